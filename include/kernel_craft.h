@@ -315,6 +315,150 @@ int kc_quantize_fp8_smooth_mul_bf16(const uint16_t* d_input,
                                     float* d_scales, int64_t rows,
                                     int64_t cols, kc_stream_t stream);
 
+/* MXFP4 (OCP microscaling, 4-bit floating point; no counterpart in the
+ * reference).  A row of K values (K a multiple of 32) is K / 32 blocks: one
+ * scale byte b each, the factor 2^(b - 127) (255: NaN), and 32 E2M1 codes
+ * (sign in bit 3; magnitudes 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte, the
+ * even value in the low nibble.  codes [rows, K/2] u8, scales [rows, K/32] u8.
+ *
+ * Quantization: b = clamp(floor(log2(largest magnitude)) - 2, -127, 127) + 127
+ * (127 for a block of zeros), codes rounded to nearest even and saturated at
+ * 6.  A block with a NaN or an infinity gets b = 255 and codes 0: all of it
+ * reads back as NaN.  Dequantization is exact but where a product leaves the
+ * output type's range.  codes 4-byte aligned. */
+int kc_quantize_mxfp4_bf16(const uint16_t* d_input, uint8_t* d_codes,
+                           uint8_t* d_scales, int64_t rows, int64_t cols,
+                           kc_stream_t stream);
+int kc_quantize_mxfp4_f32(const float* d_input, uint8_t* d_codes,
+                          uint8_t* d_scales, int64_t rows, int64_t cols,
+                          kc_stream_t stream);
+int kc_dequantize_mxfp4_bf16(const uint8_t* d_codes, const uint8_t* d_scales,
+                             uint16_t* d_output, int64_t rows, int64_t cols,
+                             kc_stream_t stream);
+int kc_dequantize_mxfp4_f32(const uint8_t* d_codes, const uint8_t* d_scales,
+                            float* d_output, int64_t rows, int64_t cols,
+                            kc_stream_t stream);
+
+/* Y[m, n] = sum_k x[m, k] w[n, k], both MXFP4 (qx, sx: [M, K]; qw, sw:
+ * [N, K]), fp32 accumulation, Y [M, N] row-major bf16 (RNE) or fp32.  K a
+ * multiple of 32 (K == 0 writes Y = 0), qx and qw 16-byte aligned, any M and
+ * N. */
+int kc_gemm_mxfp4_w4a4_bf16(const uint8_t* d_qx, const uint8_t* d_sx,
+                            const uint8_t* d_qw, const uint8_t* d_sw,
+                            uint16_t* d_y, int64_t M, int64_t N, int64_t K,
+                            kc_stream_t stream);
+int kc_gemm_mxfp4_w4a4_f32(const uint8_t* d_qx, const uint8_t* d_sx,
+                           const uint8_t* d_qw, const uint8_t* d_sw, float* d_y,
+                           int64_t M, int64_t N, int64_t K, kc_stream_t stream);
+/* The same with bf16 activations x [M, K] (16-byte aligned) on MXFP4 weights:
+ * the form for single tokens and decode batches. */
+int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw,
+                       const uint16_t* d_x, uint16_t* d_y, int64_t M, int64_t N,
+                       int64_t K, kc_stream_t stream);
+
+/* The position tables of a rotation: cos and sin fp32 [table_rows,
+ * rotary_dim / 2], and one position per token.  The first rotary_dim values
+ * of a head turn in pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with
+ * interleaved != 0: (a, b) -> (a cos - b sin, b cos + a sin). */
+typedef struct kc_rope {
+    const float* cos_table;
+    const float* sin_table;
+    const int32_t* positions;
+    int64_t table_rows;
+    int rotary_dim, interleaved;
+} kc_rope;
+
+/* RMSNorm of every query and key head and its rotation in one pass (no
+ * counterpart in the reference, whose rmsnorm.cu:40-70 takes whole rows):
+ *   y = gamma * x / sqrt(mean(x^2) + eps), then the rotation, in fp32 and
+ * rounded once.  q [tokens, q_heads, head_dim] with q_stride elements from one
+ * token to the next (a view of a fused projection's rows), k likewise;
+ * gammas [head_dim]; q_out [tokens, q_heads, head_dim] and k_out contiguous.
+ * A token with a negative position (padding) gets rows of zeros, one past
+ * the table rows of NaN.  head_dim up to 1024. */
+int kc_qk_norm_rope_bf16(const uint16_t* d_q, int64_t q_stride,
+                         const uint16_t* d_k, int64_t k_stride,
+                         const uint16_t* d_q_gamma, const uint16_t* d_k_gamma,
+                         const kc_rope* rope, float eps, int64_t tokens,
+                         int q_heads, int kv_heads, int head_dim,
+                         uint16_t* d_q_out, uint16_t* d_k_out,
+                         kc_stream_t stream);
+int kc_qk_norm_rope_f32(const float* d_q, int64_t q_stride, const float* d_k,
+                        int64_t k_stride, const float* d_q_gamma,
+                        const float* d_k_gamma, const kc_rope* rope, float eps,
+                        int64_t tokens, int q_heads, int kv_heads, int head_dim,
+                        float* d_q_out, float* d_k_out, kc_stream_t stream);
+
+/* A paged key/value cache in 8 or 4 bits (no counterpart in the reference,
+ * whose paged_attention.cu:135-142 reads fp32 pools).  Codes and scales of
+ * keys and values, a slot being page * page_size + offset in the page:
+ *   KC_KV_FP8    codes [num_pages, page_size, kv_heads, head_dim] E4M3, scales
+ *                [num_pages, page_size, kv_heads] fp32: each row quantized as
+ *                kc_quantize_fp8_per_token_* does
+ *   KC_KV_MXFP4  codes [..., head_dim / 2] and scales [..., head_dim / 32] u8
+ *                as above (head_dim a multiple of 32)
+ * head_dim up to 1024. */
+typedef enum kc_kv_format { KC_KV_FP8 = 0, KC_KV_MXFP4 = 1 } kc_kv_format;
+typedef struct kc_kv_cache {
+    void* k_codes;
+    void* k_scales;
+    void* v_codes;
+    void* v_scales;
+    int64_t num_pages;
+    int page_size, kv_heads, head_dim, format;
+} kc_kv_cache;
+
+/* Quantizes keys and values [tokens, kv_heads, head_dim] (k_stride, v_stride
+ * elements between tokens) into the slots (int64) of their tokens.  Slots
+ * outside the pool (-1: padding) are skipped; two tokens of a call must not
+ * share a slot. */
+int kc_kv_cache_write_bf16(const uint16_t* d_k, int64_t k_stride,
+                           const uint16_t* d_v, int64_t v_stride,
+                           const int64_t* d_slots, int64_t tokens,
+                           const kc_kv_cache* cache, kc_stream_t stream);
+int kc_kv_cache_write_f32(const float* d_k, int64_t k_stride, const float* d_v,
+                          int64_t v_stride, const int64_t* d_slots,
+                          int64_t tokens, const kc_kv_cache* cache,
+                          kc_stream_t stream);
+
+/* kc_qk_norm_rope_* with the keys and the values v quantized into the cache
+ * in the same pass; bit-identical to that call and kc_kv_cache_write_* on its
+ * keys.  A token whose position is not in the table writes nothing to the
+ * cache. */
+int kc_qk_norm_rope_cache_bf16(const uint16_t* d_q, int64_t q_stride,
+                               const uint16_t* d_k, int64_t k_stride,
+                               const uint16_t* d_v, int64_t v_stride,
+                               const uint16_t* d_q_gamma,
+                               const uint16_t* d_k_gamma, const kc_rope* rope,
+                               float eps, int64_t tokens, int q_heads,
+                               const int64_t* d_slots, const kc_kv_cache* cache,
+                               uint16_t* d_q_out, kc_stream_t stream);
+int kc_qk_norm_rope_cache_f32(const float* d_q, int64_t q_stride,
+                              const float* d_k, int64_t k_stride,
+                              const float* d_v, int64_t v_stride,
+                              const float* d_q_gamma, const float* d_k_gamma,
+                              const kc_rope* rope, float eps, int64_t tokens,
+                              int q_heads, const int64_t* d_slots,
+                              const kc_kv_cache* cache, float* d_q_out,
+                              kc_stream_t stream);
+
+/* The cached keys and values of a packed batch, k and v [total_tokens,
+ * kv_heads, head_dim]: token t of sequence b (cu_seqlens[b] <= t <
+ * cu_seqlens[b + 1], int32 [seqs + 1]) reads position t - cu_seqlens[b] of
+ * it, in page block_table[b, position / page_size] (int32 [seqs,
+ * max_pages]).  A position whose page is missing (past max_pages, or an entry
+ * outside the pool) reads as NaN; rows past the last sequence are left as
+ * they were. */
+int kc_kv_cache_read_bf16(const kc_kv_cache* cache,
+                          const int32_t* d_block_table, int64_t max_pages,
+                          const int32_t* d_cu_seqlens, int seqs,
+                          int64_t total_tokens, uint16_t* d_k, uint16_t* d_v,
+                          kc_stream_t stream);
+int kc_kv_cache_read_f32(const kc_kv_cache* cache, const int32_t* d_block_table,
+                         int64_t max_pages, const int32_t* d_cu_seqlens,
+                         int seqs, int64_t total_tokens, float* d_k, float* d_v,
+                         kc_stream_t stream);
+
 /* ======================================================================
  * Part 4 -- out-of-scope reference symbols (stubs).  Signatures from the
  * reference files cited; bound by kernel_craft_torch_ops.py:101-168 and

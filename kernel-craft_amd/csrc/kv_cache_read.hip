@@ -1,0 +1,185 @@
+// kv_cache_read.hip -- the quantized paged key/value cache back to rows of
+// bf16 or fp32 on gfx950 (what qk_norm_rope.hip wrote): for token t of the
+// packed batch, sequence b with cu_seqlens[b] <= t < cu_seqlens[b + 1] and
+// position t - cu_seqlens[b] in it, page block_table[b][position / page_size].
+//
+// Bound by memory: 1 (FP8) or 0.53 (MXFP4) bytes in and 2 or 4 out per value.
+// A workgroup takes a tile of tokens: its first threads find one token's slot
+// each (a binary search of cu_seqlens, all searches of the tile at once instead
+// of one before every row), then all threads walk the tile's rows in units of
+// 8 values.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv_cache.hpp"
+
+namespace {
+
+using namespace kc::mx;
+using kc::kWave;
+
+constexpr int kThreads = 256;
+constexpr int kMaxTile = 64;
+
+template <bool BF16>
+using Elem = std::conditional_t<BF16, uint16_t, float>;
+
+struct Args {
+    const uint8_t* codes[2];   // keys, values
+    const void* scales[2];
+    void* out[2];
+    const int32_t *table, *cu;
+    int64_t max_pages, num_pages, total;
+    int page_size, kv_heads, D, seqs, tile;
+};
+
+constexpr int64_t kBad = -1, kOutside = -2;
+
+// Slot of token t; kBad where its page is missing, kOutside where it belongs to
+// no sequence.
+__device__ __forceinline__ int64_t slot_of(const Args& p, int64_t t) {
+    if (t >= p.total || t < p.cu[0] || t >= p.cu[p.seqs]) return kOutside;
+    int lo = 0, hi = p.seqs - 1;  // first b with cu[b + 1] > t
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (p.cu[mid + 1] > t) hi = mid;
+        else lo = mid + 1;
+    }
+    const int64_t pos = t - p.cu[lo];
+    if (pos < 0) return kBad;  // cu_seqlens that do not ascend
+    const int64_t page_at = pos / p.page_size;
+    if (page_at >= p.max_pages) return kBad;
+    const int32_t page = p.table[lo * p.max_pages + page_at];
+    if (page < 0 || page >= p.num_pages) return kBad;
+    return static_cast<int64_t>(page) * p.page_size + (pos - page_at * p.page_size);
+}
+
+template <bool BF16, bool FP8, bool VEC>
+__global__ __launch_bounds__(kThreads) void kv_read_kernel(const Args p) {
+    __shared__ int64_t slot[kMaxTile];
+    const int which = blockIdx.y, tid = threadIdx.x;
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
+    if (tid < p.tile) slot[tid] = slot_of(p, t0 + tid);
+    __syncthreads();
+    const uint8_t* codes = p.codes[which];
+    Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out[which]);
+    constexpr int W = VEC ? 8 : 1;                 // values per unit
+    const int units = p.kv_heads * p.D / W, per_head = p.D / W;
+    const int step_t = kThreads / units, step_u = kThreads - step_t * units;
+    int tt = tid / units, u = tid - tt * units;
+    const float nan = __uint_as_float(0x7FC00000u);
+    while (tt < p.tile) {
+        const int64_t s = slot[tt];
+        if (s != kOutside) {
+            const int h = u / per_head, d = (u - h * per_head) * W;
+            const int64_t row = s * p.kv_heads + h;          // kBad reads nothing
+            const int64_t to = ((t0 + tt) * p.kv_heads + h) * p.D + d;
+            if constexpr (VEC) {
+                f32x4 lo = {nan, nan, nan, nan}, hi = lo;
+                if (s != kBad) {
+                    if constexpr (FP8) {
+                        const u32x2 c = *reinterpret_cast<const u32x2*>(codes + row * p.D + d);
+                        const float sc = static_cast<const float*>(p.scales[which])[row];
+                        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.x), false);
+                        const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.x), true);
+                        const auto e = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.y), false);
+                        const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.y), true);
+                        lo = f32x4{a[0] * sc, a[1] * sc, b[0] * sc, b[1] * sc};
+                        hi = f32x4{e[0] * sc, e[1] * sc, f[0] * sc, f[1] * sc};
+                    } else {
+                        const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + (row * p.D + d) / 2);
+                        const uint8_t sb = static_cast<const uint8_t*>(p.scales[which])[(row * p.D + d) / kBlock];
+                        decode8_f32(c, scale_value(sb), lo, hi);
+                    }
+                }
+                if constexpr (BF16) {
+                    *reinterpret_cast<u32x4*>(out + to) =
+                        u32x4{kc::pack_bf16x2(lo.x, lo.y), kc::pack_bf16x2(lo.z, lo.w), kc::pack_bf16x2(hi.x, hi.y),
+                              kc::pack_bf16x2(hi.z, hi.w)};
+                } else {
+                    f32x4* o = reinterpret_cast<f32x4*>(out + to);
+                    o[0] = lo;
+                    o[1] = hi;
+                }
+            } else {
+                float v = nan;
+                if (s != kBad) {
+                    if constexpr (FP8) {
+                        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes[row * p.D + d]), false);
+                        v = a[0] * static_cast<const float*>(p.scales[which])[row];
+                    } else {
+                        const uint32_t c = codes[(row * p.D + d) / 2];
+                        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0);
+                        v = (d & 1 ? a.y : a.x) *
+                            scale_value(static_cast<const uint8_t*>(p.scales[which])[(row * p.D + d) / kBlock]);
+                    }
+                }
+                if constexpr (BF16) out[to] = kc::f32_to_bf16(v);
+                else out[to] = v;
+            }
+        }
+        tt += step_t;
+        u += step_u;
+        if (u >= units) {
+            u -= units;
+            ++tt;
+        }
+    }
+}
+
+template <bool BF16>
+int cache_read(const char* fn, const kc_kv_cache* cache, const int32_t* table, int64_t max_pages, const int32_t* cu,
+               int seqs, int64_t total, Elem<BF16>* k, Elem<BF16>* v, hipStream_t stream) {
+    const int st = kc::kv::check_cache(fn, cache);
+    if (st != KC_SUCCESS) return st;
+    if (max_pages < 0 || seqs < 0 || total < 0)
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: negative shape", fn);
+    if (seqs == 0 || total == 0) return KC_SUCCESS;
+    if (!cu || !k || !v || (max_pages > 0 && !table))
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
+    Args p{};
+    p.codes[0] = static_cast<const uint8_t*>(cache->k_codes);
+    p.codes[1] = static_cast<const uint8_t*>(cache->v_codes);
+    p.scales[0] = cache->k_scales;
+    p.scales[1] = cache->v_scales;
+    p.out[0] = k;
+    p.out[1] = v;
+    p.table = table;
+    p.cu = cu;
+    p.max_pages = max_pages;
+    p.num_pages = cache->num_pages;
+    p.total = total;
+    p.page_size = cache->page_size;
+    p.kv_heads = cache->kv_heads;
+    p.D = cache->head_dim;
+    p.seqs = seqs;
+    const bool fp8 = cache->format == KC_KV_FP8;
+    const uintptr_t in = fp8 ? 8 : 4;
+    const bool vec = p.D % 8 == 0 && kc::aligned(k, 16) && kc::aligned(v, 16) && kc::aligned(p.codes[0], in) &&
+                     kc::aligned(p.codes[1], in);
+    p.tile = static_cast<int>(std::clamp<int64_t>(total / 1024, 4, kMaxTile));
+    const int64_t grid = (total + p.tile - 1) / p.tile;
+    if (grid > kc::kv::kMaxGrid / 2) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
+    const dim3 g(static_cast<unsigned>(grid), 2);
+    if (fp8 && vec) kv_read_kernel<BF16, true, true><<<g, kThreads, 0, stream>>>(p);
+    else if (fp8) kv_read_kernel<BF16, true, false><<<g, kThreads, 0, stream>>>(p);
+    else if (vec) kv_read_kernel<BF16, false, true><<<g, kThreads, 0, stream>>>(p);
+    else kv_read_kernel<BF16, false, false><<<g, kThreads, 0, stream>>>(p);
+    return kc::check_launch(fn);
+}
+
+}  // namespace
+
+extern "C" int kc_kv_cache_read_bf16(const kc_kv_cache* cache, const int32_t* d_block_table, int64_t max_pages,
+                                     const int32_t* d_cu_seqlens, int seqs, int64_t total_tokens, uint16_t* d_k,
+                                     uint16_t* d_v, kc_stream_t stream) {
+    return cache_read<true>("kc_kv_cache_read_bf16", cache, d_block_table, max_pages, d_cu_seqlens, seqs, total_tokens,
+                            d_k, d_v, stream);
+}
+
+extern "C" int kc_kv_cache_read_f32(const kc_kv_cache* cache, const int32_t* d_block_table, int64_t max_pages,
+                                    const int32_t* d_cu_seqlens, int seqs, int64_t total_tokens, float* d_k, float* d_v,
+                                    kc_stream_t stream) {
+    return cache_read<false>("kc_kv_cache_read_f32", cache, d_block_table, max_pages, d_cu_seqlens, seqs, total_tokens,
+                             d_k, d_v, stream);
+}

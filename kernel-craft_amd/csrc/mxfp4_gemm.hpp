@@ -1,0 +1,17 @@
+// mxfp4_gemm.hpp -- host helpers shared by the MXFP4 products.
+#pragma once
+
+#include "mxfp4.hpp"
+
+namespace kc {
+namespace mx {
+
+// Shapes of Y [M, N] = X [M, K] W [N, K]^T; y checked where Y has elements.
+int check_gemm(const char* fn, int64_t M, int64_t N, int64_t K, const void* y);
+
+// Y = 0 (an empty contraction).
+template <bool YBF16>
+int fill_zero(const char* fn, void* y, int64_t n, hipStream_t stream);
+
+}  // namespace mx
+}  // namespace kc

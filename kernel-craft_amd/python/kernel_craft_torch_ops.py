@@ -30,7 +30,8 @@ What this module adds:
 * there is no CPU fallback: a CPU tensor is an error;
 * operators for the entry points the reference lacks (bf16 GEMV and its
   chain, the M > 1 GEMM, RMSNorm and its fusions, bf16 and fused-SmoothQuant
-  FP8 quantization, the FP8 GEMM, checkpoint conversion).
+  FP8 quantization, the FP8 GEMM, checkpoint conversion, MXFP4 quantization
+  and products, head norms with rotation, the quantized key/value cache).
 
 Usage
 -----
@@ -142,6 +143,21 @@ PROTOTYPES = {
     "kc_rmsnorm_bf16": ([_vp, _vp, _vp, _i, _i, _f, _vp], _i),
     "kc_rmsnorm_gemv_int4_bf16": ([_vp, _vp, _f, _vp, _vp, _vp, _vp, _i, _i, _i, _vp], _i),
     "kc_rmsnorm_quantize_fp8_bf16": ([_vp, _vp, _f, _vp, _vp, _i64, _i64, _vp], _i),
+    "kc_quantize_mxfp4_bf16": ([_vp, _vp, _vp, _i64, _i64, _vp], _i),
+    "kc_quantize_mxfp4_f32": ([_vp, _vp, _vp, _i64, _i64, _vp], _i),
+    "kc_dequantize_mxfp4_bf16": ([_vp, _vp, _vp, _i64, _i64, _vp], _i),
+    "kc_dequantize_mxfp4_f32": ([_vp, _vp, _vp, _i64, _i64, _vp], _i),
+    "kc_gemm_mxfp4_w4a4_bf16": ([_vp] * 5 + [_i64, _i64, _i64, _vp], _i),
+    "kc_gemm_mxfp4_w4a4_f32": ([_vp] * 5 + [_i64, _i64, _i64, _vp], _i),
+    "kc_gemm_mxfp4_bf16": ([_vp] * 4 + [_i64, _i64, _i64, _vp], _i),
+    **{f"kc_qk_norm_rope_{t}": ([_vp, _i64, _vp, _i64, _vp, _vp, _vp, _f, _i64, _i, _i, _i, _vp,
+                                 _vp, _vp], _i) for t in ("bf16", "f32")},
+    **{f"kc_qk_norm_rope_cache_{t}": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _f, _i64,
+                                       _i, _vp, _vp, _vp, _vp], _i) for t in ("bf16", "f32")},
+    **{f"kc_kv_cache_write_{t}": ([_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp], _i)
+       for t in ("bf16", "f32")},
+    **{f"kc_kv_cache_read_{t}": ([_vp, _vp, _i64, _vp, _i, _i64, _vp, _vp, _vp], _i)
+       for t in ("bf16", "f32")},
 }
 
 
@@ -777,6 +793,328 @@ def fp8_quantize_smooth(x, smooth, mode: str = "div") -> Tuple:
         st = fn(_ptr(x), _ptr(smooth), _ptr(q), _ptr(s), rows, cols, _stream())
     _check("fp8_quantize_smooth", st)
     return q, s
+
+
+# ---------------------------------------------------------------------------
+# MXFP4, head norms with rotation, the quantized cache (no reference
+# counterpart)
+# ---------------------------------------------------------------------------
+
+
+def _one_gpu(op: str, *tensors):
+    """The device that all tensors live on; ValueError unless it is one GPU."""
+    _on_gpu(op, *tensors)
+    device = tensors[0].device
+    for t in tensors:
+        if t.device != device:
+            raise ValueError(f"{op}: tensors on {device} and {t.device}; they must be on one GPU")
+    return device
+
+
+def _launch(device, fn, *args) -> int:
+    """fn(*args, stream) on the current stream of ``device``."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        return fn(*args, _stream())
+    with torch.cuda.device(device):
+        return fn(*args, _stream())
+
+
+def _mx(op: str, codes, scales, names=("codes", "scales")):
+    """Validated (codes, scales, rows, cols) of an MXFP4 matrix: u8 codes [rows, cols / 2]
+    and u8 scales [rows, cols / 32]."""
+    import torch
+    codes = _arg(f"{op}: {names[0]}", codes, torch.uint8)
+    scales = _arg(f"{op}: {names[1]}", scales, torch.uint8)
+    if (codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0]
+            or scales.shape[1] * 16 != codes.shape[1]):
+        raise ValueError(f"{op}: {names[0]} {tuple(codes.shape)} and {names[1]} "
+                         f"{tuple(scales.shape)} must be [rows, K / 2] and [rows, K / 32]")
+    return codes, scales, codes.shape[0], codes.shape[1] * 2
+
+
+def mxfp4_quantize(x) -> Tuple:
+    """bf16 or fp32 x [rows, K] (K a multiple of 32) -> MXFP4 (u8 codes [rows, K / 2], low nibble =
+    even k; u8 scales [rows, K / 32], the factor 2^(byte - 127)): activations per token, or a
+    weight matrix [N, K].  A block with a NaN or an infinity becomes all NaN
+    (kc_quantize_mxfp4_*)."""
+    import torch
+    x = _arg("mxfp4_quantize: x", x, (torch.bfloat16, torch.float32))
+    if x.dim() != 2 or x.shape[1] % 32:
+        raise ValueError(f"mxfp4_quantize: x {tuple(x.shape)} must be [rows, K], K a multiple of 32")
+    device = _one_gpu("mxfp4_quantize", x)
+    rows, cols = x.shape
+    codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=device)
+    scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=device)
+    lib = _get_lib()
+    fn = lib.kc_quantize_mxfp4_bf16 if x.dtype == torch.bfloat16 else lib.kc_quantize_mxfp4_f32
+    with kernel_span("mxfp4_quantize", rows=rows, cols=cols):
+        st = _launch(device, fn, _ptr(x), _ptr(codes), _ptr(scales), rows, cols)
+    _check("mxfp4_quantize", st)
+    return codes, scales
+
+
+def mxfp4_dequantize(codes, scales, out_dtype=None):
+    """The values [rows, K] of MXFP4 codes and scales, torch.bfloat16 (default) or torch.float32:
+    exact but where a value leaves the type's range (kc_dequantize_mxfp4_*)."""
+    import torch
+    out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"mxfp4_dequantize: out_dtype must be bfloat16 or float32, not {out_dtype}")
+    codes, scales, rows, cols = _mx("mxfp4_dequantize", codes, scales)
+    device = _one_gpu("mxfp4_dequantize", codes, scales)
+    out = torch.empty(rows, cols, dtype=out_dtype, device=device)
+    lib = _get_lib()
+    fn = lib.kc_dequantize_mxfp4_bf16 if out_dtype == torch.bfloat16 else lib.kc_dequantize_mxfp4_f32
+    with kernel_span("mxfp4_dequantize", rows=rows, cols=cols):
+        st = _launch(device, fn, _ptr(codes), _ptr(scales), _ptr(out), rows, cols)
+    _check("mxfp4_dequantize", st)
+    return out
+
+
+def mxfp4_gemm_w4a4(qx, sx, qw, sw, out_dtype=None):
+    """Y [M, N] = X W^T of two MXFP4 matrices on the 4-bit matrix cores, fp32 accumulation:
+    (qx, sx) [M, K] from mxfp4_quantize on the activations, (qw, sw) [N, K] from it on the
+    weights.  Any M and N; out_dtype torch.bfloat16 (default) or torch.float32
+    (kc_gemm_mxfp4_w4a4_*)."""
+    import torch
+    out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"mxfp4_gemm_w4a4: out_dtype must be bfloat16 or float32, not {out_dtype}")
+    qx, sx, M, K = _mx("mxfp4_gemm_w4a4", qx, sx, ("qx", "sx"))
+    qw, sw, N, Kw = _mx("mxfp4_gemm_w4a4", qw, sw, ("qw", "sw"))
+    if K != Kw:
+        raise ValueError(f"mxfp4_gemm_w4a4: x has K={K}, w has K={Kw}")
+    device = _one_gpu("mxfp4_gemm_w4a4", qx, sx, qw, sw)
+    y = torch.empty(M, N, dtype=out_dtype, device=device)
+    lib = _get_lib()
+    fn = lib.kc_gemm_mxfp4_w4a4_bf16 if out_dtype == torch.bfloat16 else lib.kc_gemm_mxfp4_w4a4_f32
+    with kernel_span("mxfp4_gemm_w4a4", m=M, n=N, k=K):
+        st = _launch(device, fn, _ptr(qx), _ptr(sx), _ptr(qw), _ptr(sw), _ptr(y), M, N, K)
+    _check("mxfp4_gemm_w4a4", st)
+    return y
+
+
+def mxfp4_gemm_bf16(qw, sw, x):
+    """Y [M, N] bf16 = X W^T for bf16 X [M, K] and MXFP4 weights (qw, sw) [N, K], fp32
+    accumulation: the form for single tokens and decode batches (kc_gemm_mxfp4_bf16)."""
+    import torch
+    qw, sw, N, K = _mx("mxfp4_gemm_bf16", qw, sw, ("qw", "sw"))
+    x = _arg("mxfp4_gemm_bf16: x", x, torch.bfloat16)
+    if x.dim() != 2 or x.shape[1] != K:
+        raise ValueError(f"mxfp4_gemm_bf16: x must be [M, {K}], not {list(x.shape)}")
+    device = _one_gpu("mxfp4_gemm_bf16", qw, sw, x)
+    M = x.shape[0]
+    y = torch.empty(M, N, dtype=torch.bfloat16, device=device)
+    with kernel_span("mxfp4_gemm_bf16", m=M, n=N, k=K):
+        st = _launch(device, _get_lib().kc_gemm_mxfp4_bf16, _ptr(qw), _ptr(sw), _ptr(x), _ptr(y), M,
+                     N, K)
+    _check("mxfp4_gemm_bf16", st)
+    return y
+
+
+class Rope(ctypes.Structure):
+    """kc_rope (include/kernel_craft.h)."""
+    _fields_ = [("cos_table", ctypes.c_void_p), ("sin_table", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("table_rows", ctypes.c_int64),
+                ("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int)]
+
+
+class KvCache(ctypes.Structure):
+    """kc_kv_cache (include/kernel_craft.h)."""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_codes", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("format", ctypes.c_int)]
+
+
+def _heads(name: str, t, dtypes, tokens: Optional[int] = None, heads: Optional[int] = None,
+           head_dim: Optional[int] = None):
+    """``t`` [tokens, heads, head_dim] with the heads of a token one after the other (a view of a
+    fused projection's rows stays one, anything else is copied); ValueError for another type or
+    shape."""
+    allowed = dtypes if isinstance(dtypes, tuple) else (dtypes,)
+    if t.dtype not in allowed:
+        raise ValueError(f"{name} has dtype {t.dtype}; expected "
+                         f"{' or '.join(str(d) for d in allowed)}")
+    want = (tokens, heads, head_dim)
+    if t.dim() != 3 or any(w is not None and w != n for w, n in zip(want, t.shape)):
+        raise ValueError(f"{name} {tuple(t.shape)} must be [tokens, heads, head_dim]"
+                         + ("" if tokens is None else f" with {want}"))
+    _, H, D = t.shape
+    s = t.stride()
+    if (D > 1 and s[2] != 1) or (H > 1 and s[1] != D):
+        return t.contiguous()
+    return t
+
+
+def _rope(op: str, dtype, T: int, D: int, q_gamma, k_gamma, cos, sin, positions, interleaved: bool):
+    """Validated (q_gamma, k_gamma, cos, sin, positions, kc_rope)."""
+    import torch
+    q_gamma = _arg(f"{op}: q_gamma", q_gamma, dtype)
+    k_gamma = _arg(f"{op}: k_gamma", k_gamma, dtype)
+    cos = _arg(f"{op}: cos", cos, torch.float32)
+    sin = _arg(f"{op}: sin", sin, torch.float32)
+    positions = _arg(f"{op}: positions", positions, torch.int32)
+    if q_gamma.shape != (D,) or k_gamma.shape != (D,):
+        raise ValueError(f"{op}: q_gamma and k_gamma must be [{D}]")
+    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > D:
+        raise ValueError(f"{op}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must both be "
+                         f"[table rows, rotary_dim / 2] with rotary_dim at most {D}")
+    if positions.shape != (T,):
+        raise ValueError(f"{op}: positions {tuple(positions.shape)} must be [{T}]")
+    return q_gamma, k_gamma, cos, sin, positions, Rope(
+        _ptr(cos), _ptr(sin), _ptr(positions), cos.shape[0], 2 * cos.shape[1], bool(interleaved))
+
+
+def _kv_cache(op: str, k_codes, k_scales, v_codes, v_scales):
+    """(kc_kv_cache, kv_heads, head_dim) of a cache's four tensors, which must be contiguous
+    (they are written to); fp32 scales mean FP8 rows, u8 scales MXFP4 rows."""
+    import torch
+    fp8 = k_scales.dtype == torch.float32
+    for name, t, dtypes in (("k_codes", k_codes, (torch.int8, torch.uint8) if fp8 else (torch.uint8,)),
+                            ("v_codes", v_codes, (k_codes.dtype,)),
+                            ("k_scales", k_scales, (torch.float32, torch.uint8)),
+                            ("v_scales", v_scales, (k_scales.dtype,))):
+        if t.dtype not in dtypes:
+            raise ValueError(f"{op}: {name} has dtype {t.dtype}; expected "
+                             f"{' or '.join(str(d) for d in dtypes)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{op}: {name} must be contiguous")
+    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+        raise ValueError(f"{op}: k_codes {tuple(k_codes.shape)} and v_codes {tuple(v_codes.shape)} "
+                         "must both be [pages, page_size, kv_heads, codes of a head]")
+    pages, page, heads, width = k_codes.shape
+    D = width if fp8 else 2 * width
+    want = (pages, page, heads) if fp8 else (pages, page, heads, D // 32)
+    if k_scales.shape != want or v_scales.shape != want or (not fp8 and D % 32):
+        raise ValueError(f"{op}: k_scales {tuple(k_scales.shape)} and v_scales "
+                         f"{tuple(v_scales.shape)} must be {want} (head_dim {D})")
+    return KvCache(_ptr(k_codes), _ptr(k_scales), _ptr(v_codes), _ptr(v_scales), pages, page, heads,
+                   D, 0 if fp8 else 1), heads, D
+
+
+def qk_norm_rope(q, k, q_gamma, k_gamma, cos, sin, positions, eps: float = 1e-6,
+                 interleaved: bool = False) -> Tuple:
+    """RMSNorm of each query and key head and its rotation in one pass, fp32 arithmetic rounded
+    once: q [T, q_heads, D] and k [T, kv_heads, D] bf16 or fp32 (views of a fused projection's
+    output are read in place), gammas [D] of their type, cos and sin fp32 [table rows, R / 2],
+    positions int32 [T].  The first R values of a head turn in pairs (i, i + R / 2), or
+    (2i, 2i + 1) if ``interleaved``.  Returns new contiguous (q, k).  Tokens with a negative
+    position give zeros, positions past the tables NaN (kc_qk_norm_rope_*)."""
+    import torch
+    op = "qk_norm_rope"
+    q = _heads(f"{op}: q", q, (torch.bfloat16, torch.float32))
+    T, Hq, D = q.shape
+    k = _heads(f"{op}: k", k, q.dtype, T, None, D)
+    q_gamma, k_gamma, cos, sin, positions, rope = _rope(op, q.dtype, T, D, q_gamma, k_gamma, cos,
+                                                        sin, positions, interleaved)
+    device = _one_gpu(op, q, k, q_gamma, k_gamma, cos, sin, positions)
+    Hkv = k.shape[1]
+    q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=device)
+    k_out = torch.empty(T, Hkv, D, dtype=q.dtype, device=device)
+    lib = _get_lib()
+    fn = lib.kc_qk_norm_rope_bf16 if q.dtype == torch.bfloat16 else lib.kc_qk_norm_rope_f32
+    with kernel_span(op, tokens=T, heads=Hq, kv_heads=Hkv, head_dim=D):
+        st = _launch(device, fn, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(q_gamma),
+                     _ptr(k_gamma), ctypes.byref(rope), eps, T, Hq, Hkv, D, _ptr(q_out), _ptr(k_out))
+    _check(op, st)
+    return q_out, k_out
+
+
+def qk_norm_rope_cache(q, k, v, q_gamma, k_gamma, cos, sin, positions, slots, k_codes, k_scales,
+                       v_codes, v_scales, eps: float = 1e-6, interleaved: bool = False):
+    """qk_norm_rope with the keys and the values v [T, kv_heads, D] quantized into the cache
+    (kv_cache_write's tensors and slots) in the same pass; the same bits as the two calls.
+    Returns q.  A token whose position is negative or past the tables writes nothing to the
+    cache (kc_qk_norm_rope_cache_*)."""
+    import torch
+    op = "qk_norm_rope_cache"
+    q = _heads(f"{op}: q", q, (torch.bfloat16, torch.float32))
+    T, Hq, D = q.shape
+    cache, Hkv, Dc = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
+    if D != Dc:
+        raise ValueError(f"{op}: q has head_dim {D}, the cache {Dc}")
+    k = _heads(f"{op}: k", k, q.dtype, T, Hkv, D)
+    v = _heads(f"{op}: v", v, q.dtype, T, Hkv, D)
+    q_gamma, k_gamma, cos, sin, positions, rope = _rope(op, q.dtype, T, D, q_gamma, k_gamma, cos,
+                                                        sin, positions, interleaved)
+    slots = _arg(f"{op}: slots", slots, torch.int64)
+    if slots.shape != (T,):
+        raise ValueError(f"{op}: slots {tuple(slots.shape)} must be [{T}]")
+    device = _one_gpu(op, q, k, v, q_gamma, k_gamma, cos, sin, positions, slots, k_codes, k_scales,
+                      v_codes, v_scales)
+    q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=device)
+    lib = _get_lib()
+    fn = (lib.kc_qk_norm_rope_cache_bf16 if q.dtype == torch.bfloat16
+          else lib.kc_qk_norm_rope_cache_f32)
+    with kernel_span(op, tokens=T, heads=Hq, kv_heads=Hkv, head_dim=D):
+        st = _launch(device, fn, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0),
+                     _ptr(q_gamma), _ptr(k_gamma), ctypes.byref(rope), eps, T, Hq, _ptr(slots),
+                     ctypes.byref(cache), _ptr(q_out))
+    _check(op, st)
+    return q_out
+
+
+def kv_cache_write(k, v, slots, k_codes, k_scales, v_codes, v_scales) -> None:
+    """Quantizes bf16 or fp32 keys and values [T, kv_heads, D] into a paged cache, token t into
+    slot slots[t] (int64, page * page_size + offset).  Slots outside the pool (-1: padding)
+    are skipped; two tokens of a call must not name the same slot.
+
+    An FP8 cache: int8 codes [pages, page_size, kv_heads, D] with fp32 scales [pages, page_size,
+    kv_heads], rows quantized as fp8_quantize_rows does.  An MXFP4 cache: u8 codes [...,
+    D / 2] with u8 scales [..., D / 32], rows as mxfp4_quantize.  The scales' type tells
+    which (kc_kv_cache_write_*)."""
+    import torch
+    op = "kv_cache_write"
+    cache, H, D = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
+    k = _heads(f"{op}: k", k, (torch.bfloat16, torch.float32))
+    T = k.shape[0]
+    k = _heads(f"{op}: k", k, k.dtype, T, H, D)
+    v = _heads(f"{op}: v", v, k.dtype, T, H, D)
+    slots = _arg(f"{op}: slots", slots, torch.int64)
+    if slots.shape != (T,):
+        raise ValueError(f"{op}: slots {tuple(slots.shape)} must be [{T}]")
+    device = _one_gpu(op, k, v, slots, k_codes, k_scales, v_codes, v_scales)
+    lib = _get_lib()
+    fn = lib.kc_kv_cache_write_bf16 if k.dtype == torch.bfloat16 else lib.kc_kv_cache_write_f32
+    with kernel_span(op, tokens=T, kv_heads=H, head_dim=D):
+        st = _launch(device, fn, _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(slots), T,
+                     ctypes.byref(cache))
+    _check(op, st)
+
+
+def kv_cache_read(k_codes, k_scales, v_codes, v_scales, block_table, cu_seqlens, total_tokens: int,
+                  out_dtype=None) -> Tuple:
+    """The keys and values of a packed batch from the cache, (k, v) [total_tokens, kv_heads, D],
+    torch.bfloat16 (default) or torch.float32: token t of sequence b (cu_seqlens[b] <= t <
+    cu_seqlens[b + 1], int32 [sequences + 1]) is position t - cu_seqlens[b], in page
+    block_table[b, position // page_size] (int32 [sequences, most pages]).  A position whose page
+    is missing or outside the pool reads as NaN; rows past the last sequence are not written
+    (kc_kv_cache_read_*)."""
+    import torch
+    op = "kv_cache_read"
+    out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{op}: out_dtype must be bfloat16 or float32, not {out_dtype}")
+    cache, H, D = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
+    block_table = _arg(f"{op}: block_table", block_table, torch.int32)
+    cu_seqlens = _arg(f"{op}: cu_seqlens", cu_seqlens, torch.int32)
+    if block_table.dim() != 2 or cu_seqlens.shape != (block_table.shape[0] + 1,):
+        raise ValueError(f"{op}: block_table {tuple(block_table.shape)} and cu_seqlens "
+                         f"{tuple(cu_seqlens.shape)} must be [sequences, pages] and [sequences + 1]")
+    if total_tokens < 0:
+        raise ValueError(f"{op}: total_tokens={total_tokens} is negative")
+    device = _one_gpu(op, k_codes, k_scales, v_codes, v_scales, block_table, cu_seqlens)
+    k = torch.empty(total_tokens, H, D, dtype=out_dtype, device=device)
+    v = torch.empty_like(k)
+    lib = _get_lib()
+    fn = lib.kc_kv_cache_read_bf16 if out_dtype == torch.bfloat16 else lib.kc_kv_cache_read_f32
+    with kernel_span(op, tokens=total_tokens, kv_heads=H, head_dim=D):
+        st = _launch(device, fn, ctypes.byref(cache), _ptr(block_table), block_table.shape[1],
+                     _ptr(cu_seqlens), block_table.shape[0], total_tokens, _ptr(k), _ptr(v))
+    _check(op, st)
+    return k, v
 
 
 # ---------------------------------------------------------------------------
