@@ -1,5 +1,25 @@
-// mxfp4_gemm_a16.hip -- bf16 activations times MXFP4 weights on gfx950:
+// mxfp4_gemm_a16.hip -- bf16 activations times MXFP4 weights on gfx950, the linear
+// layer of single tokens and decode batches.  No counterpart in the reference.
+//
 //   Y[m, n] = sum_k x[m, k] * e2m1(qw[n, k]) 2^(sw[n, k / 32] - 127)
+//
+// An E2M1 value times a power of two is a bf16 value, so the weights are decoded in
+// registers (v_cvt_scalef32_pk_bf16_fp4: two codes and their scale in one
+// instruction) and multiplied on the bf16 matrix cores with fp32 accumulation; the
+// only rounding is that of Y.  Weights outside bf16's range (scale bytes under 2
+// or over 252 with large codes) are rounded or overflow as bf16 values do.
+//
+// Bound by the weight stream (0.53 bytes a weight).  A workgroup of KW waves owns
+// RT tiles of 16 weight rows and MT tiles of 16 tokens; wave w takes K steps w,
+// w + KW, ... of 256 values, and the partial sums meet in LDS in a fixed order.
+// Tokens past 16 MT are further workgroups.
+//
+// A weight load carries 8 whole rows of a step (128 bytes, a cache line each); a
+// lane and its neighbour l ^ 1 exchange one 16-byte chunk, after which lane
+// (i, kb) holds blocks 2 kb and 2 kb + 1 of row row_of(i) = i / 2 + 8 (i % 2).  A
+// 4 x 4 transpose of dwords over the lanes l % 16 (two permlane swaps) then
+// leaves dword g of block b with lane (i, g): the 8 values the matrix core wants from
+// it when X is read in its own order, 64 neighbouring bytes of each row.
 #include <algorithm>
 
 #include "mxfp4_gemm.hpp"
@@ -7,39 +27,235 @@
 namespace {
 
 using namespace kc::mx;
-using kc::kWave;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kThreads = 256;
+constexpr int kStep = 256;   // values of K per step
+constexpr int kBK = 128;     // their bytes
 
-// One wave per 16 x 16 tile of Y.
-__global__ __launch_bounds__(kThreads) void gemm_mxfp4_a16_kernel(const uint8_t* __restrict__ qw,
-                                                                  const uint8_t* __restrict__ sw,
-                                                                  const uint16_t* __restrict__ x,
-                                                                  uint16_t* __restrict__ y, int64_t M, int64_t N,
-                                                                  int64_t K, int64_t tiles_n, int64_t tiles) {
+__device__ __forceinline__ uint32_t swap_pair(uint32_t v) {  // lane l reads lane l ^ 1
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true));
+}
+
+// v[c] of lane (i, g) becomes v[g] of lane (i, c).
+__device__ __forceinline__ void transpose4(uint32_t (&v)[4]) {
+    auto swap32 = [](uint32_t& a, uint32_t& b) {  // lanes 32-63 of a with lanes 0-31 of b
+        const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+        a = r[0];
+        b = r[1];
+    };
+    auto swap16 = [](uint32_t& a, uint32_t& b) {  // odd rows of 16 lanes of a with even rows of b
+        const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+        a = r[0];
+        b = r[1];
+    };
+    swap32(v[0], v[2]);
+    swap32(v[1], v[3]);
+    swap16(v[0], v[1]);
+    swap16(v[2], v[3]);
+}
+
+// 8 codes -> 8 bf16 values at scale byte b.
+__device__ __forceinline__ bf16x8 decode(uint32_t c, uint32_t b) {
+    const float s = scale_operand(b);
+    const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1);
+    const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), t = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3);
+    return bf16x8{p.x, p.y, q.x, q.y, r.x, r.y, t.x, t.y};
+}
+
+template <int MT, int RT, int KW, int DX>
+__global__ __launch_bounds__(KW * 64) void gemm_mxfp4_a16_kernel(const uint8_t* __restrict__ qw, const uint8_t* __restrict__ sw,
+                                                                 const uint16_t* __restrict__ x, uint16_t* __restrict__ y,
+                                                                 int M, int N, int K, bool vec) {
+    __shared__ f32x4 red[KW][RT * MT][64];
     const int lane = threadIdx.x & 63;
-    const int64_t tile = static_cast<int64_t>(blockIdx.x) * (kThreads / kWave) + (threadIdx.x >> 6);
-    if (tile >= tiles) return;
-    const int i = lane & 15, g = lane >> 4;
-    const int64_t m0 = tile / tiles_n * 16, n0 = tile % tiles_n * 16, blocks = K / kBlock;
-    const int64_t xr = min(m0 + i, M - 1), wr = min(n0 + i, N - 1);
-    f32x4 acc = {0, 0, 0, 0};
-    for (int64_t b = 0; b < blocks; ++b) {
-        const u32x4 xv = *reinterpret_cast<const u32x4*>(x + xr * K + b * 32 + 8 * g);
-        const uint32_t c = *reinterpret_cast<const uint32_t*>(qw + (wr * blocks + b) * 16 + 4 * g);
-        const u32x4 wv = decode8_bf16(c, scale_value(sw[wr * blocks + b]));
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv), __builtin_bit_cast(bf16x8, xv),
-                                                      acc, 0, 0, 0);
-    }
-    const int64_t m = m0 + i;
-    if (m >= M) return;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int i = lane & 15, kb = lane >> 4;
+    const bool even = (lane & 1) == 0;
+    const int n0 = static_cast<int>(blockIdx.x) * 16 * RT, m0 = static_cast<int>(blockIdx.y) * 16 * MT;
+    const int kbytes = K / 2, blocks = K / kBlock;
+    const uint8_t* wbase = qw + static_cast<int64_t>(n0) * kbytes;
+    const uint8_t* wsbase = sw + static_cast<int64_t>(n0) * blocks;
+    const uint16_t* xbase = x + static_cast<int64_t>(m0) * K;
+    const int chunk = 2 * kb + (i & 1), r8 = i >> 1, orow = (i >> 1) + 8 * (i & 1);
+    uint32_t woff[RT][2], wsoff[RT], xoff[MT];
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        const int64_t n = n0 + 4 * g + v;
-        if (n < N) y[m * N + n] = kc::f32_to_bf16(acc[v]);
+    for (int r = 0; r < RT; ++r) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            woff[r][h] = static_cast<uint32_t>(min(n0 + 16 * r + 8 * h + r8, N - 1) - n0) * static_cast<uint32_t>(kbytes) + 16u * chunk;
+        wsoff[r] = static_cast<uint32_t>(min(n0 + 16 * r + orow, N - 1) - n0) * static_cast<uint32_t>(blocks);
     }
+#pragma unroll
+    for (int c = 0; c < MT; ++c)
+        xoff[c] = static_cast<uint32_t>(min(m0 + 16 * c + i, M - 1) - m0) * static_cast<uint32_t>(K) + 8u * kb;
+
+    f32x4 acc[RT][MT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < MT; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int full = K / kStep;
+    const int mine = full > wave ? (full - wave + KW - 1) / KW : 0;  // K steps wave, wave + KW, ...
+
+    // The weights of one step; a tile's registers take the next step's as soon as
+    // they have been decoded, so that RT - 1 tiles are always on their way.
+    u32x4 wf[RT][2];
+    u32x2 ws[RT];
+    u32x4 xf[DX][MT][8];
+    auto load_w = [&](int r, int j) {
+        const int step = wave + KW * min(j, mine - 1);
+        const uint8_t* wp = wbase + step * kBK;
+        wf[r][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][0]));
+        wf[r][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][1]));
+        __builtin_memcpy(&ws[r], wsbase + 8 * step + wsoff[r], 8);
+    };
+    auto load_x = [&](int slot, int j) {
+        const uint16_t* xp = xbase + (wave + KW * min(j, mine - 1)) * kStep;
+#pragma unroll
+        for (int c = 0; c < MT; ++c)
+#pragma unroll
+            for (int b = 0; b < 8; ++b) xf[slot][c][b] = *reinterpret_cast<const u32x4*>(xp + xoff[c] + 32 * b);
+    };
+    auto multiply = [&](int r, const u32x4 (&w)[2], u32x2 sc, const u32x4 (&xv)[MT][8], auto then) {
+        const uint32_t a[4] = {w[0].x, w[0].y, w[0].z, w[0].w}, b[4] = {w[1].x, w[1].y, w[1].z, w[1].w};
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const uint32_t an = swap_pair(a[d]), bn = swap_pair(b[d]);
+            lo[d] = even ? a[d] : bn;
+            hi[d] = even ? an : b[d];
+        }
+        then();
+        transpose4(lo);
+        transpose4(hi);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {  // blocks 2 s and 2 s + 1
+            const uint32_t word = s < 2 ? sc.x : sc.y;
+            const bf16x8 w0 = decode(lo[s], (word >> (16 * (s & 1))) & 255);
+            const bf16x8 w1 = decode(hi[s], (word >> (16 * (s & 1) + 8)) & 255);
+#pragma unroll
+            for (int c = 0; c < MT; ++c)
+                acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w0, __builtin_bit_cast(bf16x8, xv[c][2 * s]), acc[r][c], 0, 0, 0);
+#pragma unroll
+            for (int c = 0; c < MT; ++c)
+                acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w1, __builtin_bit_cast(bf16x8, xv[c][2 * s + 1]), acc[r][c], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (mine > 0) {
+        load_x(0, 0);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) load_w(r, 0);
+        if (DX == 2) load_x(DX - 1, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        auto step = [&](int slot, int j) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const u32x2 sc = ws[r];
+                multiply(r, wf[r], sc, xf[slot], [&] { load_w(r, j + 1); });
+            }
+            load_x(slot, j + DX);
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        int j = 0;
+        for (; j + DX < mine; j += DX) {
+#pragma unroll
+            for (int d = 0; d < DX; ++d) step(d, j + d);
+        }
+#pragma unroll
+        for (int d = 0; d < DX; ++d)
+            if (j + d < mine) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const u32x2 sc = ws[r];
+                    multiply(r, wf[r], sc, xf[d], [&] {
+                        if (j + d + 1 < mine) load_w(r, j + d + 1);
+                    });
+                }
+            }
+    }
+    if (K % kStep != 0 && wave == full % KW) {
+        // The partial last step: zeros past K in both operands.
+        const int valid = K - full * kStep;
+        u32x4 w[RT][2], xv[MT][8];
+        u32x2 sc[RT];
+        const u32x4 z{0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            w[r][0] = w[r][1] = z;
+            if (32 * chunk < valid) {
+                w[r][0] = *reinterpret_cast<const u32x4*>(wbase + full * kBK + woff[r][0]);
+                w[r][1] = *reinterpret_cast<const u32x4*>(wbase + full * kBK + woff[r][1]);
+            }
+            uint32_t d[2] = {0, 0};
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+                if (32 * b < valid) d[b >> 2] |= static_cast<uint32_t>(wsbase[wsoff[r] + 8 * full + b]) << (8 * (b & 3));
+            sc[r] = u32x2{d[0], d[1]};
+        }
+#pragma unroll
+        for (int c = 0; c < MT; ++c)
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                xv[c][b] = z;
+                if (32 * b < valid) xv[c][b] = *reinterpret_cast<const u32x4*>(xbase + full * kStep + xoff[c] + 32 * b);
+            }
+#pragma unroll
+        for (int r = 0; r < RT; ++r) multiply(r, w[r], sc[r], xv, [] {});
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int c = 0; c < MT; ++c) red[wave][r * MT + c][lane] = acc[r][c];
+    __syncthreads();
+    for (int t = wave; t < RT * MT; t += KW) {
+        f32x4 v = red[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < KW; ++w) {
+            const f32x4 o = red[w][t][lane];
+            v = f32x4{v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w};
+        }
+        // D: lane (i, g) holds operand rows 4 g + v of W, outputs n = 2 g, 2 g + 8,
+        // 2 g + 1, 2 g + 9 (v = 0 .. 3), of token i
+        const int m = m0 + 16 * (t % MT) + i;
+        if (m >= M) continue;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int n = n0 + 16 * (t / MT) + 2 * kb + 8 * h;
+            if (n >= N) break;
+            const float v0 = h ? v.y : v.x, v1 = h ? v.w : v.z;
+            uint16_t* o = y + static_cast<int64_t>(m) * N + n;
+            if (vec) {
+                *reinterpret_cast<uint32_t*>(o) = kc::pack_bf16x2(v0, v1);
+            } else {
+                o[0] = kc::f32_to_bf16(v0);
+                if (n + 1 < N) o[1] = kc::f32_to_bf16(v1);
+            }
+        }
+    }
+}
+
+template <int MT, int RT, int KW, int DX>
+int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t* x, uint16_t* y, int M, int N, int K,
+           hipStream_t stream) {
+    const dim3 grid((N + 16 * RT - 1) / (16 * RT), (M + 16 * MT - 1) / (16 * MT));
+    gemm_mxfp4_a16_kernel<MT, RT, KW, DX><<<grid, KW * 64, 0, stream>>>(qw, sw, x, y, M, N, K,
+                                                                       N % 2 == 0 && kc::aligned(y, 4));
+    return kc::check_launch(fn);
+}
+
+// Row tiles per workgroup: the fewest that leave at most one workgroup per CU,
+// since every workgroup reads all of its tokens' X; seven at most.
+template <int MT>
+int skinny(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t* x, uint16_t* y, int M, int N, int K,
+           hipStream_t stream) {
+    constexpr int kCus = 256;
+    const int64_t wgs = int64_t{(N + 15) / 16} * ((M + 16 * MT - 1) / (16 * MT));
+    if (wgs <= kCus) return launch<MT, 1, MT == 1 ? 8 : 4, 1>(fn, qw, sw, x, y, M, N, K, stream);
+    if (wgs <= 2 * kCus) return launch<MT, 2, 8, 1>(fn, qw, sw, x, y, M, N, K, stream);
+    if (wgs <= 4 * kCus) return launch<MT, 4, 4, MT == 2 ? 2 : 1>(fn, qw, sw, x, y, M, N, K, stream);
+    return launch<MT, 7, 4, MT == 2 ? 2 : 1>(fn, qw, sw, x, y, M, N, K, stream);
 }
 
 }  // namespace
@@ -53,8 +269,8 @@ extern "C" int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw, cons
     if (!d_qw || !d_sw || !d_x) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
     if (!kc::aligned(d_qw, 16) || !kc::aligned(d_x, 16))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the codes and x must be 16-byte aligned", fn);
-    const int64_t tn = (N + 15) / 16, tiles = tn * ((M + 15) / 16);
-    gemm_mxfp4_a16_kernel<<<static_cast<unsigned>((tiles + 3) / 4), kThreads, 0, stream>>>(d_qw, d_sw, d_x, d_y, M, N, K,
-                                                                                          tn, tiles);
-    return kc::check_launch(fn);
+    const int m = static_cast<int>(M), n = static_cast<int>(N), k = static_cast<int>(K);
+    if (m <= 16) return skinny<1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+    if (m <= 32) return skinny<2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+    return skinny<4>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
 }
