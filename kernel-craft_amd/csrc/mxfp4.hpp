@@ -63,13 +63,24 @@ __device__ __forceinline__ uint32_t absmax_bits_f32(f32x4 a, f32x4 b) {
     return max(m0, m1);
 }
 
-// Largest of v over the lanes that differ in bits 0 (and 1) of their number.
+// The same of 4 fp32 values as words.
+__device__ __forceinline__ uint32_t absmax_bits_f32(u32x4 v) {
+    constexpr uint32_t m = 0x7FFFFFFFu;
+    return max(max(v.x & m, v.y & m), max(v.z & m, v.w & m));
+}
+
+// Largest of v over the lanes that differ in bits 0 (to 1, to 2) of their number.
 __device__ __forceinline__ uint32_t max_pair(uint32_t v) {
     return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true)));
 }
 __device__ __forceinline__ uint32_t max_quad(uint32_t v) {
     v = max_pair(v);
     return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true)));
+}
+
+__device__ __forceinline__ uint32_t max_oct(uint32_t v) {
+    v = max_quad(v);  // four lanes agree: the mirror of 8 lanes is lane ^ 4
+    return max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 0xF, 0xF, true)));
 }
 
 // 8 values -> 8 codes (value i in nibble i) at scale byte b != 255.
@@ -92,6 +103,15 @@ __device__ __forceinline__ uint32_t encode8_f32(f32x4 a, f32x4 b, uint32_t sb) {
     return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, b.z, b.w, s, 3);
 }
 
+// 4 fp32 values as words -> 4 codes in 16 bits.
+__device__ __forceinline__ uint32_t encode4_f32(u32x4 v, uint32_t sb) {
+    const float s = scale_operand(sb);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(w[0]), __uint_as_float(w[1]), s, 0);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, __uint_as_float(w[2]), __uint_as_float(w[3]), s, 1);
+}
+
 // 8 codes -> 8 fp32 values times s: the conversion gives the E2M1 value, the
 // multiplication is exact but where it leaves fp32's range.
 __device__ __forceinline__ void decode8_f32(uint32_t c, float s, f32x4& a, f32x4& b) {
@@ -103,7 +123,14 @@ __device__ __forceinline__ void decode8_f32(uint32_t c, float s, f32x4& a, f32x4
     b = f32x4{r.x * s, r.y * s, t.x * s, t.y * s};
 }
 
-// The same as packed bf16 (every E2M1 value times a power of two is a bf16
+// The same of 4 codes in the low 16 bits.
+__device__ __forceinline__ f32x4 decode4_f32(uint32_t c, float s) {
+    const f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0);
+    const f32x2 q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+    return f32x4{p.x * s, p.y * s, q.x * s, q.y * s};
+}
+
+// 8 codes as packed bf16 (every E2M1 value times a power of two is a bf16
 // value, but where it leaves the range).
 __device__ __forceinline__ u32x4 decode8_bf16(uint32_t c, float s) {
     f32x4 a, b;
