@@ -5,9 +5,9 @@
 //
 // Bound by memory: 1 (FP8) or 0.53 (MXFP4) bytes in and 2 or 4 out per value.
 // A workgroup takes a tile of tokens: its first threads find one token's slot
-// each (a binary search of cu_seqlens, all searches of the tile at once instead
-// of one before every row), then all threads walk the tile's rows in units of
-// 8 values.
+// each (a binary search of cu_seqlens, in LDS up to 1023 sequences, all searches of
+// the tile at once instead of one before every row), then all threads walk the tile's rows in units of
+// 8 values, four rows in flight each.
 #include <algorithm>
 #include <type_traits>
 
@@ -35,17 +35,19 @@ struct Args {
 
 constexpr int64_t kBad = -1, kOutside = -2;
 
-// Slot of token t; kBad where its page is missing, kOutside where it belongs to
+constexpr int kStarts = 1024;  // starts of sequences held in LDS
+
+// Slot of token t, the starts of the sequences at cu; kBad where its page is missing, kOutside where it belongs to
 // no sequence.
-__device__ __forceinline__ int64_t slot_of(const Args& p, int64_t t) {
-    if (t >= p.total || t < p.cu[0] || t >= p.cu[p.seqs]) return kOutside;
+__device__ __forceinline__ int64_t slot_of(const Args& p, const int32_t* cu, int64_t t) {
+    if (t >= p.total || t < cu[0] || t >= cu[p.seqs]) return kOutside;
     int lo = 0, hi = p.seqs - 1;  // first b with cu[b + 1] > t
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (p.cu[mid + 1] > t) hi = mid;
+        if (cu[mid + 1] > t) hi = mid;
         else lo = mid + 1;
     }
-    const int64_t pos = t - p.cu[lo];
+    const int64_t pos = t - cu[lo];
     if (pos < 0) return kBad;  // cu_seqlens that do not ascend
     const int64_t page_at = pos / p.page_size;
     if (page_at >= p.max_pages) return kBad;
@@ -59,70 +61,79 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const Args p) {
     __shared__ int64_t slot[kMaxTile];
     const int which = blockIdx.y, tid = threadIdx.x;
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
-    if (tid < p.tile) slot[tid] = slot_of(p, t0 + tid);
+    if (p.seqs < kStarts) {
+        __shared__ int32_t starts[kStarts];
+        for (int i = tid; i <= p.seqs; i += kThreads) starts[i] = p.cu[i];
+        __syncthreads();
+        if (tid < p.tile) slot[tid] = slot_of(p, starts, t0 + tid);
+    } else if (tid < p.tile) {
+        slot[tid] = slot_of(p, p.cu, t0 + tid);
+    }
     __syncthreads();
     const uint8_t* codes = p.codes[which];
     Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out[which]);
     constexpr int W = VEC ? 8 : 1;                 // values per unit
+    constexpr int kAhead = 4;                      // rows in flight per thread
     const int units = p.kv_heads * p.D / W, per_head = p.D / W;
-    const int step_t = kThreads / units, step_u = kThreads - step_t * units;
-    int tt = tid / units, u = tid - tt * units;
+    // A thread keeps its unit of the row and walks the tile's tokens: the head and
+    // the place in it cost two divisions a thread.
+    const int together = max(1, kThreads / units);  // tokens side by side
+    const int first = tid / units;
+    if (units <= kThreads && first >= together) return;
     const float nan = __uint_as_float(0x7FC00000u);
-    while (tt < p.tile) {
-        const int64_t s = slot[tt];
-        if (s != kOutside) {
-            const int h = u / per_head, d = (u - h * per_head) * W;
-            const int64_t row = s * p.kv_heads + h;          // kBad reads nothing
-            const int64_t to = ((t0 + tt) * p.kv_heads + h) * p.D + d;
-            if constexpr (VEC) {
-                f32x4 lo = {nan, nan, nan, nan}, hi = lo;
-                if (s != kBad) {
-                    if constexpr (FP8) {
-                        const u32x2 c = *reinterpret_cast<const u32x2*>(codes + row * p.D + d);
-                        const float sc = static_cast<const float*>(p.scales[which])[row];
-                        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.x), false);
-                        const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.x), true);
-                        const auto e = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.y), false);
-                        const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c.y), true);
-                        lo = f32x4{a[0] * sc, a[1] * sc, b[0] * sc, b[1] * sc};
-                        hi = f32x4{e[0] * sc, e[1] * sc, f[0] * sc, f[1] * sc};
-                    } else {
-                        const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + (row * p.D + d) / 2);
-                        const uint8_t sb = static_cast<const uint8_t*>(p.scales[which])[(row * p.D + d) / kBlock];
-                        decode8_f32(c, scale_value(sb), lo, hi);
-                    }
+    for (int u = units <= kThreads ? tid - first * units : tid; u < units; u += kThreads) {
+        const int h = u / per_head, d = (u - h * per_head) * W;
+        for (int tt = units <= kThreads ? first : 0; tt < p.tile; tt += kAhead * together) {
+            int64_t s[kAhead];
+            u32x2 c[kAhead];
+            float sc[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                const int at = tt + i * together;
+                s[i] = at < p.tile ? slot[at] : kOutside;
+                c[i] = u32x2{0u, 0u};
+                sc[i] = nan;
+                if (s[i] < 0) continue;
+                const int64_t row = s[i] * p.kv_heads + h;
+                const int64_t v = row * p.D + d;
+                if constexpr (FP8) {
+                    if constexpr (VEC) c[i] = *reinterpret_cast<const u32x2*>(codes + v);
+                    else c[i].x = codes[v];
+                    sc[i] = static_cast<const float*>(p.scales[which])[row];
+                } else {
+                    if constexpr (VEC) c[i].x = *reinterpret_cast<const uint32_t*>(codes + v / 2);
+                    else c[i].x = codes[v / 2] >> (4 * (d & 1));
+                    sc[i] = scale_value(static_cast<const uint8_t*>(p.scales[which])[v / kBlock]);
                 }
-                if constexpr (BF16) {
-                    *reinterpret_cast<u32x4*>(out + to) =
-                        u32x4{kc::pack_bf16x2(lo.x, lo.y), kc::pack_bf16x2(lo.z, lo.w), kc::pack_bf16x2(hi.x, hi.y),
-                              kc::pack_bf16x2(hi.z, hi.w)};
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (s[i] == kOutside) continue;
+                const int64_t to = ((t0 + tt + i * together) * p.kv_heads + h) * p.D + d;
+                f32x4 lo, hi;
+                if constexpr (FP8) {
+                    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].x), false);
+                    const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].x), true);
+                    const auto e = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].y), false);
+                    const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].y), true);
+                    lo = f32x4{a[0] * sc[i], a[1] * sc[i], b[0] * sc[i], b[1] * sc[i]};
+                    hi = f32x4{e[0] * sc[i], e[1] * sc[i], f[0] * sc[i], f[1] * sc[i]};
+                } else {
+                    decode8_f32(c[i].x, sc[i], lo, hi);
+                }
+                if constexpr (!VEC) {
+                    if constexpr (BF16) out[to] = kc::f32_to_bf16(lo.x);
+                    else out[to] = lo.x;
+                } else if constexpr (BF16) {
+                    __builtin_nontemporal_store(u32x4{kc::pack_bf16x2(lo.x, lo.y), kc::pack_bf16x2(lo.z, lo.w),
+                                                      kc::pack_bf16x2(hi.x, hi.y), kc::pack_bf16x2(hi.z, hi.w)},
+                                                reinterpret_cast<u32x4*>(out + to));
                 } else {
                     f32x4* o = reinterpret_cast<f32x4*>(out + to);
                     o[0] = lo;
                     o[1] = hi;
                 }
-            } else {
-                float v = nan;
-                if (s != kBad) {
-                    if constexpr (FP8) {
-                        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes[row * p.D + d]), false);
-                        v = a[0] * static_cast<const float*>(p.scales[which])[row];
-                    } else {
-                        const uint32_t c = codes[(row * p.D + d) / 2];
-                        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0);
-                        v = (d & 1 ? a.y : a.x) *
-                            scale_value(static_cast<const uint8_t*>(p.scales[which])[(row * p.D + d) / kBlock]);
-                    }
-                }
-                if constexpr (BF16) out[to] = kc::f32_to_bf16(v);
-                else out[to] = v;
             }
-        }
-        tt += step_t;
-        u += step_u;
-        if (u >= units) {
-            u -= units;
-            ++tt;
         }
     }
 }
@@ -157,7 +168,10 @@ int cache_read(const char* fn, const kc_kv_cache* cache, const int32_t* table, i
     const uintptr_t in = fp8 ? 8 : 4;
     const bool vec = p.D % 8 == 0 && kc::aligned(k, 16) && kc::aligned(v, 16) && kc::aligned(p.codes[0], in) &&
                      kc::aligned(p.codes[1], in);
-    p.tile = static_cast<int>(std::clamp<int64_t>(total / 1024, 4, kMaxTile));
+    // the largest tile that still leaves 4096 of them for each of the two (larger
+    // ones end unevenly: 43 000 tokens 60.8 us at 32, 54 at 8)
+    p.tile = 8;
+    while (p.tile < kMaxTile && total / (2 * p.tile) >= 4096) p.tile *= 2;
     const int64_t grid = (total + p.tile - 1) / p.tile;
     if (grid > kc::kv::kMaxGrid / 2) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
     const dim3 g(static_cast<unsigned>(grid), 2);

@@ -17,16 +17,21 @@
 //
 // Everything here is bound by memory: a head goes in once and out once.
 //
-// Vector kernel.  A slot is 8 values (16 bytes of bf16).  Lane j of the
-// lanes that share a head takes two slots: those of its rotation pairs, j and
-// j + R/16 (interleaved and past R: 2j and 2j + 1), so that both partners of
-// every pair are in one lane and no value crosses lanes but in the sum of
-// squares.  D = 128 needs 8 lanes: a wave holds 8 heads of one token at a time
-// and keeps the token's 8 cos and sin per lane in registers over its heads.
+// Vector kernel.  A slot is W neighbouring values, 16 bytes where R allows (8 bf16,
+// 4 fp32), else 4 bf16.  Lane j of the lanes that share a head takes two slots:
+// those of its rotation pairs, j and j + R / 2W, so that both partners of every pair
+// are in one lane and no value crosses lanes but in the sum of squares.  Where no
+// pair asks for it (interleaved heads, values past R, cached values) the lanes of a
+// head read two runs of neighbouring slots (fp32, interleaved, 16384 tokens of 40
+// heads 192 -> 129 us against slots 2j and 2j + 1), or 2j and 2j + 1 where they store
+// both as one and for heads that are no multiple of 64 values, whose blocks of 32
+// then stay in neighbouring lanes.  bf16 D = 128 needs 8 lanes: a wave holds 8 heads of one token
+// at a time, loads the next 8 while it works on them, and keeps the token's 8 cos and
+// sin and the gammas of its two slots in registers over its heads.
 //
 // The sum of squares runs over the lane's first slot, then its second, one FMA
-// a value, then over the lanes (xor butterfly).  The general kernel (any D up to
-// 1024, strides and alignment; one wave per head, the row in LDS) adds in the
+// a value, then over the lanes (lane ^ 1, ^ 2, ^ 4, ...).  The general kernel (any D up
+// to 1024, strides and alignment; one wave per head, the row in LDS) adds in the
 // same order where the slots exist, so both give the same bits.
 #include <algorithm>
 #include <type_traits>
@@ -61,46 +66,66 @@ struct Args {
     int q_heads, kv_heads, D, R;
     float eps;
     bool interleaved;
+    int width;                        // values of a slot, 0: no slots
+    bool runs;                        // two runs of slots a head, not pairs
     int lanes_log2;                   // lanes of a head
     int groups, splits, per_split;    // waves of a token and the head groups of each
 };
 
-// 8 values of a row, as fp32.
-template <bool BF16>
-__device__ __forceinline__ void load8(const void* base, int64_t at, float (&v)[8]) {
-    if constexpr (BF16) {
-        const u32x4 d = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + at);
-        const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+// A slot as it lies in memory, and as fp32 values.
+template <bool BF16, int W>
+struct Slot {
+    static constexpr int kWords = W * (BF16 ? 2 : 4) / 4;
+    typedef uint32_t Vec __attribute__((ext_vector_type(kWords)));
+    Vec raw;
+    __device__ __forceinline__ void load(const void* base, int64_t at) {
+        raw = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(static_cast<const Elem<BF16>*>(base) + at));
+    }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        }
-    } else {
-        const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + at);
-        const f32x4 a = p[0], b = p[1];
+        for (int i = 0; i < kWords; ++i) raw[i] = 0;
+    }
+    __device__ __forceinline__ void get(float (&v)[W]) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
+        for (int i = 0; i < kWords; ++i) {
+            const uint32_t w = raw[i];
+            if constexpr (BF16) {
+                v[2 * i] = __uint_as_float(w << 16);
+                v[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+            } else {
+                v[i] = __uint_as_float(w);
+            }
         }
     }
+    __device__ __forceinline__ void set(const float (&v)[W]) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (BF16) raw[i] = kc::pack_bf16x2(v[2 * i], v[2 * i + 1]);
+            else raw[i] = __float_as_uint(v[i]);
+        }
+    }
+    __device__ __forceinline__ void store(void* base, int64_t at) const {
+        __builtin_nontemporal_store(raw, reinterpret_cast<Vec*>(static_cast<Elem<BF16>*>(base) + at));
+    }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float(static_cast<uint32_t>(
+        __builtin_amdgcn_mov_dpp(static_cast<int>(__float_as_uint(v)), CTRL, 0xF, 0xF, true)));
 }
 
-template <bool BF16>
-__device__ __forceinline__ void store8(void* base, int64_t at, const float (&v)[8]) {
-    if constexpr (BF16) {
-        u32x4 d;
-        d.x = kc::pack_bf16x2(v[0], v[1]);
-        d.y = kc::pack_bf16x2(v[2], v[3]);
-        d.z = kc::pack_bf16x2(v[4], v[5]);
-        d.w = kc::pack_bf16x2(v[6], v[7]);
-        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(base) + at) = d;
-    } else {
-        f32x4* p = reinterpret_cast<f32x4*>(static_cast<float*>(base) + at);
-        p[0] = f32x4{v[0], v[1], v[2], v[3]};
-        p[1] = f32x4{v[4], v[5], v[6], v[7]};
-    }
+// op over the 2^lg lanes of a head, lane ^ 1 first (once 4 (8) lanes agree, the
+// mirror of 8 (16) lanes is lane ^ 4 (^ 8)).
+template <typename Op>
+__device__ __forceinline__ float over_head(float v, int lg, Op op) {
+    if (lg >= 1) v = op(v, dpp<0xB1>(v));
+    if (lg >= 2) v = op(v, dpp<0x4E>(v));
+    if (lg >= 3) v = op(v, dpp<0x141>(v));
+    if (lg >= 4) v = op(v, dpp<0x140>(v));
+    if (lg >= 5) v = op(v, __shfl_xor(v, 16, kWave));
+    if (lg >= 6) v = op(v, __shfl_xor(v, 32, kWave));
+    return v;
 }
 
 template <bool BF16>
@@ -144,145 +169,254 @@ __device__ __forceinline__ Token token_of(const Args& p, int64_t t) {
     return k;
 }
 
-// 8 values -> 8 E4M3 codes.
-template <bool FAST>
-__device__ __forceinline__ u32x2 fp8_codes(const float (&v)[8], const RowDiv& d) {
+// W values -> W E4M3 codes.
+template <int W>
+__device__ __forceinline__ void store_fp8(uint8_t* dst, const float (&v)[W], const RowDiv& d) {
     using kc::fp8::e4m3x4_div;
-    return u32x2{e4m3x4_div<FAST>(kc::fp8::f32x4{v[0], v[1], v[2], v[3]}, d),
-                 e4m3x4_div<FAST>(kc::fp8::f32x4{v[4], v[5], v[6], v[7]}, d)};
+    uint32_t c[W / 4];
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+        const kc::fp8::f32x4 q{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        c[i] = d.fast ? e4m3x4_div<true>(q, d) : e4m3x4_div<false>(q, d);
+    }
+    if constexpr (W == 16) *reinterpret_cast<u32x4*>(dst) = u32x4{c[0], c[1], c[2], c[3]};
+    else if constexpr (W == 8) *reinterpret_cast<u32x2*>(dst) = u32x2{c[0], c[1]};
+    else *reinterpret_cast<uint32_t*>(dst) = c[0];
 }
 
-__device__ __forceinline__ uint32_t absmax_bits8(const float (&v)[8]) {
-    return absmax_bits_f32(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]});
+template <int W>
+__device__ __forceinline__ uint32_t absmax_bits(const float (&v)[W]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return m;
 }
 
-__device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t b) {
-    return b == kNaN ? 0u : encode8_f32(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]}, b);
+template <int W>
+__device__ __forceinline__ void store_mx(uint8_t* dst, const float (&v)[W], uint32_t b) {
+    if constexpr (W == 8) {
+        *reinterpret_cast<uint32_t*>(dst) =
+            b == kNaN ? 0u : encode8_f32(f32x4{v[0], v[1], v[2], v[3]}, f32x4{v[4], v[5], v[6], v[7]}, b);
+    } else {
+        const uint32_t c = encode4_f32(u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                                             __float_as_uint(v[3])}, b);
+        *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(b == kNaN ? 0u : c);
+    }
 }
 
-template <bool BF16, bool NORM, int SINK>
+// The two slots of lane j of `lanes`: `apart`, the head's pairs are half a rotation
+// apart (`half` slots).
+struct Slots {
+    int a, b;
+};
+__device__ __forceinline__ Slots slots_of(int j, int lanes, int half, bool apart, bool runs) {
+    if (apart && j < half) return {j, j + half};
+    if (!runs) return {2 * j, 2 * j + 1};
+    return {apart ? j + half : j, j + lanes};  // past a rotation that takes slots 0 .. 2 half - 1, or none
+}
+
+// What lane j has of head group g.
+struct Place {
+    bool live, is_q, is_v, apart;
+    int hh;
+    Slots s;
+};
+
+template <bool BF16, int W, bool NORM, int SINK>
 __global__ __launch_bounds__(kThreads) void heads_kernel(const Args p) {
+    using S = Slot<BF16, W>;
     const int lane = threadIdx.x & (kWave - 1);
-    const int64_t w = static_cast<int64_t>(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t t = w / p.splits;
     if (t >= p.tokens) return;
     const int part = static_cast<int>(w - t * p.splits);
-    const int D = p.D, half = p.R >> 4;  // slots of half a rotation
+    const int D = p.D, half = p.R / (2 * W);  // slots of half a rotation
     const int lg = p.lanes_log2, hp = kWave >> lg, j = lane & ((1 << lg) - 1);
     const Token tok = token_of<NORM, SINK>(p, t);
     const int n_q = NORM ? p.q_heads : 0, n_all = n_q + p.kv_heads + (SINK != kPlain ? p.kv_heads : 0);
-    const bool has = j < (D >> 4);
+    const int lanes = D / (2 * W);
+    const bool has = j < lanes, pairs_apart = NORM && !p.interleaved;
 
-    float c[8] = {}, s[8] = {};
+    auto place = [&](int g) {
+        Place o;
+        const int h = g * hp + (lane >> lg);
+        o.live = has && h < n_all;
+        o.is_q = h < n_q;
+        o.is_v = SINK != kPlain && h >= n_q + p.kv_heads;
+        o.hh = o.is_q ? h : o.is_v ? h - n_q - p.kv_heads : h - n_q;
+        o.apart = pairs_apart && !o.is_v;
+        o.s = slots_of(j, lanes, half, o.apart, p.runs);
+        return o;
+    };
+    auto fetch = [&](int g, S& a, S& b) {
+        const Place o = place(g);
+        a.clear();
+        b.clear();
+        if (o.live) {
+            const void* src = o.is_q ? p.q : o.is_v ? p.v : p.k;
+            const int64_t at = t * (o.is_q ? p.q_stride : o.is_v ? p.v_stride : p.k_stride) + static_cast<int64_t>(o.hh) * D;
+            a.load(src, at + W * o.s.a);
+            b.load(src, at + W * o.s.b);
+        }
+    };
+    S na, nb;  // the next group's slots
+    const int g0 = part * p.per_split, g_end = min(p.groups, g0 + p.per_split);
+    if (g0 < g_end) fetch(g0, na, nb);
+
+    float c[W] = {}, s[W] = {};
+    S qa, qb, ka, kb;  // gammas of a query's and a key's slots
     if constexpr (NORM) {
-        if (has && j < half && tok.in_table) {
-            load8<false>(p.cos_t, tok.row * (p.R >> 1) + 8 * j, c);
-            load8<false>(p.sin_t, tok.row * (p.R >> 1) + 8 * j, s);
+        // angles: W of the lane's pairs, or W / 2 of each slot's
+        const int turned = p.R / W;
+        const Slots qs = slots_of(j, lanes, half, pairs_apart, p.runs);
+        if (has && tok.in_table) {
+            const float *ct = p.cos_t + tok.row * (p.R >> 1), *st = p.sin_t + tok.row * (p.R >> 1);
+            auto angles = [&](int to, int from, auto n) {
+                constexpr int kN = decltype(n)::value;
+                typedef float Vec __attribute__((ext_vector_type(kN)));
+                const Vec cv = *reinterpret_cast<const Vec*>(ct + from), sv = *reinterpret_cast<const Vec*>(st + from);
+#pragma unroll
+                for (int e = 0; e < kN; ++e) {
+                    c[to + e] = cv[e];
+                    s[to + e] = sv[e];
+                }
+            };
+            if (pairs_apart) {
+                if (j < half) {
+                    angles(0, W * j, std::integral_constant<int, 4>{});
+                    if constexpr (W == 8) angles(4, W * j + 4, std::integral_constant<int, 4>{});
+                }
+            } else {
+                if (qs.a < turned) angles(0, W / 2 * qs.a, std::integral_constant<int, W / 2>{});
+                if (qs.b < turned) angles(W / 2, W / 2 * qs.b, std::integral_constant<int, W / 2>{});
+            }
+        }
+        qa.clear(), qb.clear(), ka.clear(), kb.clear();
+        if (has) {
+            if (p.q_heads > 0) {
+                qa.load(p.q_gamma, W * qs.a);
+                qb.load(p.q_gamma, W * qs.b);
+            }
+            if (p.kv_heads > 0) {
+                ka.load(p.k_gamma, W * qs.a);
+                kb.load(p.k_gamma, W * qs.b);
+            }
         }
     }
-    const int g_end = min(p.groups, (part + 1) * p.per_split);
-    for (int g = part * p.per_split; g < g_end; ++g) {
-        const int h = g * hp + (lane >> lg);
-        const bool live = has && h < n_all;
-        const bool is_q = h < n_q, is_v = SINK != kPlain && h >= n_q + p.kv_heads;
-        const int hh = is_q ? h : is_v ? h - n_q - p.kv_heads : h - n_q;
-        const bool turns = NORM && !is_v && j < half;
-        const bool apart = turns && !p.interleaved;  // slots j and j + half
-        const int sa = apart ? j : 2 * j, sb = apart ? j + half : 2 * j + 1;
-        const void* src = is_q ? p.q : is_v ? p.v : p.k;
-        const int64_t at = t * (is_q ? p.q_stride : is_v ? p.v_stride : p.k_stride) + static_cast<int64_t>(hh) * D;
-        float a[8], b[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.0f;
-        if (live) {
-            load8<BF16>(src, at + 8 * sa, a);
-            load8<BF16>(src, at + 8 * sb, b);
-        }
+    for (int g = g0; g < g_end; ++g) {
+        const S ra = na, rb = nb;
+        if (g + 1 < g_end) fetch(g + 1, na, nb);
+        const Place o = place(g);
+        float a[W], b[W];
+        ra.get(a);
+        rb.get(b);
         if constexpr (NORM) {
             float ss = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], ss);
+            for (int i = 0; i < W; ++i) ss = fmaf(a[i], a[i], ss);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(b[i], b[i], ss);
-            for (int off = (1 << lg) >> 1; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, kWave);
+            for (int i = 0; i < W; ++i) ss = fmaf(b[i], b[i], ss);
+            ss = over_head(ss, lg, [](float u, float v) { return u + v; });
             const float inv = rms_inverse(ss, D, p.eps);
-            if (live && !is_v) {
-                float ga[8], gb[8];
-                load8<BF16>(is_q ? p.q_gamma : p.k_gamma, 8 * sa, ga);
-                load8<BF16>(is_q ? p.q_gamma : p.k_gamma, 8 * sb, gb);
+            if (!o.is_v) {
+                float ga[W], gb[W];
+                S xa = ka, xb = kb;
+                if (o.is_q) xa = qa, xb = qb;
+                xa.get(ga);
+                xb.get(gb);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < W; ++i) {
                     a[i] = (ga[i] * a[i]) * inv;
                     b[i] = (gb[i] * b[i]) * inv;
                 }
-                if (turns) {
-                    if (apart) {
+                if (pairs_apart) {
+                    if (j < half) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) rotate(a[i], b[i], c[i], s[i]);
-                    } else {
+                        for (int i = 0; i < W; ++i) rotate(a[i], b[i], c[i], s[i]);
+                    }
+                } else {
+                    if (o.s.a < p.R / W) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            rotate(a[2 * i], a[2 * i + 1], c[i], s[i]);
-                            rotate(b[2 * i], b[2 * i + 1], c[4 + i], s[4 + i]);
-                        }
+                        for (int i = 0; i < W / 2; ++i) rotate(a[2 * i], a[2 * i + 1], c[i], s[i]);
+                    }
+                    if (o.s.b < p.R / W) {
+#pragma unroll
+                        for (int i = 0; i < W / 2; ++i) rotate(b[2 * i], b[2 * i + 1], c[W / 2 + i], s[W / 2 + i]);
                     }
                 }
                 if (!tok.in_table) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) a[i] = b[i] = tok.fill;
+                    for (int i = 0; i < W; ++i) a[i] = b[i] = tok.fill;
                 }
             }
         }
-        if (live && (is_q || SINK == kPlain)) {
-            void* out = is_q ? p.q_out : p.k_out;
-            const int64_t o = (t * (is_q ? p.q_heads : p.kv_heads) + hh) * D;
-            store8<BF16>(out, o + 8 * sa, a);
-            store8<BF16>(out, o + 8 * sb, b);
+        if (SINK == kPlain || (NORM && o.is_q)) {
+            if (o.live) {
+                S out;
+                void* base = o.is_q ? p.q_out : p.k_out;
+                const int64_t to = (t * (o.is_q ? p.q_heads : p.kv_heads) + o.hh) * D;
+                out.set(a);
+                out.store(base, to + W * o.s.a);
+                out.set(b);
+                out.store(base, to + W * o.s.b);
+            }
         }
         if constexpr (SINK == kPlain) continue;
+        if (NORM && (g + 1) * hp <= n_q) continue;  // queries only
         // keys as they would be stored; a value is of the type already
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            a[i] = kc::fp8::quiet(rounded<BF16>(a[i]));
-            b[i] = kc::fp8::quiet(rounded<BF16>(b[i]));
+        if constexpr (NORM && BF16) {
+            S v;
+            v.set(a);
+            v.get(a);
+            v.set(b);
+            v.get(b);
         }
-        const bool out = live && !is_q && tok.cached;
-        const int64_t row = tok.slot * p.kv_heads + hh;
-        uint8_t* codes = is_v ? p.v_codes : p.k_codes;
-        void* scales = is_v ? p.v_scales : p.k_scales;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            a[i] = kc::fp8::quiet(a[i]);
+            b[i] = kc::fp8::quiet(b[i]);
+        }
+        const bool out = o.live && !o.is_q && tok.cached;
+        const int64_t row = tok.slot * p.kv_heads + o.hh;
+        uint8_t* codes = o.is_v ? p.v_codes : p.k_codes;
+        void* scales = o.is_v ? p.v_scales : p.k_scales;
         if constexpr (SINK == kFp8) {
             float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(b[i])));
-            for (int off = (1 << lg) >> 1; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
+            for (int i = 0; i < W; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(b[i])));
+            m = over_head(m, lg, [](float u, float v) { return fmaxf(u, v); });
             if (out) {
                 const RowDiv d = kc::fp8::row_div(m);
-                u32x2 ca, cb;
-                if (d.fast) {
-                    ca = fp8_codes<true>(a, d);
-                    cb = fp8_codes<true>(b, d);
-                } else {
-                    ca = fp8_codes<false>(a, d);
-                    cb = fp8_codes<false>(b, d);
+                if constexpr (NORM) {
+                    store_fp8<W>(codes + row * D + W * o.s.a, a, d);
+                    store_fp8<W>(codes + row * D + W * o.s.b, b, d);
+                } else {  // neighbouring slots
+                    float v[2 * W];
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        v[i] = a[i];
+                        v[W + i] = b[i];
+                    }
+                    store_fp8<2 * W>(codes + row * D + W * o.s.a, v, d);
                 }
-                u32x2* dst = reinterpret_cast<u32x2*>(codes + row * D);
-                dst[sa] = ca;
-                dst[sb] = cb;
                 if (j == 0) static_cast<float*>(scales)[row] = d.s;
             }
         } else {
-            // A block is four slots: four lanes' first (second) slots where
-            // they lie apart, two lanes' slot pairs elsewhere.
-            const uint32_t ma = absmax_bits8(a), mb = absmax_bits8(b);
-            const uint32_t qa = max_quad(ma), qb = max_quad(mb), pr = max_pair(max(ma, mb));
-            const uint32_t ba = scale_byte(apart ? qa : pr), bb = scale_byte(apart ? qb : pr);
+            // A block is 32 / W slots: of so many lanes' first (second) slots in a run,
+            // of half as many lanes' slot pairs.
+            const bool run = p.runs || (o.apart && j < half);
+            const uint32_t ma = absmax_bits<W>(a), mb = absmax_bits<W>(b), mab = max(ma, mb);
+            const uint32_t ra2 = W == 8 ? max_quad(ma) : max_oct(ma), rb2 = W == 8 ? max_quad(mb) : max_oct(mb);
+            const uint32_t pr = W == 8 ? max_pair(mab) : max_quad(mab);
+            const uint32_t ba = scale_byte(run ? ra2 : pr), bb = scale_byte(run ? rb2 : pr);
             if (out) {
-                uint32_t* dst = reinterpret_cast<uint32_t*>(codes + row * (D / 2));
-                dst[sa] = mx_codes(a, ba);
-                dst[sb] = mx_codes(b, bb);
+                uint8_t* dst = codes + row * (D / 2);
+                store_mx<W>(dst + W / 2 * o.s.a, a, ba);
+                store_mx<W>(dst + W / 2 * o.s.b, b, bb);
+                constexpr int kSlots = kBlock / W;
                 uint8_t* sc = static_cast<uint8_t*>(scales) + row * (D / kBlock);
-                if ((sa & 3) == 0) sc[sa >> 2] = static_cast<uint8_t>(ba);
-                if (apart && (sb & 3) == 0) sc[sb >> 2] = static_cast<uint8_t>(bb);
+                if (o.s.a % kSlots == 0) sc[o.s.a / kSlots] = static_cast<uint8_t>(ba);
+                if (run && o.s.b % kSlots == 0) sc[o.s.b / kSlots] = static_cast<uint8_t>(bb);
             }
         }
     }
@@ -290,7 +424,7 @@ __global__ __launch_bounds__(kThreads) void heads_kernel(const Args p) {
 
 // Any D up to 1024, any alignment: one wave per head, the row in LDS as fp32.
 template <bool BF16, bool NORM, int SINK>
-__global__ __launch_bounds__(kThreads) void heads_general_kernel(const Args p, int64_t rows, bool slotted) {
+__global__ __launch_bounds__(kThreads) void heads_general_kernel(const Args p, int64_t rows) {
     using T = Elem<BF16>;
     __shared__ float lds[kWaves][kc::kv::kMaxHeadDim];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
@@ -313,18 +447,18 @@ __global__ __launch_bounds__(kThreads) void heads_general_kernel(const Args p, i
     __syncthreads();
     if constexpr (NORM) {
         float ss = 0.0f;
-        if (slotted) {  // the vector kernel's order
-            const int half = R >> 4;
-            if (lane < (D >> 4)) {
-                const bool apart = lane < half && !p.interleaved;
-                const int sa = apart ? lane : 2 * lane, sb = apart ? lane + half : 2 * lane + 1;
-                for (int i = 0; i < 8; ++i) ss = fmaf(row[8 * sa + i], row[8 * sa + i], ss);
-                for (int i = 0; i < 8; ++i) ss = fmaf(row[8 * sb + i], row[8 * sb + i], ss);
+        if (p.width > 0) {  // the vector kernel's order
+            const int W = p.width, half = R / (2 * W);
+            if (lane < D / (2 * W)) {
+                const Slots s = slots_of(lane, D / (2 * W), half, !p.interleaved && !is_v, p.runs);
+                for (int i = 0; i < W; ++i) ss = fmaf(row[W * s.a + i], row[W * s.a + i], ss);
+                for (int i = 0; i < W; ++i) ss = fmaf(row[W * s.b + i], row[W * s.b + i], ss);
             }
         } else {
             for (int i = lane; i < D; i += kWave) ss = fmaf(row[i], row[i], ss);
         }
-        const float inv = rms_inverse(kc::wave_sum(ss), D, p.eps);
+        for (int off = 1; off < kWave; off <<= 1) ss += __shfl_xor(ss, off, kWave);
+        const float inv = rms_inverse(ss, D, p.eps);
         __syncthreads();
         if (!is_v) {
             const T* gamma = static_cast<const T*>(is_q ? p.q_gamma : p.k_gamma);
@@ -382,22 +516,28 @@ __global__ __launch_bounds__(kThreads) void heads_general_kernel(const Args p, i
 template <bool BF16, bool NORM, int SINK>
 int launch(const char* fn, Args& p, hipStream_t stream) {
     const int heads = (NORM ? p.q_heads : 0) + p.kv_heads + (SINK != kPlain ? p.kv_heads : 0);
-    const int D = p.D, align_elems = BF16 ? 8 : 4;
-    const bool slotted = D % 16 == 0 && D <= 512 && p.R % 16 == 0;
-    auto rows_ok = [&](const void* ptr, int64_t stride) { return kc::aligned(ptr, 16) && stride % align_elems == 0; };
-    bool vec = slotted && rows_ok(p.k, p.k_stride);
+    const int D = p.D;
+    // 16-byte slots where both halves of the rotation are whole slots, else 4 bf16
+    const int wide = BF16 ? 8 : 4;
+    p.width = D % (2 * wide) == 0 && p.R % (2 * wide) == 0 ? wide : D % 8 == 0 && p.R % 8 == 0 ? 4 : 0;
+    if (p.width > 0 && D / (2 * p.width) > kWave) p.width = 0;
+    p.runs = NORM && D % 64 == 0;  // without a rotation neighbouring slots, stored as one
+    const uintptr_t bytes = p.width * sizeof(Elem<BF16>);
+    auto whole = [&](const void* ptr) { return kc::aligned(ptr, bytes); };
+    auto rows_ok = [&](const void* ptr, int64_t stride) { return whole(ptr) && stride % p.width == 0; };
+    bool vec = p.width > 0 && rows_ok(p.k, p.k_stride);
     if (NORM)
-        vec = vec && rows_ok(p.q, p.q_stride) && kc::aligned(p.q_gamma, 16) && kc::aligned(p.k_gamma, 16) &&
-              kc::aligned(p.cos_t, 16) && kc::aligned(p.sin_t, 16) && kc::aligned(p.q_out, 16);
-    if (SINK == kPlain) vec = vec && kc::aligned(p.k_out, 16);
+        vec = vec && rows_ok(p.q, p.q_stride) && whole(p.q_gamma) && whole(p.k_gamma) && kc::aligned(p.cos_t, 16) &&
+              kc::aligned(p.sin_t, 16) && whole(p.q_out);
+    if (SINK == kPlain) vec = vec && whole(p.k_out);
     else vec = vec && rows_ok(p.v, p.v_stride);
-    if (SINK == kFp8) vec = vec && kc::aligned(p.k_codes, 8) && kc::aligned(p.v_codes, 8);
+    if (SINK == kFp8) vec = vec && kc::aligned(p.k_codes, (NORM ? 1 : 2) * p.width) && kc::aligned(p.v_codes, (NORM ? 1 : 2) * p.width);
     if (SINK == kMx)  // whole blocks in the lanes that share a maximum
         vec = vec && kc::aligned(p.k_codes, 4) && kc::aligned(p.v_codes, 4) &&
               (!NORM || p.interleaved || p.R % 64 == 0);
     if (vec) {
         p.lanes_log2 = 0;
-        while ((1 << p.lanes_log2) * 16 < D) ++p.lanes_log2;
+        while ((1 << p.lanes_log2) * 2 * p.width < D) ++p.lanes_log2;
         const int hp = kWave >> p.lanes_log2;
         p.groups = (heads + hp - 1) / hp;
         // A wave per token once that fills the chip (8 waves on each of 1024
@@ -406,11 +546,14 @@ int launch(const char* fn, Args& p, hipStream_t stream) {
         p.per_split = (p.groups + p.splits - 1) / p.splits;
         const int64_t grid = (p.tokens * p.splits + kWaves - 1) / kWaves;
         if (grid > kc::kv::kMaxGrid) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
-        heads_kernel<BF16, NORM, SINK><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+        if (p.width == wide)
+            heads_kernel<BF16, BF16 ? 8 : 4, NORM, SINK><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
+        else
+            heads_kernel<BF16, 4, NORM, SINK><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p);
     } else {
         const int64_t rows = p.tokens * heads, grid = (rows + kWaves - 1) / kWaves;
         if (grid > kc::kv::kMaxGrid) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
-        heads_general_kernel<BF16, NORM, SINK><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, rows, slotted);
+        heads_general_kernel<BF16, NORM, SINK><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, rows);
     }
     return kc::check_launch(fn);
 }

@@ -61,7 +61,7 @@ SHAPES = [  # T, q heads, kv heads, D, R, interleaved
     (6, 2, 2, 256, 128, False), (2, 4, 1, 512, 512, False), (3, 2, 1, 16, 16, False), (3, 2, 1, 48, 16, True),
     (3, 3, 1, 40, 40, False), (2, 2, 1, 33, 20, True), (2, 1, 1, 1, 0, False), (2, 2, 1, 576, 64, False),
     (3, 2, 1, 1024, 1024, False), (2, 2, 2, 100, 50, True), (300, 7, 1, 64, 64, False), (2100, 4, 1, 128, 128, False),
-    (11, 0, 2, 64, 64, False), (11, 2, 0, 64, 64, True), (5, 40, 8, 128, 0, False),
+    (4, 3, 1, 80, 40, False), (4, 3, 1, 56, 24, True), (11, 0, 2, 64, 64, False), (11, 2, 0, 64, 64, True), (5, 40, 8, 128, 0, False),
 ]
 
 
@@ -204,9 +204,12 @@ def test_write_then_read(gpu, ops, T, H, D, page, fmt, dtype):
 @pytest.mark.parametrize("T,Hq,Hkv,D,R,inter", [(1, 32, 8, 128, 128, False), (5, 7, 1, 64, 64, True),
                                                 (9, 4, 2, 96, 32, False), (9, 4, 2, 96, 64, False),
                                                 (6, 2, 2, 32, 32, False), (40, 16, 4, 256, 128, False),
+                                                (9, 4, 2, 80, 40, False), (5, 4, 2, 224, 40, True),
                                                 (3, 2, 1, 576, 64, False), (2300, 4, 2, 128, 128, False),
                                                 (4, 0, 3, 64, 64, False)])
 def test_fused_equals_the_two_calls(gpu, ops, T, Hq, Hkv, D, R, inter, dtype, fmt):
+    if fmt == "mxfp4" and D % 32:
+        pytest.skip("MXFP4 rows are whole blocks")
     dt = getattr(gpu, dtype)
     q, k, v, qg, kg = _heads(gpu, T, Hq, Hkv, D, dt, seed=T + D)
     cos, sin = _tables(gpu, 64, R // 2)
