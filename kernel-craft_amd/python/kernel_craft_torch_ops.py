@@ -801,36 +801,44 @@ def fp8_quantize_smooth(x, smooth, mode: str = "div") -> Tuple:
 # ---------------------------------------------------------------------------
 
 
-def _one_gpu(op: str, *tensors):
-    """The device that all tensors live on; ValueError unless it is one GPU."""
-    _on_gpu(op, *tensors)
-    device = tensors[0].device
+def _one_gpu(op: str, *tensors) -> int:
+    """The number of the GPU that all tensors live on; ValueError unless it is one GPU."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t.device != device:
-            raise ValueError(f"{op}: tensors on {device} and {t.device}; they must be on one GPU")
-    return device
+        if t.get_device() != index or index < 0:
+            _on_gpu(op, *tensors)
+            raise ValueError(f"{op}: tensors on {tensors[0].device} and {t.device}; they must be "
+                             "on one GPU")
+    return index
 
 
-def _launch(device, fn, *args) -> int:
-    """fn(*args, stream) on the current stream of ``device``."""
+def _launch(index: int, fn, *args) -> int:
+    """fn(*args, stream) on the current stream of GPU ``index``."""
     import torch
-    if device.index == torch.cuda.current_device():
+    if index == torch.cuda.current_device():
         return fn(*args, _stream())
-    with torch.cuda.device(device):
+    with torch.cuda.device(index):
         return fn(*args, _stream())
+
+
+def _take(op: str, name: str, t, dtype):
+    """_arg without the element count; its message is put together only when it is needed."""
+    if t.dtype is not dtype:
+        raise ValueError(f"{op}: {name} has dtype {t.dtype}; expected {dtype}")
+    return t.contiguous()
 
 
 def _mx(op: str, codes, scales, names=("codes", "scales")):
     """Validated (codes, scales, rows, cols) of an MXFP4 matrix: u8 codes [rows, cols / 2]
     and u8 scales [rows, cols / 32]."""
     import torch
-    codes = _arg(f"{op}: {names[0]}", codes, torch.uint8)
-    scales = _arg(f"{op}: {names[1]}", scales, torch.uint8)
-    if (codes.dim() != 2 or scales.dim() != 2 or scales.shape[0] != codes.shape[0]
-            or scales.shape[1] * 16 != codes.shape[1]):
-        raise ValueError(f"{op}: {names[0]} {tuple(codes.shape)} and {names[1]} "
-                         f"{tuple(scales.shape)} must be [rows, K / 2] and [rows, K / 32]")
-    return codes, scales, codes.shape[0], codes.shape[1] * 2
+    codes = _take(op, names[0], codes, torch.uint8)
+    scales = _take(op, names[1], scales, torch.uint8)
+    c, s = codes.shape, scales.shape
+    if len(c) != 2 or len(s) != 2 or s[0] != c[0] or s[1] * 16 != c[1]:
+        raise ValueError(f"{op}: {names[0]} {tuple(c)} and {names[1]} {tuple(s)} must be "
+                         "[rows, K / 2] and [rows, K / 32]")
+    return codes, scales, c[0], c[1] * 2
 
 
 def mxfp4_quantize(x) -> Tuple:
@@ -842,14 +850,14 @@ def mxfp4_quantize(x) -> Tuple:
     x = _arg("mxfp4_quantize: x", x, (torch.bfloat16, torch.float32))
     if x.dim() != 2 or x.shape[1] % 32:
         raise ValueError(f"mxfp4_quantize: x {tuple(x.shape)} must be [rows, K], K a multiple of 32")
-    device = _one_gpu("mxfp4_quantize", x)
+    gpu = _one_gpu("mxfp4_quantize", x)
     rows, cols = x.shape
-    codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=device)
-    scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=device)
+    codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
     lib = _get_lib()
     fn = lib.kc_quantize_mxfp4_bf16 if x.dtype == torch.bfloat16 else lib.kc_quantize_mxfp4_f32
     with kernel_span("mxfp4_quantize", rows=rows, cols=cols):
-        st = _launch(device, fn, _ptr(x), _ptr(codes), _ptr(scales), rows, cols)
+        st = _launch(gpu, fn, _ptr(x), _ptr(codes), _ptr(scales), rows, cols)
     _check("mxfp4_quantize", st)
     return codes, scales
 
@@ -862,12 +870,12 @@ def mxfp4_dequantize(codes, scales, out_dtype=None):
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"mxfp4_dequantize: out_dtype must be bfloat16 or float32, not {out_dtype}")
     codes, scales, rows, cols = _mx("mxfp4_dequantize", codes, scales)
-    device = _one_gpu("mxfp4_dequantize", codes, scales)
-    out = torch.empty(rows, cols, dtype=out_dtype, device=device)
+    gpu = _one_gpu("mxfp4_dequantize", codes, scales)
+    out = torch.empty(rows, cols, dtype=out_dtype, device=codes.device)
     lib = _get_lib()
     fn = lib.kc_dequantize_mxfp4_bf16 if out_dtype == torch.bfloat16 else lib.kc_dequantize_mxfp4_f32
     with kernel_span("mxfp4_dequantize", rows=rows, cols=cols):
-        st = _launch(device, fn, _ptr(codes), _ptr(scales), _ptr(out), rows, cols)
+        st = _launch(gpu, fn, _ptr(codes), _ptr(scales), _ptr(out), rows, cols)
     _check("mxfp4_dequantize", st)
     return out
 
@@ -885,12 +893,12 @@ def mxfp4_gemm_w4a4(qx, sx, qw, sw, out_dtype=None):
     qw, sw, N, Kw = _mx("mxfp4_gemm_w4a4", qw, sw, ("qw", "sw"))
     if K != Kw:
         raise ValueError(f"mxfp4_gemm_w4a4: x has K={K}, w has K={Kw}")
-    device = _one_gpu("mxfp4_gemm_w4a4", qx, sx, qw, sw)
-    y = torch.empty(M, N, dtype=out_dtype, device=device)
+    gpu = _one_gpu("mxfp4_gemm_w4a4", qx, sx, qw, sw)
+    y = torch.empty(M, N, dtype=out_dtype, device=qx.device)
     lib = _get_lib()
     fn = lib.kc_gemm_mxfp4_w4a4_bf16 if out_dtype == torch.bfloat16 else lib.kc_gemm_mxfp4_w4a4_f32
     with kernel_span("mxfp4_gemm_w4a4", m=M, n=N, k=K):
-        st = _launch(device, fn, _ptr(qx), _ptr(sx), _ptr(qw), _ptr(sw), _ptr(y), M, N, K)
+        st = _launch(gpu, fn, _ptr(qx), _ptr(sx), _ptr(qw), _ptr(sw), _ptr(y), M, N, K)
     _check("mxfp4_gemm_w4a4", st)
     return y
 
@@ -900,14 +908,14 @@ def mxfp4_gemm_bf16(qw, sw, x):
     accumulation: the form for single tokens and decode batches (kc_gemm_mxfp4_bf16)."""
     import torch
     qw, sw, N, K = _mx("mxfp4_gemm_bf16", qw, sw, ("qw", "sw"))
-    x = _arg("mxfp4_gemm_bf16: x", x, torch.bfloat16)
+    x = _take("mxfp4_gemm_bf16", "x", x, torch.bfloat16)
     if x.dim() != 2 or x.shape[1] != K:
         raise ValueError(f"mxfp4_gemm_bf16: x must be [M, {K}], not {list(x.shape)}")
-    device = _one_gpu("mxfp4_gemm_bf16", qw, sw, x)
+    gpu = _one_gpu("mxfp4_gemm_bf16", qw, sw, x)
     M = x.shape[0]
-    y = torch.empty(M, N, dtype=torch.bfloat16, device=device)
+    y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
     with kernel_span("mxfp4_gemm_bf16", m=M, n=N, k=K):
-        st = _launch(device, _get_lib().kc_gemm_mxfp4_bf16, _ptr(qw), _ptr(sw), _ptr(x), _ptr(y), M,
+        st = _launch(gpu, _get_lib().kc_gemm_mxfp4_bf16, _ptr(qw), _ptr(sw), _ptr(x), _ptr(y), M,
                      N, K)
     _check("mxfp4_gemm_bf16", st)
     return y
@@ -928,22 +936,19 @@ class KvCache(ctypes.Structure):
                 ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int), ("format", ctypes.c_int)]
 
 
-def _heads(name: str, t, dtypes, tokens: Optional[int] = None, heads: Optional[int] = None,
-           head_dim: Optional[int] = None):
+def _heads(op: str, name: str, t, dtypes, want=(None, None, None)):
     """``t`` [tokens, heads, head_dim] with the heads of a token one after the other (a view of a
     fused projection's rows stays one, anything else is copied); ValueError for another type or
     shape."""
-    allowed = dtypes if isinstance(dtypes, tuple) else (dtypes,)
-    if t.dtype not in allowed:
-        raise ValueError(f"{name} has dtype {t.dtype}; expected "
-                         f"{' or '.join(str(d) for d in allowed)}")
-    want = (tokens, heads, head_dim)
-    if t.dim() != 3 or any(w is not None and w != n for w, n in zip(want, t.shape)):
-        raise ValueError(f"{name} {tuple(t.shape)} must be [tokens, heads, head_dim]"
-                         + ("" if tokens is None else f" with {want}"))
-    _, H, D = t.shape
-    s = t.stride()
-    if (D > 1 and s[2] != 1) or (H > 1 and s[1] != D):
+    if t.dtype not in dtypes:
+        raise ValueError(f"{op}: {name} has dtype {t.dtype}; expected "
+                         f"{' or '.join(str(d) for d in dtypes)}")
+    shape = t.shape
+    if len(shape) != 3 or any(w is not None and w != n for w, n in zip(want, shape)):
+        raise ValueError(f"{op}: {name} {tuple(shape)} must be [tokens, heads, head_dim]"
+                         + (f" with {want}" if any(w is not None for w in want) else ""))
+    _, across, inner = t.stride()
+    if (shape[2] > 1 and inner != 1) or (shape[1] > 1 and across != shape[2]):
         return t.contiguous()
     return t
 
@@ -951,27 +956,28 @@ def _heads(name: str, t, dtypes, tokens: Optional[int] = None, heads: Optional[i
 def _rope(op: str, dtype, T: int, D: int, q_gamma, k_gamma, cos, sin, positions, interleaved: bool):
     """Validated (q_gamma, k_gamma, cos, sin, positions, kc_rope)."""
     import torch
-    q_gamma = _arg(f"{op}: q_gamma", q_gamma, dtype)
-    k_gamma = _arg(f"{op}: k_gamma", k_gamma, dtype)
-    cos = _arg(f"{op}: cos", cos, torch.float32)
-    sin = _arg(f"{op}: sin", sin, torch.float32)
-    positions = _arg(f"{op}: positions", positions, torch.int32)
+    q_gamma = _take(op, "q_gamma", q_gamma, dtype)
+    k_gamma = _take(op, "k_gamma", k_gamma, dtype)
+    cos = _take(op, "cos", cos, torch.float32)
+    sin = _take(op, "sin", sin, torch.float32)
+    positions = _take(op, "positions", positions, torch.int32)
     if q_gamma.shape != (D,) or k_gamma.shape != (D,):
         raise ValueError(f"{op}: q_gamma and k_gamma must be [{D}]")
-    if cos.dim() != 2 or cos.shape != sin.shape or 2 * cos.shape[1] > D:
-        raise ValueError(f"{op}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must both be "
+    table = cos.shape
+    if len(table) != 2 or table != sin.shape or 2 * table[1] > D:
+        raise ValueError(f"{op}: cos {tuple(table)} and sin {tuple(sin.shape)} must both be "
                          f"[table rows, rotary_dim / 2] with rotary_dim at most {D}")
     if positions.shape != (T,):
         raise ValueError(f"{op}: positions {tuple(positions.shape)} must be [{T}]")
     return q_gamma, k_gamma, cos, sin, positions, Rope(
-        _ptr(cos), _ptr(sin), _ptr(positions), cos.shape[0], 2 * cos.shape[1], bool(interleaved))
+        _ptr(cos), _ptr(sin), _ptr(positions), table[0], 2 * table[1], bool(interleaved))
 
 
 def _kv_cache(op: str, k_codes, k_scales, v_codes, v_scales):
     """(kc_kv_cache, kv_heads, head_dim) of a cache's four tensors, which must be contiguous
     (they are written to); fp32 scales mean FP8 rows, u8 scales MXFP4 rows."""
     import torch
-    fp8 = k_scales.dtype == torch.float32
+    fp8 = k_scales.dtype is torch.float32
     for name, t, dtypes in (("k_codes", k_codes, (torch.int8, torch.uint8) if fp8 else (torch.uint8,)),
                             ("v_codes", v_codes, (k_codes.dtype,)),
                             ("k_scales", k_scales, (torch.float32, torch.uint8)),
@@ -1004,19 +1010,19 @@ def qk_norm_rope(q, k, q_gamma, k_gamma, cos, sin, positions, eps: float = 1e-6,
     position give zeros, positions past the tables NaN (kc_qk_norm_rope_*)."""
     import torch
     op = "qk_norm_rope"
-    q = _heads(f"{op}: q", q, (torch.bfloat16, torch.float32))
+    q = _heads(op, "q", q, (torch.bfloat16, torch.float32))
     T, Hq, D = q.shape
-    k = _heads(f"{op}: k", k, q.dtype, T, None, D)
+    k = _heads(op, "k", k, (q.dtype,), (T, None, D))
     q_gamma, k_gamma, cos, sin, positions, rope = _rope(op, q.dtype, T, D, q_gamma, k_gamma, cos,
                                                         sin, positions, interleaved)
-    device = _one_gpu(op, q, k, q_gamma, k_gamma, cos, sin, positions)
+    gpu = _one_gpu(op, q, k, q_gamma, k_gamma, cos, sin, positions)
     Hkv = k.shape[1]
-    q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=device)
-    k_out = torch.empty(T, Hkv, D, dtype=q.dtype, device=device)
+    q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(T, Hkv, D, dtype=q.dtype, device=q.device)
     lib = _get_lib()
     fn = lib.kc_qk_norm_rope_bf16 if q.dtype == torch.bfloat16 else lib.kc_qk_norm_rope_f32
     with kernel_span(op, tokens=T, heads=Hq, kv_heads=Hkv, head_dim=D):
-        st = _launch(device, fn, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(q_gamma),
+        st = _launch(gpu, fn, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(q_gamma),
                      _ptr(k_gamma), ctypes.byref(rope), eps, T, Hq, Hkv, D, _ptr(q_out), _ptr(k_out))
     _check(op, st)
     return q_out, k_out
@@ -1030,26 +1036,26 @@ def qk_norm_rope_cache(q, k, v, q_gamma, k_gamma, cos, sin, positions, slots, k_
     cache (kc_qk_norm_rope_cache_*)."""
     import torch
     op = "qk_norm_rope_cache"
-    q = _heads(f"{op}: q", q, (torch.bfloat16, torch.float32))
+    q = _heads(op, "q", q, (torch.bfloat16, torch.float32))
     T, Hq, D = q.shape
     cache, Hkv, Dc = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
     if D != Dc:
         raise ValueError(f"{op}: q has head_dim {D}, the cache {Dc}")
-    k = _heads(f"{op}: k", k, q.dtype, T, Hkv, D)
-    v = _heads(f"{op}: v", v, q.dtype, T, Hkv, D)
+    k = _heads(op, "k", k, (q.dtype,), (T, Hkv, D))
+    v = _heads(op, "v", v, (q.dtype,), (T, Hkv, D))
     q_gamma, k_gamma, cos, sin, positions, rope = _rope(op, q.dtype, T, D, q_gamma, k_gamma, cos,
                                                         sin, positions, interleaved)
-    slots = _arg(f"{op}: slots", slots, torch.int64)
+    slots = _take(op, "slots", slots, torch.int64)
     if slots.shape != (T,):
         raise ValueError(f"{op}: slots {tuple(slots.shape)} must be [{T}]")
-    device = _one_gpu(op, q, k, v, q_gamma, k_gamma, cos, sin, positions, slots, k_codes, k_scales,
+    gpu = _one_gpu(op, q, k, v, q_gamma, k_gamma, cos, sin, positions, slots, k_codes, k_scales,
                       v_codes, v_scales)
-    q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=device)
+    q_out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
     lib = _get_lib()
     fn = (lib.kc_qk_norm_rope_cache_bf16 if q.dtype == torch.bfloat16
           else lib.kc_qk_norm_rope_cache_f32)
     with kernel_span(op, tokens=T, heads=Hq, kv_heads=Hkv, head_dim=D):
-        st = _launch(device, fn, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0),
+        st = _launch(gpu, fn, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0),
                      _ptr(q_gamma), _ptr(k_gamma), ctypes.byref(rope), eps, T, Hq, _ptr(slots),
                      ctypes.byref(cache), _ptr(q_out))
     _check(op, st)
@@ -1068,18 +1074,17 @@ def kv_cache_write(k, v, slots, k_codes, k_scales, v_codes, v_scales) -> None:
     import torch
     op = "kv_cache_write"
     cache, H, D = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
-    k = _heads(f"{op}: k", k, (torch.bfloat16, torch.float32))
+    k = _heads(op, "k", k, (torch.bfloat16, torch.float32), (None, H, D))
     T = k.shape[0]
-    k = _heads(f"{op}: k", k, k.dtype, T, H, D)
-    v = _heads(f"{op}: v", v, k.dtype, T, H, D)
-    slots = _arg(f"{op}: slots", slots, torch.int64)
+    v = _heads(op, "v", v, (k.dtype,), (T, H, D))
+    slots = _take(op, "slots", slots, torch.int64)
     if slots.shape != (T,):
         raise ValueError(f"{op}: slots {tuple(slots.shape)} must be [{T}]")
-    device = _one_gpu(op, k, v, slots, k_codes, k_scales, v_codes, v_scales)
+    gpu = _one_gpu(op, k, v, slots, k_codes, k_scales, v_codes, v_scales)
     lib = _get_lib()
     fn = lib.kc_kv_cache_write_bf16 if k.dtype == torch.bfloat16 else lib.kc_kv_cache_write_f32
     with kernel_span(op, tokens=T, kv_heads=H, head_dim=D):
-        st = _launch(device, fn, _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(slots), T,
+        st = _launch(gpu, fn, _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(slots), T,
                      ctypes.byref(cache))
     _check(op, st)
 
@@ -1098,20 +1103,20 @@ def kv_cache_read(k_codes, k_scales, v_codes, v_scales, block_table, cu_seqlens,
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"{op}: out_dtype must be bfloat16 or float32, not {out_dtype}")
     cache, H, D = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
-    block_table = _arg(f"{op}: block_table", block_table, torch.int32)
-    cu_seqlens = _arg(f"{op}: cu_seqlens", cu_seqlens, torch.int32)
+    block_table = _take(op, "block_table", block_table, torch.int32)
+    cu_seqlens = _take(op, "cu_seqlens", cu_seqlens, torch.int32)
     if block_table.dim() != 2 or cu_seqlens.shape != (block_table.shape[0] + 1,):
         raise ValueError(f"{op}: block_table {tuple(block_table.shape)} and cu_seqlens "
                          f"{tuple(cu_seqlens.shape)} must be [sequences, pages] and [sequences + 1]")
     if total_tokens < 0:
         raise ValueError(f"{op}: total_tokens={total_tokens} is negative")
-    device = _one_gpu(op, k_codes, k_scales, v_codes, v_scales, block_table, cu_seqlens)
-    k = torch.empty(total_tokens, H, D, dtype=out_dtype, device=device)
+    gpu = _one_gpu(op, k_codes, k_scales, v_codes, v_scales, block_table, cu_seqlens)
+    k = torch.empty(total_tokens, H, D, dtype=out_dtype, device=k_codes.device)
     v = torch.empty_like(k)
     lib = _get_lib()
     fn = lib.kc_kv_cache_read_bf16 if out_dtype == torch.bfloat16 else lib.kc_kv_cache_read_f32
     with kernel_span(op, tokens=total_tokens, kv_heads=H, head_dim=D):
-        st = _launch(device, fn, ctypes.byref(cache), _ptr(block_table), block_table.shape[1],
+        st = _launch(gpu, fn, ctypes.byref(cache), _ptr(block_table), block_table.shape[1],
                      _ptr(cu_seqlens), block_table.shape[0], total_tokens, _ptr(k), _ptr(v))
     _check(op, st)
     return k, v
