@@ -18,5 +18,10 @@ template <bool YBF16>
 int gemm_tile(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int64_t M,
               int64_t N, int64_t K, hipStream_t stream);
 
+// One token of bf16 activations (mxfp4_gemv.hip); false, nothing launched, for
+// shapes that are left to the matrix cores.
+bool gemv(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t* x, uint16_t* y, int N, int K,
+          hipStream_t stream, int* status);
+
 }  // namespace mx
 }  // namespace kc

@@ -1,5 +1,5 @@
 // mxfp4_gemm_a16.hip -- bf16 activations times MXFP4 weights on gfx950, the linear
-// layer of single tokens and decode batches.  No counterpart in the reference.
+// layer of decode batches (one token: mxfp4_gemv.hip).  No counterpart in the reference.
 //
 //   Y[m, n] = sum_k x[m, k] * e2m1(qw[n, k]) 2^(sw[n, k / 32] - 127)
 //
@@ -245,17 +245,31 @@ int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t*
     return kc::check_launch(fn);
 }
 
-// Row tiles per workgroup: the fewest that leave at most one workgroup per CU,
-// since every workgroup reads all of its tokens' X; seven at most.
-template <int MT>
-int skinny(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t* x, uint16_t* y, int M, int N, int K,
-           hipStream_t stream) {
-    constexpr int kCus = 256;
-    const int64_t wgs = int64_t{(N + 15) / 16} * ((M + 16 * MT - 1) / (16 * MT));
-    if (wgs <= kCus) return launch<MT, 1, MT == 1 ? 8 : 4, 1>(fn, qw, sw, x, y, M, N, K, stream);
-    if (wgs <= 2 * kCus) return launch<MT, 2, 8, 1>(fn, qw, sw, x, y, M, N, K, stream);
-    if (wgs <= 4 * kCus) return launch<MT, 4, 4, MT == 2 ? 2 : 1>(fn, qw, sw, x, y, M, N, K, stream);
-    return launch<MT, 7, 4, MT == 2 ? 2 : 1>(fn, qw, sw, x, y, M, N, K, stream);
+// Tokens (tiles of 16) and weight rows (tiles of 16) per workgroup, and what a
+// workgroup takes in hundredths of a microsecond per step of 256 values and beside
+// the steps, with every CU holding one (K 4096 and 14336).  More rows share the
+// reads of X, more tokens those of the weights and their decoding, fewer of both
+// fill the CUs: M 64, N 4096, K 14336 54 us with all tokens and one row tile, 28
+// with one tile of tokens and four of rows; M 128, N 6144, K 4096 20 with 2 and 7, 48
+// with 4 and 1; M 64, N 28672, K 4096 31 with 4 and 7, 63 with 1 and 7.
+struct Cost {
+    int mt, rt, step, fixed;
+};
+constexpr int kCus = 256;
+constexpr Cost kCosts[] = {{1, 1, 20, 300}, {1, 2, 31, 320}, {1, 4, 43, 390}, {1, 7, 70, 410}, {2, 1, 48, 310}, {2, 2, 53, 300},
+                           {2, 4, 62, 450}, {2, 7, 86, 470}, {3, 7, 107, 650}, {4, 2, 95, 460}, {4, 4, 105, 600}, {4, 7, 128, 830}};
+
+int best(int M, int N, int K) {
+    const int64_t steps = (K + kStep - 1) / kStep;
+    int which = 0;
+    int64_t least = INT64_MAX;
+    for (int i = 0; i < static_cast<int>(sizeof(kCosts) / sizeof(kCosts[0])); ++i) {
+        const Cost& c = kCosts[i];
+        const int64_t wgs = int64_t{(N + 16 * c.rt - 1) / (16 * c.rt)} * ((M + 16 * c.mt - 1) / (16 * c.mt));
+        const int64_t cost = (wgs + kCus - 1) / kCus * steps * c.step + c.fixed;
+        if (cost < least) least = cost, which = i;
+    }
+    return which;
 }
 
 }  // namespace
@@ -270,7 +284,20 @@ extern "C" int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw, cons
     if (!kc::aligned(d_qw, 16) || !kc::aligned(d_x, 16))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the codes and x must be 16-byte aligned", fn);
     const int m = static_cast<int>(M), n = static_cast<int>(N), k = static_cast<int>(K);
-    if (m <= 16) return skinny<1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-    if (m <= 32) return skinny<2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-    return skinny<4>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+    int done = KC_SUCCESS;
+    if (m == 1 && kc::mx::gemv(fn, d_qw, d_sw, d_x, d_y, n, k, stream, &done)) return done;
+    switch (best(m, n, k)) {
+        case 0: return launch<1, 1, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 1: return launch<1, 2, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 2: return launch<1, 4, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 3: return launch<1, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 4: return launch<2, 1, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 5: return launch<2, 2, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 6: return launch<2, 4, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 7: return launch<2, 7, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 8: return launch<3, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 9: return launch<4, 2, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 10: return launch<4, 4, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        default: return launch<4, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+    }
 }

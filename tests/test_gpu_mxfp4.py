@@ -215,7 +215,9 @@ def test_w4a4_nan_scale_stays_in_its_row_and_column(gpu, ops, M):
 
 A16_SHAPES = [(1, 1, 32), (1, 17, 64), (3, 40, 96), (1, 4096, 4096), (7, 1000, 1056), (13, 2048, 4096),
               (16, 16, 128), (17, 515, 544), (31, 96, 2048), (33, 129, 320), (48, 600, 1024), (64, 1100, 14336),
-              (65, 300, 800), (128, 260, 4096), (130, 33, 288), (1, 28672, 512)]
+              (65, 300, 800), (128, 260, 4096), (130, 33, 288), (1, 28672, 512), (1, 77, 2048), (1, 1000, 2080),
+              (1, 130, 16384), (1, 50, 16416), (1, 301, 10240), (40, 4097, 320), (20, 9000, 288), (60, 17000, 256),
+              (33, 28672, 256), (200, 8200, 96)]
 
 
 @pytest.mark.parametrize("M,N,K", A16_SHAPES)
