@@ -1,23 +1,27 @@
 // mxfp4_gemm.hip -- the product of two MXFP4 matrices on gfx950's scaled matrix
-// cores: entry points, and the kernel for decode batches (M <= 64).  More rows:
-// mxfp4_gemm_tile.hip.  No counterpart in the reference.
+// cores: entry points, and the kernel for decode batches (M <= 16, or 64 on layers of
+// few rows).  More: mxfp4_gemm_tile.hip.  No counterpart in the reference.
 //
 //   Y[m, n] = sum_b 2^(sx[m, b] + sw[n, b] - 254) sum_{k in block b} e2m1(qx[m, k]) e2m1(qw[n, k])
 //
-// M <= 64 is bound by the weight stream (0.53 bytes a weight).  A workgroup of KW
-// waves owns RT tiles of 16 weight rows and all MT = ceil(M / 16) tiles of X; wave w
-// takes K steps w, w + KW, ... of 128 bytes (256 values), D of them in flight in
-// registers, and the KW partial sums of every output meet in LDS in a fixed
-// order.  No barrier stands in the K loop and no operand goes through LDS:
-// with K split over the waves no two of them read the same bytes.
+// gemm_mxfp4_skinny_kernel is bound by the weight stream (0.53 bytes a weight).  A workgroup of KW
+// waves owns RT tiles of 16 weight rows and all MT = ceil(M / 16) tiles of X; K advances
+// in spans of 1024 values, 512 bytes of every row, which the waves take in turn, and
+// the KW partial sums of every output meet in LDS in a fixed order.  No barrier
+// stands in the K loop and no operand goes through LDS: with K split over the waves no
+// two of them read the same bytes.  A step's registers take the next span's as soon as
+// they have been multiplied.
 //
-// A load carries 8 whole rows of a step (128 bytes, a cache line each): lane l
-// takes 16-byte chunk 2 (l / 16) + l % 2 of row 8 h + (l % 16) / 2.  A lane and its
+// A load carries 8 whole rows of a quarter span, a step (128 bytes, a cache line each):
+// lane l takes 16-byte chunk 2 (l / 16) + l % 2 of row 8 h + (l % 16) / 2.  A lane and its
 // neighbour l ^ 1 exchange one chunk each, after which lane (i, kb) holds chunks
 // 2 kb and 2 kb + 1, two blocks of 32, of row row_of(i) = i / 2 + 8 (i % 2): the
-// operands of two matrix-core instructions of 128 values.  The blocks' scale bytes
-// are neighbours and come as one 16-bit load.
+// operands of two matrix-core instructions of 128 values.  The 32 scale bytes of a row's
+// span come with one load of 8 bytes, step kb's, to lane (i, kb); a 4 x 4 transpose of
+// 16-bit pairs over the lanes l % 16 leaves each lane its own two blocks' bytes of all
+// four steps (a 16-bit load a step costs the load unit as many lines as the codes).
 #include <algorithm>
+#include <type_traits>
 
 #include "mxfp4_gemm.hpp"
 
@@ -25,9 +29,8 @@ namespace {
 
 using namespace kc::mx;
 
-typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kBK = 128;       // bytes of K per step
+constexpr int kSpan = 4 * kBK;  // and per span
 constexpr int kSkinnyM = 64;
 
 struct Frag {
@@ -39,18 +42,28 @@ __device__ __forceinline__ uint32_t swap_pair(uint32_t v) {  // lane l reads lan
 }
 
 // Chunks 2 kb (lo) and 2 kb + 1 (hi) of the lane's operand row.
-__device__ __forceinline__ void as_operands(const Frag& f, bool even, i32x8& lo, i32x8& hi) {
-    const uint32_t a[4] = {f.h0.x, f.h0.y, f.h0.z, f.h0.w}, b[4] = {f.h1.x, f.h1.y, f.h1.z, f.h1.w};
-    lo = hi = i32x8{0, 0, 0, 0, 0, 0, 0, 0};
+__device__ __forceinline__ void as_operands(const Frag& f, bool even, u32x4& lo, u32x4& hi) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-        const uint32_t an = swap_pair(a[d]), bn = swap_pair(b[d]);
-        lo[d] = static_cast<int32_t>(even ? a[d] : bn);
-        hi[d] = static_cast<int32_t>(even ? an : b[d]);
+        const uint32_t a = f.h0[d], b = f.h1[d], an = swap_pair(a), bn = swap_pair(b);
+        lo[d] = even ? a : bn;
+        hi[d] = even ? an : b;
     }
 }
 
-template <int MT, int RT, int KW, int D, bool YBF16>
+// Lane (i, g) holds pairs 0 .. 3 of step g (16 bits each, two to a word); it gets pair g
+// of steps 0, 1 (x) and 2, 3 (y).
+__device__ __forceinline__ u32x2 transpose_pairs(u32x2 v, uint32_t select) {
+    uint32_t a = v.x, b = v.y;
+    const auto q = __builtin_amdgcn_permlane32_swap(a, b, false, false);  // lanes 32-63 of a with 0-31 of b
+    a = q[0];
+    b = q[1];
+    const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);  // even row's in [0], odd row's in [1]
+    const auto s = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return u32x2{__builtin_amdgcn_perm(r[1], r[0], select), __builtin_amdgcn_perm(s[1], s[0], select)};
+}
+
+template <int MT, int RT, int KW, bool YBF16>
 __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
     const uint8_t* __restrict__ qx, const uint8_t* __restrict__ sx, const uint8_t* __restrict__ qw,
     const uint8_t* __restrict__ sw, void* __restrict__ y, int M, int N, int K, bool vec) {
@@ -59,6 +72,7 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int i = lane & 15, kb = lane >> 4;
     const bool even = (lane & 1) == 0;
+    const uint32_t select = kb & 1 ? 0x07060302u : 0x05040100u;  // high or low halves of two words
     const int n0 = static_cast<int>(blockIdx.x) * 16 * RT;
     const int kbytes = K / 2, blocks = K / kBlock;
     const uint8_t* wbase = qw + static_cast<int64_t>(n0) * kbytes;
@@ -70,14 +84,14 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             woff[r][h] = static_cast<uint32_t>(min(n0 + 16 * r + 8 * h + r8, N - 1) - n0) * static_cast<uint32_t>(kbytes) + 16u * chunk;
-        wsoff[r] = static_cast<uint32_t>(min(n0 + 16 * r + orow, N - 1) - n0) * static_cast<uint32_t>(blocks) + 2u * kb;
+        wsoff[r] = static_cast<uint32_t>(min(n0 + 16 * r + orow, N - 1) - n0) * static_cast<uint32_t>(blocks);
     }
 #pragma unroll
     for (int c = 0; c < MT; ++c) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             xoff[c][h] = static_cast<uint32_t>(min(16 * c + 8 * h + r8, M - 1)) * static_cast<uint32_t>(kbytes) + 16u * chunk;
-        xsoff[c] = static_cast<uint32_t>(min(16 * c + orow, M - 1)) * static_cast<uint32_t>(blocks) + 2u * kb;
+        xsoff[c] = static_cast<uint32_t>(min(16 * c + orow, M - 1)) * static_cast<uint32_t>(blocks);
     }
 
     f32x4 acc[RT][MT];
@@ -85,83 +99,100 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int c = 0; c < MT; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int full = kbytes / kBK;
-    const int mine = full > wave ? (full - wave + KW - 1) / KW : 0;  // K steps wave, wave + KW, ...
+    const int spans = kbytes / kSpan;
+    const int mine = spans > wave ? (spans - wave + KW - 1) / KW : 0;  // spans wave, wave + KW, ...
 
-    Frag wf[D][RT], xf[D][MT];
-    uint32_t ws[D][RT], xs[D][MT];
-    auto pair_at = [](const uint8_t* p) {
-        uint16_t v;
-        __builtin_memcpy(&v, p, 2);
-        return static_cast<uint32_t>(v);
-    };
-    auto load = [&](int slot, int j) {
-        const int step = wave + KW * min(j, mine - 1);
-        const uint8_t *wp = wbase + step * kBK, *xp = qx + step * kBK, *wsp = wsbase + 8 * step, *xsp = sx + 8 * step;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            wf[slot][r].h0 = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][0]));
-            wf[slot][r].h1 = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][1]));
-            ws[slot][r] = pair_at(wsp + wsoff[r]);
-        }
-#pragma unroll
-        for (int c = 0; c < MT; ++c) {
-            xf[slot][c].h0 = *reinterpret_cast<const u32x4*>(xp + xoff[c][0]);
-            xf[slot][c].h1 = *reinterpret_cast<const u32x4*>(xp + xoff[c][1]);
-            xs[slot][c] = pair_at(xsp + xsoff[c]);
-        }
-    };
-    auto multiply = [&](const Frag (&w)[RT], const Frag (&x)[MT], const uint32_t (&wsc)[RT], const uint32_t (&xsc)[MT]) {
-        i32x8 b0[MT], b1[MT];
+    // acc += W X^T of one step, its scales at `byte` and the next of their words
+    auto multiply = [&](const Frag (&w)[RT], const Frag (&x)[MT], const uint32_t (&wsc)[RT], const uint32_t (&xsc)[MT],
+                        auto bc) {
+        constexpr int byte = decltype(bc)::value;
+        u32x4 b0[MT], b1[MT];
 #pragma unroll
         for (int c = 0; c < MT; ++c) as_operands(x[c], even, b0[c], b1[c]);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            i32x8 a0, a1;
+            u32x4 a0, a1;
             as_operands(w[r], even, a0, a1);
 #pragma unroll
-            for (int c = 0; c < MT; ++c)
-                acc[r][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                    a0, b0[c], acc[r][c], 4, 4, 0, static_cast<int>(wsc[r]), 0, static_cast<int>(xsc[c]));
+            for (int c = 0; c < MT; ++c) mfma<byte, true>(acc[r][c], a0, b0[c], wsc[r], xsc[c]);
 #pragma unroll
-            for (int c = 0; c < MT; ++c)
-                acc[r][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                    a1, b1[c], acc[r][c], 4, 4, 1, static_cast<int>(wsc[r]), 1, static_cast<int>(xsc[c]));
+            for (int c = 0; c < MT; ++c) mfma<byte + 1, true>(acc[r][c], a1, b1[c], wsc[r], xsc[c]);
         }
     };
-    if (mine > 0) {
+    Frag wf[4][RT], xf[4][MT];
+    u32x2 ws[RT], xs[MT];
+    auto load = [&](int s, int span) {
+        const uint8_t *wp = wbase + span * kSpan + s * kBK, *xp = qx + span * kSpan + s * kBK;
 #pragma unroll
-        for (int d = 0; d < D; ++d) load(d, d);
-        __builtin_amdgcn_sched_barrier(0);
-        int j = 0;
-        for (; j + D < mine; j += D) {
-#pragma unroll
-            for (int d = 0; d < D; ++d) {
-                multiply(wf[d], xf[d], ws[d], xs[d]);
-                load(d, j + D + d);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int r = 0; r < RT; ++r) {
+            wf[s][r].h0 = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][0]));
+            wf[s][r].h1 = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][1]));
         }
 #pragma unroll
-        for (int d = 0; d < D; ++d)
-            if (j + d < mine) multiply(wf[d], xf[d], ws[d], xs[d]);
+        for (int c = 0; c < MT; ++c) {
+            xf[s][c].h0 = *reinterpret_cast<const u32x4*>(xp + xoff[c][0]);
+            xf[s][c].h1 = *reinterpret_cast<const u32x4*>(xp + xoff[c][1]);
+        }
+    };
+    auto load_scales = [&](int span) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) __builtin_memcpy(&ws[r], wsbase + 32 * span + wsoff[r] + 8 * kb, 8);
+#pragma unroll
+        for (int c = 0; c < MT; ++c) __builtin_memcpy(&xs[c], sx + 32 * span + xsoff[c] + 8 * kb, 8);
+    };
+    if (mine > 0) {
+        load_scales(wave);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) load(s, wave);
+        __builtin_amdgcn_sched_barrier(0);
+        auto span = [&](int next, auto mc) {
+            constexpr bool more = decltype(mc)::value;
+            uint32_t wsc[2][RT], xsc[2][MT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const u32x2 v = transpose_pairs(ws[r], select);
+                wsc[0][r] = v.x;
+                wsc[1][r] = v.y;
+            }
+#pragma unroll
+            for (int c = 0; c < MT; ++c) {
+                const u32x2 v = transpose_pairs(xs[c], select);
+                xsc[0][c] = v.x;
+                xsc[1][c] = v.y;
+            }
+            if constexpr (more) load_scales(next);
+            auto step = [&](auto sc) {
+                constexpr int s = decltype(sc)::value;
+                multiply(wf[s], xf[s], wsc[s / 2], xsc[s / 2], std::integral_constant<int, 2 * (s % 2)>{});
+                if constexpr (more) load(s, next);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            step(std::integral_constant<int, 0>{});
+            step(std::integral_constant<int, 1>{});
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
+        };
+        for (int j = 1; j < mine; ++j) span(wave + KW * j, std::true_type{});
+        span(0, std::false_type{});
     }
-    if (kbytes % kBK != 0 && wave == full % KW) {
-        // The partial last step: no codes and scale bytes 0 past K.
-        const int kvalid = kbytes - full * kBK;
+    // The steps behind the last whole span, one a wave: no codes and scale bytes 0 past K.
+    for (int step = 4 * spans; step * kBK < kbytes; ++step) {
+        if (step % KW != wave) continue;
+        const int kvalid = kbytes - step * kBK;
         auto tail = [&](const uint8_t* base, const uint32_t (&off)[2]) {
             const u32x4 z{0u, 0u, 0u, 0u};
             Frag f{z, z};
             if (16 * chunk < kvalid) {
-                f.h0 = *reinterpret_cast<const u32x4*>(base + full * kBK + off[0]);
-                f.h1 = *reinterpret_cast<const u32x4*>(base + full * kBK + off[1]);
+                f.h0 = *reinterpret_cast<const u32x4*>(base + step * kBK + off[0]);
+                f.h1 = *reinterpret_cast<const u32x4*>(base + step * kBK + off[1]);
             }
             return f;
         };
         auto tail_scales = [&](const uint8_t* p) {
+            p += 8 * step + 2 * kb;
             uint32_t v = 0;
-            if (32 * kb < kvalid) v = p[8 * full];
-            if (32 * kb + 16 < kvalid) v |= static_cast<uint32_t>(p[8 * full + 1]) << 8;
+            if (32 * kb < kvalid) v = p[0];
+            if (32 * kb + 16 < kvalid) v |= static_cast<uint32_t>(p[1]) << 8;
             return v;
         };
         Frag w[RT], x[MT];
@@ -176,8 +207,9 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
             x[c] = tail(qx, xoff[c]);
             xsc[c] = tail_scales(sx + xsoff[c]);
         }
-        multiply(w, x, wsc, xsc);
+        multiply(w, x, wsc, xsc, std::integral_constant<int, 0>{});
     }
+    settle();
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -217,30 +249,24 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
     }
 }
 
-template <int MT, int RT, int KW, int D, bool YBF16>
+template <int MT, int RT, int KW, bool YBF16>
 int launch_skinny(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int M,
                   int N, int K, hipStream_t stream) {
-    gemm_mxfp4_skinny_kernel<MT, RT, KW, D, YBF16><<<static_cast<unsigned>((N + 16 * RT - 1) / (16 * RT)), KW * 64, 0, stream>>>(
+    gemm_mxfp4_skinny_kernel<MT, RT, KW, YBF16><<<static_cast<unsigned>((N + 16 * RT - 1) / (16 * RT)), KW * 64, 0, stream>>>(
         qx, sx, qw, sw, y, M, N, K, N % 2 == 0 && kc::aligned(y, 4));
     return kc::check_launch(fn);
 }
 
-// Row tiles per workgroup: the fewest that leave at most one workgroup per CU,
-// since every workgroup reads all of X (M 32, K 4096: N 6144 8.4 us at one tile, 7.0
-// at two, 9.4 at four; N 28672 19.7 at two, 17.8 at four, 16.2 at seven; M 64
-// 32.6, 25.0, 20.5); four on two workgroups a CU where X is one tile and N large (M 8,
-// N 28672, K 8192 26.1 against 28.6 at seven; M 16, K 4096 15.2 and 15.4).  At one row
-// tile eight waves with one tile of X, four with more (M 1, K 4096 3.9 against 4.2
-// us; M 64, N 6144 13.3 against 12.5, M 32, K 14336 15.1 against 13.0).
+// Row tiles per workgroup, us at 1, 2 and 4 of them: one tile of X N 4096, K 14336 8.4,
+// 10.9, 15.7, N 11008, K 5120 7.5, 8.5, 8.7, N 28672, K 4096 15.0, 13.7, 14.7; two tiles
+// N 4096, K 14336 10.7, 13.2, 19.6, N 6144, K 4096 7.0, 6.3, 8.4; four 15.1, 19.3, 29.8 and
+// 11.6, 8.5, 12.3.  Eight waves instead of four: one tile of X 4.2 against 4.1 us (N 4096,
+// K 4096) and 8.2 against 8.4 (K 14336), more tiles spill.
 template <int MT, bool YBF16>
 int skinny(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int M, int N,
            int K, hipStream_t stream) {
-    constexpr int kRowsPerTile = 16 * 256;
-    if (N <= kRowsPerTile)
-        return launch_skinny<MT, 1, MT == 1 ? 8 : 4, 2, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
-    if (N <= 2 * kRowsPerTile) return launch_skinny<MT, 2, 8, 2, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
-    if (MT == 1 || N <= 4 * kRowsPerTile) return launch_skinny<MT, 4, 4, 2, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
-    return launch_skinny<MT, 7, 4, 1, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+    if (N <= (MT == 1 ? 12288 : 4096)) return launch_skinny<MT, 1, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+    return launch_skinny<MT, 2, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
 }
 
 template <bool YBF16>
@@ -252,7 +278,9 @@ int gemm(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw
     if (!qx || !sx || !qw || !sw) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
     if (!kc::aligned(qx, 16) || !kc::aligned(qw, 16))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the codes must be 16-byte aligned", fn);
-    if (M > kSkinnyM) return kc::mx::gemm_tile<YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+    // More than one tile of tokens on layers of many rows read X less often from LDS
+    // (M 32, N 28672, K 4096 16.4 -> 14.8 us; M 64 20.5 -> 15.4; M 64, N 6144 stays at 8.5).
+    if (M > kSkinnyM || (M > 16 && N > 8192)) return kc::mx::gemm_tile<YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
     const int m = static_cast<int>(M), n = static_cast<int>(N), k = static_cast<int>(K);
     switch ((m + 15) / 16) {
         case 1: return skinny<1, YBF16>(fn, qx, sx, qw, sw, y, m, n, k, stream);

@@ -6,6 +6,33 @@
 namespace kc {
 namespace mx {
 
+// acc += a b^T of one 16 x 16 x 128 tile, the scales in byte BYTE of sa and sb.
+// In assembly for the accumulator's "a" and the operands' four registers: with 256
+// accumulator registers and most of the others in use, the compiler's allocation keeps
+// moving accumulators between the two halves of the register file (640 moves per 512
+// of these), and the builtin's eight-register operands spill where loads fill most
+// registers.  Nothing but these instructions touches the accumulators until
+// settle().  NOP: the operands may come from the instruction just before (the wait
+// states that the compiler adds between a vector instruction and a matrix one that
+// reads its result); operands that LDS or memory wrote need none.
+template <int BYTE, bool NOP = false>
+__device__ __forceinline__ void mfma(f32x4& acc, u32x4 a, u32x4 b, uint32_t sa, uint32_t sb) {
+    if constexpr (NOP) asm volatile("s_nop 3" : "+v"(a), "+v"(b), "+v"(sa), "+v"(sb));
+#define KC_MFMA(sel)                                                                                        \
+    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " sel " cbsz:4 blgp:4" \
+        : "+a"(acc)                                                                                         \
+        : "v"(a), "v"(b), "v"(sa), "v"(sb))
+    if constexpr (BYTE == 0) KC_MFMA("op_sel_hi:[0,0,0]");
+    else if constexpr (BYTE == 1) KC_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
+    else if constexpr (BYTE == 2) KC_MFMA("op_sel_hi:[1,1,0]");
+    else KC_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
+#undef KC_MFMA
+}
+
+// The last results are in their registers (the compiler does not know the
+// latency of the assembly above).
+__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+
 // Shapes of Y [M, N] = X [M, K] W [N, K]^T; y checked where Y has elements.
 int check_gemm(const char* fn, int64_t M, int64_t N, int64_t K, const void* y);
 
@@ -22,6 +49,11 @@ int gemm_tile(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_
 // shapes that are left to the matrix cores.
 bool gemv(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t* x, uint16_t* y, int N, int K,
           hipStream_t stream, int* status);
+
+// bf16 activations in tiles of 16 mt tokens x 128 rows (mxfp4_gemm_a16_tile.hip): K a
+// multiple of 128, sw 4-byte aligned.
+int gemm_a16_tile(const char* fn, int mt, const uint8_t* qw, const uint8_t* sw, const uint16_t* x, uint16_t* y, int M, int N,
+                  int K, hipStream_t stream);
 
 }  // namespace mx
 }  // namespace kc

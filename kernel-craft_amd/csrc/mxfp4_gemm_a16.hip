@@ -252,19 +252,25 @@ int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t*
 // fill the CUs: M 64, N 4096, K 14336 54 us with all tokens and one row tile, 28
 // with one tile of tokens and four of rows; M 128, N 6144, K 4096 20 with 2 and 7, 48
 // with 4 and 1; M 64, N 28672, K 4096 31 with 4 and 7, 63 with 1 and 7.
+// The last three are the kernel of mxfp4_gemm_a16_tile.hip (128 rows; K a multiple of
+// 128): M 32, N 28672, K 4096 20.4 -> 19.0 us, M 64 30.7 -> 24.5, M 128 59 -> 44; M 128,
+// N 6144 20.4 -> 16.0; M 512, N 4096 44 -> 23; M 2048 144 -> 90.
 struct Cost {
     int mt, rt, step, fixed;
 };
 constexpr int kCus = 256;
+constexpr int kTileRt = 8;  // 128 rows: the other kernel
 constexpr Cost kCosts[] = {{1, 1, 20, 300}, {1, 2, 31, 320}, {1, 4, 43, 390}, {1, 7, 70, 410}, {2, 1, 48, 310}, {2, 2, 53, 300},
-                           {2, 4, 62, 450}, {2, 7, 86, 470}, {3, 7, 107, 650}, {4, 2, 95, 460}, {4, 4, 105, 600}, {4, 7, 128, 830}};
+                           {2, 4, 62, 450}, {2, 7, 86, 470}, {3, 7, 107, 650}, {4, 2, 95, 460}, {4, 4, 105, 600}, {4, 7, 128, 830},
+                           {2, kTileRt, 100, 200}, {3, kTileRt, 103, 300}, {4, kTileRt, 115, 500}};
 
-int best(int M, int N, int K) {
+int best(int M, int N, int K, bool tile) {
     const int64_t steps = (K + kStep - 1) / kStep;
     int which = 0;
     int64_t least = INT64_MAX;
     for (int i = 0; i < static_cast<int>(sizeof(kCosts) / sizeof(kCosts[0])); ++i) {
         const Cost& c = kCosts[i];
+        if (c.rt == kTileRt && !tile) continue;
         const int64_t wgs = int64_t{(N + 16 * c.rt - 1) / (16 * c.rt)} * ((M + 16 * c.mt - 1) / (16 * c.mt));
         const int64_t cost = (wgs + kCus - 1) / kCus * steps * c.step + c.fixed;
         if (cost < least) least = cost, which = i;
@@ -286,7 +292,7 @@ extern "C" int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw, cons
     const int m = static_cast<int>(M), n = static_cast<int>(N), k = static_cast<int>(K);
     int done = KC_SUCCESS;
     if (m == 1 && kc::mx::gemv(fn, d_qw, d_sw, d_x, d_y, n, k, stream, &done)) return done;
-    switch (best(m, n, k)) {
+    switch (best(m, n, k, k % 128 == 0 && kc::aligned(d_sw, 4))) {
         case 0: return launch<1, 1, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         case 1: return launch<1, 2, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         case 2: return launch<1, 4, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
@@ -298,6 +304,9 @@ extern "C" int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw, cons
         case 8: return launch<3, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         case 9: return launch<4, 2, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         case 10: return launch<4, 4, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        default: return launch<4, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 11: return launch<4, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 12: return kc::mx::gemm_a16_tile(fn, 2, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 13: return kc::mx::gemm_a16_tile(fn, 3, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        default: return kc::mx::gemm_a16_tile(fn, 4, d_qw, d_sw, d_x, d_y, m, n, k, stream);
     }
 }

@@ -55,28 +55,6 @@ __device__ __forceinline__ void lds_dma16(uint32_t voff, const void* sbase, uint
                  : "memory", "m0");
 }
 
-// acc += a b^T of one 16 x 16 x 128 tile, the scales in byte BYTE of sa and sb.
-// In assembly for the accumulator's "a": with 256 accumulator registers and most of
-// the others in use, the compiler's allocation keeps moving accumulators between
-// the two halves of the register file (640 moves per 512 of these).  Nothing
-// but these instructions touches the accumulators until settle().
-template <int BYTE>
-__device__ __forceinline__ void mfma(f32x4& acc, u32x4 a, u32x4 b, uint32_t sa, uint32_t sb) {
-#define KC_MFMA(sel)                                                                                        \
-    asm("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 " sel " cbsz:4 blgp:4" \
-        : "+a"(acc)                                                                                         \
-        : "v"(a), "v"(b), "v"(sa), "v"(sb))
-    if constexpr (BYTE == 0) KC_MFMA("op_sel_hi:[0,0,0]");
-    else if constexpr (BYTE == 1) KC_MFMA("op_sel:[1,1,0] op_sel_hi:[0,0,0]");
-    else if constexpr (BYTE == 2) KC_MFMA("op_sel_hi:[1,1,0]");
-    else KC_MFMA("op_sel:[1,1,0] op_sel_hi:[1,1,0]");
-#undef KC_MFMA
-}
-
-// The last results are in their registers (the compiler does not know the
-// latency of the assembly above).
-__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
-
 template <int TM_, int TN_, int WGM, int WGN, int ST>
 struct Shape {
     static constexpr int kRowsM = 16 * TM_ * WGM, kRowsN = 16 * TN_ * WGN, kRows = kRowsM + kRowsN;
@@ -357,7 +335,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
     // time, and leave in pieces of 16 bytes per lane.
     settle();
     const int64_t mw = m0 + 16 * TM * wm, nw = n0 + 16 * TN * wn;
-    if constexpr (YBF16) {
+    if constexpr (YBF16 && TN > 1) {
         if (vec) {
             constexpr int kChunks = 2 * TN;              // 16-byte chunks of a row
             constexpr int kPasses = 16 * kChunks / 64;   // of the wave
@@ -392,11 +370,12 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
         for (int j = 0; j < TN; ++j) {
             const int64_t n = nw + 16 * j + 4 * kb;
             const f32x4 v = acc[i][j];
-            if constexpr (!YBF16) {
-                if (vec && n < N) {
-                    *reinterpret_cast<f32x4*>(static_cast<float*>(y) + m * N + n) = v;
-                    continue;
-                }
+            if (vec && n < N) {
+                if constexpr (YBF16)
+                    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(y) + m * N + n) =
+                        u32x2{kc::pack_bf16x2(v.x, v.y), kc::pack_bf16x2(v.z, v.w)};
+                else *reinterpret_cast<f32x4*>(static_cast<float*>(y) + m * N + n) = v;
+                continue;
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -427,7 +406,7 @@ int launch(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* 
 // as one of two.  Measured with K 1024 to 14336 on grids of 64 to 1024 tiles; the
 // least expected time wins.  Against the 256 x 256 tile: M 128, N 4096, K 4096 28.6
 // -> 7.9 us (64 x 64); M 1000, N 4096, K 14336 103 -> 44.5 (128 x 128, four buffers,
-// one a CU); M 2048, N 4096, K 4096 34.4 -> 27.0 (256 x 128); M 4096, N 4096 39.7 and
+// one a CU); M 64, N 28672, K 4096 38 -> 15.4 (64 x 128); M 65, N 4096, K 4096 7.3 (32 x 64); M 2048, N 4096, K 4096 34.4 -> 27.0 (256 x 128); M 4096, N 4096 39.7 and
 // M 300, N 28672 38.4 stay (256 x 128: 50.9 and 46.1).
 struct TileCost {
     int rows_m, rows_n, step, fixed, step2, fixed2;  // step2, fixed2: two of them (0: one a CU)
@@ -436,8 +415,10 @@ constexpr int kCus = 256;
 constexpr TileCost kTiles[] = {{256, 256, 205, 300, 0, 0},
                                {256, 128, 150, 200, 0, 0},
                                {128, 128, 103, 100, 155, 250},
-                               {128, 128, 80, 200, 0, 0},
-                               {64, 64, 48, 150, 66, 200}};
+                               {128, 128, 80, 500, 0, 0},
+                               {64, 64, 48, 150, 85, 200},
+                               {64, 128, 85, 150, 0, 0},
+                               {32, 64, 46, 20, 88, 200}};
 
 int best_tile(int64_t M, int64_t N, int64_t K) {
     const int64_t steps = (K + 2 * kBK - 1) / (2 * kBK);
@@ -467,7 +448,9 @@ int gemm_tile(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_
         case 1: return launch<8, 4, 2, 2, 2, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
         case 2: return launch<4, 4, 2, 2, 2, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
         case 3: return launch<4, 4, 2, 2, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
-        default: return launch<2, 2, 2, 2, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+        case 4: return launch<2, 2, 2, 2, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+        case 5: return launch<4, 2, 1, 4, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+        default: return launch<2, 1, 1, 4, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
     }
 }
 

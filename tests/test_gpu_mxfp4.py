@@ -152,7 +152,8 @@ def _mx(rng, rows, cols, lo=120, hi=134):
 W4A4_SHAPES = [(1, 1, 32), (1, 16, 64), (2, 33, 96), (5, 100, 160), (16, 16, 128), (17, 31, 288), (33, 257, 512),
                (64, 300, 1024), (65, 129, 1056), (100, 513, 4096), (128, 256, 2048), (255, 260, 544),
                (256, 256, 256), (257, 511, 768), (300, 1000, 1312), (513, 1025, 320), (1, 4096, 4096),
-               (8, 6144, 4096), (32, 1100, 14336), (700, 264, 96)]
+               (8, 6144, 4096), (32, 1100, 14336), (700, 264, 96), (20, 8200, 288), (33, 9001, 1024), (64, 12300, 544),
+              (50, 28672, 256), (5, 13000, 2080), (130, 4100, 1600), (1100, 3000, 1056), (2100, 2100, 2112), (64, 8192, 992)]
 
 
 @pytest.mark.parametrize("out", ["bfloat16", "float32"])
@@ -217,7 +218,8 @@ A16_SHAPES = [(1, 1, 32), (1, 17, 64), (3, 40, 96), (1, 4096, 4096), (7, 1000, 1
               (16, 16, 128), (17, 515, 544), (31, 96, 2048), (33, 129, 320), (48, 600, 1024), (64, 1100, 14336),
               (65, 300, 800), (128, 260, 4096), (130, 33, 288), (1, 28672, 512), (1, 77, 2048), (1, 1000, 2080),
               (1, 130, 16384), (1, 50, 16416), (1, 301, 10240), (40, 4097, 320), (20, 9000, 288), (60, 17000, 256),
-              (33, 28672, 256), (200, 8200, 96)]
+              (33, 28672, 256), (200, 8200, 96), (128, 6144, 384), (500, 4100, 640),
+              (64, 20003, 256), (300, 1000, 1152), (32, 28672, 128)]
 
 
 @pytest.mark.parametrize("M,N,K", A16_SHAPES)
