@@ -209,7 +209,7 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
         }
         multiply(w, x, wsc, xsc, std::integral_constant<int, 0>{});
     }
-    settle();
+    settle(acc);
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -309,7 +309,7 @@ int check_gemm(const char* fn, int64_t M, int64_t N, int64_t K, const void* y) {
     if (M == 0 || N == 0) return KC_SUCCESS;
     if (!y) return set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
     // 32-bit lane offsets (256 rows of K / 2 bytes), tile counts and launch sizes
-    if (K > (1 << 24) || M > (1 << 30) || N > (1 << 30) || ((M + 15) / 16) > (int64_t{1} << 26) / ((N + 15) / 16))
+    if (K > (1 << 24) || M > (1 << 28) || N > (1 << 28) || ((M + 15) / 16) > (int64_t{1} << 26) / ((N + 15) / 16))
         return set_error(KC_ERR_INVALID_ARGUMENT, "%s: M=%lld N=%lld K=%lld too large", fn, (long long)M, (long long)N,
                          (long long)K);
     return KC_SUCCESS;

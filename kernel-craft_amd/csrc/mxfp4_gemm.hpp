@@ -1,6 +1,8 @@
 // mxfp4_gemm.hpp -- host helpers shared by the MXFP4 products.
 #pragma once
 
+#include <atomic>
+
 #include "mxfp4.hpp"
 
 namespace kc {
@@ -29,9 +31,32 @@ __device__ __forceinline__ void mfma(f32x4& acc, u32x4 a, u32x4 b, uint32_t sa, 
 #undef KC_MFMA
 }
 
-// The last results are in their registers (the compiler does not know the
-// latency of the assembly above).
-__device__ __forceinline__ void settle() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
+// Waits until the last results are in their registers (the compiler does not know the
+// latency of the assembly above): every later use of an accumulator depends on this.
+template <int I, int J>
+__device__ __forceinline__ void settle(f32x4 (&acc)[I][J]) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < J; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// Lets KERNEL use `bytes` of dynamic LDS on the current device (once per device: the
+// limit is the loaded function's).
+template <auto KERNEL>
+int raise_lds_limit(const char* fn, int bytes) {
+    static std::atomic<uint64_t> done{0};
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess) return set_error(KC_ERR_HIP, "%s: no current device", fn);
+    const uint64_t bit = uint64_t{1} << (device & 63);
+    if (done.load(std::memory_order_acquire) & bit) return KC_SUCCESS;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+        hipSuccess)
+        return set_error(KC_ERR_HIP, "%s: cannot raise the LDS limit", fn);
+    done.fetch_or(bit, std::memory_order_release);
+    return KC_SUCCESS;
+}
 
 // Shapes of Y [M, N] = X [M, K] W [N, K]^T; y checked where Y has elements.
 int check_gemm(const char* fn, int64_t M, int64_t N, int64_t K, const void* y);

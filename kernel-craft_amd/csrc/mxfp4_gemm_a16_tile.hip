@@ -189,9 +189,8 @@ template <int MT>
 int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t* x, uint16_t* y, int M, int N, int K,
            hipStream_t stream) {
     using S = Shape<MT>;
-    static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_mxfp4_a16_tile_kernel<MT>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) == hipSuccess;
-    if (!ok) return kc::set_error(KC_ERR_HIP, "%s: cannot raise the LDS limit", fn);
+    const int st = raise_lds_limit<gemm_mxfp4_a16_tile_kernel<MT>>(fn, S::kLds);
+    if (st != KC_SUCCESS) return st;
     const dim3 grid((N + kRowsN - 1) / kRowsN, (M + 16 * MT - 1) / (16 * MT));
     gemm_mxfp4_a16_tile_kernel<MT><<<grid, kThreads, S::kLds, stream>>>(qw, sw, x, y, M, N, K,
                                                                         N % 4 == 0 && kc::aligned(y, 8));

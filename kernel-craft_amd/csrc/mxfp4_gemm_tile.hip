@@ -333,7 +333,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
     // D of a 16 x 16 tile: lane (j, g) holds columns n = 4 g + v of row m = j.
     // bf16 rows are put together in the wave's own LDS, 16 rows of 16 TN columns at a
     // time, and leave in pieces of 16 bytes per lane.
-    settle();
+    settle(acc);
     const int64_t mw = m0 + 16 * TM * wm, nw = n0 + 16 * TN * wn;
     if constexpr (YBF16 && TN > 1) {
         if (vec) {
@@ -391,9 +391,8 @@ template <int TM, int TN, int WGM, int WGN, int ST, bool YBF16>
 int launch(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int64_t M,
            int64_t N, int64_t K, hipStream_t stream) {
     using S = Shape<TM, TN, WGM, WGN, ST>;
-    static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(gemm_mxfp4_tile_kernel<TM, TN, WGM, WGN, ST, YBF16>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds) == hipSuccess;
-    if (!ok) return kc::set_error(KC_ERR_HIP, "%s: cannot raise the LDS limit", fn);
+    const int st = raise_lds_limit<gemm_mxfp4_tile_kernel<TM, TN, WGM, WGN, ST, YBF16>>(fn, S::kLds);
+    if (st != KC_SUCCESS) return st;
     const int64_t tm = (M + S::kRowsM - 1) / S::kRowsM, tn = (N + S::kRowsN - 1) / S::kRowsN;
     const bool vec = YBF16 ? N % 8 == 0 && kc::aligned(y, 16) : N % 4 == 0 && kc::aligned(y, 16);
     gemm_mxfp4_tile_kernel<TM, TN, WGM, WGN, ST, YBF16><<<static_cast<unsigned>(tm * tn), S::kThreads, S::kLds, stream>>>(

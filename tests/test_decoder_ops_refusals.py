@@ -128,6 +128,9 @@ def _rp(**kw):
     (lambda L: L.kc_gemm_mxfp4_bf16(P, P, P, P, 4, 4, 16, None), "multiple of 32"),
     (lambda L: L.kc_gemm_mxfp4_bf16(P, P, ODD, P, 4, 4, 64, None), "aligned"),
     (lambda L: L.kc_gemm_mxfp4_bf16(P, P, P, None, 4, 4, 64, None), "null"),
+    (lambda L: L.kc_gemm_mxfp4_bf16(P, P, P, P, 1 << 21, 4, 64, None), "too large"),
+    (lambda L: L.kc_gemm_mxfp4_bf16(P, P, P, P, 4, 4, 1 << 25, None), "too large"),
+    (lambda L: L.kc_gemm_mxfp4_w4a4_f32(P, P, P, P, P, 4, 1 << 29, 64, None), "too large"),
     (lambda L: L.kc_qk_norm_rope_bf16(P, 256, P, 256, P, P, None, 1e-6, 3, 2, 2, 64, P, P, None), "null rope"),
     (lambda L: L.kc_qk_norm_rope_bf16(P, 256, P, 256, P, P, _rp(rotary_dim=66), 1e-6, 3, 2, 2, 64, P, P, None),
      "rotary_dim"),
