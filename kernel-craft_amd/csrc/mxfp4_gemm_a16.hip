@@ -9,18 +9,27 @@
 // only rounding is that of Y.  Weights outside bf16's range (scale bytes under 2
 // or over 252 with large codes) are rounded or overflow as bf16 values do.
 //
-// Bound by the weight stream (0.53 bytes a weight).  A workgroup of KW waves owns
-// RT tiles of 16 weight rows and MT tiles of 16 tokens; wave w takes K steps w,
-// w + KW, ... of 256 values, and the partial sums meet in LDS in a fixed order.
-// Tokens past 16 MT are further workgroups.
+// Bound by the weight stream (0.53 bytes a weight) on wide layers (M 13, N 28672, K 4096
+// 13.8 us, 4.7 TB/s), by the reads of X, one for every RT tiles of rows, on narrow ones.
+// A workgroup of KW waves owns RT tiles of 16 weight rows and MT tiles of 16 tokens; K
+// advances in spans of four steps of 256 values, which the waves take in turn, and
+// their partial sums meet in LDS in a fixed order.  Tokens past 16 MT are further
+// workgroups.  KW is 8 where one or two tiles of rows leave room (M 13, N 4096,
+// K 14336 15.7 -> 15.1 us), 4 elsewhere (M 13, N 28672, K 4096 with four tiles 17.2 at
+// 8, 15.5 at 4).  The registers hold DX steps of X: two where they fit (N 11008,
+// K 5120 13.7 -> 12.5 us), one for the two smallest tiles (no gain) and the largest.
 //
 // A weight load carries 8 whole rows of a step (128 bytes, a cache line each); a
 // lane and its neighbour l ^ 1 exchange one 16-byte chunk, after which lane
 // (i, kb) holds blocks 2 kb and 2 kb + 1 of row row_of(i) = i / 2 + 8 (i % 2).  A
 // 4 x 4 transpose of dwords over the lanes l % 16 (two permlane swaps) then
 // leaves dword g of block b with lane (i, g): the 8 values the matrix core wants from
-// it when X is read in its own order, 64 neighbouring bytes of each row.
+// it when X is read in its own order, 64 neighbouring bytes of each row.  The 32 scale
+// bytes of a row's span come with one load of 8 bytes, step kb's, to lane (i, kb), and
+// two more swaps hand a step's to all of the row's lanes (a load of 8 bytes a step
+// costs the load unit as many lines as the codes: M 13, N 28672, K 4096 16.5 us).
 #include <algorithm>
+#include <type_traits>
 
 #include "mxfp4_gemm.hpp"
 
@@ -63,10 +72,22 @@ __device__ __forceinline__ bf16x8 decode(uint32_t c, uint32_t b) {
     return bf16x8{p.x, p.y, q.x, q.y, r.x, r.y, t.x, t.y};
 }
 
+// v of the lanes (i, S), in all lanes (i, .).
+template <int S>
+__device__ __forceinline__ uint32_t of_group(uint32_t v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);  // groups 0, 1 twice; 2, 3 twice
+    const uint32_t h = r[S >> 1];
+    const auto q = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+    return q[S & 1];
+}
+
 template <int MT, int RT, int KW, int DX>
 __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_a16_kernel(const uint8_t* __restrict__ qw, const uint8_t* __restrict__ sw,
                                                                  const uint16_t* __restrict__ x, uint16_t* __restrict__ y,
                                                                  int M, int N, int K, bool vec) {
+    // More would not fit a wave's 512 registers, and a variant that spills is not to be
+    // used: a spilled half of an address has been left out of its reload.
+    static_assert(RT * MT <= 21 && RT * MT * DX <= 28, "more registers than a wave has");
     __shared__ f32x4 red[KW][RT * MT][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -95,23 +116,22 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_a16_kernel(const uint8_t* 
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int c = 0; c < MT; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int full = K / kStep;
-    const int mine = full > wave ? (full - wave + KW - 1) / KW : 0;  // K steps wave, wave + KW, ...
+    const int spans = K / (4 * kStep);
+    const int mine = spans > wave ? (spans - wave + KW - 1) / KW : 0;  // spans wave, wave + KW, ...
 
     // The weights of one step; a tile's registers take the next step's as soon as
     // they have been decoded, so that RT - 1 tiles are always on their way.
     u32x4 wf[RT][2];
-    u32x2 ws[RT];
+    u32x2 ws[RT];                // scales of the span: step kb's
     u32x4 xf[DX][MT][8];
-    auto load_w = [&](int r, int j) {
-        const int step = wave + KW * min(j, mine - 1);
+    auto load_w = [&](int r, int step) {
         const uint8_t* wp = wbase + step * kBK;
         wf[r][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][0]));
         wf[r][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + woff[r][1]));
-        __builtin_memcpy(&ws[r], wsbase + 8 * step + wsoff[r], 8);
     };
-    auto load_x = [&](int slot, int j) {
-        const uint16_t* xp = xbase + (wave + KW * min(j, mine - 1)) * kStep;
+    auto load_scales = [&](int r, int span) { __builtin_memcpy(&ws[r], wsbase + 32 * span + wsoff[r] + 8 * kb, 8); };
+    auto load_x = [&](int slot, int step) {
+        const uint16_t* xp = xbase + step * kStep;
 #pragma unroll
         for (int c = 0; c < MT; ++c)
 #pragma unroll
@@ -144,40 +164,44 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_a16_kernel(const uint8_t* 
         __builtin_amdgcn_sched_barrier(0);
     };
     if (mine > 0) {
-        load_x(0, 0);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) load_w(r, 0);
-        if (DX == 2) load_x(DX - 1, 1);
+        for (int r = 0; r < RT; ++r) load_scales(r, wave);
+#pragma unroll
+        for (int d = 0; d < DX; ++d) load_x(d, 4 * wave + d);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) load_w(r, 4 * wave);
         __builtin_amdgcn_sched_barrier(0);
-        auto step = [&](int slot, int j) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const u32x2 sc = ws[r];
-                multiply(r, wf[r], sc, xf[slot], [&] { load_w(r, j + 1); });
-            }
-            load_x(slot, j + DX);
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        int j = 0;
-        for (; j + DX < mine; j += DX) {
-#pragma unroll
-            for (int d = 0; d < DX; ++d) step(d, j + d);
-        }
-#pragma unroll
-        for (int d = 0; d < DX; ++d)
-            if (j + d < mine) {
+        // one span; `more`: the next one's loads follow its own
+        auto span = [&](int at, auto mc) {
+            constexpr bool more = decltype(mc)::value;
+            const int next = at + KW;
+            auto step = [&](auto sc) {
+                constexpr int s = decltype(sc)::value;
 #pragma unroll
                 for (int r = 0; r < RT; ++r) {
-                    const u32x2 sc = ws[r];
-                    multiply(r, wf[r], sc, xf[d], [&] {
-                        if (j + d + 1 < mine) load_w(r, j + d + 1);
+                    const u32x2 scale = {of_group<s>(ws[r].x), of_group<s>(ws[r].y)};
+                    multiply(r, wf[r], scale, xf[s % DX], [&] {
+                        if constexpr (s < 3) load_w(r, 4 * at + s + 1);
+                        else if constexpr (more) load_w(r, 4 * next);
+                        if constexpr (s == 3 && more) load_scales(r, next);
                     });
                 }
-            }
+                if constexpr (s + DX < 4) load_x(s % DX, 4 * at + s + DX);
+                else if constexpr (more) load_x(s % DX, 4 * next + s + DX - 4);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            step(std::integral_constant<int, 0>{});
+            step(std::integral_constant<int, 1>{});
+            step(std::integral_constant<int, 2>{});
+            step(std::integral_constant<int, 3>{});
+        };
+        for (int j = 0; j + 1 < mine; ++j) span(wave + KW * j, std::true_type{});
+        span(wave + KW * (mine - 1), std::false_type{});
     }
-    if (K % kStep != 0 && wave == full % KW) {
-        // The partial last step: zeros past K in both operands.
-        const int valid = K - full * kStep;
+    // The steps behind the last whole span, one a wave: zeros past K in both operands.
+    for (int step = 4 * spans; step * kStep < K; ++step) {
+        if (step % KW != wave) continue;
+        const int valid = K - step * kStep;
         u32x4 w[RT][2], xv[MT][8];
         u32x2 sc[RT];
         const u32x4 z{0u, 0u, 0u, 0u};
@@ -185,13 +209,13 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_a16_kernel(const uint8_t* 
         for (int r = 0; r < RT; ++r) {
             w[r][0] = w[r][1] = z;
             if (32 * chunk < valid) {
-                w[r][0] = *reinterpret_cast<const u32x4*>(wbase + full * kBK + woff[r][0]);
-                w[r][1] = *reinterpret_cast<const u32x4*>(wbase + full * kBK + woff[r][1]);
+                w[r][0] = *reinterpret_cast<const u32x4*>(wbase + step * kBK + woff[r][0]);
+                w[r][1] = *reinterpret_cast<const u32x4*>(wbase + step * kBK + woff[r][1]);
             }
             uint32_t d[2] = {0, 0};
 #pragma unroll
             for (int b = 0; b < 8; ++b)
-                if (32 * b < valid) d[b >> 2] |= static_cast<uint32_t>(wsbase[wsoff[r] + 8 * full + b]) << (8 * (b & 3));
+                if (32 * b < valid) d[b >> 2] |= static_cast<uint32_t>(wsbase[wsoff[r] + 8 * step + b]) << (8 * (b & 3));
             sc[r] = u32x2{d[0], d[1]};
         }
 #pragma unroll
@@ -199,7 +223,7 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_a16_kernel(const uint8_t* 
 #pragma unroll
             for (int b = 0; b < 8; ++b) {
                 xv[c][b] = z;
-                if (32 * b < valid) xv[c][b] = *reinterpret_cast<const u32x4*>(xbase + full * kStep + xoff[c] + 32 * b);
+                if (32 * b < valid) xv[c][b] = *reinterpret_cast<const u32x4*>(xbase + step * kStep + xoff[c] + 32 * b);
             }
 #pragma unroll
         for (int r = 0; r < RT; ++r) multiply(r, w[r], sc[r], xv, [] {});
@@ -247,22 +271,21 @@ int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t*
 
 // Tokens (tiles of 16) and weight rows (tiles of 16) per workgroup, and what a
 // workgroup takes in hundredths of a microsecond per step of 256 values and beside
-// the steps, with every CU holding one (K 4096 and 14336).  More rows share the
-// reads of X, more tokens those of the weights and their decoding, fewer of both
-// fill the CUs: M 64, N 4096, K 14336 54 us with all tokens and one row tile, 28
-// with one tile of tokens and four of rows; M 128, N 6144, K 4096 20 with 2 and 7, 48
-// with 4 and 1; M 64, N 28672, K 4096 31 with 4 and 7, 63 with 1 and 7.
+// the steps, with every CU holding one (fitted to K 4096, 8192 and 14336).  More rows
+// share the reads of X, more tokens those of the weights and their decoding, fewer of
+// both fill the CUs: M 13, N 28672, K 4096 13.8 us with 1 and 7, 15.5 with 1 and 4, 26.6
+// with 1 and 1; M 13, N 4096, K 14336 15.1 with 1 and 1, 23.4 with 1 and 4; M 64, same
+// N and K 24.8 with 1 and 4, 37.3 with 2 and 4, 62 with 3 and 7; M 32, N 28672, K 4096
+// 18.6 with 2 and 7, 30.4 with 1 and 4.
 // The last three are the kernel of mxfp4_gemm_a16_tile.hip (128 rows; K a multiple of
-// 128): M 32, N 28672, K 4096 20.4 -> 19.0 us, M 64 30.7 -> 24.5, M 128 59 -> 44; M 128,
-// N 6144 20.4 -> 16.0; M 512, N 4096 44 -> 23; M 2048 144 -> 90.
+// 128): M 64, N 28672, K 4096 24 us against 36 with 2 and 7; M 128 44 (59 before).
 struct Cost {
     int mt, rt, step, fixed;
 };
 constexpr int kCus = 256;
 constexpr int kTileRt = 8;  // 128 rows: the other kernel
-constexpr Cost kCosts[] = {{1, 1, 20, 300}, {1, 2, 31, 320}, {1, 4, 43, 390}, {1, 7, 70, 410}, {2, 1, 48, 310}, {2, 2, 53, 300},
-                           {2, 4, 62, 450}, {2, 7, 86, 470}, {3, 7, 107, 650}, {4, 2, 95, 460}, {4, 4, 105, 600}, {4, 7, 128, 830},
-                           {2, kTileRt, 100, 200}, {3, kTileRt, 103, 300}, {4, kTileRt, 115, 500}};
+constexpr Cost kCosts[] = {{1, 1, 22, 260}, {1, 2, 27, 265}, {1, 4, 47, 200}, {1, 7, 85, 100}, {2, 4, 64, 310}, {2, 7, 98, 250},
+                           {3, 7, 100, 370}, {2, kTileRt, 100, 300}, {3, kTileRt, 103, 300}, {4, kTileRt, 115, 500}};
 
 int best(int M, int N, int K, bool tile) {
     const int64_t steps = (K + kStep - 1) / kStep;
@@ -297,18 +320,13 @@ extern "C" int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw, cons
     switch (best(m, n, k, k % 128 == 0 && kc::aligned(d_sw, 4))) {
         case 0: return launch<1, 1, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         case 1: return launch<1, 2, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 2: return launch<1, 4, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 3: return launch<1, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 4: return launch<2, 1, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 5: return launch<2, 2, 8, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 6: return launch<2, 4, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 7: return launch<2, 7, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 8: return launch<3, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 9: return launch<4, 2, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 10: return launch<4, 4, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 11: return launch<4, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 12: return kc::mx::gemm_a16_tile(fn, 2, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        case 13: return kc::mx::gemm_a16_tile(fn, 3, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 2: return launch<1, 4, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 3: return launch<1, 7, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 4: return launch<2, 4, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 5: return launch<2, 7, 4, 2>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 6: return launch<3, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 7: return kc::mx::gemm_a16_tile(fn, 2, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 8: return kc::mx::gemm_a16_tile(fn, 3, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         default: return kc::mx::gemm_a16_tile(fn, 4, d_qw, d_sw, d_x, d_y, m, n, k, stream);
     }
 }
