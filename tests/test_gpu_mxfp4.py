@@ -219,7 +219,10 @@ A16_SHAPES = [(1, 1, 32), (1, 17, 64), (3, 40, 96), (1, 4096, 4096), (7, 1000, 1
               (65, 300, 800), (128, 260, 4096), (130, 33, 288), (1, 28672, 512), (1, 77, 2048), (1, 1000, 2080),
               (1, 130, 16384), (1, 50, 16416), (1, 301, 10240), (40, 4097, 320), (20, 9000, 288), (60, 17000, 256),
               (33, 28672, 256), (200, 8200, 96), (128, 6144, 384), (500, 4100, 640),
-              (64, 20003, 256), (300, 1000, 1152), (32, 28672, 128)]
+              (64, 20003, 256), (300, 1000, 1152), (32, 28672, 128),
+              # several spans of 1024 a wave and a tail, in every tile shape
+              (5, 300, 9248), (5, 4200, 9248), (13, 9000, 5152), (9, 17000, 5152), (20, 9000, 5152),
+              (20, 17000, 5152), (48, 17000, 5152)]
 
 
 @pytest.mark.parametrize("M,N,K", A16_SHAPES)
