@@ -3,7 +3,8 @@
 // packed batch, sequence b with cu_seqlens[b] <= t < cu_seqlens[b + 1] and
 // position t - cu_seqlens[b] in it, page block_table[b][position / page_size].
 //
-// Bound by memory: 1 (FP8) or 0.53 (MXFP4) bytes in and 2 or 4 out per value.
+// Bound by memory: 1 (FP8) or 0.53 (MXFP4) bytes in and 2 or 4 out per value (43 000
+// tokens of 8 heads of 128, FP8 to bf16, keys and values: 264 MB in 53 us, 5.0 TB/s).
 // A workgroup takes a tile of tokens: its first threads find one token's slot
 // each (a binary search of cu_seqlens, in LDS up to 1023 sequences, all searches of
 // the tile at once instead of one before every row), then all threads walk the tile's rows in units of

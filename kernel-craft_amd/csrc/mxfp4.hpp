@@ -56,13 +56,6 @@ __device__ __forceinline__ uint32_t absmax_bits_bf16(u32x4 v) {
     return static_cast<uint32_t>(m.x > m.y ? m.x : m.y) << 16;
 }
 
-__device__ __forceinline__ uint32_t absmax_bits_f32(f32x4 a, f32x4 b) {
-    auto mag = [](float f) { return __float_as_uint(f) & 0x7FFFFFFFu; };
-    const uint32_t m0 = max(max(mag(a.x), mag(a.y)), max(mag(a.z), mag(a.w)));
-    const uint32_t m1 = max(max(mag(b.x), mag(b.y)), max(mag(b.z), mag(b.w)));
-    return max(m0, m1);
-}
-
 // The same of 4 fp32 values as words.
 __device__ __forceinline__ uint32_t absmax_bits_f32(u32x4 v) {
     constexpr uint32_t m = 0x7FFFFFFFu;

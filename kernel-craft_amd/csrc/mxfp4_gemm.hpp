@@ -65,7 +65,8 @@ int check_gemm(const char* fn, int64_t M, int64_t N, int64_t K, const void* y);
 template <bool YBF16>
 int fill_zero(const char* fn, void* y, int64_t n, hipStream_t stream);
 
-// M > 64 (mxfp4_gemm_tile.hip); arguments checked by the caller, K > 0.
+// More rows than a decode batch (mxfp4_gemm_tile.hip); arguments checked by the caller,
+// K > 0.
 template <bool YBF16>
 int gemm_tile(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int64_t M,
               int64_t N, int64_t K, hipStream_t stream);

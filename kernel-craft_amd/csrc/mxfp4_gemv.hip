@@ -12,11 +12,11 @@
 // multiplied with the block's scale, a power of two.  The lanes meet in DPP sums, the
 // waves in LDS.
 //
-// Measured (us, against the matrix-core kernel for one token): N 28672, K 4096 11.5
-// and 15.5 (62 MB; 10.4 at 6 TB/s); K 8192 22.4 and 29.8; N 4096, K 4096 4.0 and 4.6,
-// K 14336 8.1 and 9.8; with a block per lane missing (K 1024) 3.2 and 2.4, so K under
-// 2048 stays there, and so do two tokens (15.8 and 15.6 us: the sums over lanes cost
-// as much as the dot products).  Two rows a wave 12.4 us, eight 13.3, sixteen 16.9.
+// Measured (us, against the matrix-core kernel for one token): N 28672, K 4096 12.3
+// and 13.5 (62 MB; 10.4 at 6 TB/s); K 8192 24.3 and 29.6; K 2048 8.0 and 9.6; N 4096, K 4096
+// 4.4 and 5.1, K 14336 9.4 and 10.2; with a block per lane missing (K 1024) 3.2 and 2.4, so
+// K under 2048 stays there, and so do two tokens (15.8 and 13.2 us: the sums over lanes
+// cost as much as the dot products).  Two rows a wave 12.4 us, eight 13.3, sixteen 16.9.
 #include "mxfp4_gemm.hpp"
 
 namespace {
