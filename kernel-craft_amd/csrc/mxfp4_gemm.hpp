@@ -32,14 +32,19 @@ __device__ __forceinline__ void mfma(f32x4& acc, u32x4 a, u32x4 b, uint32_t sa, 
 }
 
 // Waits until the last results are in their registers (the compiler does not know the
-// latency of the assembly above): every later use of an accumulator depends on this.
+// latency of the assembly above): every instruction that makes an accumulator comes
+// before the wait, every later use of one behind it.
 template <int I, int J>
 __device__ __forceinline__ void settle(f32x4 (&acc)[I][J]) {
+    auto tie = [&] {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) asm volatile("" : "+a"(acc[i][j]));
+    };
+    tie();
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int j = 0; j < J; ++j) asm volatile("" : "+a"(acc[i][j]));
+    tie();
 }
 
 // Lets KERNEL use `bytes` of dynamic LDS on the current device (once per device: the
