@@ -19,11 +19,14 @@
 // written there too.  8 x 8 on four waves needs three quarters of the LDS clocks that
 // its MFMAs take, 8 x 4 on eight waves all of them.
 //
-// Scales.  Four steps need 32 scale bytes of every row.  Each thread fetches its
-// rows' bytes one group of four steps ahead, sorts them so that a lane's bytes
-// are neighbours ([row][kb][step, half]) and leaves them in LDS; a lane then
-// holds the 16 bytes a block of rows needs for four steps in two registers, and
-// the MFMA picks its byte by number.
+// Scales.  Four steps need 32 scale bytes of every row.  Their bytes come one group of
+// four steps ahead; each thread sorts its rows' so that a lane's bytes are neighbours
+// ([row][kb][step, half]) and leaves them in LDS; a lane then holds the 16 bytes a block
+// of rows needs for four steps in two registers, and the MFMA picks its byte by number.
+// They come through registers where two buffers make every step wait for all loads
+// anyway.  With more (SDMA) they go straight into LDS as the operands do: the
+// compiler's wait for a load into registers would be for every load in flight, once a
+// group (M 1000, N 4096, K 14336 45.6 -> 42.3 us, K 16384 50.7 -> 46.6).
 //
 // Tails.  Rows past M (N) load the last row and feed outputs that are not stored.
 // K past the last group of four steps runs in a loop without the overlap; chunks
@@ -55,7 +58,7 @@ __device__ __forceinline__ void lds_dma16(uint32_t voff, const void* sbase, uint
                  : "memory", "m0");
 }
 
-template <int TM_, int TN_, int WGM, int WGN, int ST>
+template <int TM_, int TN_, int WGM, int WGN, int ST, bool SDMA>
 struct Shape {
     static constexpr int kRowsM = 16 * TM_ * WGM, kRowsN = 16 * TN_ * WGN, kRows = kRowsM + kRowsN;
     static constexpr int kWaves = WGM * WGN, kThreads = 64 * kWaves;
@@ -63,18 +66,21 @@ struct Shape {
     static constexpr int kLoads = kPerM + kPerN;
     static constexpr int kStage = kRows * kBK;
     static constexpr int kScaleOff = ST * kStage;                // [row][kb][8 bytes]
-    static constexpr int kLds = kScaleOff + kRows * 32;
+    static constexpr int kRawOff = kScaleOff + kRows * 32;       // [row][32 bytes] as they come
+    static constexpr int kLds = SDMA ? kRawOff + kRows * 32 : kRawOff;
+    static constexpr int kScaleLoads = (kRows / 32 + kWaves - 1) / kWaves;  // of a wave and group
     static constexpr int kRowsPerThread = (kRows + kThreads - 1) / kThreads;
     static_assert(kPerM * 8 * kWaves == kRowsM && kPerN * 8 * kWaves == kRowsN, "whole loads per wave");
     static_assert(kLds <= 160 * 1024, "LDS");
+    static_assert(!SDMA || (ST <= 4 && kRows % 32 == 0), "scales have landed two steps on; whole loads");
 };
 
-template <int TM, int TN, int WGM, int WGN, int ST, bool YBF16>
+template <int TM, int TN, int WGM, int WGN, int ST, bool SDMA, bool YBF16>
 __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
     const uint8_t* __restrict__ qx, const uint8_t* __restrict__ sx, const uint8_t* __restrict__ qw,
     const uint8_t* __restrict__ sw, void* __restrict__ y, int64_t M, int64_t N, int K, int tiles_m, int tiles_n,
     bool vec) {
-    using S = Shape<TM, TN, WGM, WGN, ST>;
+    using S = Shape<TM, TN, WGM, WGN, ST, SDMA>;
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -155,6 +161,30 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
             }
         }
     };
+    // SDMA: the same straight into LDS, 32 rows a load, half a row per lane
+    auto dma_scales = [&](int g) {
+#pragma unroll
+        for (int u = 0; u < S::kScaleLoads; ++u) {
+            const int first = 32 * (wave + S::kWaves * u);
+            if (first >= S::kRows) continue;
+            const bool m = first < S::kRowsM;
+            const int r = first + (lane >> 1) - (m ? 0 : S::kRowsM);
+            const uint32_t at = static_cast<uint32_t>(min(r, (m ? xrows : wrows) - 1)) * static_cast<uint32_t>(blocks) + 16 * (lane & 1);
+            lds_dma16(at, (m ? sx + m0 * blocks : sw + n0 * blocks) + 32 * g,
+                      __builtin_amdgcn_readfirstlane(lds0 + S::kRawOff + 32 * first));
+        }
+    };
+    auto raw_scales = [&] {
+#pragma unroll
+        for (int t = 0; t < S::kRowsPerThread; ++t) {
+            const int r = tid + t * S::kThreads;
+            if (r < S::kRows) {
+                const u32x4* p = reinterpret_cast<const u32x4*>(lds + S::kRawOff + 32 * r);
+                sreg[t][0] = p[0];
+                sreg[t][1] = p[1];
+            }
+        }
+    };
     auto fetch_scales_partial = [&](int g) {
 #pragma unroll
         for (int t = 0; t < S::kRowsPerThread; ++t) {
@@ -226,11 +256,20 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
 
     if (groups > 0) {
         const int last = kGroup * groups - 1;
-        fetch_scales(0);
-        store_scales();
+        if constexpr (SDMA) {
+            dma_scales(0);
+        } else {
+            fetch_scales(0);
+            store_scales();
+        }
 #pragma unroll
         for (int s = 0; s < ST; ++s) dma(min(s, last));
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::kLoads * (ST - 1)) : "memory");
+        if constexpr (SDMA) {
+            raw_scales();
+            store_scales();
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
         read_scales(0);
 #pragma unroll
         for (int j = 0; j < TN; ++j) read_b(j, stage_at(0), 0);
@@ -260,13 +299,22 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
 #pragma unroll
             for (int i = 0; i < kWait; ++i) mfma_row(pc, second, i, [](int) {});
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::kLoads * (ST - 2)) : "memory");
-            if constexpr (p == 0) {
-                if (g + 1 < groups) fetch_scales(g + 1);
+            if constexpr (SDMA) {  // two barriers on the loads are among the waited for
+                if constexpr (p == 0) dma_scales(min(g + 1, groups - 1));
+                if constexpr (p == 2) {
+                    raw_scales();
+                    store_scales();
+                }
+                if constexpr (p == 3) read_scales(0);
+            } else {
+                if constexpr (p == 0) {
+                    if (g + 1 < groups) fetch_scales(g + 1);
+                }
+                if constexpr (p == 1) {
+                    if (g + 1 < groups) store_scales();
+                }
+                if constexpr (p == 2) read_scales(0);
             }
-            if constexpr (p == 1) {
-                if (g + 1 < groups) store_scales();
-            }
-            if constexpr (p == 2) read_scales(0);
             const int k0 = min(s + ST, last) * kBK;
             const uint32_t st = stage_lds(s);
 #pragma unroll
@@ -387,37 +435,48 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
     }
 }
 
-template <int TM, int TN, int WGM, int WGN, int ST, bool YBF16>
-int launch(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int64_t M,
-           int64_t N, int64_t K, hipStream_t stream) {
-    using S = Shape<TM, TN, WGM, WGN, ST>;
-    const int st = raise_lds_limit<gemm_mxfp4_tile_kernel<TM, TN, WGM, WGN, ST, YBF16>>(fn, S::kLds);
+template <int TM, int TN, int WGM, int WGN, int ST, bool SDMA, bool YBF16>
+int launch_tile(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int64_t M,
+                int64_t N, int64_t K, hipStream_t stream) {
+    using S = Shape<TM, TN, WGM, WGN, ST, SDMA>;
+    const int st = raise_lds_limit<gemm_mxfp4_tile_kernel<TM, TN, WGM, WGN, ST, SDMA, YBF16>>(fn, S::kLds);
     if (st != KC_SUCCESS) return st;
     const int64_t tm = (M + S::kRowsM - 1) / S::kRowsM, tn = (N + S::kRowsN - 1) / S::kRowsN;
     const bool vec = YBF16 ? N % 8 == 0 && kc::aligned(y, 16) : N % 4 == 0 && kc::aligned(y, 16);
-    gemm_mxfp4_tile_kernel<TM, TN, WGM, WGN, ST, YBF16><<<static_cast<unsigned>(tm * tn), S::kThreads, S::kLds, stream>>>(
+    gemm_mxfp4_tile_kernel<TM, TN, WGM, WGN, ST, SDMA, YBF16><<<static_cast<unsigned>(tm * tn), S::kThreads, S::kLds, stream>>>(
         qx, sx, qw, sw, y, M, N, static_cast<int>(K), static_cast<int>(tm), static_cast<int>(tn), vec);
     return kc::check_launch(fn);
+}
+
+template <int TM, int TN, int WGM, int WGN, int ST, bool YBF16>
+int launch(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int64_t M,
+           int64_t N, int64_t K, hipStream_t stream) {
+    if constexpr (ST > 2) {
+        if (K % (4 * kBlock) == 0 && kc::aligned(sx, 4) && kc::aligned(sw, 4))
+            return launch_tile<TM, TN, WGM, WGN, ST, true, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+    }
+    return launch_tile<TM, TN, WGM, WGN, ST, false, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
 }
 
 // Tiles, and what one costs a CU in hundredths of a microsecond: per step of 256
 // values, and beside the steps (start, first loads, stores), alone on its CU and
 // as one of two.  Measured with K 1024 to 14336 on grids of 64 to 1024 tiles; the
-// least expected time wins.  Against the 256 x 256 tile: M 128, N 4096, K 4096 28.6
-// -> 7.9 us (64 x 64); M 1000, N 4096, K 14336 103 -> 44.5 (128 x 128, four buffers,
-// one a CU); M 64, N 28672, K 4096 38 -> 15.4 (64 x 128); M 65, N 4096, K 4096 7.3 (32 x 64); M 2048, N 4096, K 4096 34.4 -> 27.0 (256 x 128); M 4096, N 4096 39.7 and
-// M 300, N 28672 38.4 stay (256 x 128: 50.9 and 46.1).
+// least expected time wins (27 shapes: the fastest tile, but for 5 % on one).  Against
+// the 256 x 256 tile: M 128, N 4096, K 4096 29.1 -> 6.8 us (32 x 64); M 1000, N 4096,
+// K 14336 103 -> 42.2 (128 x 128, four buffers, one a CU); M 500, N 6144, K 4096 32.9 -> 15.0
+// (the same); M 64, N 28672, K 4096 32.0 -> 15.1 (64 x 128); M 2048, N 4096, K 4096 34.2 ->
+// 27.0 (256 x 128); M 3000, N 4096 34.6 and M 300, N 28672 38.1 stay (256 x 128: 43.5 and 46.6).
 struct TileCost {
     int rows_m, rows_n, step, fixed, step2, fixed2;  // step2, fixed2: two of them (0: one a CU)
 };
 constexpr int kCus = 256;
 constexpr TileCost kTiles[] = {{256, 256, 205, 300, 0, 0},
-                               {256, 128, 150, 200, 0, 0},
-                               {128, 128, 103, 100, 155, 250},
-                               {128, 128, 80, 500, 0, 0},
-                               {64, 64, 48, 150, 85, 200},
-                               {64, 128, 85, 150, 0, 0},
-                               {32, 64, 46, 20, 88, 200}};
+                               {256, 128, 145, 200, 0, 0},
+                               {128, 128, 91, 300, 145, 240},
+                               {128, 128, 66, 500, 0, 0},
+                               {64, 64, 35, 260, 62, 210},
+                               {64, 128, 52, 340, 0, 0},
+                               {32, 64, 30, 190, 45, 150}};
 
 int best_tile(int64_t M, int64_t N, int64_t K) {
     const int64_t steps = (K + 2 * kBK - 1) / (2 * kBK);

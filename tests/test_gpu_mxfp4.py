@@ -153,7 +153,10 @@ W4A4_SHAPES = [(1, 1, 32), (1, 16, 64), (2, 33, 96), (5, 100, 160), (16, 16, 128
                (64, 300, 1024), (65, 129, 1056), (100, 513, 4096), (128, 256, 2048), (255, 260, 544),
                (256, 256, 256), (257, 511, 768), (300, 1000, 1312), (513, 1025, 320), (1, 4096, 4096),
                (8, 6144, 4096), (32, 1100, 14336), (700, 264, 96), (20, 8200, 288), (33, 9001, 1024), (64, 12300, 544),
-              (50, 28672, 256), (5, 13000, 2080), (130, 4100, 1600), (1100, 3000, 1056), (2100, 2100, 2112), (64, 8192, 992)]
+              (50, 28672, 256), (5, 13000, 2080), (130, 4100, 1600), (1100, 3000, 1056), (2100, 2100, 2112), (64, 8192, 992),
+              # several groups of steps, K a multiple of 128 and not, on every larger tile
+              (500, 6144, 2176), (700, 5000, 2208), (300, 4096, 2176), (300, 4096, 2080), (300, 4096, 4224),
+              (300, 4096, 4128), (300, 28672, 2112), (400, 2100, 2176)]
 
 
 @pytest.mark.parametrize("out", ["bfloat16", "float32"])
@@ -180,6 +183,22 @@ def test_w4a4_scales(gpu, ops, M, N, K):
     assert (np.abs(_f64(y) - exact) <= K * 2.0 ** -23 * size).all()
     y = ops.mxfp4_gemm_w4a4(*args)
     assert (np.abs(_f64(y) - exact) <= K * 2.0 ** -23 * size + 2.0 ** -8 * np.abs(exact)).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 300, 2176), (100, 513, 2176), (300, 4096, 2176), (500, 6144, 2176), (40, 9000, 4224)])
+def test_products_with_scales_at_odd_addresses(gpu, ops, M, N, K):
+    """Codes must be aligned, scale bytes need not be.  W4A4 sums in one order
+    wherever they lie; bf16 activations may take another kernel."""
+    rng = np.random.default_rng(M + N + K)
+    (qx, sx), (qw, sw) = _mx(rng, M, K), _mx(rng, N, K)
+    x, w = _bf16(gpu, rng.standard_normal((M, K))), ref.values(qw, sw)
+    exact, size = _f64(x) @ w.T, np.abs(_f64(x)) @ np.abs(w).T
+    qx, sx, qw, sw = [_t(gpu, a) for a in (qx, sx, qw, sw)]
+    y = ops.mxfp4_gemm_w4a4(qx, sx, qw, sw)
+    for by in (1, 2, 3):
+        assert gpu.equal(ops.mxfp4_gemm_w4a4(qx, _shift(gpu, sx, by), qw, _shift(gpu, sw, by)), y)
+        a16 = ops.mxfp4_gemm_bf16(qw, _shift(gpu, sw, by), x)
+        assert (np.abs(_f64(a16) - exact) <= K * 2.0 ** -23 * size + 2.0 ** -8 * np.abs(exact)).all()
 
 
 @pytest.mark.parametrize("M", [1, 40, 300])
