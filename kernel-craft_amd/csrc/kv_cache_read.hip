@@ -3,12 +3,13 @@
 // packed batch, sequence b with cu_seqlens[b] <= t < cu_seqlens[b + 1] and
 // position t - cu_seqlens[b] in it, page block_table[b][position / page_size].
 //
-// Bound by memory: 1 (FP8) or 0.53 (MXFP4) bytes in and 2 or 4 out per value (43 000
-// tokens of 8 heads of 128, FP8 to bf16, keys and values: 264 MB in 53 us, 5.0 TB/s).
-// A workgroup takes a tile of tokens: its first threads find one token's slot
-// each (a binary search of cu_seqlens, in LDS up to 1023 sequences, all searches of
-// the tile at once instead of one before every row), then all threads walk the tile's rows in units of
-// 8 values, four rows in flight each.
+// Bound by memory: 1 (FP8) or 0.53 (MXFP4) bytes in and 2 or 4 out per value (45 000
+// tokens of 8 heads of 128, keys and values: FP8 to bf16 50 us, 5.4 TB/s, MXFP4 34.9,
+// 6.3; FP8 to fp32 84).  A workgroup takes a tile of tokens: its first threads find one
+// token's slot each (a binary search of cu_seqlens, in LDS up to 1023 sequences, all
+// searches of the tile at once instead of one before every row), then all threads walk
+// the rows in units of 16 bytes of output, four keys and four values in flight each
+// (keys and values in workgroups of their own, each with its search: 53.5 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -21,6 +22,7 @@ using kc::kWave;
 
 constexpr int kThreads = 256;
 constexpr int kMaxTile = 64;
+constexpr int kAhead = 4;  // rows of keys, and of values, in flight per thread
 
 template <bool BF16>
 using Elem = std::conditional_t<BF16, uint16_t, float>;
@@ -60,7 +62,7 @@ __device__ __forceinline__ int64_t slot_of(const Args& p, const int32_t* cu, int
 template <bool BF16, bool FP8, bool VEC>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(const Args p) {
     __shared__ int64_t slot[kMaxTile];
-    const int which = blockIdx.y, tid = threadIdx.x;
+    const int tid = threadIdx.x;
     const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.tile;
     if (p.seqs < kStarts) {
         __shared__ int32_t starts[kStarts];
@@ -71,10 +73,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const Args p) {
         slot[tid] = slot_of(p, p.cu, t0 + tid);
     }
     __syncthreads();
-    const uint8_t* codes = p.codes[which];
-    Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out[which]);
-    constexpr int W = VEC ? 8 : 1;                 // values per unit
-    constexpr int kAhead = 4;                      // rows in flight per thread
+    constexpr int W = !VEC ? 1 : BF16 ? 8 : 4;     // values per unit: a lane writes 16 bytes
     const int units = p.kv_heads * p.D / W, per_head = p.D / W;
     // A thread keeps its unit of the row and walks the tile's tokens: the head and
     // the place in it cost two divisions a thread.
@@ -86,53 +85,66 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const Args p) {
         const int h = u / per_head, d = (u - h * per_head) * W;
         for (int tt = units <= kThreads ? first : 0; tt < p.tile; tt += kAhead * together) {
             int64_t s[kAhead];
-            u32x2 c[kAhead];
-            float sc[kAhead];
+            u32x2 c[2][kAhead];
+            float sc[2][kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
                 const int at = tt + i * together;
                 s[i] = at < p.tile ? slot[at] : kOutside;
-                c[i] = u32x2{0u, 0u};
-                sc[i] = nan;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    c[w][i] = u32x2{0u, 0u};
+                    sc[w][i] = nan;
+                }
                 if (s[i] < 0) continue;
                 const int64_t row = s[i] * p.kv_heads + h;
                 const int64_t v = row * p.D + d;
-                if constexpr (FP8) {
-                    if constexpr (VEC) c[i] = *reinterpret_cast<const u32x2*>(codes + v);
-                    else c[i].x = codes[v];
-                    sc[i] = static_cast<const float*>(p.scales[which])[row];
-                } else {
-                    if constexpr (VEC) c[i].x = *reinterpret_cast<const uint32_t*>(codes + v / 2);
-                    else c[i].x = codes[v / 2] >> (4 * (d & 1));
-                    sc[i] = scale_value(static_cast<const uint8_t*>(p.scales[which])[v / kBlock]);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint8_t* codes = p.codes[w];
+                    if constexpr (FP8) {
+                        if constexpr (W == 8) c[w][i] = *reinterpret_cast<const u32x2*>(codes + v);
+                        else if constexpr (W == 4) c[w][i].x = *reinterpret_cast<const uint32_t*>(codes + v);
+                        else c[w][i].x = codes[v];
+                        sc[w][i] = static_cast<const float*>(p.scales[w])[row];
+                    } else {
+                        if constexpr (W == 8) c[w][i].x = *reinterpret_cast<const uint32_t*>(codes + v / 2);
+                        else if constexpr (W == 4) c[w][i].x = *reinterpret_cast<const uint16_t*>(codes + v / 2);
+                        else c[w][i].x = codes[v / 2] >> (4 * (d & 1));
+                        sc[w][i] = scale_value(static_cast<const uint8_t*>(p.scales[w])[v / kBlock]);
+                    }
                 }
             }
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
                 if (s[i] == kOutside) continue;
                 const int64_t to = ((t0 + tt + i * together) * p.kv_heads + h) * p.D + d;
-                f32x4 lo, hi;
-                if constexpr (FP8) {
-                    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].x), false);
-                    const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].x), true);
-                    const auto e = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].y), false);
-                    const auto f = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c[i].y), true);
-                    lo = f32x4{a[0] * sc[i], a[1] * sc[i], b[0] * sc[i], b[1] * sc[i]};
-                    hi = f32x4{e[0] * sc[i], e[1] * sc[i], f[0] * sc[i], f[1] * sc[i]};
-                } else {
-                    decode8_f32(c[i].x, sc[i], lo, hi);
-                }
-                if constexpr (!VEC) {
-                    if constexpr (BF16) out[to] = kc::f32_to_bf16(lo.x);
-                    else out[to] = lo.x;
-                } else if constexpr (BF16) {
-                    __builtin_nontemporal_store(u32x4{kc::pack_bf16x2(lo.x, lo.y), kc::pack_bf16x2(lo.z, lo.w),
-                                                      kc::pack_bf16x2(hi.x, hi.y), kc::pack_bf16x2(hi.z, hi.w)},
-                                                reinterpret_cast<u32x4*>(out + to));
-                } else {
-                    f32x4* o = reinterpret_cast<f32x4*>(out + to);
-                    o[0] = lo;
-                    o[1] = hi;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out[w]);
+                    const u32x2 cw = c[w][i];
+                    const float f = sc[w][i];
+                    f32x4 lo, hi;
+                    if constexpr (FP8) {
+                        const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(cw.x), false);
+                        const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(cw.x), true);
+                        const auto e = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(cw.y), false);
+                        const auto g = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(cw.y), true);
+                        lo = f32x4{a[0] * f, a[1] * f, b[0] * f, b[1] * f};
+                        hi = f32x4{e[0] * f, e[1] * f, g[0] * f, g[1] * f};
+                    } else {
+                        decode8_f32(cw.x, f, lo, hi);
+                    }
+                    if constexpr (!VEC) {
+                        if constexpr (BF16) out[to] = kc::f32_to_bf16(lo.x);
+                        else out[to] = lo.x;
+                    } else if constexpr (BF16) {
+                        __builtin_nontemporal_store(u32x4{kc::pack_bf16x2(lo.x, lo.y), kc::pack_bf16x2(lo.z, lo.w),
+                                                          kc::pack_bf16x2(hi.x, hi.y), kc::pack_bf16x2(hi.z, hi.w)},
+                                                    reinterpret_cast<u32x4*>(out + to));
+                    } else {
+                        __builtin_nontemporal_store(lo, reinterpret_cast<f32x4*>(out + to));
+                    }
                 }
             }
         }
@@ -169,13 +181,16 @@ int cache_read(const char* fn, const kc_kv_cache* cache, const int32_t* table, i
     const uintptr_t in = fp8 ? 8 : 4;
     const bool vec = p.D % 8 == 0 && kc::aligned(k, 16) && kc::aligned(v, 16) && kc::aligned(p.codes[0], in) &&
                      kc::aligned(p.codes[1], in);
-    // the largest tile that still leaves 4096 of them for each of the two (larger
-    // ones end unevenly: 43 000 tokens 60.8 us at 32, 54 at 8)
-    p.tile = 8;
-    while (p.tile < kMaxTile && total / (2 * p.tile) >= 4096) p.tile *= 2;
+    // Tokens of a workgroup: what its threads take at once where 512 workgroups are left,
+    // more while 4096 are (larger ones end unevenly: 43 000 tokens 60.8 us at 32, 54 at 8,
+    // keys and values apart; one head of 128 11.0 us at 8,
+    // 8.3 at 64).
+    const int units = p.kv_heads * p.D / (!vec ? 1 : BF16 ? 8 : 4), at_once = kAhead * std::max(1, kThreads / units);
+    p.tile = 4;
+    while (p.tile < kMaxTile && total / (2 * p.tile) >= (2 * p.tile <= at_once ? 512 : 4096)) p.tile *= 2;
     const int64_t grid = (total + p.tile - 1) / p.tile;
-    if (grid > kc::kv::kMaxGrid / 2) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
-    const dim3 g(static_cast<unsigned>(grid), 2);
+    if (grid > kc::kv::kMaxGrid) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
+    const unsigned g = static_cast<unsigned>(grid);
     if (fp8 && vec) kv_read_kernel<BF16, true, true><<<g, kThreads, 0, stream>>>(p);
     else if (fp8) kv_read_kernel<BF16, true, false><<<g, kThreads, 0, stream>>>(p);
     else if (vec) kv_read_kernel<BF16, false, true><<<g, kThreads, 0, stream>>>(p);
