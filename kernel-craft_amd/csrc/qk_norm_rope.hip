@@ -552,12 +552,19 @@ int launch(const char* fn, Args& p, hipStream_t stream) {
         p.per_split = (p.groups + p.splits - 1) / p.splits;
         const int64_t grid = (p.tokens * p.splits + kWaves - 1) / kWaves;
         if (grid > kc::kv::kMaxGrid) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
-        // Nontemporal loads gain 3 to 5 % where a head is whole 128-byte lines and lose
-        // where loads share lines (D 96: 20.9 -> 28.8 us for 8192 tokens of 32 heads).
+        // Nontemporal loads gain 3 to 8 % where the heads cannot lie in the Infinity Cache
+        // (256 MB), in which a projection has just left them, and lose where they do (32 + 8
+        // bf16 heads of 128: 2048 tokens 11.7 us against 10.3 with plain loads, 4096 17.9 and
+        // 16.2, 8192 33.6 and 35.7), or where a load of a head's lanes is no whole 128-byte
+        // lines: heads of 96 (20.9 -> 28.8 us for 8192 tokens of 32), half rotations of 64
+        // bytes (heads of 64 18.4 -> 21.9).
+        const int64_t line = 128 / sizeof(Elem<BF16>);
+        const bool stream_heads = p.tokens * heads * D * static_cast<int64_t>(sizeof(Elem<BF16>)) > (int64_t{64} << 20) &&
+                                  D % line == 0 && (!NORM || p.interleaved || p.R % (2 * line) == 0);
         const unsigned blocks = static_cast<unsigned>(grid);
         constexpr int kWide = BF16 ? 8 : 4;
         if (p.width < wide) heads_kernel<BF16, 4, NORM, SINK, false><<<blocks, kThreads, 0, stream>>>(p);
-        else if (D * sizeof(Elem<BF16>) % 128 == 0) heads_kernel<BF16, kWide, NORM, SINK, true><<<blocks, kThreads, 0, stream>>>(p);
+        else if (stream_heads) heads_kernel<BF16, kWide, NORM, SINK, true><<<blocks, kThreads, 0, stream>>>(p);
         else heads_kernel<BF16, kWide, NORM, SINK, false><<<blocks, kThreads, 0, stream>>>(p);
     } else {
         const int64_t rows = p.tokens * heads, grid = (rows + kWaves - 1) / kWaves;

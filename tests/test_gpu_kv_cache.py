@@ -225,6 +225,38 @@ def test_fused_equals_the_two_calls(gpu, ops, T, Hq, Hkv, D, R, inter, dtype, fm
     assert all(gpu.equal(a, b) for a, b in zip(one, two))
 
 
+@pytest.mark.parametrize("dtype,fmt,inter", [("bfloat16", "fp8", False), ("bfloat16", "mxfp4", True),
+                                             ("float32", "fp8", True), ("float32", "mxfp4", False)])
+def test_long_batches_equal_their_parts(gpu, ops, dtype, fmt, inter):
+    """More than 64 MB of heads are read past the cache: the same bits as the batch in
+    parts, in which they are not."""
+    T, Hq, Hkv, D, parts = (9601 if dtype == "bfloat16" else 4801), 8, 20, 128, 4
+    q, k, v, gq, gk = _heads(gpu, T, Hq, Hkv, D, getattr(gpu, dtype))
+    cos, sin = _tables(gpu, 1000, D // 2)
+    pos = (gpu.arange(T, device="cuda") % 1003 - 1).int()
+    slots = gpu.randperm(T + 7, device="cuda")[:T] - 3
+    args = lambda a, b: (q[a:b], k[a:b], gq, gk, cos, sin, pos[a:b])
+    cuts = [T * i // parts for i in range(parts + 1)]
+    pieces = [ops.qk_norm_rope(*args(a, b), interleaved=inter) for a, b in zip(cuts, cuts[1:])]
+    got = ops.qk_norm_rope(*args(0, T), interleaved=inter)
+    for whole, part in zip(got, zip(*pieces)):
+        assert gpu.equal(whole.view(gpu.uint8), gpu.cat(part).view(gpu.uint8))
+    caches = []
+    for step in ("whole", "parts", "whole", "parts"):
+        cache = _pool(gpu, T // 16 + 1, 16, Hkv, D, fmt)
+        ends = [0, T] if step == "whole" else cuts
+        for a, b in zip(ends, ends[1:]):
+            if len(caches) < 2:
+                ops.qk_norm_rope_cache(q[a:b], k[a:b], v[a:b], gq, gk, cos, sin, pos[a:b], slots[a:b], *cache,
+                                       interleaved=inter)
+            else:
+                ops.kv_cache_write(k[a:b], v[a:b], slots[a:b], *cache)
+        caches.append(cache)
+    for one, other in (caches[:2], caches[2:]):
+        for a, b in zip(one, other):
+            assert gpu.equal(a.view(gpu.uint8), b.view(gpu.uint8))
+
+
 @pytest.mark.parametrize("fmt,D", [("fp8", 64), ("fp8", 33), ("mxfp4", 64)])
 def test_read_of_a_ragged_batch(gpu, ops, fmt, D):
     """Empty sequences, a page that ends inside the batch, missing pages, pages
