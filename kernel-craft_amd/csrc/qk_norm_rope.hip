@@ -79,8 +79,8 @@ struct Slot {
     typedef uint32_t Vec __attribute__((ext_vector_type(kWords)));
     Vec raw;
     template <bool STREAM = false>
-    __device__ __forceinline__ void load(const void* base, int64_t at) {
-        const Vec* p = reinterpret_cast<const Vec*>(static_cast<const Elem<BF16>*>(base) + at);
+    __device__ __forceinline__ void load(const Elem<BF16>* base, uint32_t at) {
+        const Vec* p = reinterpret_cast<const Vec*>(base + at);
         if constexpr (STREAM) raw = __builtin_nontemporal_load(p);
         else raw = *p;
     }
@@ -107,8 +107,8 @@ struct Slot {
             else raw[i] = __float_as_uint(v[i]);
         }
     }
-    __device__ __forceinline__ void store(void* base, int64_t at) const {
-        __builtin_nontemporal_store(raw, reinterpret_cast<Vec*>(static_cast<Elem<BF16>*>(base) + at));
+    __device__ __forceinline__ void store(Elem<BF16>* base, uint32_t at) const {
+        __builtin_nontemporal_store(raw, reinterpret_cast<Vec*>(base + at));
     }
 };
 
@@ -218,17 +218,21 @@ __device__ __forceinline__ Slots slots_of(int j, int lanes, int half, bool apart
     return {apart ? j + half : j, j + lanes};  // past a rotation that takes slots 0 .. 2 half - 1, or none
 }
 
-// What lane j has of head group g.
+// What lane j has of head group g: head `hh` of its tensor (EVEN: the first lane's) and `sub`
+// more, two slots.
 struct Place {
     bool live, is_q, is_v, apart;
-    int hh;
+    int hh, sub;
     Slots s;
 };
 
 // Five waves a SIMD: the fused kernels would take registers for four otherwise (8000
 // tokens with an 8-bit cache 44 -> 40 us).
-// STREAM: nontemporal loads of the heads.
-template <bool BF16, int W, bool NORM, int SINK, bool STREAM>
+// STREAM: nontemporal loads of the heads.  EVEN: a group is of one tensor, so that its
+// addresses and what becomes of it are the wave's and not each lane's (8000 tokens, FP8
+// cache 41 -> 37 us, 4-bit cache 36 -> 33: two thirds of the clocks went to vector
+// instructions).
+template <bool BF16, int W, bool NORM, int SINK, bool STREAM, bool EVEN>
 __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
     using S = Slot<BF16, W>;
     const int lane = threadIdx.x & (kWave - 1);
@@ -243,13 +247,15 @@ __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
     const int lanes = D / (2 * W);
     const bool has = j < lanes, pairs_apart = NORM && !p.interleaved;
 
+    using E = Elem<BF16>;
     auto place = [&](int g) {
         Place o;
-        const int h = g * hp + (lane >> lg);
-        o.live = has && h < n_all;
+        const int h = g * hp + (EVEN ? 0 : lane >> lg);
+        o.live = has && (EVEN || h < n_all);
         o.is_q = h < n_q;
         o.is_v = SINK != kPlain && h >= n_q + p.kv_heads;
         o.hh = o.is_q ? h : o.is_v ? h - n_q - p.kv_heads : h - n_q;
+        o.sub = EVEN ? lane >> lg : 0;
         o.apart = pairs_apart && !o.is_v;
         o.s = slots_of(j, lanes, half, o.apart, p.runs);
         return o;
@@ -259,8 +265,9 @@ __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
         a.clear();
         b.clear();
         if (o.live) {
-            const void* src = o.is_q ? p.q : o.is_v ? p.v : p.k;
-            const int64_t at = t * (o.is_q ? p.q_stride : o.is_v ? p.v_stride : p.k_stride) + static_cast<int64_t>(o.hh) * D;
+            const E* src = static_cast<const E*>(o.is_q ? p.q : o.is_v ? p.v : p.k);
+            src += t * (o.is_q ? p.q_stride : o.is_v ? p.v_stride : p.k_stride) + static_cast<int64_t>(o.hh) * D;
+            const uint32_t at = o.sub * D;
             a.template load<STREAM>(src, at + W * o.s.a);
             b.template load<STREAM>(src, at + W * o.s.b);
         }
@@ -300,12 +307,12 @@ __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
         qa.clear(), qb.clear(), ka.clear(), kb.clear();
         if (has) {
             if (p.q_heads > 0) {
-                qa.load(p.q_gamma, W * qs.a);
-                qb.load(p.q_gamma, W * qs.b);
+                qa.load(static_cast<const E*>(p.q_gamma), W * qs.a);
+                qb.load(static_cast<const E*>(p.q_gamma), W * qs.b);
             }
             if (p.kv_heads > 0) {
-                ka.load(p.k_gamma, W * qs.a);
-                kb.load(p.k_gamma, W * qs.b);
+                ka.load(static_cast<const E*>(p.k_gamma), W * qs.a);
+                kb.load(static_cast<const E*>(p.k_gamma), W * qs.b);
             }
         }
     }
@@ -336,7 +343,7 @@ __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
                     b[i] = (gb[i] * b[i]) * inv;
                 }
                 if (pairs_apart) {
-                    if (j < half) {
+                    if (p.R == D || j < half) {
 #pragma unroll
                         for (int i = 0; i < W; ++i) rotate(a[i], b[i], c[i], s[i]);
                     }
@@ -359,8 +366,8 @@ __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
         if (SINK == kPlain || (NORM && o.is_q)) {
             if (o.live) {
                 S out;
-                void* base = o.is_q ? p.q_out : p.k_out;
-                const int64_t to = (t * (o.is_q ? p.q_heads : p.kv_heads) + o.hh) * D;
+                E* base = static_cast<E*>(o.is_q ? p.q_out : p.k_out) + (t * (o.is_q ? p.q_heads : p.kv_heads) + o.hh) * D;
+                const uint32_t to = o.sub * D;
                 out.set(a);
                 out.store(base, to + W * o.s.a);
                 out.set(b);
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
             b[i] = kc::fp8::quiet(b[i]);
         }
         const bool out = o.live && !o.is_q && tok.cached;
-        const int64_t row = tok.slot * p.kv_heads + o.hh;
+        const int64_t row = tok.slot * p.kv_heads + o.hh + o.sub;
         uint8_t* codes = o.is_v ? p.v_codes : p.k_codes;
         void* scales = o.is_v ? p.v_scales : p.k_scales;
         if constexpr (SINK == kFp8) {
@@ -563,9 +570,12 @@ int launch(const char* fn, Args& p, hipStream_t stream) {
                                   D % line == 0 && (!NORM || p.interleaved || p.R % (2 * line) == 0);
         const unsigned blocks = static_cast<unsigned>(grid);
         constexpr int kWide = BF16 ? 8 : 4;
-        if (p.width < wide) heads_kernel<BF16, 4, NORM, SINK, false><<<blocks, kThreads, 0, stream>>>(p);
-        else if (stream_heads) heads_kernel<BF16, kWide, NORM, SINK, true><<<blocks, kThreads, 0, stream>>>(p);
-        else heads_kernel<BF16, kWide, NORM, SINK, false><<<blocks, kThreads, 0, stream>>>(p);
+        const bool even = (NORM ? p.q_heads : 0) % hp == 0 && p.kv_heads % hp == 0;
+        if (p.width < wide) heads_kernel<BF16, 4, NORM, SINK, false, false><<<blocks, kThreads, 0, stream>>>(p);
+        else if (stream_heads && even) heads_kernel<BF16, kWide, NORM, SINK, true, true><<<blocks, kThreads, 0, stream>>>(p);
+        else if (stream_heads) heads_kernel<BF16, kWide, NORM, SINK, true, false><<<blocks, kThreads, 0, stream>>>(p);
+        else if (even) heads_kernel<BF16, kWide, NORM, SINK, false, true><<<blocks, kThreads, 0, stream>>>(p);
+        else heads_kernel<BF16, kWide, NORM, SINK, false, false><<<blocks, kThreads, 0, stream>>>(p);
     } else {
         const int64_t rows = p.tokens * heads, grid = (rows + kWaves - 1) / kWaves;
         if (grid > kc::kv::kMaxGrid) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
