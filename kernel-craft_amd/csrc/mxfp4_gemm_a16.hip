@@ -277,15 +277,16 @@ int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t*
 // with 1 and 1; M 13, N 4096, K 14336 15.1 with 1 and 1, 23.4 with 1 and 4; M 64, same
 // N and K 24.8 with 1 and 4, 37.3 with 2 and 4, 62 with 3 and 7; M 32, N 28672, K 4096
 // 18.6 with 2 and 7, 30.4 with 1 and 4.
-// The last three are the kernel of mxfp4_gemm_a16_tile.hip (128 rows; K a multiple of
-// 128): M 64, N 28672, K 4096 24 us against 36 with 2 and 7; M 128 44 (59 before).
+// The last four are the kernel of mxfp4_gemm_a16_tile.hip (128 rows; K a multiple of
+// 128): M 64, N 28672, K 4096 24 us against 36 with 2 and 7; M 128 39 with 128 tokens, 44
+// with 64; M 2048, N 4096 78 and 88.
 struct Cost {
     int mt, rt, step, fixed;
 };
 constexpr int kCus = 256;
 constexpr int kTileRt = 8;  // 128 rows: the other kernel
 constexpr Cost kCosts[] = {{1, 1, 22, 260}, {1, 2, 27, 265}, {1, 4, 47, 200}, {1, 7, 85, 100}, {2, 4, 64, 310}, {2, 7, 98, 250},
-                           {3, 7, 100, 370}, {2, kTileRt, 100, 300}, {3, kTileRt, 103, 300}, {4, kTileRt, 115, 500}};
+                           {3, 7, 100, 370}, {2, kTileRt, 100, 300}, {3, kTileRt, 103, 300}, {4, kTileRt, 115, 500}, {8, kTileRt, 215, 480}};
 
 int best(int M, int N, int K, bool tile) {
     const int64_t steps = (K + kStep - 1) / kStep;
@@ -327,6 +328,7 @@ extern "C" int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw, cons
         case 6: return launch<3, 7, 4, 1>(fn, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         case 7: return kc::mx::gemm_a16_tile(fn, 2, d_qw, d_sw, d_x, d_y, m, n, k, stream);
         case 8: return kc::mx::gemm_a16_tile(fn, 3, d_qw, d_sw, d_x, d_y, m, n, k, stream);
-        default: return kc::mx::gemm_a16_tile(fn, 4, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        case 9: return kc::mx::gemm_a16_tile(fn, 4, d_qw, d_sw, d_x, d_y, m, n, k, stream);
+        default: return kc::mx::gemm_a16_tile(fn, 8, d_qw, d_sw, d_x, d_y, m, n, k, stream);
     }
 }
