@@ -278,15 +278,17 @@ int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t*
 // N and K 24.8 with 1 and 4, 37.3 with 2 and 4, 62 with 3 and 7; M 32, N 28672, K 4096
 // 18.6 with 2 and 7, 30.4 with 1 and 4.
 // The last four are the kernel of mxfp4_gemm_a16_tile.hip (128 rows; K a multiple of
-// 128): M 64, N 28672, K 4096 24 us against 36 with 2 and 7; M 128 39 with 128 tokens, 44
-// with 64; M 2048, N 4096 78 and 88.
+// 128): M 64, N 28672, K 4096 23 us against 36 with 2 and 7; M 128 36 with 128 tokens, 40
+// with 64; M 2048, N 4096 72 and 81; M 64, N 14336 16.5 in tiles of 32 tokens, 21.2 in one
+// of 64; M 128, N 6144 15.6 and 19.7 (18.6 with 1 and 7).
 struct Cost {
     int mt, rt, step, fixed;
 };
 constexpr int kCus = 256;
 constexpr int kTileRt = 8;  // 128 rows: the other kernel
-constexpr Cost kCosts[] = {{1, 1, 22, 260}, {1, 2, 27, 265}, {1, 4, 47, 200}, {1, 7, 85, 100}, {2, 4, 64, 310}, {2, 7, 98, 250},
-                           {3, 7, 100, 370}, {2, kTileRt, 100, 300}, {3, kTileRt, 103, 300}, {4, kTileRt, 115, 500}, {8, kTileRt, 215, 480}};
+constexpr Cost kCosts[] = {{1, 1, 22, 260}, {1, 2, 27, 265}, {1, 4, 40, 260}, {1, 7, 84, 100}, {2, 4, 64, 310}, {2, 7, 88, 250},
+                           {3, 7, 100, 370}, {2, kTileRt, 84, 150}, {3, kTileRt, 84, 250}, {4, kTileRt, 107, 130},
+                           {8, kTileRt, 175, 200}};
 
 int best(int M, int N, int K, bool tile) {
     const int64_t steps = (K + kStep - 1) / kStep;

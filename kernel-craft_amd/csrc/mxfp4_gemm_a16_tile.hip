@@ -5,18 +5,21 @@
 // A workgroup computes 16 MT TG tokens x 128 rows of W with eight waves: half of them
 // take the first blocks of every step of STEP values of K and half the others, and the
 // two halves meet in LDS at the end; the four waves of a half share the tokens in TG
-// groups and the rows.  X, the codes and the scales of a step go
-// from global memory straight into LDS through a ring of ST buffers, so every byte
-// of X is fetched once per 128 rows and no register holds a load in flight.  Rows are
-// whole in LDS (512 bytes of X, 128 of codes) with their 16-byte chunks XOR-swizzled
-// by the row: lane (i, g) then reads 16 bytes of X row i and the dword g of a block of
-// W row i, 8 values of K each, without bank conflicts, decodes the codes with their
-// scale (v_cvt_scalef32_pk_bf16_fp4) and multiplies on the bf16 matrix cores.
+// groups and the rows.  X, the codes and the scales of a step go from global memory
+// straight into LDS through a ring of ST buffers, so every byte of X is fetched once per
+// 128 rows and no register holds a load in flight.  Rows are whole in LDS (512 bytes of
+// X, 128 of codes) with their 16-byte chunks XOR-swizzled by the row: lane (i, g) then
+// reads 16 bytes of X row i and the dword g of a block of W row i, 8 values of K each,
+// without bank conflicts, decodes the codes with their scale
+// (v_cvt_scalef32_pk_bf16_fp4) and multiplies on the bf16 matrix cores.
 //
-// Bound by LDS, which every step is written to and read from: M 64, N 28672, K 4096 24 us,
-// the weights alone 10.5; M 128 39 (17.3 and 26 on 32 workgroups of 22 and 35 are left
-// without the matrix instructions, 19 and 32 without the loads).  128 tokens take half
-// the reads of W and its decoding, and steps of 128 values, since 256 leave one buffer.
+// A step's operands are read, and the loads of a later one issued, between the matrix
+// instructions of the step before: all of them ahead of the matrix instructions keep a
+// wave, which issues in order, from those until LDS has taken them (M 128, N 4096,
+// K 4096 in tiles of 64 tokens 21.8 -> 17.8 us, of 128 36 -> 30.5).  Full grids are bound by
+// the arrival of the steps (512 bytes of X a token and 128 of codes a row, 10 TB/s): M 64,
+// N 28672, K 4096 23 us, the weights alone 10.5; M 128 36.  128 tokens take half the
+// reads of W and its decoding, and steps of 128 values, since 256 leave one buffer.
 //
 // Rows past M or N load the last row and feed outputs that are not stored.  K is a
 // multiple of 128: in a last half step the second half of the waves has nothing to
@@ -108,19 +111,20 @@ __global__ __launch_bounds__(kThreads) void gemm_mxfp4_a16_tile_kernel(const uin
         wchunk[u] = 16u * (slot ^ w_swizzle(r));
     }
     const uint32_t srow = static_cast<uint32_t>(min(n0 + 16 * wave + lane / kSWords, N - 1) - n0) * blocks;
-    auto load = [&](int s, int buffer) {
-        const uint32_t st = __builtin_amdgcn_readfirstlane(lds0 + (buffer % S::ST) * S::kStage);
+    // load u of step s; then all of them
+    auto load_one = [&](int u, int s, uint32_t st) {
         const uint32_t k0 = static_cast<uint32_t>(s) * STEP;
-#pragma unroll
-        for (int u = 0; u < S::kXLoads; ++u)
+        if (u < S::kXLoads) {
             lds_dma16(xrow[u] + min(2 * k0 + xchunk[u], 2u * K - 16), xbase, st + 1024 * (S::kXLoads * wave + u));
-#pragma unroll
-        for (int u = 0; u < S::kWLoads; ++u)
-            lds_dma16(wrow[u] + min(k0 / 2 + wchunk[u], kbytes - 16), wbase, st + S::kX + 1024 * (S::kWLoads * wave + u));
-        if (lane < 16 * kSWords)
+        } else if (u < S::kXLoads + S::kWLoads) {
+            const int v = u - S::kXLoads;
+            lds_dma16(wrow[v] + min(k0 / 2 + wchunk[v], kbytes - 16), wbase, st + S::kX + 1024 * (S::kWLoads * wave + v));
+        } else if (lane < 16 * kSWords) {
             lds_dma4(srow + min(k0 / kBlock + 4 * (lane % kSWords), blocks - 4), sbase,
                      st + S::kX + S::kW + 16 * S::kSRow * wave);
+        }
     };
+    auto buffer = [&](int s) { return __builtin_amdgcn_readfirstlane(lds0 + (s % S::ST) * S::kStage); };
 
     f32x4 acc[kRT][MT];
 #pragma unroll
@@ -129,47 +133,84 @@ __global__ __launch_bounds__(kThreads) void gemm_mxfp4_a16_tile_kernel(const uin
         for (int c = 0; c < MT; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     asm volatile("" ::"s"(y), "s"(M), "s"(N));
 
-    const int last = steps - 1;
-    constexpr int kAhead = S::ST - 1;  // steps on their way while one is multiplied
-#pragma unroll
-    for (int p = 0; p < kAhead; ++p) load(min(p, last), p);
-    for (int s = 0; s < steps; ++s) {
-        // step s has landed, and everyone has read step s - 1, whose buffer is next
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::kLoads * (kAhead - 1)) : "memory");
-        load(min(s + kAhead, last), s + kAhead);
-        if (kg == 1 && static_cast<uint32_t>(s) * STEP + STEP / 2 >= static_cast<uint32_t>(K)) continue;  // nothing past K
-        const uint8_t* st = lds + (s % S::ST) * S::kStage;
+    // What a wave multiplies of a step, its half: read from LDS between the matrix
+    // instructions of the step before.
+    struct Operands {
         uint32_t sc[kRT];  // bytes of the half's blocks
-#pragma unroll
-        for (int r = 0; r < kRT; ++r) {
-            sc[r] = *reinterpret_cast<const uint32_t*>(st + S::kX + S::kW + S::kSRow * (16 * kRT * wn + 16 * r + i) +
-                                                       (kSWords == 2 ? 4 * kg : 0));
-            if constexpr (kSWords == 1) sc[r] >>= 16 * kg;
-        }
-        // every read of the step ahead of its first use
         uint32_t code[kHalf][kRT];
         bf16x8 xv[kHalf][MT];
+    };
+    auto read = [&](int b, int r, const uint8_t* st, Operands& o) {  // a share of block b
+        const int blk = kHalf * kg + b, row = 16 * kRT * wn + 16 * r + i;
+        if (b == 0)
+            o.sc[r] = *reinterpret_cast<const uint32_t*>(st + S::kX + S::kW + S::kSRow * row + (kSWords == 2 ? 4 * kg : 0));
+        o.code[b][r] = *reinterpret_cast<const uint32_t*>(st + S::kX + row * S::kWRow + 16 * (blk ^ w_swizzle(row)) + 4 * g);
+#pragma unroll
+        for (int c = r * MT / kRT; c < (r + 1) * MT / kRT; ++c)
+            o.xv[b][c] = *reinterpret_cast<const bf16x8*>(st + (16 * (MT * tg + c) + i) * S::kXRow + 16 * ((4 * blk + g) ^ i));
+    };
+    auto multiply = [&](int b, int r, const Operands& o) {
+        const bf16x8 wv = decode(o.code[b][r], (o.sc[r] >> (8 * b + (kSWords == 2 ? 0 : 16 * kg))) & 255);
+#pragma unroll
+        for (int c = 0; c < MT; ++c) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, o.xv[b][c], acc[r][c], 0, 0, 0);
+    };
+    const int last = steps - 1;
+    Operands even, odd;
+#pragma unroll
+    for (int p = 0; p < S::ST; ++p)
+#pragma unroll
+        for (int u = 0; u < S::kLoads; ++u) load_one(u, min(p, last), buffer(p));
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(S::kLoads * (S::ST - 1)) : "memory");
+#pragma unroll
+    for (int b = 0; b < kHalf; ++b)
+#pragma unroll
+        for (int r = 0; r < kRT; ++r) read(b, r, lds, even);
+    // Step s + 1 has landed and everyone holds step s in registers, so its buffer takes
+    // step s + ST.  Steps past the last load the last one.
+    auto step = [&](int s, Operands& now, Operands& next) {
+        // the compiler's wait for these reads stands here, and not behind the next ones
 #pragma unroll
         for (int b = 0; b < kHalf; ++b) {
-            const int blk = kHalf * kg + b;
 #pragma unroll
-            for (int r = 0; r < kRT; ++r) {
-                const int row = 16 * kRT * wn + 16 * r + i;
-                code[b][r] = *reinterpret_cast<const uint32_t*>(st + S::kX + row * S::kWRow + 16 * (blk ^ w_swizzle(row)) + 4 * g);
-            }
+            for (int r = 0; r < kRT; ++r) asm volatile("" : "+v"(now.code[b][r]));
 #pragma unroll
-            for (int c = 0; c < MT; ++c)
-                xv[b][c] = *reinterpret_cast<const bf16x8*>(st + (16 * (MT * tg + c) + i) * S::kXRow + 16 * ((4 * blk + g) ^ i));
+            for (int c = 0; c < MT; ++c) asm volatile("" : "+v"(now.xv[b][c]));
         }
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < kRT; ++r) asm volatile("" : "+v"(now.sc[r]));
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(S::kLoads * (S::ST - 2)) : "memory");
+        const uint8_t* nxt = lds + ((s + 1) % S::ST) * S::kStage;
+        const uint32_t st = buffer(s);
+        constexpr int kParts = kHalf * kRT;
 #pragma unroll
         for (int b = 0; b < kHalf; ++b)
 #pragma unroll
             for (int r = 0; r < kRT; ++r) {
-                const bf16x8 wv = decode(code[b][r], (sc[r] >> (8 * b)) & 255);
+                const int q = b * kRT + r;
+                read(b, r, nxt, next);
+                multiply(b, r, now);
 #pragma unroll
-                for (int c = 0; c < MT; ++c) acc[r][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[b][c], acc[r][c], 0, 0, 0);
+                for (int u = q * S::kLoads / kParts; u < (q + 1) * S::kLoads / kParts; ++u) load_one(u, min(s + S::ST, last), st);
+                __builtin_amdgcn_sched_barrier(0);
             }
+    };
+    auto finish = [&](int s, const Operands& now) {
+        if (kg == 1 && static_cast<uint32_t>(s) * STEP + STEP / 2 >= static_cast<uint32_t>(K)) return;  // nothing past K
+#pragma unroll
+        for (int b = 0; b < kHalf; ++b)
+#pragma unroll
+            for (int r = 0; r < kRT; ++r) multiply(b, r, now);
+    };
+    int s = 0;
+    for (; s + 2 < steps; s += 2) {
+        step(s, even, odd);
+        step(s + 1, odd, even);
+    }
+    if (s + 1 < steps) {
+        step(s, even, odd);
+        finish(s + 1, odd);
+    } else {
+        finish(s, even);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     f32x4* red = reinterpret_cast<f32x4*>(lds);  // [tile of the wave][16 x 16 tile][lane]

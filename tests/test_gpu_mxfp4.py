@@ -241,7 +241,10 @@ A16_SHAPES = [(1, 1, 32), (1, 17, 64), (3, 40, 96), (1, 4096, 4096), (7, 1000, 1
               (64, 20003, 256), (300, 1000, 1152), (32, 28672, 128),
               # several spans of 1024 a wave and a tail, in every tile shape
               (5, 300, 9248), (5, 4200, 9248), (13, 9000, 5152), (9, 17000, 5152), (20, 9000, 5152),
-              (20, 17000, 5152), (48, 17000, 5152)]
+              (20, 17000, 5152), (48, 17000, 5152),
+              # the tiles in LDS: even and odd steps, a half step at the end
+              (100, 4500, 2176), (100, 4500, 2304), (45, 16500, 2176), (60, 16500, 2304), (60, 16500, 2176),
+              (100, 22000, 2176), (120, 16500, 1024)]
 
 
 @pytest.mark.parametrize("M,N,K", A16_SHAPES)
