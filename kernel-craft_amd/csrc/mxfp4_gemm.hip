@@ -1,6 +1,6 @@
 // mxfp4_gemm.hip -- the product of two MXFP4 matrices on gfx950's scaled matrix
-// cores: entry points, and the kernel for decode batches (M <= 16, or 64 on layers of
-// few rows).  More: mxfp4_gemm_tile.hip.  No counterpart in the reference.
+// cores: entry points, and the kernel for decode batches (M <= 16, or 48 and 64 on layers
+// of few rows).  More: mxfp4_gemm_tile.hip.  No counterpart in the reference.
 //
 //   Y[m, n] = sum_b 2^(sx[m, b] + sw[n, b] - 254) sum_{k in block b} e2m1(qx[m, k]) e2m1(qw[n, k])
 //
@@ -259,14 +259,16 @@ int launch_skinny(const char* fn, const uint8_t* qx, const uint8_t* sx, const ui
 
 // Row tiles per workgroup, us at 1, 2 and 4 of them: one tile of X N 4096, K 14336 8.4,
 // 10.9, 15.7, N 11008, K 5120 7.5, 8.5, 8.7, N 28672, K 4096 15.0, 13.7, 14.7; two tiles
-// N 4096, K 14336 10.7, 13.2, 19.6, N 6144, K 4096 7.0, 6.3, 8.4; four 15.1, 19.3, 29.8 and
-// 11.6, 8.5, 12.3.  Eight waves instead of four: one tile of X 4.2 against 4.1 us (N 4096,
+// N 4096, K 14336 10.7, 13.2, 19.6, N 6144, K 4096 7.0, 6.3, 8.4; four N 4096, K 14336 15.1,
+// 19.3, 29.8.  Eight waves instead of four: one tile of X 4.2 against 4.1 us (N 4096,
 // K 4096) and 8.2 against 8.4 (K 14336), more tiles spill.
 template <int MT, bool YBF16>
 int skinny(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw, const uint8_t* sw, void* y, int M, int N,
            int K, hipStream_t stream) {
-    if (N <= (MT == 1 ? 12288 : 4096)) return launch_skinny<MT, 1, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
-    return launch_skinny<MT, 2, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+    if constexpr (MT < 4) {  // four tiles come with at most 4096 rows
+        if (N > (MT == 1 ? 12288 : 4096)) return launch_skinny<MT, 2, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+    }
+    return launch_skinny<MT, 1, 4, YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
 }
 
 template <bool YBF16>
@@ -279,8 +281,10 @@ int gemm(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* qw
     if (!kc::aligned(qx, 16) || !kc::aligned(qw, 16))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the codes must be 16-byte aligned", fn);
     // More than one tile of tokens on layers of many rows read X less often from LDS
-    // (M 32, N 28672, K 4096 16.4 -> 14.8 us; M 64 20.5 -> 15.4; M 64, N 6144 stays at 8.5).
-    if (M > kSkinnyM || (M > 16 && N > 8192)) return kc::mx::gemm_tile<YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
+    // (M 32, N 28672, K 4096 16.4 -> 14.8 us; M 64 20.5 -> 15.4), and so do four tiles on more
+    // than 4096 (M 64, N 6144, K 2048 6.5 -> 4.9, K 4096 8.6 -> 7.9, K 14336 the same; M 48 7.4
+    // there, 7.8 in LDS tiles; M 64, N 4096, K 4096 6.6 and 6.5, K 14336 15.1 and 19.4).
+    if (M > kSkinnyM || (M > 16 && N > 8192) || (M > 48 && N > 4096)) return kc::mx::gemm_tile<YBF16>(fn, qx, sx, qw, sw, y, M, N, K, stream);
     const int m = static_cast<int>(M), n = static_cast<int>(N), k = static_cast<int>(K);
     switch ((m + 15) / 16) {
         case 1: return skinny<1, YBF16>(fn, qx, sx, qw, sw, y, m, n, k, stream);

@@ -156,7 +156,10 @@ W4A4_SHAPES = [(1, 1, 32), (1, 16, 64), (2, 33, 96), (5, 100, 160), (16, 16, 128
               (50, 28672, 256), (5, 13000, 2080), (130, 4100, 1600), (1100, 3000, 1056), (2100, 2100, 2112), (64, 8192, 992),
               # several groups of steps, K a multiple of 128 and not, on every larger tile
               (500, 6144, 2176), (700, 5000, 2208), (300, 4096, 2176), (300, 4096, 2080), (300, 4096, 4224),
-              (300, 4096, 4128), (300, 28672, 2112), (400, 2100, 2176)]
+              (300, 4096, 4128), (300, 28672, 2112), (400, 2100, 2176),
+              # several spans a wave and a tail with one to four tiles of tokens, one and two of rows
+              (9, 3000, 5152), (9, 12500, 5152), (25, 3000, 5152), (25, 5000, 5152), (40, 3000, 5152),
+              (40, 6100, 5152), (60, 3000, 5152)]
 
 
 @pytest.mark.parametrize("out", ["bfloat16", "float32"])
