@@ -94,7 +94,7 @@ __device__ __forceinline__ void load_tile_lds(const int8_t* src, int64_t rows, i
         const int chunk = (lane & 7) ^ swizzle(row);
         const int64_t k = min(k0 + 16 * chunk, K - 16);
         const int64_t r = min(r0 + row, rows - 1);
-        lds_dma16(src + r * K + k, base + 8 * i * kBK);
+        kc::lds_dma16(src + r * K + k, base + 8 * i * kBK);
     }
 }
 

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "kc_common.hpp"
+#include "lds_dma.hpp"
 
 namespace kc {
 namespace fp8 {
@@ -21,18 +22,6 @@ constexpr int kE8M0One = 127;  // block scale 2^0
 constexpr int kSchedMfma = 0x008, kSchedDsRead = 0x100;
 
 __device__ __forceinline__ int swizzle(int row) { return (row >> 1) & 7; }
-
-// One global_load_lds_dwordx4: 16 bytes per lane from `g` into LDS at
-// lds_base + 16 * lane.  Written as inline assembly so that the compiler's
-// LDS-wait bookkeeping does not see it: with such a load in flight the
-// compiler cannot count the ordinary LDS reads and drains them all before
-// every use.  The kernel waits for these loads itself (vmcnt(0) before the
-// barrier that publishes the buffer), and the "memory" clobber keeps LDS
-// reads and writes on their side of it.
-__device__ __forceinline__ void lds_dma16(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base)
-                 : "memory", "m0");
-}
 
 __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) {
     return static_cast<uint32_t>(reinterpret_cast<size_t>((lds_void*)p));

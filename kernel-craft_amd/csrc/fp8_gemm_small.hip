@@ -299,12 +299,6 @@ struct TileShape {
     static constexpr int kLds = kScales + (kRowsM + kRowsN) * 4;
 };
 
-// lds_dma16 from a scalar base and a 32-bit lane offset.
-__device__ __forceinline__ void lds_dma16s(uint32_t voff, const void* sbase, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base)
-                 : "memory", "m0");
-}
-
 // Lane offsets of one wave's loads of a step (ROWS rows of 128 bytes, WAVES
 // waves): load i carries rows 8 (kPer wave + i) .. + 7 of the tile, lane l row
 // l / 8 of them, chunk (l % 8) ^ swizzle(row); rows past `rows` read the last
@@ -374,17 +368,17 @@ __global__ __launch_bounds__(64 * WGM * WGN * KG) void gemm_fp8_tile_kernel(
         const uint32_t st = __builtin_amdgcn_readfirstlane(lds0 + (it % ST) * S::kStage);
         if (s < full) {
 #pragma unroll
-            for (int i = 0; i < kPerM; ++i) lds_dma16s(xo[i], xbase + k0, st + 1024 * (kPerM * wg + i));
+            for (int i = 0; i < kPerM; ++i) kc::lds_dma16(xo[i], xbase + k0, st + 1024 * (kPerM * wg + i));
 #pragma unroll
-            for (int i = 0; i < kPerN; ++i) lds_dma16s(wo[i], wbase + k0, st + S::kRowsM * kBK + 1024 * (kPerN * wg + i));
+            for (int i = 0; i < kPerN; ++i) kc::lds_dma16(wo[i], wbase + k0, st + S::kRowsM * kBK + 1024 * (kPerN * wg + i));
         } else {
             uint32_t xt[kPerM], wt[kPerN];
             row_offsets<S::kRowsM, S::kWavesG>(xt, xrows, static_cast<uint32_t>(K), wg, lane, kvalid);
             row_offsets<S::kRowsN, S::kWavesG>(wt, wrows, static_cast<uint32_t>(K), wg, lane, kvalid);
 #pragma unroll
-            for (int i = 0; i < kPerM; ++i) lds_dma16s(xt[i], xbase + k0, st + 1024 * (kPerM * wg + i));
+            for (int i = 0; i < kPerM; ++i) kc::lds_dma16(xt[i], xbase + k0, st + 1024 * (kPerM * wg + i));
 #pragma unroll
-            for (int i = 0; i < kPerN; ++i) lds_dma16s(wt[i], wbase + k0, st + S::kRowsM * kBK + 1024 * (kPerN * wg + i));
+            for (int i = 0; i < kPerN; ++i) kc::lds_dma16(wt[i], wbase + k0, st + S::kRowsM * kBK + 1024 * (kPerN * wg + i));
         }
     };
     struct Ops {
@@ -442,8 +436,8 @@ __global__ __launch_bounds__(64 * WGM * WGN * KG) void gemm_fp8_tile_kernel(
             }
 #pragma unroll
             for (int u = q * kL / kM; u < (q + 1) * kL / kM; ++u) {
-                if (u < kPerM) lds_dma16s(xo[u], xbase + k0, st + 1024 * (kPerM * wg + u));
-                else lds_dma16s(wo[u - kPerM], wbase + k0, st + S::kRowsM * kBK + 1024 * (kPerN * wg + u - kPerM));
+                if (u < kPerM) kc::lds_dma16(xo[u], xbase + k0, st + 1024 * (kPerM * wg + u));
+                else kc::lds_dma16(wo[u - kPerM], wbase + k0, st + S::kRowsM * kBK + 1024 * (kPerN * wg + u - kPerM));
             }
         }
     };

@@ -27,6 +27,7 @@
 
 #include "int4_decode.hpp"
 #include "kc_common.hpp"
+#include "lds_dma.hpp"
 
 namespace {
 
@@ -107,11 +108,6 @@ struct RunParams {
 };
 
 
-__device__ __forceinline__ void x_dma16(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base)
-                 : "memory", "m0");
-}
-
 // s_waitcnt vmcnt(n), n a constant once the caller's loop is unrolled; the
 // wait reads and writes `after` (work the caller does just before), so it is
 // not hoisted above it.
@@ -183,8 +179,8 @@ __device__ __forceinline__ void run_tile(const RunOp* op, int tile, char* lds) {
             for (int t0 = 0; t0 < KW * kXQ; t0 += kActive) {
                 const int t = t0 + wave;
                 const int kwp = t / kXQ, j = t - kwp * kXQ;
-                x_dma16(o.x + ((kwp * kWave + lane) * kXQ + j) * 8,
-                        __builtin_amdgcn_readfirstlane(base + t * kWave * 16));
+                kc::lds_dma16(o.x + ((kwp * kWave + lane) * kXQ + j) * 8,
+                              __builtin_amdgcn_readfirstlane(base + t * kWave * 16));
             }
             const uint32_t soff = static_cast<uint32_t>(g) * 4u, zoff = static_cast<uint32_t>(g >> 1);
 #pragma unroll

@@ -68,6 +68,7 @@
 
 #include "int4_gemm.hpp"
 #include "kc_common.hpp"
+#include "lds_dma.hpp"
 
 namespace {
 
@@ -1280,16 +1281,6 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return static_cast<uint32_t>(reinterpret_cast<size_t>((lds_void_t*)p));
 }
 
-// One global_load_lds_dwordx4: 16 bytes per lane from sbase + voff into LDS
-// at lds_base + 16 lane.  `after` is a register the load is made to depend
-// on (a value computed from the last LDS read of the slot it overwrites), so
-// it is issued after that read has returned.
-__device__ __forceinline__ void dma16(uint32_t voff, const void* sbase, uint32_t lds_base, uint32_t after) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base),
-                 "v"(after)
-                 : "memory", "m0");
-}
-
 template <int N>
 __device__ __forceinline__ void wait_vmcnt() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -1427,16 +1418,16 @@ __global__ __launch_bounds__(kKsWaves * kWave) void gemm_int4_kslds_kernel(
         const uint8_t* base = xbytes + 256 * min(T, tl);
 #pragma unroll
         for (int j = 0; j < kXB - 4; ++j)
-            dma16(xg[j & 3], base + static_cast<size_t>(8 * j) * K, x_lds + 1024 * j, after);
+            kc::lds_dma16_after(xg[j & 3], base + static_cast<size_t>(8 * j) * K, x_lds + 1024 * j, after);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dma16(xe[e], base, x_lds + 1024 * (kXB - 4 + e), after);
+        for (int e = 0; e < 4; ++e) kc::lds_dma16_after(xe[e], base, x_lds + 1024 * (kXB - 4 + e), after);
     };
     auto issue_w = [&](int rt, int T, uint32_t after) {
-        dma16(woff[rt], packed + 16 * kTStep<SHUF> * min(T, tl), w_lds + 1024 * rt, after);
+        kc::lds_dma16_after(woff[rt], packed + 16 * kTStep<SHUF> * min(T, tl), w_lds + 1024 * rt, after);
     };
     // load h of tile rt for the pair of T-blocks 2 p, 2 p + 1
     auto issue_wh = [&](int rt, int p, int h, uint32_t after) {
-        dma16(woffp[rt][h], packed + 128 * min(p, tl >> 1), w_lds + 2048 * rt + 1024 * h, after);
+        kc::lds_dma16_after(woffp[rt][h], packed + 128 * min(p, tl >> 1), w_lds + 2048 * rt + 1024 * h, after);
     };
     auto issue_wp = [&](int rt, int p, uint32_t after) {
         issue_wh(rt, p, 0, after);

@@ -3,6 +3,7 @@
 
 #include <atomic>
 
+#include "lds_dma.hpp"
 #include "mxfp4.hpp"
 
 namespace kc {

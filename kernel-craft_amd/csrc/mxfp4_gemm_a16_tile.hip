@@ -54,16 +54,6 @@ struct Shape {
     static_assert(ST >= 3 && kWn * TG * kRT * MT * 1024 <= kLds, "LDS");
 };
 
-// 16 (4) bytes per lane from sbase + voff into LDS at lds_base + 16 (4) * lane.
-__device__ __forceinline__ void lds_dma16(uint32_t voff, const void* sbase, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base)
-                 : "memory", "m0");
-}
-__device__ __forceinline__ void lds_dma4(uint32_t voff, const void* sbase, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base)
-                 : "memory", "m0");
-}
-
 __device__ __forceinline__ bf16x8 decode(uint32_t c, uint32_t b) {
     const float s = scale_operand(b);
     const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), q = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1);
@@ -115,12 +105,12 @@ __global__ __launch_bounds__(kThreads) void gemm_mxfp4_a16_tile_kernel(const uin
     auto load_one = [&](int u, int s, uint32_t st) {
         const uint32_t k0 = static_cast<uint32_t>(s) * STEP;
         if (u < S::kXLoads) {
-            lds_dma16(xrow[u] + min(2 * k0 + xchunk[u], 2u * K - 16), xbase, st + 1024 * (S::kXLoads * wave + u));
+            kc::lds_dma16(xrow[u] + min(2 * k0 + xchunk[u], 2u * K - 16), xbase, st + 1024 * (S::kXLoads * wave + u));
         } else if (u < S::kXLoads + S::kWLoads) {
             const int v = u - S::kXLoads;
-            lds_dma16(wrow[v] + min(k0 / 2 + wchunk[v], kbytes - 16), wbase, st + S::kX + 1024 * (S::kWLoads * wave + v));
+            kc::lds_dma16(wrow[v] + min(k0 / 2 + wchunk[v], kbytes - 16), wbase, st + S::kX + 1024 * (S::kWLoads * wave + v));
         } else if (lane < 16 * kSWords) {
-            lds_dma4(srow + min(k0 / kBlock + 4 * (lane % kSWords), blocks - 4), sbase,
+            kc::lds_dma4(srow + min(k0 / kBlock + 4 * (lane % kSWords), blocks - 4), sbase,
                      st + S::kX + S::kW + 16 * S::kSRow * wave);
         }
     };

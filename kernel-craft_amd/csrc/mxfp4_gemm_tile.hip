@@ -58,14 +58,6 @@ __device__ __forceinline__ int swizzle(int row) {
     return (j & 1) | (j >> 1 & 2) | ((j << 1 ^ j) & 4);
 }
 
-// 16 bytes per lane from sbase + voff into LDS at lds_base + 16 * lane.  In
-// assembly, so that the compiler does not wait for it at every LDS read: the
-// kernel waits itself before the barrier that publishes the buffer.
-__device__ __forceinline__ void lds_dma16(uint32_t voff, const void* sbase, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds_base)
-                 : "memory", "m0");
-}
-
 template <int TM_, int TN_, int WGM, int WGN, int ST, bool SDMA>
 struct Shape {
     static constexpr int kRowsM = 16 * TM_ * WGM, kRowsN = 16 * TN_ * WGN, kRows = kRowsM + kRowsN;
@@ -130,8 +122,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<size_t>((lds_void*)lds));
     auto stage_at = [&](int s) { return lds + (s % ST) * S::kStage; };
     auto dma_one = [&](int u, int k0, uint32_t st) {
-        if (u < S::kPerM) lds_dma16(xo[u], xbase + k0, st + 1024 * (S::kPerM * wave + u));
-        else lds_dma16(wo[u - S::kPerM], wbase + k0, st + S::kRowsM * kBK + 1024 * (S::kPerN * wave + u - S::kPerM));
+        if (u < S::kPerM) kc::lds_dma16(xo[u], xbase + k0, st + 1024 * (S::kPerM * wave + u));
+        else kc::lds_dma16(wo[u - S::kPerM], wbase + k0, st + S::kRowsM * kBK + 1024 * (S::kPerN * wave + u - S::kPerM));
     };
     auto stage_lds = [&](int s) { return __builtin_amdgcn_readfirstlane(lds0 + (s % ST) * S::kStage); };
     auto dma = [&](int s) {  // a whole step
@@ -149,7 +141,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
             const int row = row_in(per, v);
             const uint32_t at = static_cast<uint32_t>(min(row, (m ? xrows : wrows) - 1)) * kbytes +
                                 min(static_cast<uint32_t>(s) * kBK + 16 * ((lane & 7) ^ swizzle(row)), last);
-            lds_dma16(at, m ? xbase : wbase, st + (m ? 0 : S::kRowsM * kBK) + 1024 * (per * wave + v));
+            kc::lds_dma16(at, m ? xbase : wbase, st + (m ? 0 : S::kRowsM * kBK) + 1024 * (per * wave + v));
         }
     };
 
@@ -178,7 +170,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
             const bool m = first < S::kRowsM;
             const int r = first + (lane >> 1) - (m ? 0 : S::kRowsM);
             const uint32_t at = static_cast<uint32_t>(min(r, (m ? xrows : wrows) - 1)) * static_cast<uint32_t>(blocks) + 16 * (lane & 1);
-            lds_dma16(at, (m ? sx + m0 * blocks : sw + n0 * blocks) + 32 * g,
+            kc::lds_dma16(at, (m ? sx + m0 * blocks : sw + n0 * blocks) + 32 * g,
                       __builtin_amdgcn_readfirstlane(lds0 + S::kRawOff + 32 * first));
         }
     };

@@ -26,6 +26,7 @@
 
 #include "int4_decode.hpp"
 #include "kc_common.hpp"
+#include "lds_dma.hpp"
 
 namespace {
 
@@ -364,14 +365,6 @@ __global__ __launch_bounds__(WPB * kWave) void gemv_int4_fast_kernel(
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void lds_void_t;
 
-// One global_load_lds_dwordx4: 16 bytes per lane from g into LDS at
-// lds_base + 16 lane.  Inline assembly, so that the compiler's LDS-wait
-// bookkeeping does not see it; the kernel waits for these loads itself.
-__device__ __forceinline__ void x_dma16(const void* g, uint32_t lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds_base)
-                 : "memory", "m0");
-}
-
 // s_waitcnt vmcnt(n) for n in [0, 7] (a constant once the caller's loop is
 // unrolled).  The wait reads and writes `after` (a value the caller computes
 // just before, e.g. the previous row's sum), so it is not hoisted above that
@@ -450,8 +443,8 @@ __global__ __launch_bounds__(KW * RGW * kWave) void gemv_int4_xl_kernel(
         for (int t0 = 0; t0 < KW * kXQ; t0 += KW * RGW) {
             const int t = t0 + wave;
             const int kwp = t / kXQ, j = t - kwp * kXQ;
-            x_dma16(static_cast<const u32x4*>(x) + (kwp * kWave + lane) * kXQ + j,
-                    __builtin_amdgcn_readfirstlane(base + t * kWave * 16));
+            kc::lds_dma16(static_cast<const u32x4*>(x) + (kwp * kWave + lane) * kXQ + j,
+                          __builtin_amdgcn_readfirstlane(base + t * kWave * 16));
         }
         const uint32_t soff = static_cast<uint32_t>(g) * 4u, zoff = static_cast<uint32_t>(g >> 1);
 #pragma unroll
