@@ -99,6 +99,7 @@ __global__ __launch_bounds__(KW * 64) void gemm_mxfp4_skinny_kernel(
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int c = 0; c < MT; ++c) acc[r][c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    start(acc);
     const int spans = kbytes / kSpan;
     const int mine = spans > wave ? (spans - wave + KW - 1) / KW : 0;  // spans wave, wave + KW, ...
 

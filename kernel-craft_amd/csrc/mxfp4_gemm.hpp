@@ -14,10 +14,10 @@ namespace mx {
 // accumulator registers and most of the others in use, the compiler's allocation keeps
 // moving accumulators between the two halves of the register file (640 moves per 512
 // of these), and the builtin's eight-register operands spill where loads fill most
-// registers.  Nothing but these instructions touches the accumulators until
-// settle().  NOP: the operands may come from the instruction just before (the wait
-// states that the compiler adds between a vector instruction and a matrix one that
-// reads its result); operands that LDS or memory wrote need none.
+// registers.  Nothing but these instructions touches the accumulators between
+// start() and settle().  NOP: the operands may come from the instruction just before
+// (the wait states that the compiler adds between a vector instruction and a matrix one
+// that reads its result); operands that LDS or memory wrote need none.
 template <int BYTE, bool NOP = false>
 __device__ __forceinline__ void mfma(f32x4& acc, u32x4 a, u32x4 b, uint32_t sa, uint32_t sb) {
     if constexpr (NOP) asm volatile("s_nop 3" : "+v"(a), "+v"(b), "+v"(sa), "+v"(sb));
@@ -32,20 +32,32 @@ __device__ __forceinline__ void mfma(f32x4& acc, u32x4 a, u32x4 b, uint32_t sa, 
 #undef KC_MFMA
 }
 
+// Ties every accumulator to this place: what made it comes before, its uses behind.
+template <int I, int J>
+__device__ __forceinline__ void tie(f32x4 (&acc)[I][J]) {
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < J; ++j) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// Behind the accumulators' first values: vector instructions write them, and a matrix
+// instruction that reads one has to be two wait states behind.
+template <int I, int J>
+__device__ __forceinline__ void start(f32x4 (&acc)[I][J]) {
+    tie(acc);
+    asm volatile("s_nop 1" ::: "memory");
+    tie(acc);
+}
+
 // Waits until the last results are in their registers (the compiler does not know the
 // latency of the assembly above): every instruction that makes an accumulator comes
 // before the wait, every later use of one behind it.
 template <int I, int J>
 __device__ __forceinline__ void settle(f32x4 (&acc)[I][J]) {
-    auto tie = [&] {
-#pragma unroll
-        for (int i = 0; i < I; ++i)
-#pragma unroll
-            for (int j = 0; j < J; ++j) asm volatile("" : "+a"(acc[i][j]));
-    };
-    tie();
+    tie(acc);
     asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-    tie();
+    tie(acc);
 }
 
 // Lets KERNEL use `bytes` of dynamic LDS on the current device (once per device: the

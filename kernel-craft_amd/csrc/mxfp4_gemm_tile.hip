@@ -241,6 +241,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void gemm_mxfp4_tile_kernel(
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    start(acc);
     // scalar loads still in flight would make every LDS wait a full drain
     asm volatile("" ::"s"(y), "s"(M), "s"(N));
 

@@ -2,11 +2,16 @@
 
 The hardware does not hold back an instruction for some of the results that it
 reads.  The compiler puts s_nop between its own instructions, but sees neither
-into nor across inline assembly, which the loads into LDS of this library are.
-Checked here over every path of every kernel in the built library's disassembly:
+into nor across inline assembly, which the loads into LDS and some matrix
+products of this library are.  Checked here over every path of every kernel in
+the built library's disassembly:
 
 * M0 written by a scalar instruction -> a load into LDS, which takes its LDS
   address from it: 1 wait state.
+* A register written by a vector instruction -> a matrix instruction that reads
+  it, as operand, scale or accumulator: 2.
+* A matrix instruction's result -> anything but a matrix instruction: 5 for the
+  shortest of them, 3 more for one of 16 x 16 x 128 or 32 x 32.
 
 Every instruction is one wait state, s_nop n is n + 1; what an instruction waits
 for by itself (memory, LDS) is not counted on.
@@ -39,8 +44,17 @@ def code_objects(path):
         at = data.find(MAGIC, at + 1)
 
 
+REG = re.compile(r"\b([av])(?:(\d+)\b|\[(\d+):(\d+)\])")
 LINE = re.compile(r"^\t(\S+)\s*(.*?)\s*// ([0-9A-F]{12}):")
 TARGET = re.compile(r"<[^<>]*?(?:\+0x([0-9a-f]+))?>\s*$")
+
+
+def registers(text):
+    """The vector and accumulation registers that `text` names, as (kind, number)."""
+    out = set()
+    for kind, one, lo, hi in REG.findall(text):
+        out.update((kind, n) for n in (range(int(one), int(one) + 1) if one else range(int(lo), int(hi) + 1)))
+    return out
 
 
 class Instruction:
@@ -56,8 +70,23 @@ class Instruction:
         return [a.strip() for a in re.split(r",(?![^\[]*\])", self.text)]
 
     @property
+    def matrix(self):
+        return self.name.startswith(("v_mfma", "v_smfma"))
+
+    @property
     def into_lds(self):
         return "load_lds" in self.name or (self.name.startswith("buffer_load") and " lds" in self.text)
+
+    @property
+    def writes(self):
+        """Registers that a vector instruction writes."""
+        if "swap" in self.name:
+            return registers(self.text)
+        return registers(self.args[0])
+
+    @property
+    def reads(self):
+        return registers(",".join(self.args[1:]))
 
 
 def kernels(disassembly):
@@ -117,6 +146,13 @@ def missing_waits(code):
         if ins.into_lds:
             found += [("M0 -> load into LDS", n, ins, gap) for n, gap in near(ins, "before", 1)
                       if n.name.startswith("s_") and n.args[0] == "m0"]
+        if ins.matrix:
+            reads, result = ins.reads, registers(ins.args[0])
+            found += [("vector -> matrix", n, ins, gap) for n, gap in near(ins, "before", 2)
+                      if n.name.startswith("v_") and not n.matrix and n.writes & reads]
+            wide = "16x16x128" in ins.name or "32x32" in ins.name
+            found += [("matrix -> other", ins, n, gap) for n, gap in near(ins, "after", 8 if wide else 5)
+                      if not n.matrix and registers(n.text) & result]
     return found
 
 
@@ -135,22 +171,33 @@ def test_the_check_sees_missing_waits():
     load, m0 = "global_load_lds_dwordx4 v0, s[2:3]", "s_mov_b32 m0, s4"
     assert listing(m0, load, "s_endpgm") == ["M0 -> load into LDS"]
     assert listing(m0, "s_nop 0", load, "s_endpgm") == []
-    assert listing(load, m0, "s_cbranch_scc1 1 @0", "s_endpgm") == []
-    assert listing("s_nop 0", load, "s_branch 1 @0", m0, "s_cbranch_scc1 1 @1", load, "s_endpgm") == []
+    mfma = "v_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[8:11], v[12:15], a[4:7], v1, v2 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+    for write in ("v_accvgpr_write_b32 a5, 0", "v_mov_b32_e32 v15, v3", "v_mov_b32_e32 v2, 0",
+                  "v_permlane32_swap_b32_e32 v90, v8"):
+        assert listing(write, mfma, "s_endpgm") == ["vector -> matrix"]
+        assert listing(write, "s_waitcnt lgkmcnt(0)", mfma, "s_endpgm") == ["vector -> matrix"]
+        assert listing(write, "s_nop 1", mfma, "s_endpgm") == []
+    assert listing("s_nop 0", mfma, "v_mov_b32_e32 v1, 0", "s_cbranch_scc1 1 @1", "s_endpgm") == ["vector -> matrix"]
+    assert listing("v_mov_b32_e32 v7, 0", mfma, "s_endpgm") == []
+    read = "v_accvgpr_read_b32 v0, a7"
+    assert listing(mfma, "s_nop 6", read, "s_endpgm") == ["matrix -> other"]
+    assert listing(mfma, "s_nop 7", read, "s_endpgm") == []
+    assert listing(mfma, mfma, "s_nop 7", read, "s_endpgm") == []
 
 
 @pytest.mark.skipif(not OBJDUMP.exists(), reason="no llvm-objdump")
 def test_no_wait_state_is_missing_in_the_built_kernels(tmp_path):
     if not LIB_PATH.exists():
         pytest.fail(f"{LIB_PATH} missing: run __graft_entry__.build() first")
-    found, loads = [], 0
+    found, loads, matrix = [], 0, 0
     for i, obj in enumerate(code_objects(LIB_PATH)):
         path = tmp_path / f"{i}.co"
         path.write_bytes(obj)
         text = subprocess.run([OBJDUMP, "-d", "--no-leading-addr", path], check=True, capture_output=True, text=True).stdout
         for name, code in kernels(text):
             loads += sum(ins.into_lds for ins in code)
+            matrix += sum(ins.matrix for ins in code)
             found += [f"{name}: {kind}, {gap} wait states: {a.name} {a.text} ... {b.name} {b.text}"
                       for kind, a, b, gap in missing_waits(code)]
-    assert loads > 1000  # the library was really taken apart
+    assert loads > 1000 and matrix > 1000  # the library was really taken apart
     assert not found, f"{len(found)} missing waits, first: " + "\n".join(found[:5])
