@@ -350,8 +350,10 @@ int kc_gemm_mxfp4_w4a4_bf16(const uint8_t* d_qx, const uint8_t* d_sx,
 int kc_gemm_mxfp4_w4a4_f32(const uint8_t* d_qx, const uint8_t* d_sx,
                            const uint8_t* d_qw, const uint8_t* d_sw, float* d_y,
                            int64_t M, int64_t N, int64_t K, kc_stream_t stream);
-/* The same with bf16 activations x [M, K] (16-byte aligned) on MXFP4 weights:
- * the form for single tokens and decode batches. */
+/* The same with bf16 activations x [M, K] (16-byte aligned) on MXFP4 weights,
+ * whose values are those that kc_dequantize_mxfp4_bf16 gives (an infinity where
+ * a large code at scale byte 253 or 254 leaves bf16's range): the form for
+ * single tokens and decode batches. */
 int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw,
                        const uint16_t* d_x, uint16_t* d_y, int64_t M, int64_t N,
                        int64_t K, kc_stream_t stream);

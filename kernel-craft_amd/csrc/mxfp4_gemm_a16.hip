@@ -6,8 +6,9 @@
 // An E2M1 value times a power of two is a bf16 value, so the weights are decoded in
 // registers (v_cvt_scalef32_pk_bf16_fp4: two codes and their scale in one
 // instruction) and multiplied on the bf16 matrix cores with fp32 accumulation; the
-// only rounding is that of Y.  Weights outside bf16's range (scale bytes under 2
-// or over 252 with large codes) are rounded or overflow as bf16 values do.
+// only rounding is that of Y.  Scale bytes 0 and 1 give subnormal bf16 values, exactly;
+// a code times a scale past bf16's range (bytes 253 and 254 with large codes) is an
+// infinity, as it is dequantized.
 //
 // Bound by the weight stream (0.53 bytes a weight) on wide layers (M 13, N 28672, K 4096
 // 13.8 us, 4.7 TB/s), by the reads of X, one for every RT tiles of rows, on narrow ones.

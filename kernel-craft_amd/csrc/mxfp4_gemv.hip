@@ -7,14 +7,15 @@
 // wave's rows, so x stays in 16 registers and a wave's load is 1 KB of one row, whole
 // cache lines; all four rows of a wave are on their way before the first is used.  K is
 // split over kw waves of 64 blocks; the workgroup's 8 / kw groups of waves take four
-// rows each.  A block is decoded to bf16 without its scale
-// (v_cvt_scalef32_pk_bf16_fp4), multiplied with v_dot2_f32_bf16, and its fp32 sum
-// multiplied with the block's scale, a power of two.  The lanes meet in DPP sums, the
-// waves in LDS.
+// rows each.  A block is decoded to bf16 with its scale
+// (v_cvt_scalef32_pk_bf16_fp4), as for more tokens, so that one token's terms leave
+// fp32's range (and its weights bf16's) where many tokens' do, and multiplied with
+// v_dot2_f32_bf16.  The lanes meet in DPP sums, the waves in LDS.
 //
-// Measured (us, against the matrix-core kernel for one token): N 28672, K 4096 12.3
-// and 13.5 (62 MB; 10.4 at 6 TB/s); K 8192 24.3 and 29.6; K 2048 8.0 and 9.6; N 4096, K 4096
-// 4.4 and 5.1, K 14336 9.4 and 10.2; with a block per lane missing (K 1024) 3.2 and 2.4, so
+// Measured (us, against the matrix-core kernel for one token): N 28672, K 4096 11.9
+// and 13.5 (62 MB; 10.4 at 6 TB/s); K 8192 22.6 and 29.6; K 2048 7.2 and 9.6; N 4096, K 4096
+// 3.9 and 5.1, K 14336 7.9 and 10.2 (with the scale on the block's fp32 sum 12.0, 23.8, 7.6,
+// 4.3 and 8.5); with a block per lane missing (K 1024) 3.2 and 2.4, so
 // K under 2048 stays there, and so do two tokens (15.8 and 13.2 us: the sums over lanes
 // cost as much as the dot products).  Two rows a wave 12.4 us, eight 13.3, sixteen 16.9.
 #include "mxfp4_gemm.hpp"
@@ -43,9 +44,9 @@ __device__ __forceinline__ float sum_all(float v) {
     return v + __shfl_xor(v, 32, kWave);
 }
 
-__device__ __forceinline__ float dot8(uint32_t c, const uint32_t (&x)[4], float a) {
-    const bf16x2 w0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 0), w1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 1);
-    const bf16x2 w2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 2), w3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, 1.0f, 3);
+__device__ __forceinline__ float dot8(uint32_t c, float s, const uint32_t (&x)[4], float a) {
+    const bf16x2 w0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), w1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1);
+    const bf16x2 w2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), w3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3);
     a = __builtin_amdgcn_fdot2_f32_bf16(w0, __builtin_bit_cast(bf16x2, x[0]), a, false);
     a = __builtin_amdgcn_fdot2_f32_bf16(w1, __builtin_bit_cast(bf16x2, x[1]), a, false);
     a = __builtin_amdgcn_fdot2_f32_bf16(w2, __builtin_bit_cast(bf16x2, x[2]), a, false);
@@ -77,13 +78,14 @@ __global__ __launch_bounds__(kWaves * 64) void gemv_mxfp4_kernel(const uint8_t* 
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
         const uint32_t c[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
+        const float scale = scale_operand(s[r]);
         float a = 0.0f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const uint32_t xq[4] = {xv[q].x, xv[q].y, xv[q].z, xv[q].w};
-            a = dot8(c[q], xq, a);
+            a = dot8(c[q], scale, xq, a);
         }
-        a = sum_all(has ? a * scale_value(s[r]) : 0.0f);
+        a = sum_all(has ? a : 0.0f);
         if (lane == 0) red[wave][r] = a;
     }
     __syncthreads();

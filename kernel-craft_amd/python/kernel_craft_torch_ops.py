@@ -904,8 +904,9 @@ def mxfp4_gemm_w4a4(qx, sx, qw, sw, out_dtype=None):
 
 
 def mxfp4_gemm_bf16(qw, sw, x):
-    """Y [M, N] bf16 = X W^T for bf16 X [M, K] and MXFP4 weights (qw, sw) [N, K], fp32
-    accumulation: the form for single tokens and decode batches (kc_gemm_mxfp4_bf16)."""
+    """Y [M, N] bf16 = X W^T for bf16 X [M, K] and MXFP4 weights (qw, sw) [N, K], of the values that
+    mxfp4_dequantize gives, fp32 accumulation: the form for single tokens and decode batches
+    (kc_gemm_mxfp4_bf16)."""
     import torch
     qw, sw, N, K = _mx("mxfp4_gemm_bf16", qw, sw, ("qw", "sw"))
     x = _take("mxfp4_gemm_bf16", "x", x, torch.bfloat16)

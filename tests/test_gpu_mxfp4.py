@@ -355,3 +355,74 @@ def test_other_stream_and_graph_replays(gpu, ops, M):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, layer(x)))
+
+
+# The products with bf16 activations over the whole range of scales: Y = X W^T, W as
+# mxfp4_dequantize gives it in bf16, whichever kernel the number of tokens leads to.
+# M 1: the GEMV (K from 2048), or the matrix cores (K 96); 5 and 40 tokens in registers, 100 in LDS tiles.
+A16_KERNELS = [(1, 2080), (1, 96), (5, 2176), (40, 2080), (100, 2176)]
+
+
+def _one_block_rows(rng, N, K, byte, low=0):
+    """N rows with codes in one block each, of any scale in `byte`; all others zero.  `low`: the smallest code."""
+    qw, sw = np.zeros((N, K // 32, 16), np.uint8), np.full((N, K // 32), 127, np.uint8)
+    at, rows = rng.integers(0, K // 32, N), np.arange(N)
+    codes = rng.integers(low, 8, (N, 32), dtype=np.uint8) | (rng.integers(0, 2, (N, 32), dtype=np.uint8) << 3)
+    qw[rows, at] = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    sw[rows, at] = byte
+    return qw.reshape(N, K // 2), sw
+
+
+@pytest.mark.parametrize("M,K", A16_KERNELS)
+@pytest.mark.parametrize("first,last,x_exponent", [(0, 127, 60), (128, 252, -60), (64, 110, 120), (150, 252, -120)])
+def test_a16_every_scale(gpu, ops, M, K, first, last, x_exponent):
+    """One block a row: with activations n 2^e, |n| <= 8, its 32 terms are multiples of one
+    power of two, at most 32 * 48 * 2 of them, and exact in fp32 in any order.  Activations
+    of 2^123 on scales far below 1, and of 2^-120 on large ones, among them: the terms
+    are in fp32's range only with their scale."""
+    rng = np.random.default_rng(M + first)
+    N = 16500 if M == 100 else 520
+    byte = np.resize(np.arange(first, last + 1), N)
+    qw, sw = _one_block_rows(rng, N, K, byte)
+    x = np.ldexp(rng.integers(-8, 9, (M, K)).astype(np.float64), x_exponent)
+    y = ops.mxfp4_gemm_bf16(_t(gpu, qw), _t(gpu, sw), _bf16(gpu, x))
+    want = gpu.from_numpy(x @ ref.values(qw, sw).T).float().bfloat16()    # exact in fp32
+    assert gpu.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("M,K", A16_KERNELS)
+def test_a16_subnormal_activations(gpu, ops, M, K):
+    """bf16's subnormal activations on large scales."""
+    rng = np.random.default_rng(M)
+    N = 16500 if M == 100 else 300
+    qw, sw = _one_block_rows(rng, N, K, np.resize(np.arange(180, 250), N))
+    x = np.ldexp(rng.integers(-8, 9, (M, K)).astype(np.float64), -133)
+    y = ops.mxfp4_gemm_bf16(_t(gpu, qw), _t(gpu, sw), _bf16(gpu, x))
+    want = gpu.from_numpy(x @ ref.values(qw, sw).T).float().bfloat16()
+    assert gpu.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("M,K", A16_KERNELS)
+def test_a16_weights_past_the_range_are_bf16_infinities(gpu, ops, M, K):
+    """Scale bytes 253 and 254 with codes whose value leaves bf16's range."""
+    rng = np.random.default_rng(M)
+    N = 16500 if M == 100 else 64
+    qw, sw = _one_block_rows(rng, N, K, np.resize([253, 254], N), low=6)
+    qw &= 0x77  # positive
+    x = np.full((M, K), 2.0 ** -20)
+    w = ops.mxfp4_dequantize(_t(gpu, qw), _t(gpu, sw))
+    assert bool(gpu.isinf(w).any(1).all())
+    y = ops.mxfp4_gemm_bf16(_t(gpu, qw), _t(gpu, sw), _bf16(gpu, x))
+    assert bool((y == float("inf")).all())
+
+
+@pytest.mark.parametrize("M,K", A16_KERNELS)
+def test_a16_nan_scale_marks_its_column(gpu, ops, M, K):
+    rng = np.random.default_rng(M)
+    N = 16500 if M == 100 else 70
+    qw, sw = _mx(rng, N, K)
+    sw[9, K // 32 - 1], sw[69, 0] = 255, 255
+    y = ops.mxfp4_gemm_bf16(_t(gpu, qw), _t(gpu, sw), _bf16(gpu, rng.standard_normal((M, K))))
+    want = np.zeros(N, bool)
+    want[[9, 69]] = True
+    assert (gpu.isnan(y).cpu().numpy() == want).all()
