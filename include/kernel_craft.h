@@ -341,8 +341,8 @@ int kc_dequantize_mxfp4_f32(const uint8_t* d_codes, const uint8_t* d_scales,
 
 /* Y[m, n] = sum_k x[m, k] w[n, k], both MXFP4 (qx, sx: [M, K]; qw, sw:
  * [N, K]), fp32 accumulation, Y [M, N] row-major bf16 (RNE) or fp32.  K a
- * multiple of 32 (K == 0 writes Y = 0), qx and qw 16-byte aligned, any M and
- * N. */
+ * multiple of 32 up to 2^24 (K == 0 writes Y = 0), qx and qw 16-byte aligned,
+ * M and N up to 2^28 with at most 2^26 tiles of 16 x 16 in Y. */
 int kc_gemm_mxfp4_w4a4_bf16(const uint8_t* d_qx, const uint8_t* d_sx,
                             const uint8_t* d_qw, const uint8_t* d_sw,
                             uint16_t* d_y, int64_t M, int64_t N, int64_t K,
@@ -353,7 +353,7 @@ int kc_gemm_mxfp4_w4a4_f32(const uint8_t* d_qx, const uint8_t* d_sx,
 /* The same with bf16 activations x [M, K] (16-byte aligned) on MXFP4 weights,
  * whose values are those that kc_dequantize_mxfp4_bf16 gives (an infinity where
  * a large code at scale byte 253 or 254 leaves bf16's range): the form for
- * single tokens and decode batches. */
+ * single tokens and decode batches.  M up to 1048560, else the same limits. */
 int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw,
                        const uint16_t* d_x, uint16_t* d_y, int64_t M, int64_t N,
                        int64_t K, kc_stream_t stream);

@@ -314,7 +314,7 @@ extern "C" int kc_gemm_mxfp4_bf16(const uint8_t* d_qw, const uint8_t* d_sw, cons
     if (st != KC_SUCCESS || M == 0 || N == 0) return st;
     if (K == 0) return kc::mx::fill_zero<true>(fn, d_y, M * N, stream);
     if (M > 16 * 65535)  // tiles of tokens are the grid's second dimension
-        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: M=%lld too large", fn, (long long)M);
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: M=%lld too large, at most %d", fn, (long long)M, 16 * 65535);
     if (!d_qw || !d_sw || !d_x) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
     if (!kc::aligned(d_qw, 16) || !kc::aligned(d_x, 16))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the codes and x must be 16-byte aligned", fn);

@@ -883,8 +883,8 @@ def mxfp4_dequantize(codes, scales, out_dtype=None):
 def mxfp4_gemm_w4a4(qx, sx, qw, sw, out_dtype=None):
     """Y [M, N] = X W^T of two MXFP4 matrices on the 4-bit matrix cores, fp32 accumulation:
     (qx, sx) [M, K] from mxfp4_quantize on the activations, (qw, sw) [N, K] from it on the
-    weights.  Any M and N; out_dtype torch.bfloat16 (default) or torch.float32
-    (kc_gemm_mxfp4_w4a4_*)."""
+    weights.  M and N up to 2^28 with at most 2^26 tiles of 16 x 16 in Y, K up to 2^24;
+    out_dtype torch.bfloat16 (default) or torch.float32 (kc_gemm_mxfp4_w4a4_*)."""
     import torch
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
     if out_dtype not in (torch.bfloat16, torch.float32):
@@ -905,8 +905,8 @@ def mxfp4_gemm_w4a4(qx, sx, qw, sw, out_dtype=None):
 
 def mxfp4_gemm_bf16(qw, sw, x):
     """Y [M, N] bf16 = X W^T for bf16 X [M, K] and MXFP4 weights (qw, sw) [N, K], of the values that
-    mxfp4_dequantize gives, fp32 accumulation: the form for single tokens and decode batches
-    (kc_gemm_mxfp4_bf16)."""
+    mxfp4_dequantize gives, fp32 accumulation: the form for single tokens and decode batches.
+    M up to 1048560 tokens, else mxfp4_gemm_w4a4's limits (kc_gemm_mxfp4_bf16)."""
     import torch
     qw, sw, N, K = _mx("mxfp4_gemm_bf16", qw, sw, ("qw", "sw"))
     x = _take("mxfp4_gemm_bf16", "x", x, torch.bfloat16)

@@ -193,3 +193,18 @@ def test_plain_forms_agree():
     x[0, 40] = np.nan
     codes, scales = ref.quantize(x)
     assert list(scales[0]) == [127, 255] and not codes[0, 16:].any()
+
+
+@pytest.mark.parametrize("call,why", [
+    (lambda L: L.kc_gemm_mxfp4_bf16(P, P, P, P, 1048561, 4, 64, None), "at most 1048560"),
+    (lambda L: L.kc_gemm_mxfp4_bf16(P, P, P, P, 16, (1 << 28) + 1, 64, None), "too large"),
+    (lambda L: L.kc_gemm_mxfp4_w4a4_bf16(P, P, P, P, P, 16 << 13, (16 << 13) + 1, 64, None), "too large"),
+    (lambda L: L.kc_gemm_mxfp4_w4a4_f32(P, P, P, P, P, 4, 4, (1 << 24) + 32, None), "too large"),
+])
+def test_products_refuse_what_is_just_past_their_limits(call, why):
+    """The limits that the header names."""
+    L = kc_abi.lib()
+    L.kc_get_last_error()
+    assert call(L) == 1
+    assert why in L.kc_last_error_string().decode()
+    assert L.kc_get_last_error() == 1
