@@ -435,3 +435,45 @@ def test_decoder_layer_front(gpu, ops, fmt):
     rel = lambda a, b: float((a.double().cpu() - b).norm() / b.norm())  # noqa: E731
     assert rel(torch.cat(rows), wq_) <= 2.0 ** -6
     assert rel(kv[0], wk) <= half_step + 2.0 ** -6 and rel(kv[1], wv) <= half_step + 2.0 ** -6
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(32, 8), (16, 16)])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+def test_long_bf16_batches_of_whole_head_groups_equal_their_parts(gpu, ops, fmt, inter, Hq, Hkv):
+    """More than 64 MB of heads (read past the cache) whose groups of 8, a wave's, are of one
+    tensor: the same bits as the batch in parts, in which they are not read past it.
+    32 + 8 heads pass 64 MB with their norm, 16 + 16 also when keys and values are written alone."""
+    T, D, parts = 8211, 128, 5
+    q, k, v, gq, gk = _heads(gpu, T, Hq, Hkv, D, gpu.bfloat16, seed=Hq)
+    cos, sin = _tables(gpu, 1000, D // 2)
+    pos = (gpu.arange(T, device="cuda") % 1003 - 1).int()
+    slots = gpu.randperm(T + 7, device="cuda")[:T] - 3
+    cuts = [T * i // parts for i in range(parts + 1)]
+    assert T * (Hq + Hkv) * D * 2 > 64 << 20 and (Hkv == 8 or T * 2 * Hkv * D * 2 > 64 << 20)
+
+    def over(ends, call):
+        return [call(slice(a, b)) for a, b in zip(ends, ends[1:])]
+
+    def norm(s):
+        return ops.qk_norm_rope(q[s], k[s], gq, gk, cos, sin, pos[s], interleaved=inter)
+
+    whole, pieces = norm(slice(0, T)), over(cuts, norm)
+    for i in range(2):
+        assert gpu.equal(whole[i].view(gpu.uint8), gpu.cat([p[i] for p in pieces]).view(gpu.uint8))
+    caches = [_pool(gpu, T // 16 + 1, 16, Hkv, D, fmt) for _ in range(5)]
+
+    def fused(cache):
+        return lambda s: ops.qk_norm_rope_cache(q[s], k[s], v[s], gq, gk, cos, sin, pos[s], slots[s], *cache,
+                                                interleaved=inter)
+
+    y = over([0, T], fused(caches[0])) + [gpu.cat(over(cuts, fused(caches[1])))]
+    assert all(gpu.equal(t.view(gpu.uint8), whole[0].view(gpu.uint8)) for t in y)
+    over([0, T], lambda s: ops.kv_cache_write(k[s], v[s], slots[s], *caches[2]))
+    over(cuts, lambda s: ops.kv_cache_write(k[s], v[s], slots[s], *caches[3]))
+    # the fused write's keys are the normed ones, where a position is in the table
+    kept = gpu.where((pos >= 0) & (pos < 1000), slots, -1)
+    ops.kv_cache_write(whole[1], v, kept, *caches[4])
+    for one, other in ((0, 1), (2, 3), (0, 4)):
+        for a, b in zip(caches[one], caches[other]):
+            assert gpu.equal(a.view(gpu.uint8), b.view(gpu.uint8))
