@@ -449,8 +449,8 @@ int kc_qk_norm_rope_cache_f32(const float* d_q, int64_t q_stride,
  * cu_seqlens[b + 1], int32 [seqs + 1]) reads position t - cu_seqlens[b] of
  * it, in page block_table[b, position / page_size] (int32 [seqs,
  * max_pages]).  A position whose page is missing (past max_pages, or an entry
- * outside the pool) reads as NaN; rows past the last sequence are left as
- * they were. */
+ * outside the pool) reads as NaN; rows before the first sequence
+ * (cu_seqlens[0] > 0) and past the last are left as they were. */
 int kc_kv_cache_read_bf16(const kc_kv_cache* cache,
                           const int32_t* d_block_table, int64_t max_pages,
                           const int32_t* d_cu_seqlens, int seqs,

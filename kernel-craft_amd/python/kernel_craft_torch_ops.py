@@ -1096,8 +1096,8 @@ def kv_cache_read(k_codes, k_scales, v_codes, v_scales, block_table, cu_seqlens,
     torch.bfloat16 (default) or torch.float32: token t of sequence b (cu_seqlens[b] <= t <
     cu_seqlens[b + 1], int32 [sequences + 1]) is position t - cu_seqlens[b], in page
     block_table[b, position // page_size] (int32 [sequences, most pages]).  A position whose page
-    is missing or outside the pool reads as NaN; rows past the last sequence are not written
-    (kc_kv_cache_read_*)."""
+    is missing or outside the pool reads as NaN; rows before the first sequence (cu_seqlens[0] >
+    0) and past the last are not written (kc_kv_cache_read_*)."""
     import torch
     op = "kv_cache_read"
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype

@@ -477,3 +477,58 @@ def test_long_bf16_batches_of_whole_head_groups_equal_their_parts(gpu, ops, fmt,
     for one, other in ((0, 1), (2, 3), (0, 4)):
         for a, b in zip(caches[one], caches[other]):
             assert gpu.equal(a.view(gpu.uint8), b.view(gpu.uint8))
+
+
+@pytest.mark.parametrize("fmt,D", [("fp8", 64), ("fp8", 33), ("mxfp4", 64)])
+@pytest.mark.parametrize("starts", [[0, 9, 4, 8], [3, 1, 6, 8], [0, -5, 4, 7], [2, 2 ** 30, -2 ** 31, 2 ** 31 - 1], [8, 8, 0, 0]])
+def test_read_with_descending_starts_keeps_to_pool_and_outputs(gpu, ops, starts, fmt, D):
+    """Starts that do not ascend are the caller's mistake: each row is a row of the pool,
+    keys' and values' the same one, or all NaN, or left as it was; nothing is
+    written outside the outputs.  Every slot holds values of its own."""
+    import ctypes
+    from kc_abi import check, ptr, stream
+    H, page, pages, total, guard = 2, 4, 3, 8, 5
+    g = gpu.Generator("cuda").manual_seed(2)
+    pool = _pool(gpu, pages, page, H, D, fmt)
+    rows = [gpu.randn(pages * page, H, D, generator=g, device="cuda") for _ in range(2)]
+    ops.kv_cache_write(*rows, gpu.arange(pages * page, device="cuda"), *pool)
+    every = ops.kv_cache_read(*pool, gpu.arange(pages, device="cuda", dtype=gpu.int32)[None],
+                              gpu.tensor([0, pages * page], dtype=gpu.int32, device="cuda"), pages * page,
+                              out_dtype=gpu.float32)
+    cu = gpu.tensor(starts, dtype=gpu.int32, device="cuda")
+    table = gpu.tensor([[0, 2], [1, -1], [2, 7]], dtype=gpu.int32, device="cuda")
+    outs = [gpu.full((total + 2 * guard, H, D), 42.0, device="cuda") for _ in range(2)]
+    cache, _, _ = ops._kv_cache("test", *pool)
+    check("read", ops._get_lib().kc_kv_cache_read_f32(ctypes.byref(cache), ptr(table), 2, ptr(cu), 3, total,
+                                                      ptr(outs[0][guard:]), ptr(outs[1][guard:]), stream()))
+    for y in outs:
+        assert bool((y[:guard] == 42.0).all()) and bool((y[guard + total:] == 42.0).all())
+    for t in range(guard, guard + total):
+        def kind(y, src):
+            if bool((y == 42.0).all()):
+                return "left"
+            if bool(gpu.isnan(y).all()):
+                return "NaN"
+            same = (src == y).flatten(1).all(1).nonzero().flatten().tolist()
+            assert len(same) == 1, "not a row of the pool"
+            return same[0]
+        assert kind(outs[0][t], every[0]) == kind(outs[1][t], every[1])
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+def test_read_leaves_rows_before_the_first_sequence(gpu, ops, fmt):
+    """Sequences that start behind the outputs' first rows: those rows are left as they were."""
+    import ctypes
+    from kc_abi import check, ptr, stream
+    pool = _pool(gpu, 2, 4, 1, 64, fmt)
+    ops.kv_cache_write(gpu.randn(8, 1, 64, device="cuda"), gpu.randn(8, 1, 64, device="cuda"),
+                       gpu.arange(8, device="cuda"), *pool)
+    cu = gpu.tensor([3, 5, 9], dtype=gpu.int32, device="cuda")
+    table = gpu.tensor([[0], [1]], dtype=gpu.int32, device="cuda")
+    outs = [gpu.full((11, 1, 64), 42.0, device="cuda") for _ in range(2)]
+    cache, _, _ = ops._kv_cache("test", *pool)
+    check("read", ops._get_lib().kc_kv_cache_read_f32(ctypes.byref(cache), ptr(table), 1, ptr(cu), 2, 11, ptr(outs[0]),
+                                                      ptr(outs[1]), stream()))
+    want = ops.kv_cache_read(*pool, table, cu - 3, 6, out_dtype=gpu.float32)
+    for y, w in zip(outs, want):
+        assert bool((y[[0, 1, 2, 9, 10]] == 42.0).all()) and gpu.equal(y[3:9], w)
