@@ -532,3 +532,36 @@ def test_read_leaves_rows_before_the_first_sequence(gpu, ops, fmt):
     want = ops.kv_cache_read(*pool, table, cu - 3, 6, out_dtype=gpu.float32)
     for y, w in zip(outs, want):
         assert bool((y[[0, 1, 2, 9, 10]] == 42.0).all()) and gpu.equal(y[3:9], w)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("D", [128, 80, 33])
+def test_fp8_scales_are_the_rounded_quotient(gpu, ops, D, dtype, fused):
+    """Rows whose largest magnitude is 7 n: x / scale then meets midpoints of E4M3 exactly, so a
+    scale that is off by one step of fp32 (a multiplication with a rounded 1 / 448)
+    shows in the codes.  Scales and codes against 64 bits, bit for bit."""
+    T, H, dt = 300, 2, getattr(gpu, dtype)
+    rng = np.random.default_rng(D)
+    x = rng.integers(-120, 121, (T, H, D)).astype(np.float64)
+    top = 7.0 * rng.integers(1, 18, (T, H))
+    x = np.clip(x, -top[..., None], top[..., None])
+    x[..., 0] = top
+    x = np.ldexp(x, rng.integers(-30, 30, (T, H, 1)))
+    v = gpu.from_numpy(x).cuda().to(dt)
+    assert np.array_equal(_np(v), x)
+    pool = _pool(gpu, T, 1, H, D, "fp8")
+    slots = gpu.arange(T, device="cuda")
+    if fused:
+        one = gpu.ones(D, device="cuda").to(dt)
+        none = gpu.zeros(1, 0, device="cuda")
+        ops.qk_norm_rope_cache(v, v, v, one, one, none, none, gpu.zeros(T, device="cuda", dtype=gpu.int32), slots, *pool)
+    else:
+        ops.kv_cache_write(v, v, slots, *pool)
+    scale = (np.abs(x).max(-1) / 448.0).astype(np.float32)
+    a = x / scale.astype(np.float64)[..., None]
+    ulp = np.exp2(np.maximum(np.floor(np.log2(np.maximum(np.abs(a), 2.0 ** -30))), -6) - 3)
+    want = np.rint(a / ulp) * ulp
+    for i in (2,) if fused else (0, 2):
+        np.testing.assert_array_equal(pool[i + 1][:, 0].cpu().numpy(), scale)
+        np.testing.assert_array_equal(pool[i][:, 0].view(gpu.float8_e4m3fn).double().cpu().numpy(), want)
