@@ -8,6 +8,8 @@ the built library's disassembly:
 
 * M0 written by a scalar instruction -> a load into LDS, which takes its LDS
   address from it: 1 wait state.
+* A scalar register written by a vector instruction (v_readfirstlane) -> a memory
+  instruction that takes its address from it: 5.
 * A register written by a vector instruction -> a matrix instruction that reads
   it, as operand, scale or accumulator: 2.
 * A matrix instruction's result -> anything but a matrix instruction: 5 for the
@@ -45,6 +47,7 @@ def code_objects(path):
 
 
 REG = re.compile(r"\b([av])(?:(\d+)\b|\[(\d+):(\d+)\])")
+SCALAR = re.compile(r"\bs(?:(\d+)\b|\[(\d+):(\d+)\])")
 LINE = re.compile(r"^\t(\S+)\s*(.*?)\s*// ([0-9A-F]{12}):")
 TARGET = re.compile(r"<[^<>]*?(?:\+0x([0-9a-f]+))?>\s*$")
 
@@ -54,6 +57,14 @@ def registers(text):
     out = set()
     for kind, one, lo, hi in REG.findall(text):
         out.update((kind, n) for n in (range(int(one), int(one) + 1) if one else range(int(lo), int(hi) + 1)))
+    return out
+
+
+def scalars(text):
+    """The scalar registers that `text` names."""
+    out = set()
+    for one, lo, hi in SCALAR.findall(text):
+        out.update(range(int(one), int(one) + 1) if one else range(int(lo), int(hi) + 1))
     return out
 
 
@@ -76,6 +87,10 @@ class Instruction:
     @property
     def into_lds(self):
         return "load_lds" in self.name or (self.name.startswith("buffer_load") and " lds" in self.text)
+
+    @property
+    def memory(self):
+        return self.name.startswith(("global_", "buffer_", "flat_", "scratch_"))
 
     @property
     def writes(self):
@@ -146,6 +161,9 @@ def missing_waits(code):
         if ins.into_lds:
             found += [("M0 -> load into LDS", n, ins, gap) for n, gap in near(ins, "before", 1)
                       if n.name.startswith("s_") and n.args[0] == "m0"]
+        if ins.memory and (address := scalars(ins.text)):
+            found += [("vector -> address", n, ins, gap) for n, gap in near(ins, "before", 5)
+                      if n.name.startswith("v_") and not n.matrix and scalars(n.args[0]) & address]
         if ins.matrix:
             reads, result = ins.reads, registers(ins.args[0])
             found += [("vector -> matrix", n, ins, gap) for n, gap in near(ins, "before", 2)
@@ -171,6 +189,8 @@ def test_the_check_sees_missing_waits():
     load, m0 = "global_load_lds_dwordx4 v0, s[2:3]", "s_mov_b32 m0, s4"
     assert listing(m0, load, "s_endpgm") == ["M0 -> load into LDS"]
     assert listing(m0, "s_nop 0", load, "s_endpgm") == []
+    assert listing("v_readfirstlane_b32 s3, v1", "s_nop 3", load, "s_endpgm") == ["vector -> address"]
+    assert listing("v_readfirstlane_b32 s3, v1", "s_nop 4", load, "s_endpgm") == []
     mfma = "v_mfma_scale_f32_16x16x128_f8f6f4 a[4:7], v[8:11], v[12:15], a[4:7], v1, v2 op_sel_hi:[0,0,0] cbsz:4 blgp:4"
     for write in ("v_accvgpr_write_b32 a5, 0", "v_mov_b32_e32 v15, v3", "v_mov_b32_e32 v2, 0",
                   "v_permlane32_swap_b32_e32 v90, v8"):
