@@ -526,9 +526,9 @@ __global__ __launch_bounds__(kThreads) void heads_general_kernel(const Args p, i
     }
 }
 
+// As many tokens as one launch holds.
 template <bool BF16, bool NORM, int SINK>
-int launch(const char* fn, Args& p, hipStream_t stream) {
-    const int heads = (NORM ? p.q_heads : 0) + p.kv_heads + (SINK != kPlain ? p.kv_heads : 0);
+int launch_part(const char* fn, Args& p, int heads, hipStream_t stream) {
     const int D = p.D;
     // 16-byte slots where both halves of the rotation are whole slots, else 4 bf16
     const int wide = BF16 ? 8 : 4;
@@ -558,7 +558,6 @@ int launch(const char* fn, Args& p, hipStream_t stream) {
         p.splits = static_cast<int>(std::clamp<int64_t>((8192 + p.tokens - 1) / p.tokens, 1, p.groups));
         p.per_split = (p.groups + p.splits - 1) / p.splits;
         const int64_t grid = (p.tokens * p.splits + kWaves - 1) / kWaves;
-        if (grid > kc::kv::kMaxGrid) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
         // Nontemporal loads gain 3 to 8 % where the heads cannot lie in the Infinity Cache
         // (256 MB), in which a projection has just left them, and lose where they do (32 + 8
         // bf16 heads of 128: 2048 tokens 11.7 us against 10.3 with plain loads, 4096 17.9 and
@@ -578,10 +577,38 @@ int launch(const char* fn, Args& p, hipStream_t stream) {
         else heads_kernel<BF16, kWide, NORM, SINK, false, false><<<blocks, kThreads, 0, stream>>>(p);
     } else {
         const int64_t rows = p.tokens * heads, grid = (rows + kWaves - 1) / kWaves;
-        if (grid > kc::kv::kMaxGrid) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: too many tokens", fn);
         heads_general_kernel<BF16, NORM, SINK><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, rows);
     }
     return kc::check_launch(fn);
+}
+
+// A wave takes one head at least, so a launch holds every batch of up to kMaxGrid kWaves
+// heads; more are further launches.
+template <bool BF16, bool NORM, int SINK>
+int launch(const char* fn, Args& p, hipStream_t stream) {
+    using E = Elem<BF16>;
+    const int heads = (NORM ? p.q_heads : 0) + p.kv_heads + (SINK != kPlain ? p.kv_heads : 0);
+    const int64_t most = kc::kv::kMaxGrid * kWaves / heads, tokens = p.tokens;
+    for (int64_t t = 0; t < tokens; t += most) {
+        Args part = p;
+        part.tokens = std::min(most, tokens - t);
+        auto input = [&](const void*& x, int64_t stride) {
+            if (x) x = static_cast<const E*>(x) + t * stride;
+        };
+        auto output = [&](void*& y, int64_t n) {
+            if (y) y = static_cast<E*>(y) + t * n * p.D;
+        };
+        input(part.q, p.q_stride);
+        input(part.k, p.k_stride);
+        input(part.v, p.v_stride);
+        output(part.q_out, p.q_heads);
+        output(part.k_out, p.kv_heads);
+        if (part.positions) part.positions += t;
+        if (part.slots) part.slots += t;
+        const int st = launch_part<BF16, NORM, SINK>(fn, part, heads, stream);
+        if (st != KC_SUCCESS) return st;
+    }
+    return KC_SUCCESS;
 }
 
 int check_rope(const char* fn, const kc_rope* r, int head_dim, int64_t tokens) {

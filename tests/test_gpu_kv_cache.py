@@ -565,3 +565,31 @@ def test_fp8_scales_are_the_rounded_quotient(gpu, ops, D, dtype, fused):
     for i in (2,) if fused else (0, 2):
         np.testing.assert_array_equal(pool[i + 1][:, 0].cpu().numpy(), scale)
         np.testing.assert_array_equal(pool[i][:, 0].view(gpu.float8_e4m3fn).double().cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_more_rows_than_one_launch_holds(gpu, ops, dtype):
+    """Over 2^26 heads in one call (of 2 values: one wave each): the rows around every place
+    where a further launch can start, and the last ones, as by themselves."""
+    dt, T, D, Hkv = getattr(gpu, dtype), (1 << 25) + 77, 2, 1
+    g = gpu.Generator("cuda").manual_seed(5)
+    q, k, v = (gpu.randn(T, Hkv, D, generator=g, device="cuda").to(dt) for _ in range(3))
+    qg, kg = ((1 + 0.3 * gpu.randn(D, generator=g, device="cuda")).to(dt) for _ in range(2))
+    cos, sin = _tables(gpu, 50, 1)
+    pos = (gpu.arange(T, device="cuda") % 50).int()
+    slots = T - 1 - gpu.arange(T, device="cuda")
+    most = (1 << 24) - 1
+    at = sorted({a for n in (2, 3) for a in range(0, T, 4 * most // n)} | {T})
+    near = [slice(max(0, a - 40), min(T, a + 40)) for a in at]
+    whole = ops.qk_norm_rope(q, k, qg, kg, cos, sin, pos)
+    pools = [_pool(gpu, T, 1, Hkv, D, "fp8", 1) for _ in range(2)]
+    y = ops.qk_norm_rope_cache(q, k, v, qg, kg, cos, sin, pos, slots, *pools[0])
+    ops.kv_cache_write(whole[1], v, slots, *pools[1])
+    assert gpu.equal(y, whole[0]) and all(gpu.equal(a, b) for a, b in zip(*pools))
+    for s in near:
+        part = ops.qk_norm_rope(q[s], k[s], qg, kg, cos, sin, pos[s])
+        assert all(gpu.equal(a[s], b) for a, b in zip(whole, part))
+        for i, x in ((0, whole[1]), (2, v)):
+            c, scale = _rows_expected(gpu, ops, x[s], "fp8")
+            assert gpu.equal(pools[0][i].flatten(0, 1)[slots[s]], c)
+            assert gpu.equal(pools[0][i + 1].flatten(0, 1)[slots[s]], scale)
