@@ -50,7 +50,7 @@ constexpr int kWaves = kThreads / kWave;
 template <bool BF16>
 using Elem = std::conditional_t<BF16, uint16_t, float>;
 
-enum Sink { kPlain, kFp8, kMx };
+enum Sink { kPlain, kFp8, kMx, kMxAcross };  // kMxAcross: blocks of 32 in any lanes' slots
 
 struct Args {
     const void *q, *k, *v;            // heads of a token are D apart
@@ -207,6 +207,13 @@ __device__ __forceinline__ void store_mx(uint8_t* dst, const float (&v)[W], uint
     }
 }
 
+// What the lanes of a wave wrote to its LDS before, they read behind it (LDS takes a wave's
+// accesses in order).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // The two slots of lane j of `lanes`: `apart`, the head's pairs are half a rotation
 // apart (`half` slots).
 struct Slots {
@@ -235,6 +242,7 @@ struct Place {
 template <bool BF16, int W, bool NORM, int SINK, bool STREAM, bool EVEN>
 __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
     using S = Slot<BF16, W>;
+    __shared__ __align__(16) uint32_t slot_tops[SINK == kMxAcross ? kWaves : 1][2 * kWave];
     const int lane = threadIdx.x & (kWave - 1);
     const int64_t w = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t t = w / p.splits;
@@ -415,18 +423,46 @@ __global__ __launch_bounds__(kThreads, 5) void heads_kernel(const Args p) {
                 if (j == 0) static_cast<float*>(scales)[row] = d.s;
             }
         } else {
-            // A block is 32 / W slots: of so many lanes' first (second) slots in a run,
-            // of half as many lanes' slot pairs.
-            const bool run = p.runs || (o.apart && j < half);
-            const uint32_t ma = absmax_bits<W>(a), mb = absmax_bits<W>(b), mab = max(ma, mb);
-            const uint32_t ra2 = W == 8 ? max_quad(ma) : max_oct(ma), rb2 = W == 8 ? max_quad(mb) : max_oct(mb);
-            const uint32_t pr = W == 8 ? max_pair(mab) : max_quad(mab);
-            const uint32_t ba = scale_byte(run ? ra2 : pr), bb = scale_byte(run ? rb2 : pr);
+            constexpr int kSlots = kBlock / W;
+            const uint32_t ma = absmax_bits<W>(a), mb = absmax_bits<W>(b);
+            uint32_t ba, bb;
+            bool run;
+            if constexpr (SINK == kMxAcross) {
+                // Half a rotation is no whole number of blocks: the slots' maxima meet
+                // in the wave's own LDS, in the head's order (8000 tokens of 32 + 8 bf16
+                // heads of 96, all of them turned, 31.5 us, of 128 with a quarter turned
+                // 38.6; by one wave a head 196 and 204).
+                uint32_t* tops = slot_tops[threadIdx.x >> 6] + (lane >> lg << (lg + 1));
+                if (has) {
+                    tops[o.s.a] = ma;
+                    tops[o.s.b] = mb;
+                }
+                wave_sync();
+                auto top = [&](int slot) {
+                    const u32x4* q = reinterpret_cast<const u32x4*>(tops + slot / kSlots * kSlots);
+                    uint32_t m = 0;
+#pragma unroll
+                    for (int i = 0; i < kSlots / 4; ++i) m = max(m, max(max(q[i].x, q[i].y), max(q[i].z, q[i].w)));
+                    return m;
+                };
+                ba = scale_byte(has ? top(o.s.a) : 0u);
+                bb = scale_byte(has ? top(o.s.b) : 0u);
+                run = true;
+                wave_sync();
+            } else {
+                // A block is 32 / W slots: of so many lanes' first (second) slots in a run,
+                // of half as many lanes' slot pairs.
+                run = p.runs || (o.apart && j < half);
+                const uint32_t mab = max(ma, mb);
+                const uint32_t ra2 = W == 8 ? max_quad(ma) : max_oct(ma), rb2 = W == 8 ? max_quad(mb) : max_oct(mb);
+                const uint32_t pr = W == 8 ? max_pair(mab) : max_quad(mab);
+                ba = scale_byte(run ? ra2 : pr);
+                bb = scale_byte(run ? rb2 : pr);
+            }
             if (out) {
                 uint8_t* dst = codes + row * (D / 2);
                 store_mx<W>(dst + W / 2 * o.s.a, a, ba);
                 store_mx<W>(dst + W / 2 * o.s.b, b, bb);
-                constexpr int kSlots = kBlock / W;
                 uint8_t* sc = static_cast<uint8_t*>(scales) + row * (D / kBlock);
                 if (o.s.a % kSlots == 0) sc[o.s.a / kSlots] = static_cast<uint8_t>(ba);
                 if (run && o.s.b % kSlots == 0) sc[o.s.b / kSlots] = static_cast<uint8_t>(bb);
@@ -545,9 +581,7 @@ int launch_part(const char* fn, Args& p, int heads, hipStream_t stream) {
     if (SINK == kPlain) vec = vec && whole(p.k_out);
     else vec = vec && rows_ok(p.v, p.v_stride);
     if (SINK == kFp8) vec = vec && kc::aligned(p.k_codes, (NORM ? 1 : 2) * p.width) && kc::aligned(p.v_codes, (NORM ? 1 : 2) * p.width);
-    if (SINK == kMx)  // whole blocks in the lanes that share a maximum
-        vec = vec && kc::aligned(p.k_codes, 4) && kc::aligned(p.v_codes, 4) &&
-              (!NORM || p.interleaved || p.R % 64 == 0);
+    if (SINK == kMx) vec = vec && kc::aligned(p.k_codes, 4) && kc::aligned(p.v_codes, 4);
     if (vec) {
         p.lanes_log2 = 0;
         while ((1 << p.lanes_log2) * 2 * p.width < D) ++p.lanes_log2;
@@ -570,11 +604,20 @@ int launch_part(const char* fn, Args& p, int heads, hipStream_t stream) {
         const unsigned blocks = static_cast<unsigned>(grid);
         constexpr int kWide = BF16 ? 8 : 4;
         const bool even = (NORM ? p.q_heads : 0) % hp == 0 && p.kv_heads % hp == 0;
-        if (p.width < wide) heads_kernel<BF16, 4, NORM, SINK, false, false><<<blocks, kThreads, 0, stream>>>(p);
-        else if (stream_heads && even) heads_kernel<BF16, kWide, NORM, SINK, true, true><<<blocks, kThreads, 0, stream>>>(p);
-        else if (stream_heads) heads_kernel<BF16, kWide, NORM, SINK, true, false><<<blocks, kThreads, 0, stream>>>(p);
-        else if (even) heads_kernel<BF16, kWide, NORM, SINK, false, true><<<blocks, kThreads, 0, stream>>>(p);
-        else heads_kernel<BF16, kWide, NORM, SINK, false, false><<<blocks, kThreads, 0, stream>>>(p);
+        auto run = [&](auto sink) {
+            constexpr int kTo = decltype(sink)::value;
+            if (p.width < wide) heads_kernel<BF16, 4, NORM, kTo, false, false><<<blocks, kThreads, 0, stream>>>(p);
+            else if (stream_heads && even) heads_kernel<BF16, kWide, NORM, kTo, true, true><<<blocks, kThreads, 0, stream>>>(p);
+            else if (stream_heads) heads_kernel<BF16, kWide, NORM, kTo, true, false><<<blocks, kThreads, 0, stream>>>(p);
+            else if (even) heads_kernel<BF16, kWide, NORM, kTo, false, true><<<blocks, kThreads, 0, stream>>>(p);
+            else heads_kernel<BF16, kWide, NORM, kTo, false, false><<<blocks, kThreads, 0, stream>>>(p);
+        };
+        if constexpr (NORM && SINK == kMx) {
+            if (!p.interleaved && p.R % 64 != 0) run(std::integral_constant<int, kMxAcross>{});
+            else run(std::integral_constant<int, kMx>{});
+        } else {
+            run(std::integral_constant<int, SINK>{});
+        }
     } else {
         const int64_t rows = p.tokens * heads, grid = (rows + kWaves - 1) / kWaves;
         heads_general_kernel<BF16, NORM, SINK><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(p, rows);

@@ -593,3 +593,63 @@ def test_more_rows_than_one_launch_holds(gpu, ops, dtype):
             c, scale = _rows_expected(gpu, ops, x[s], "fp8")
             assert gpu.equal(pools[0][i].flatten(0, 1)[slots[s]], c)
             assert gpu.equal(pools[0][i + 1].flatten(0, 1)[slots[s]], scale)
+
+
+ACROSS = [(32, 16), (32, 8), (64, 16), (64, 40), (96, 96), (96, 32), (96, 48), (128, 32), (128, 96), (128, 24), (160, 80),
+          (192, 96), (224, 224), (256, 96), (512, 160), (576, 48), (1024, 96)]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("Hq,Hkv,T", [(8, 8, 5), (7, 3, 9), (0, 1, 1), (4, 2, 700)])
+@pytest.mark.parametrize("D,R", ACROSS)
+def test_mxfp4_blocks_across_half_rotations(gpu, ops, D, R, Hq, Hkv, T, dtype):
+    """Half-split heads whose half rotation is no whole number of blocks of 32: the fused
+    call's cache is that of the two calls, with zeros, a NaN and an infinity among the values."""
+    dt = getattr(gpu, dtype)
+    q, k, v, qg, kg = _heads(gpu, T, Hq, Hkv, D, dt, seed=D + R)
+    v[0, 0, D - 1] = float("inf")
+    v[-1, -1, :8] = float("nan")
+    k[-1, 0, D // 2] = float("nan")
+    v[T // 2, 0] = 0
+    cos, sin = _tables(gpu, 64, R // 2)
+    pos = (gpu.arange(T, device="cuda") % 64).int()
+    pages = T // 16 + 2
+    slots = gpu.randperm(pages * 16, device="cuda")[:T]
+    one, two = (_pool(gpu, pages, 16, Hkv, D, "mxfp4", 1) for _ in range(2))
+    yq = ops.qk_norm_rope_cache(q, k, v, qg, kg, cos, sin, pos, slots, *one)
+    wq, wk = ops.qk_norm_rope(q, k, qg, kg, cos, sin, pos)
+    ops.kv_cache_write(wk, v, slots, *two)
+    assert gpu.equal(yq, wq)
+    assert all(gpu.equal(a, b) for a, b in zip(one, two))
+
+
+@pytest.mark.parametrize("D,R", [(96, 96), (128, 32)])
+def test_mxfp4_fused_write_is_no_slower_than_two_calls(gpu, ops, D, R):
+    """Half a rotation that is no whole number of blocks keeps the kernel that a whole one has
+    (one wave a head was 4 to 5 times the two calls' time; the bound is 1.5)."""
+    torch, T, Hq, Hkv = gpu, 8000, 32, 8
+    q, k, v, qg, kg = _heads(torch, T, Hq, Hkv, D, torch.bfloat16)
+    cos, sin = _tables(torch, 100, R // 2)
+    pos, slots = (torch.arange(T, device="cuda") % 100).int(), torch.randperm(T, device="cuda")
+    pool = _pool(torch, T // 16, 16, Hkv, D, "mxfp4")
+
+    def fused():
+        ops.qk_norm_rope_cache(q, k, v, qg, kg, cos, sin, pos, slots, *pool)
+
+    def two():
+        ops.kv_cache_write(ops.qk_norm_rope(q, k, qg, kg, cos, sin, pos)[1], v, slots, *pool)
+
+    def least(f):
+        f()
+        times = []
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                f()
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert least(fused) <= 1.5 * least(two)
