@@ -70,7 +70,7 @@ def fp8_bytes(rows: int, cols: int) -> int:
 
 
 GEMV_SOURCES = ("kernel-craft_amd/csrc/gemv_chain.hip", "kernel-craft_amd/csrc/int4_decode.hpp",
-                "kernel-craft_amd/csrc/kc_common.hpp")
+                "kernel-craft_amd/csrc/kc_common.hpp", "kernel-craft_amd/csrc/lds_dma.hpp")
 
 
 def source_sha256(paths=GEMV_SOURCES) -> str:
