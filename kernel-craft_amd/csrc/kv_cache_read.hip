@@ -4,8 +4,8 @@
 // position t - cu_seqlens[b] in it, page block_table[b][position / page_size].
 //
 // Bound by memory: 1 (FP8) or 0.53 (MXFP4) bytes in and 2 or 4 out per value (45 000
-// tokens of 8 heads of 128, keys and values: FP8 to bf16 50 us, 5.4 TB/s, MXFP4 34.9,
-// 6.3; FP8 to fp32 84).  A workgroup takes a tile of tokens: its first threads find one
+// tokens of 8 heads of 128, keys and values: FP8 to bf16 50 to 54 us, 5.2 to 5.6 TB/s,
+// MXFP4 35 to 36; FP8 to fp32 84).  A workgroup takes a tile of tokens: its first threads find one
 // token's slot each (a binary search of cu_seqlens, in LDS up to 1023 sequences, all
 // searches of the tile at once instead of one before every row), then all threads walk
 // the rows in units of 16 bytes of output, four keys and four values in flight each

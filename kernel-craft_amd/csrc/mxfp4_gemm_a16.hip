@@ -274,14 +274,16 @@ int launch(const char* fn, const uint8_t* qw, const uint8_t* sw, const uint16_t*
 // workgroup takes in hundredths of a microsecond per step of 256 values and beside
 // the steps, with every CU holding one (fitted to K 4096, 8192 and 14336).  More rows
 // share the reads of X, more tokens those of the weights and their decoding, fewer of
-// both fill the CUs: M 13, N 28672, K 4096 13.8 us with 1 and 7, 15.5 with 1 and 4, 26.6
-// with 1 and 1; M 13, N 4096, K 14336 15.1 with 1 and 1, 23.4 with 1 and 4; M 64, same
-// N and K 24.8 with 1 and 4, 37.3 with 2 and 4, 62 with 3 and 7; M 32, N 28672, K 4096
-// 18.6 with 2 and 7, 30.4 with 1 and 4.
+// both fill the CUs: M 13, N 28672, K 4096 14.1 us with 1 and 7, 15.4 with 1 and 4, 29.8
+// with 1 and 1; M 13, N 4096, K 14336 14.9 with 1 and 1, 23.2 with 1 and 4; M 64, same
+// N and K 24.5 with 1 and 4, 37.0 with 2 and 4, 62 with 3 and 7; M 32, N 28672, K 4096
+// 19.8 with 2 and 7, 30.4 with 1 and 4.
 // The last four are the kernel of mxfp4_gemm_a16_tile.hip (128 rows; K a multiple of
-// 128): M 64, N 28672, K 4096 23 us against 36 with 2 and 7; M 128 36 with 128 tokens, 40
-// with 64; M 2048, N 4096 72 and 81; M 64, N 14336 16.5 in tiles of 32 tokens, 21.2 in one
-// of 64; M 128, N 6144 15.6 and 19.7 (18.6 with 1 and 7).
+// 128): M 64, N 28672, K 4096 24 us against 38 with 2 and 7; M 128 39 with 128 tokens, 43
+// with 64; M 2048, N 4096 78 and 86; M 64, N 14336 16.9 in tiles of 32 tokens, 21.2 in one
+// of 64; M 128, N 6144 15.5 and 19.4 (27 with 1 and 7).  The expected times are up to 10 % over and 30 % under the
+// measured ones (most where X comes from L2 many times); on 21 shapes of 2 to 2048 tokens
+// the least of them is the fastest.
 struct Cost {
     int mt, rt, step, fixed;
 };

@@ -18,7 +18,7 @@
 // wave, which issues in order, from those until LDS has taken them (M 128, N 4096,
 // K 4096 in tiles of 64 tokens 21.8 -> 17.8 us, of 128 36 -> 30.5).  Full grids are bound by
 // the arrival of the steps (512 bytes of X a token and 128 of codes a row, 10 TB/s): M 64,
-// N 28672, K 4096 23 us, the weights alone 10.5; M 128 36.  128 tokens take half the
+// N 28672, K 4096 24 us, the weights alone 10.5; M 128 38.  128 tokens take half the
 // reads of W and its decoding, and steps of 128 values, since 256 leave one buffer.
 //
 // Rows past M or N load the last row and feed outputs that are not stored.  K is a

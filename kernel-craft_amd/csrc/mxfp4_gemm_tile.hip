@@ -16,8 +16,9 @@
 //
 // LDS sets the wave tile: per half step a wave reads TM + TN operands (8 clocks
 // each) for TM TN MFMAs of 16 clocks on its own SIMD, and the tile's bytes are
-// written there too.  8 x 8 on four waves needs three quarters of the LDS clocks that
-// its MFMAs take, 8 x 4 on eight waves all of them.
+// written there too (128 a clock).  8 x 8 on four waves needs three quarters of the LDS
+// clocks that its MFMAs take, 8 x 4 on eight waves all of them, 4 x 2 on eight waves
+// (128 x 128) about 910 (counted) for 512 of MFMAs, of the 1290 that a step takes there.
 //
 // Scales.  Four steps need 32 scale bytes of every row.  Their bytes come one group of
 // four steps ahead; each thread sorts its rows' so that a lane's bytes are neighbours
@@ -52,7 +53,7 @@ constexpr int kGroupM = 4;    // row tiles walked together
 // the upper half, then the others (rows 0-3 and 12-15 of chunk c with rows 4-11 of chunk
 // c + 2): the pairs of rows take the eight slots in an order that gives each such sixteen
 // different banks.  With row / 2 for the order they meet two by two: M 1000, N 4096, K 14336
-// 5.6e6 clocks of conflicts against 1.9e6, and the prefill product 0.6 % slower.
+// 5.6e6 clocks of conflicts against 1.9e6 (on four waves; 2.7e6 on eight), and the prefill product 0.6 % slower.
 __device__ __forceinline__ int swizzle(int row) {
     const int j = row >> 1;
     return (j & 1) | (j >> 1 & 2) | ((j << 1 ^ j) & 4);
@@ -462,7 +463,8 @@ int launch(const char* fn, const uint8_t* qx, const uint8_t* sx, const uint8_t* 
 // Tiles, and what one costs a CU in hundredths of a microsecond: per step of 256
 // values, and beside the steps (start, first loads, stores), alone on its CU and
 // as one of two.  Measured with K 1024 to 14336 on grids of 64 to 1024 tiles; the
-// least expected time wins (27 shapes: the fastest tile, but for 5 % on one).  Against
+// least expected time wins (22 shapes of 64 to 8192 rows: the fastest tile on 18, 8 % from it on
+// one, 3 % at most on the others).  Against
 // the 256 x 256 tile: M 128, N 4096, K 4096 29.1 -> 6.8 us (32 x 64); M 1000, N 4096,
 // K 14336 103 -> 41.5 (128 x 128, eight waves and four buffers, one a CU; four waves 43.1);
 // M 500, N 6144, K 4096 32.9 -> 14.8 (the same); M 64, N 28672, K 4096 32.0 -> 15.1 (64 x 128); M 2048, N 4096, K 4096 34.2 ->
