@@ -653,3 +653,51 @@ def test_mxfp4_fused_write_is_no_slower_than_two_calls(gpu, ops, D, R):
         return min(times)
 
     assert least(fused) <= 1.5 * least(two)
+
+
+@pytest.mark.parametrize("fmt,D", [("fp8", 128), ("fp8", 33), ("mxfp4", 128), ("mxfp4", 96)])
+def test_a_pool_without_pages(gpu, ops, fmt, D):
+    """No page: every slot is outside, every position reads as NaN."""
+    q, k, v, qg, kg = _heads(gpu, 5, 4, 2, D, gpu.bfloat16)
+    cos, sin = _tables(gpu, 5, D // 2)
+    pos, slots = gpu.arange(5, device="cuda").int(), gpu.arange(5, device="cuda")
+    pool = _pool(gpu, 0, 16, 2, D, fmt)
+    ops.kv_cache_write(k, v, slots, *pool)
+    y = ops.qk_norm_rope_cache(q, k, v, qg, kg, cos, sin, pos, slots, *pool)
+    assert gpu.equal(y, ops.qk_norm_rope(q, k, qg, kg, cos, sin, pos)[0])
+    got = ops.kv_cache_read(*pool, gpu.zeros(1, 1, dtype=gpu.int32, device="cuda"),
+                            gpu.tensor([0, 5], dtype=gpu.int32, device="cuda"), 5)
+    assert all(bool(gpu.isnan(t).all()) for t in got)
+
+
+def test_calls_on_two_streams_at_once(gpu, ops):
+    """The operators keep nothing between calls: two batches on two streams, many times, give
+    what they give alone."""
+    torch = gpu
+    w, ws = ops.mxfp4_quantize(torch.randn(768, 512, device="cuda") * 0.05)
+    cos, sin = _tables(torch, 300, 32)
+    gam = torch.ones(64, device="cuda").bfloat16()
+
+    def layer(x, pool):
+        qkv = ops.mxfp4_gemm_w4a4(*ops.mxfp4_quantize(x), w, ws).unflatten(1, (12, 64))
+        T = x.shape[0]
+        pos = torch.arange(T, device="cuda", dtype=torch.int32)
+        q = ops.qk_norm_rope_cache(qkv[:, :8], qkv[:, 8:10], qkv[:, 10:], gam, gam, cos, sin, pos, pos.long(), *pool)
+        return (q, *ops.kv_cache_read(*pool, torch.arange(20, device="cuda", dtype=torch.int32)[None],
+                                      torch.tensor([0, T], dtype=torch.int32, device="cuda"), T),
+                ops.mxfp4_gemm_bf16(w, ws, x))
+
+    xs = [torch.randn(T, 512, device="cuda").bfloat16() for T in (1, 300)]
+    pools = [_pool(torch, 20, 16, 2, 64, fmt) for fmt in ("fp8", "mxfp4")]
+    want = [layer(x, p) for x, p in zip(xs, pools)]
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(layer(xs[i], pools[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(out, want[i]))

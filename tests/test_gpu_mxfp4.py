@@ -426,3 +426,28 @@ def test_a16_nan_scale_marks_its_column(gpu, ops, M, K):
     want = np.zeros(N, bool)
     want[[9, 69]] = True
     assert (gpu.isnan(y).cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("M,K", A16_KERNELS + [(20, 96), (64, 2176), (300, 2176), (300, 2080)])
+def test_quantized_nan_blocks_reach_every_product(gpu, ops, M, K):
+    """A weight block with a NaN or an infinity, as the quantizer stores it (codes 0, byte 255):
+    its column is NaN in both products, nothing else is; and so for a token's block."""
+    g = gpu.Generator("cuda").manual_seed(M)
+    N = 16500 if M == 100 else 300
+    w = gpu.randn(N, K, generator=g, device="cuda")
+    w[7, K - 1] = float("nan")
+    w[N - 1, 3] = float("inf")
+    qw, sw = ops.mxfp4_quantize(w)
+    assert int(sw[7, -1]) == 255 and not qw[7, -16:].any()
+    x = gpu.randn(M, K, generator=g, device="cuda").bfloat16()
+    cols = gpu.zeros(N, dtype=gpu.bool, device="cuda")
+    cols[[7, N - 1]] = True
+    assert gpu.equal(gpu.isnan(ops.mxfp4_gemm_bf16(qw, sw, x)), cols[None].expand(M, N))
+    for out in (gpu.bfloat16, gpu.float32):
+        assert gpu.equal(gpu.isnan(ops.mxfp4_gemm_w4a4(*ops.mxfp4_quantize(x), qw, sw, out_dtype=out)), cols[None].expand(M, N))
+    x[M // 2, K // 2] = float("nan")
+    rows = gpu.zeros(M, dtype=gpu.bool, device="cuda")
+    rows[M // 2] = True
+    want = rows[:, None] | cols
+    assert gpu.equal(gpu.isnan(ops.mxfp4_gemm_bf16(qw, sw, x)), want)
+    assert gpu.equal(gpu.isnan(ops.mxfp4_gemm_w4a4(*ops.mxfp4_quantize(x), qw, sw)), want)
