@@ -461,6 +461,126 @@ int kc_kv_cache_read_f32(const kc_kv_cache* cache, const int32_t* d_block_table,
                          int seqs, int64_t total_tokens, float* d_k, float* d_v,
                          kc_stream_t stream);
 
+/* Attention of one token per sequence over that cache (the reference's
+ * paged_attention.cu:135-142 reads fp32 pools): q and out [seqs, q_heads,
+ * head_dim] (q_stride elements from one sequence's heads to the next), q_heads
+ * a multiple of kv_heads, whose query heads stand together.
+ *   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q.k_t - max)
+ * over the positions t of the sequence: all of the seq_lens[b] (int32) that it
+ * has in the cache, the new token's own among them, or the last `window` of
+ * them (0: all).  Computed in fp32 from the values that kc_kv_cache_read_f32
+ * gives and rounded once; results do not depend on what other sequences of
+ * the batch hold beyond the order in which a long sum is split.  A sequence
+ * without tokens (a length of 0 or below) gives zeros; one with a visible
+ * position whose page is missing (past max_pages, or an entry outside the
+ * pool) gives NaN.  What the cache holds behind a sequence's end, or outside
+ * of its window, does not matter, NaN included.  At most 2^31 - 1 slots,
+ * seqs * q_heads below 2^24.
+ *
+ * The workspace (16-byte aligned) holds what the parts of a long sequence
+ * give before they are joined: kc_kv_cache_attention_workspace() bytes (-1
+ * for arguments that the call refuses), with any content, used by one call at
+ * a time. */
+int64_t kc_kv_cache_attention_workspace(const kc_kv_cache* cache,
+                                        int64_t max_pages, int seqs,
+                                        int q_heads);
+int kc_kv_cache_attention_bf16(const uint16_t* d_q, int64_t q_stride,
+                               int q_heads, const kc_kv_cache* cache,
+                               const int32_t* d_block_table, int64_t max_pages,
+                               const int32_t* d_seq_lens, int seqs, float scale,
+                               int window, void* d_workspace,
+                               int64_t workspace_bytes, uint16_t* d_out,
+                               kc_stream_t stream);
+int kc_kv_cache_attention_f32(const float* d_q, int64_t q_stride, int q_heads,
+                              const kc_kv_cache* cache,
+                              const int32_t* d_block_table, int64_t max_pages,
+                              const int32_t* d_seq_lens, int seqs, float scale,
+                              int window, void* d_workspace,
+                              int64_t workspace_bytes, float* d_out,
+                              kc_stream_t stream);
+
+/* The pages of a cache: a block table [seqs, max_pages] int32, and a stack of
+ * free pages, free_pages[0 .. free_count - 1] of num_pages int32 entries. */
+typedef struct kc_kv_pages {
+    int32_t* block_table;
+    int32_t* free_pages;
+    const int32_t* free_count;
+    int64_t max_pages, num_pages;
+    int page_size, seqs;
+} kc_kv_pages;
+
+/* Pages for the next tokens of a batch, and where those tokens go.  Request b
+ * has seq_lens[b] tokens in the cache and new_lens[b] new ones (int32 [seqs],
+ * negative counts as 0), which stand packed, request after request, in
+ * total_new rows.  In order, each request takes the pages that it lacks from
+ * the top of the stack and writes them behind its others in block_table.  It
+ * is served whole or not at all: not if it would pass max_pages, if its rows
+ * pass total_new, or if it lacks pages and they, together with what the
+ * requests before it asked for, are more than the stack has (a request that
+ * lacks none is served all the same).
+ *   seq_lens_out [seqs]   lengths with the new tokens of those served
+ *   free_count_out [1]    pages left on the stack
+ *   cu_new [seqs + 1]     first row of each request
+ *   cu_seqlens [seqs + 1] sums of seq_lens_out, for kc_kv_cache_read_*
+ *   positions [total_new], slots [total_new] (int64) of the rows for
+ *     kc_qk_norm_rope_cache_*; -1 (padding there) for requests that are not
+ *     served and for rows behind the last request
+ * (cu_* past 2^31 - 1 stay at it).  Inputs are left as they are but for new
+ * entries of block_table, and no output may overlap them, so a call that is
+ * repeated gives the same again.  seqs up to 2^24. */
+int kc_kv_cache_extend(const kc_kv_pages* pages, const int32_t* d_seq_lens,
+                       const int32_t* d_new_lens, int64_t total_new,
+                       int32_t* d_seq_lens_out, int32_t* d_free_count_out,
+                       int32_t* d_cu_new, int32_t* d_cu_seqlens,
+                       int32_t* d_positions, int64_t* d_slots,
+                       kc_stream_t stream);
+/* The pages of the sequences with finished[b] != 0 (u8 [seqs]) back onto the
+ * stack, in order: free_pages is written from free_count on (pages past
+ * num_pages are dropped), seq_lens_out is 0 for them.  block_table stays. */
+int kc_kv_cache_release(const kc_kv_pages* pages, const uint8_t* d_finished,
+                        const int32_t* d_seq_lens, int32_t* d_seq_lens_out,
+                        int32_t* d_free_count_out, kc_stream_t stream);
+
+/* The residual sum between two blocks of a decoder and the norms on both of
+ * its sides (the reference normalizes whole rows alone, rmsnorm.cu:40-70):
+ * of a block's output y [rows, cols] and the residual stream h,
+ *   b     = post_gamma ? post_gamma * y / sqrt(mean(y^2) + eps) : y
+ *   h_out = h + alpha * gate * b
+ *   n     = gamma * h_out / sqrt(mean(h_out^2) + eps), h_out before rounding
+ * in fp32, each output rounded once.  gate may be null (1), one row [cols]
+ * (gate_stride 0) or [rows, cols]; post_gamma may be null.  y, gate and the
+ * gammas (and n) are of the type in the name, h and h_out of the second type
+ * where it has two.  Strides are elements between rows; h_out, n and codes
+ * are contiguous and overlap no input.  cols up to 32768.
+ * kc_residual_rmsnorm_quantize_fp8_* quantizes n from fp32 as
+ * kc_quantize_fp8_per_token_f32 does. */
+typedef struct kc_residual {
+    const void* y;
+    const void* h;
+    const void* gate;
+    const void* post_gamma;
+    const void* gamma;
+    int64_t y_stride, h_stride, gate_stride, rows;
+    int cols;
+    float alpha, eps;
+} kc_residual;
+int kc_residual_rmsnorm_bf16(const kc_residual* args, uint16_t* d_h_out,
+                             uint16_t* d_n, kc_stream_t stream);
+int kc_residual_rmsnorm_bf16_f32(const kc_residual* args, float* d_h_out,
+                                 uint16_t* d_n, kc_stream_t stream);
+int kc_residual_rmsnorm_f32(const kc_residual* args, float* d_h_out,
+                            float* d_n, kc_stream_t stream);
+int kc_residual_rmsnorm_quantize_fp8_bf16(const kc_residual* args,
+                                          uint16_t* d_h_out, int8_t* d_codes,
+                                          float* d_scales, kc_stream_t stream);
+int kc_residual_rmsnorm_quantize_fp8_bf16_f32(const kc_residual* args,
+                                              float* d_h_out, int8_t* d_codes,
+                                              float* d_scales,
+                                              kc_stream_t stream);
+int kc_residual_rmsnorm_quantize_fp8_f32(const kc_residual* args,
+                                         float* d_h_out, int8_t* d_codes,
+                                         float* d_scales, kc_stream_t stream);
+
 /* ======================================================================
  * Part 4 -- out-of-scope reference symbols (stubs).  Signatures from the
  * reference files cited; bound by kernel_craft_torch_ops.py:101-168 and

@@ -1,0 +1,333 @@
+// kv_cache_attention.hip -- attention of each sequence's newest token over the quantized
+// paged cache on gfx950 (what qk_norm_rope.hip wrote):
+//     out[b, h] = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale q[b, h] . k_t - max)
+// over the visible positions t of sequence b, k and v the rows' values in fp32.  Here the
+// vector kernel for any head_dim and alignment, the join and the entry points; kv_attention.hpp
+// says how the work is split.
+#include <algorithm>
+#include <type_traits>
+
+#include "kv_attention.hpp"
+
+namespace {
+
+using namespace kc::kv;
+using namespace kc::mx;
+using kc::kWave;
+
+template <bool BF16>
+using Elem = std::conditional_t<BF16, uint16_t, float>;
+
+template <bool BF16>
+__device__ __forceinline__ float get(const Elem<BF16>* p, int64_t i) {
+    if constexpr (BF16) return kc::bf16_to_f32(p[i]);
+    else return p[i];
+}
+template <bool BF16>
+__device__ __forceinline__ void put(Elem<BF16>* p, int64_t i, float v) {
+    if constexpr (BF16) p[i] = kc::f32_to_bf16(v);
+    else p[i] = v;
+}
+
+constexpr int kHeads = 4;  // query heads of a wave of the vector kernel
+
+// Value d of the row `row` (slot * kv_heads + head); FP8 without its scale.
+template <bool FP8>
+__device__ __forceinline__ float value(const uint8_t* codes, const void* scales, int64_t row, int D, int d) {
+    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8(codes[row * D + d], 0);
+    const uint32_t c = codes[(row * D + d) / 2] >> (4 * (d & 1));
+    return decode4_f32(c & 15u, scale_value(static_cast<const uint8_t*>(scales)[(row * D + d) / kBlock])).x;
+}
+
+// A wave takes kHeads query heads of one key/value head.  Scores: a lane per position and
+// half of the head; output: a lane per NI values of the head.
+template <bool BF16, bool FP8, int NI>
+__global__ __launch_bounds__(256) void attention_kernel(const Attention p) {
+    __shared__ PlanShared plan;
+    extern __shared__ float lds[];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    float* ql = lds + wave * (kHeads * p.D + (kHeads + 1) * kTile);
+    float* pl = ql + kHeads * p.D;
+    int* sl = reinterpret_cast<int*>(pl + kHeads * kTile);
+    const int set = blockIdx.y * p.wg_sets + wave % p.wg_sets;
+    Stretch s = find_stretch(p, plan, wave / p.wg_sets);
+    if (s.b < 0 || set >= p.sets) return;
+    const int per_kv = (p.group + kHeads - 1) / kHeads, h = set / per_kv, q0 = (set - h * per_kv) * kHeads;
+    const int heads = min(kHeads, p.group - q0);
+    const float nan = __uint_as_float(0x7FC00000u), inf = __uint_as_float(0x7F800000u);
+
+    for (int b = s.b; b < p.seqs; ++b) {
+        const Visible vis = visible(p, b);
+        const int tiles = vis.tiles();
+        const int64_t end = min(s.end, s.first + tiles);
+        const int64_t head0 = static_cast<int64_t>(h) * p.group + q0;
+        Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(b) * p.q_heads + head0) * p.D;
+        if (tiles == 0) {
+            if (p.units != 0) continue;  // the join's
+            for (int i = lane; i < heads * p.D; i += kWave) put<BF16>(out, i, 0.0f);
+            return;
+        }
+        const Elem<BF16>* q = static_cast<const Elem<BF16>*>(p.q) + b * p.q_stride + head0 * p.D;
+        for (int i = lane; i < kHeads * p.D; i += kWave) ql[i] = i < heads * p.D ? get<BF16>(q, i) : 0.0f;
+        float m[kHeads], l[kHeads], acc[kHeads][NI];
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j) {
+            m[j] = -inf;
+            l[j] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) acc[j][i] = 0.0f;
+        }
+        for (int64_t tile = s.tile; tile < end; ++tile) {
+            const int base = (vis.first / kTile + static_cast<int>(tile - s.first)) * kTile;
+            const int t = lane & (kTile - 1), half = lane / kTile, pos = base + t;
+            const bool seen = pos >= vis.first && pos < vis.end;
+            const int slot = seen ? slot_of(p, b, pos) : -1;
+            float sc[kHeads] = {}, vs = 1.0f;
+            if (slot >= 0) {
+                const int64_t row = static_cast<int64_t>(slot) * p.kv_heads + h;
+                for (int d = half; d < p.D; d += 2) {
+                    const float k = value<FP8>(p.k_codes, p.k_scales, row, p.D, d);
+#pragma unroll
+                    for (int j = 0; j < kHeads; ++j) sc[j] = fmaf(ql[j * p.D + d], k, sc[j]);
+                }
+                float ks = p.scale;
+                if constexpr (FP8) {
+                    ks *= static_cast<const float*>(p.k_scales)[row];
+                    vs = static_cast<const float*>(p.v_scales)[row];
+                }
+#pragma unroll
+                for (int j = 0; j < kHeads; ++j) sc[j] *= ks;
+            }
+            if (half == 0) sl[t] = slot;
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j) {
+                float v = sc[j] + __shfl_xor(sc[j], kTile, kWave);
+                if (slot < 0) v = nan;
+                const float most = fmaxf(m[j], kc::wave_max(seen ? v : -inf));
+                const float at = most == -inf ? 0.0f : most, by = __builtin_amdgcn_exp2f(m[j] - at);
+                const float e = seen ? __builtin_amdgcn_exp2f(v - at) : 0.0f;
+                m[j] = most;
+                l[j] = fmaf(l[j], by, kc::wave_sum(half == 0 ? e : 0.0f));
+                if (half == 0) pl[j * kTile + t] = seen ? e * vs : 0.0f;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) acc[j][i] *= by;
+            }
+            __builtin_amdgcn_wave_barrier();
+            for (int u = 0; u < kTile; ++u) {
+                const int at = sl[u];
+                const int64_t row = static_cast<int64_t>(at) * p.kv_heads + h;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const int d = lane + i * kWave;
+                    const float v = at >= 0 && d < p.D ? value<FP8>(p.v_codes, p.v_scales, row, p.D, d) : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kHeads; ++j) acc[j][i] = fmaf(pl[j * kTile + u], v, acc[j][i]);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        const bool whole = holds_all(s, s.tile, end, tiles);
+        const int64_t segment = (static_cast<int64_t>(s.unit) + b) * p.q_heads + head0;
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j) {
+            if (j >= heads) break;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int d = lane + i * kWave;
+                if (d >= p.D) break;
+                if (whole) put<BF16>(out, j * p.D + d, acc[j][i] / l[j]);
+                else p.part_o[(segment + j) * p.D + d] = acc[j][i];
+            }
+            if (!whole && lane == 0) {
+                p.part_ml[(segment + j) * 2] = m[j];
+                p.part_ml[(segment + j) * 2 + 1] = l[j];
+            }
+        }
+        s.first += tiles;
+        s.tile = end;
+        if (p.units == 0 || end == s.end) return;
+    }
+}
+
+// A workgroup per sequence and query head.
+template <bool BF16>
+__global__ __launch_bounds__(256) void join_kernel(const Attention p) {
+    __shared__ float weight[kMaxUnits + 1], part[2][4];
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const int b = blockIdx.x, head = blockIdx.y;
+    const int64_t tile = p.starts[b], end = p.starts[b + 1], per = p.starts[p.seqs + 1];
+    Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(b) * p.q_heads + head) * p.D;
+    if (tile == end) {
+        for (int d = tid; d < p.D; d += 256) put<BF16>(out, d, 0.0f);
+        return;
+    }
+    const int unit = static_cast<int>(tile / per), n = static_cast<int>((end - 1) / per) - unit + 1;
+    if (n == 1) return;
+    const int64_t first = static_cast<int64_t>(unit + b) * p.q_heads + head;
+    const float inf = __uint_as_float(0x7F800000u);
+    float m = -inf;
+    for (int i = tid; i < n; i += 256) m = fmaxf(m, p.part_ml[(first + static_cast<int64_t>(i) * p.q_heads) * 2]);
+    m = kc::wave_max(m);
+    if (lane == 0) part[0][wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
+    if (m == -inf) m = 0.0f;
+    float l = 0.0f;
+    for (int i = tid; i < n; i += 256) {
+        const float* ml = p.part_ml + (first + static_cast<int64_t>(i) * p.q_heads) * 2;
+        const float w = __builtin_amdgcn_exp2f(ml[0] - m);
+        weight[i] = w;
+        l = fmaf(w, ml[1], l);
+    }
+    l = kc::wave_sum(l);
+    if (lane == 0) part[1][wave] = l;
+    __syncthreads();
+    l = (part[1][0] + part[1][1]) + (part[1][2] + part[1][3]);
+    for (int d = tid; d < p.D; d += 256) {
+        float o = 0.0f;
+        for (int i = 0; i < n; ++i)
+            o = fmaf(weight[i], p.part_o[(first + static_cast<int64_t>(i) * p.q_heads) * p.D + d], o);
+        put<BF16>(out, d, o / l);
+    }
+}
+
+struct Plan {
+    int sets, wg_sets, streams, units;
+    unsigned grid_x, grid_y;
+};
+
+constexpr int kMinTiles = 2;
+
+// Waves of `heads` query heads each, up to `waves` to a workgroup.
+Plan plan_of(int heads, int waves, const kc_kv_cache* c, int64_t max_pages, int seqs, int q_heads) {
+    Plan p{};
+    const int group = q_heads / c->kv_heads;
+    p.sets = c->kv_heads * ((group + heads - 1) / heads);
+    p.grid_y = static_cast<unsigned>((p.sets + waves - 1) / waves);
+    p.wg_sets = static_cast<int>((p.sets + p.grid_y - 1) / p.grid_y);
+    p.streams = std::max(1, waves / p.wg_sets);
+    const int64_t tiles = (std::min<int64_t>(max_pages * c->page_size, INT32_MAX) + kTile - 1) / kTile;
+    if (tiles <= kMinTiles) {  // nothing to split
+        p.grid_x = static_cast<unsigned>((seqs + p.streams - 1) / p.streams);
+        return p;
+    }
+    const int64_t most = (tiles * seqs + kMinTiles - 1) / kMinTiles;
+    const int64_t wgs = std::max<int64_t>(1, 512 / p.grid_y);
+    p.grid_x = static_cast<unsigned>(std::min({wgs, (most + p.streams - 1) / p.streams, int64_t{kMaxUnits / p.streams}}));
+    p.units = static_cast<int>(p.grid_x) * p.streams;
+    return p;
+}
+
+Plan vector_plan(const kc_kv_cache* c, int64_t max_pages, int seqs, int q_heads) {
+    // queries in LDS: 64 KB hold four waves of heads of up to 768
+    return plan_of(kHeads, c->head_dim > 768 ? 2 : 4, c, max_pages, seqs, q_heads);
+}
+
+int64_t starts_bytes(int seqs) { return (int64_t{seqs} + 2) * 8; }
+
+int64_t workspace_bytes(const Plan& p, int seqs, int q_heads, int D) {
+    return p.units == 0 ? 0 : (starts_bytes(seqs) + 15) / 16 * 16 + (int64_t{p.units} + seqs) * q_heads * (D + 2) * 4;
+}
+
+int check(const char* fn, const kc_kv_cache* cache, int64_t max_pages, int seqs, int q_heads) {
+    const int st = check_cache(fn, cache);
+    if (st != KC_SUCCESS) return st;
+    if (max_pages < 0 || seqs < 0 || q_heads < 0)
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: negative shape", fn);
+    if (q_heads % cache->kv_heads != 0)
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: q_heads=%d must be a multiple of kv_heads=%d", fn, q_heads,
+                             cache->kv_heads);
+    if (max_pages > INT32_MAX || q_heads > (1 << 16) - 1 || int64_t{seqs} * q_heads > kMaxGrid)
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: max_pages=%lld seqs=%d q_heads=%d too large", fn,
+                             (long long)max_pages, seqs, q_heads);
+    if (cache->num_pages * cache->page_size > INT32_MAX)
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the cache has over 2^31 - 1 slots", fn);
+    return KC_SUCCESS;
+}
+
+template <bool BF16, bool FP8>
+void launch_vector(const Attention& p, dim3 grid, int threads, hipStream_t stream) {
+    const size_t lds = static_cast<size_t>(threads / kWave) * (kHeads * p.D + (kHeads + 1) * kTile) * sizeof(float);
+    if (p.D <= 64) attention_kernel<BF16, FP8, 1><<<grid, threads, lds, stream>>>(p);
+    else if (p.D <= 256) attention_kernel<BF16, FP8, 4><<<grid, threads, lds, stream>>>(p);
+    else attention_kernel<BF16, FP8, 16><<<grid, threads, lds, stream>>>(p);
+}
+
+template <bool BF16>
+int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads, const kc_kv_cache* cache,
+              const int32_t* table, int64_t max_pages, const int32_t* lens, int seqs, float scale, int window,
+              void* workspace, int64_t bytes, Elem<BF16>* out, hipStream_t stream) {
+    const int st = check(fn, cache, max_pages, seqs, q_heads);
+    if (st != KC_SUCCESS) return st;
+    if (window < 0) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: window=%d is negative", fn, window);
+    if (seqs == 0 || q_heads == 0) return KC_SUCCESS;
+    if (!q || !lens || !out || (max_pages > 0 && !table))
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
+    Attention p{};
+    p.q = q;
+    p.out = out;
+    p.k_codes = static_cast<const uint8_t*>(cache->k_codes);
+    p.v_codes = static_cast<const uint8_t*>(cache->v_codes);
+    p.k_scales = cache->k_scales;
+    p.v_scales = cache->v_scales;
+    p.table = table;
+    p.lens = lens;
+    p.q_stride = q_stride;
+    p.max_pages = max_pages;
+    p.num_pages = cache->num_pages;
+    p.page = cache->page_size;
+    p.kv_heads = cache->kv_heads;
+    p.D = cache->head_dim;
+    p.q_heads = q_heads;
+    p.group = q_heads / cache->kv_heads;
+    p.seqs = seqs;
+    p.window = window;
+    p.scale = scale * 1.44269504088896340736f;
+    const bool fp8 = cache->format == KC_KV_FP8;
+    const Plan plan = vector_plan(cache, max_pages, seqs, q_heads);
+    p.units = plan.units;
+    p.min_tiles = kMinTiles;
+    p.streams = plan.streams;
+    p.sets = plan.sets;
+    p.wg_sets = plan.wg_sets;
+    if (bytes < workspace_bytes(plan, seqs, q_heads, p.D) || (plan.units > 0 && (!workspace || !kc::aligned(workspace, 16))))
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the workspace has %lld bytes, needs %lld, 16-byte aligned", fn,
+                             (long long)bytes, (long long)workspace_bytes(plan, seqs, q_heads, p.D));
+    p.starts = static_cast<int64_t*>(workspace);
+    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + (starts_bytes(seqs) + 15) / 16 * 16);
+    p.part_o = p.part_ml + (int64_t{plan.units} + seqs) * q_heads * 2;
+    const dim3 grid(plan.grid_x, plan.grid_y);
+    const int threads = plan.wg_sets * plan.streams * kWave;
+    if (fp8) launch_vector<BF16, true>(p, grid, threads, stream);
+    else launch_vector<BF16, false>(p, grid, threads, stream);
+    const int launched = kc::check_launch(fn);
+    if (launched != KC_SUCCESS || plan.units == 0) return launched;
+    join_kernel<BF16><<<dim3(seqs, q_heads), 256, 0, stream>>>(p);
+    return kc::check_launch(fn);
+}
+
+}  // namespace
+
+extern "C" int64_t kc_kv_cache_attention_workspace(const kc_kv_cache* cache, int64_t max_pages, int seqs,
+                                                   int q_heads) {
+    const char* fn = "kc_kv_cache_attention_workspace";
+    if (check(fn, cache, max_pages, seqs, q_heads) != KC_SUCCESS) return -1;
+    if (seqs == 0 || q_heads == 0) return 0;
+    return workspace_bytes(vector_plan(cache, max_pages, seqs, q_heads), seqs, q_heads, cache->head_dim);
+}
+
+extern "C" int kc_kv_cache_attention_bf16(const uint16_t* d_q, int64_t q_stride, int q_heads, const kc_kv_cache* cache,
+                                          const int32_t* d_block_table, int64_t max_pages, const int32_t* d_seq_lens,
+                                          int seqs, float scale, int window, void* d_workspace,
+                                          int64_t workspace_bytes, uint16_t* d_out, kc_stream_t stream) {
+    return attention<true>("kc_kv_cache_attention_bf16", d_q, q_stride, q_heads, cache, d_block_table, max_pages,
+                           d_seq_lens, seqs, scale, window, d_workspace, workspace_bytes, d_out, stream);
+}
+
+extern "C" int kc_kv_cache_attention_f32(const float* d_q, int64_t q_stride, int q_heads, const kc_kv_cache* cache,
+                                         const int32_t* d_block_table, int64_t max_pages, const int32_t* d_seq_lens,
+                                         int seqs, float scale, int window, void* d_workspace,
+                                         int64_t workspace_bytes, float* d_out, kc_stream_t stream) {
+    return attention<false>("kc_kv_cache_attention_f32", d_q, q_stride, q_heads, cache, d_block_table, max_pages,
+                            d_seq_lens, seqs, scale, window, d_workspace, workspace_bytes, d_out, stream);
+}

@@ -31,7 +31,8 @@ What this module adds:
 * operators for the entry points the reference lacks (bf16 GEMV and its
   chain, the M > 1 GEMM, RMSNorm and its fusions, bf16 and fused-SmoothQuant
   FP8 quantization, the FP8 GEMM, checkpoint conversion, MXFP4 quantization
-  and products, head norms with rotation, the quantized key/value cache).
+  and products, head norms with rotation, the quantized key/value cache, its
+  pages and attention over it, the residual sum with its norms).
 
 Usage
 -----
@@ -158,6 +159,14 @@ PROTOTYPES = {
        for t in ("bf16", "f32")},
     **{f"kc_kv_cache_read_{t}": ([_vp, _vp, _i64, _vp, _i, _i64, _vp, _vp, _vp], _i)
        for t in ("bf16", "f32")},
+    "kc_kv_cache_attention_workspace": ([_vp, _i64, _i, _i], _i64),
+    **{f"kc_kv_cache_attention_{t}": ([_vp, _i64, _i, _vp, _vp, _i64, _vp, _i, _f, _i, _vp, _i64,
+                                       _vp, _vp], _i) for t in ("bf16", "f32")},
+    "kc_kv_cache_extend": ([_vp] * 3 + [_i64] + [_vp] * 7, _i),
+    "kc_kv_cache_release": ([_vp] * 6, _i),
+    **{f"kc_residual_rmsnorm_{t}": ([_vp] * 4, _i) for t in ("bf16", "bf16_f32", "f32")},
+    **{f"kc_residual_rmsnorm_quantize_fp8_{t}": ([_vp] * 5, _i)
+       for t in ("bf16", "bf16_f32", "f32")},
 }
 
 
@@ -1121,6 +1130,238 @@ def kv_cache_read(k_codes, k_scales, v_codes, v_scales, block_table, cu_seqlens,
                      _ptr(cu_seqlens), block_table.shape[0], total_tokens, _ptr(k), _ptr(v))
     _check(op, st)
     return k, v
+
+
+def kv_cache_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens,
+                       scale: Optional[float] = None, window: int = 0):
+    """Attention of one token per sequence over the quantized cache (kv_cache_write's tensors):
+    bf16 or fp32 q [sequences, q_heads, D] -> the same, softmax(scale q k) v over the seq_lens[b]
+    (int32) positions that sequence b has in the cache, its newest token's among them, in the
+    pages block_table[b] (int32 [sequences, most pages]); only the last ``window`` of them if it
+    is not 0.  q_heads is a multiple of the cache's kv_heads, scale 1 / sqrt(D) by default.  fp32
+    arithmetic on the values that kv_cache_read gives, rounded once.  A sequence of length 0
+    gives zeros, one with a visible position whose page is missing NaN
+    (kc_kv_cache_attention_*)."""
+    import torch
+    op = "kv_cache_attention"
+    cache, Hkv, D = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
+    q = _heads(op, "q", q, (torch.bfloat16, torch.float32), (None, None, D))
+    B, Hq, _ = q.shape
+    if Hq % Hkv:
+        raise ValueError(f"{op}: q has {Hq} heads, not a multiple of the cache's {Hkv}")
+    block_table = _take(op, "block_table", block_table, torch.int32)
+    seq_lens = _take(op, "seq_lens", seq_lens, torch.int32)
+    table = block_table.shape
+    if len(table) != 2 or table[0] != B or seq_lens.shape != (B,):
+        raise ValueError(f"{op}: block_table {tuple(table)} and seq_lens {tuple(seq_lens.shape)} "
+                         f"must be [{B}, pages] and [{B}]")
+    if window < 0:
+        raise ValueError(f"{op}: window={window} is negative")
+    gpu = _one_gpu(op, q, k_codes, k_scales, v_codes, v_scales, block_table, seq_lens)
+    lib = _get_lib()
+    ref = ctypes.byref(cache)
+    need = lib.kc_kv_cache_attention_workspace(ref, table[1], B, Hq)
+    if need < 0:
+        _check(op)
+    work = torch.empty(max(need, 0), dtype=torch.uint8, device=q.device)
+    out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    fn = lib.kc_kv_cache_attention_bf16 if q.dtype == torch.bfloat16 else lib.kc_kv_cache_attention_f32
+    with kernel_span(op, sequences=B, heads=Hq, kv_heads=Hkv, head_dim=D):
+        st = _launch(gpu, fn, _ptr(q), q.stride(0), Hq, ref, _ptr(block_table), table[1],
+                     _ptr(seq_lens), B, D ** -0.5 if scale is None else scale, min(window, 2 ** 31 - 1),
+                     _ptr(work), need, _ptr(out))
+    _check(op, st)
+    return out
+
+
+class KvPages(ctypes.Structure):
+    """kc_kv_pages (include/kernel_craft.h)."""
+    _fields_ = [("block_table", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+                ("free_count", ctypes.c_void_p), ("max_pages", ctypes.c_int64),
+                ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int), ("seqs", ctypes.c_int)]
+
+
+def _kv_pages(op: str, seq_lens, block_table, free_pages, free_count, page_size: int, written):
+    """(seq_lens, free_count, kc_kv_pages) of a cache's pages; the tensor named ``written`` must
+    be contiguous, as it is written to."""
+    import torch
+    seq_lens = _take(op, "seq_lens", seq_lens, torch.int32)
+    free_count = _take(op, "free_count", free_count, torch.int32)
+    shaped = {"block_table": block_table, "free_pages": free_pages}
+    if not shaped[written].is_contiguous():
+        raise ValueError(f"{op}: {written} must be contiguous")
+    block_table = _take(op, "block_table", block_table, torch.int32)
+    free_pages = _take(op, "free_pages", free_pages, torch.int32)
+    table = block_table.shape
+    if len(table) != 2 or seq_lens.shape != table[:1]:
+        raise ValueError(f"{op}: block_table {tuple(table)} and seq_lens {tuple(seq_lens.shape)} "
+                         "must be [requests, pages] and [requests]")
+    if free_pages.dim() != 1 or free_count.shape != (1,):
+        raise ValueError(f"{op}: free_pages {tuple(free_pages.shape)} and free_count "
+                         f"{tuple(free_count.shape)} must be [pages] and [1]")
+    if page_size <= 0:
+        raise ValueError(f"{op}: page_size={page_size} must be positive")
+    # the copies that _take may have made live as long as the structure
+    pages = KvPages(_ptr(block_table), _ptr(free_pages), _ptr(free_count), table[1],
+                    free_pages.shape[0], page_size, table[0])
+    pages.keep = (block_table, free_pages, free_count)
+    return seq_lens, free_count, pages
+
+
+def kv_cache_extend(seq_lens, new_lens, block_table, free_pages, free_count, page_size: int,
+                    total_new: int) -> Tuple:
+    """Pages of the cache for the next tokens of a batch, on the GPU: request b has seq_lens[b]
+    tokens in the cache and new_lens[b] new ones (int32), which stand packed in ``total_new``
+    rows.  Each request, in order, takes the pages that it lacks from the top of the stack
+    free_pages[:free_count] (int32 [pages], [1]) and writes them behind its others in
+    block_table (int32 [requests, most pages], written in place).  It is served whole or not at
+    all: not if block_table has no room, if its rows pass total_new, or if it lacks pages and
+    they are, with those that the requests before it asked for, more than the stack has.
+
+    Returns (seq_lens, free_count, cu_new, cu_seqlens, positions, slots): the new lengths, the
+    pages left, each request's first row and first token in kv_cache_read's batch (int32
+    [requests + 1]), and for each row what qk_norm_rope_cache takes (int32 positions, int64
+    slots; -1, padding, for requests not served and rows behind the last).  The inputs stay as
+    they are but for block_table's new entries (kc_kv_cache_extend)."""
+    import torch
+    op = "kv_cache_extend"
+    seq_lens, free_count, pages = _kv_pages(op, seq_lens, block_table, free_pages, free_count,
+                                            page_size, "block_table")
+    new_lens = _take(op, "new_lens", new_lens, torch.int32)
+    B = seq_lens.shape[0]
+    if new_lens.shape != (B,):
+        raise ValueError(f"{op}: new_lens {tuple(new_lens.shape)} must be [{B}]")
+    if not 0 <= total_new < 2 ** 31:
+        raise ValueError(f"{op}: total_new={total_new} must be from 0 to 2^31 - 1")
+    gpu = _one_gpu(op, seq_lens, new_lens, block_table, free_pages, free_count)
+    dev = seq_lens.device
+    # one allocation for the int32 results
+    parts = torch.empty(3 * B + 3 + total_new, dtype=torch.int32, device=dev).split(
+        (B, 1, B + 1, B + 1, total_new))
+    slots = torch.empty(total_new, dtype=torch.int64, device=dev)
+    with kernel_span(op, requests=B, tokens=total_new, page_size=page_size):
+        st = _launch(gpu, _get_lib().kc_kv_cache_extend, ctypes.byref(pages), _ptr(seq_lens),
+                     _ptr(new_lens), total_new, *[_ptr(t) for t in parts], _ptr(slots))
+    _check(op, st)
+    return (*parts, slots)
+
+
+def kv_cache_release(finished, seq_lens, block_table, free_pages, free_count,
+                     page_size: int) -> Tuple:
+    """The pages of the sequences that ``finished`` (bool or u8 [requests]) names, back onto the
+    stack of free pages (kv_cache_extend's tensors; free_pages is written in place from
+    free_count on).  Returns (seq_lens, free_count), lengths of 0 for those sequences; their
+    entries of block_table stay (kc_kv_cache_release)."""
+    import torch
+    op = "kv_cache_release"
+    if finished.dtype not in (torch.bool, torch.uint8):
+        raise ValueError(f"{op}: finished has dtype {finished.dtype}; expected torch.bool or torch.uint8")
+    finished = finished.contiguous()
+    seq_lens, free_count, pages = _kv_pages(op, seq_lens, block_table, free_pages, free_count,
+                                            page_size, "free_pages")
+    B = seq_lens.shape[0]
+    if finished.shape != (B,):
+        raise ValueError(f"{op}: finished {tuple(finished.shape)} must be [{B}]")
+    gpu = _one_gpu(op, seq_lens, finished, block_table, free_pages, free_count)
+    lens, count = torch.empty(B + 1, dtype=torch.int32, device=seq_lens.device).split((B, 1))
+    with kernel_span(op, requests=B, page_size=page_size):
+        st = _launch(gpu, _get_lib().kc_kv_cache_release, ctypes.byref(pages), _ptr(finished),
+                     _ptr(seq_lens), _ptr(lens), _ptr(count))
+    _check(op, st)
+    return lens, count
+
+
+class Residual(ctypes.Structure):
+    """kc_residual (include/kernel_craft.h)."""
+    _fields_ = [("y", ctypes.c_void_p), ("h", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("post_gamma", ctypes.c_void_p), ("gamma", ctypes.c_void_p),
+                ("y_stride", ctypes.c_int64), ("h_stride", ctypes.c_int64),
+                ("gate_stride", ctypes.c_int64), ("rows", ctypes.c_int64), ("cols", ctypes.c_int),
+                ("alpha", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+def _residual_args(op: str, y, h, gamma, post_gamma, gate, alpha: float, eps: float):
+    """(gpu, suffix of the entry point, kc_residual) of validated arguments; rows with values one
+    after the other are read in place, anything else is copied."""
+    import torch
+    if y.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{op}: y has dtype {y.dtype}; expected torch.bfloat16 or torch.float32")
+    if h.dtype is not y.dtype and h.dtype is not torch.float32:
+        raise ValueError(f"{op}: h has dtype {h.dtype}; expected {y.dtype} or torch.float32")
+    if y.dim() != 2 or h.shape != y.shape:
+        raise ValueError(f"{op}: y {tuple(y.shape)} and h {tuple(h.shape)} must both be [rows, cols]")
+    T, D = y.shape
+    gamma = _take(op, "gamma", gamma, y.dtype)
+    given = [y, h, gamma]
+    if post_gamma is not None:
+        post_gamma = _take(op, "post_gamma", post_gamma, y.dtype)
+        given.append(post_gamma)
+    if gamma.shape != (D,) or (post_gamma is not None and post_gamma.shape != (D,)):
+        raise ValueError(f"{op}: gamma and post_gamma must be [{D}]")
+
+    def rows(t):
+        return t if t.stride(1) == 1 or D <= 1 else t.contiguous()
+
+    y, h = rows(y), rows(h)
+    gate_stride = 0
+    if gate is not None:
+        if gate.dtype is not y.dtype:
+            raise ValueError(f"{op}: gate has dtype {gate.dtype}; expected {y.dtype}")
+        if gate.shape == (D,):
+            gate = gate.contiguous()
+        elif gate.shape == (T, D):
+            gate = rows(gate)
+            gate_stride = gate.stride(0)
+        else:
+            raise ValueError(f"{op}: gate {tuple(gate.shape)} must be [{D}] or [{T}, {D}]")
+        given.append(gate)
+    gpu = _one_gpu(op, *given)
+    args = Residual(_ptr(y), _ptr(h), None if gate is None else _ptr(gate),
+                    None if post_gamma is None else _ptr(post_gamma), _ptr(gamma), y.stride(0),
+                    h.stride(0), gate_stride, T, D, alpha, eps)
+    # the copies made above live as long as the structure
+    args.keep = (y, h, gate, post_gamma, gamma)
+    suffix = "f32" if y.dtype == torch.float32 else "bf16" if h.dtype == y.dtype else "bf16_f32"
+    return gpu, suffix, args
+
+
+def residual_rmsnorm(y, h, gamma, post_gamma=None, gate=None, alpha: float = 1.0,
+                     eps: float = 1e-6) -> Tuple:
+    """The residual sum behind a decoder's block and the norm in front of the next one, in one
+    pass: of the block's output y [rows, cols] (bf16 or fp32) and the residual stream h (y's type
+    or fp32), h_new = h + alpha * gate * b with b = y, or y normed with post_gamma [cols], and
+    n = rmsnorm(h_new) * gamma.  gate is None (1), [cols] or [rows, cols].  Returns (h_new, n),
+    h_new of h's type and n of y's; fp32 arithmetic, each rounded once, n from the h_new that is
+    not rounded yet (kc_residual_rmsnorm_*)."""
+    import torch
+    op = "residual_rmsnorm"
+    gpu, suffix, args = _residual_args(op, y, h, gamma, post_gamma, gate, alpha, eps)
+    h_new = torch.empty(args.rows, args.cols, dtype=h.dtype, device=h.device)
+    n = torch.empty(args.rows, args.cols, dtype=y.dtype, device=h.device)
+    with kernel_span(op, rows=args.rows, d=args.cols):
+        st = _launch(gpu, getattr(_get_lib(), "kc_residual_rmsnorm_" + suffix), ctypes.byref(args),
+                     _ptr(h_new), _ptr(n))
+    _check(op, st)
+    return h_new, n
+
+
+def residual_rmsnorm_fp8_quantize(y, h, gamma, post_gamma=None, gate=None, alpha: float = 1.0,
+                                  eps: float = 1e-6) -> Tuple:
+    """residual_rmsnorm with n quantized per token in the same pass, from fp32 as
+    fp8_quantize_rows does: (h_new, int8 codes [rows, cols], fp32 scales [rows]), what
+    fp8_gemm_w8a8 takes (kc_residual_rmsnorm_quantize_fp8_*)."""
+    import torch
+    op = "residual_rmsnorm_fp8_quantize"
+    gpu, suffix, args = _residual_args(op, y, h, gamma, post_gamma, gate, alpha, eps)
+    h_new = torch.empty(args.rows, args.cols, dtype=h.dtype, device=h.device)
+    codes = torch.empty(args.rows, args.cols, dtype=torch.int8, device=h.device)
+    # scale 1 for empty rows (absmax 0), which the library does not write
+    scales = (torch.empty if args.cols else torch.ones)(args.rows, dtype=torch.float32, device=h.device)
+    with kernel_span(op, rows=args.rows, cols=args.cols):
+        st = _launch(gpu, getattr(_get_lib(), "kc_residual_rmsnorm_quantize_fp8_" + suffix),
+                     ctypes.byref(args), _ptr(h_new), _ptr(codes), _ptr(scales))
+    _check(op, st)
+    return h_new, codes, scales
 
 
 # ---------------------------------------------------------------------------
