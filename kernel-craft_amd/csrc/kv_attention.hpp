@@ -28,7 +28,8 @@ struct Attention {
     const void *k_scales, *v_scales;
     const int32_t *table, *lens;
     int64_t q_stride, max_pages, num_pages;
-    int page, kv_heads, D, q_heads, group, seqs, window;
+    int page, page_shift;  // page_shift: its logarithm, or -1
+    int kv_heads, D, q_heads, group, seqs, window;
     float scale;       // times log2(e)
     int units;         // stretches; 0: a stretch per sequence, and no join
     int min_tiles;     // of a stretch
@@ -138,6 +139,10 @@ __device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& 
 __device__ __forceinline__ bool holds_all(const Stretch& s, int64_t tile, int64_t end, int tiles) {
     return tile == s.first && end == s.first + tiles;
 }
+
+// The matrix-core kernel (kv_cache_attention_mfma.hip): sets of 8 query heads in bf16, 4 in fp32.
+bool mfma_takes(const kc_kv_cache& cache);
+bool launch_mfma(const Attention& p, bool bf16, bool fp8, dim3 grid, int threads, hipStream_t stream);
 
 }  // namespace kv
 }  // namespace kc

@@ -218,15 +218,19 @@ Plan plan_of(int heads, int waves, const kc_kv_cache* c, int64_t max_pages, int 
     return p;
 }
 
-Plan vector_plan(const kc_kv_cache* c, int64_t max_pages, int seqs, int q_heads) {
+Plan plan_for(const kc_kv_cache* c, bool bf16, int64_t max_pages, int seqs, int q_heads) {
+    if (mfma_takes(*c)) return plan_of(bf16 ? 8 : 4, kMaxWaves, c, max_pages, seqs, q_heads);
     // queries in LDS: 64 KB hold four waves of heads of up to 768
     return plan_of(kHeads, c->head_dim > 768 ? 2 : 4, c, max_pages, seqs, q_heads);
 }
 
 int64_t starts_bytes(int seqs) { return (int64_t{seqs} + 2) * 8; }
 
+int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
 int64_t workspace_bytes(const Plan& p, int seqs, int q_heads, int D) {
-    return p.units == 0 ? 0 : (starts_bytes(seqs) + 15) / 16 * 16 + (int64_t{p.units} + seqs) * q_heads * (D + 2) * 4;
+    const int64_t rows = (int64_t{p.units} + seqs) * q_heads;
+    return p.units == 0 ? 0 : round16(starts_bytes(seqs)) + round16(rows * 8) + rows * D * 4;
 }
 
 int check(const char* fn, const kc_kv_cache* cache, int64_t max_pages, int seqs, int q_heads) {
@@ -276,6 +280,7 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     p.max_pages = max_pages;
     p.num_pages = cache->num_pages;
     p.page = cache->page_size;
+    p.page_shift = kc::is_pow2(p.page) ? kc::ilog2(p.page) : -1;
     p.kv_heads = cache->kv_heads;
     p.D = cache->head_dim;
     p.q_heads = q_heads;
@@ -284,7 +289,7 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     p.window = window;
     p.scale = scale * 1.44269504088896340736f;
     const bool fp8 = cache->format == KC_KV_FP8;
-    const Plan plan = vector_plan(cache, max_pages, seqs, q_heads);
+    const Plan plan = plan_for(cache, BF16, max_pages, seqs, q_heads);
     p.units = plan.units;
     p.min_tiles = kMinTiles;
     p.streams = plan.streams;
@@ -294,11 +299,13 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the workspace has %lld bytes, needs %lld, 16-byte aligned", fn,
                              (long long)bytes, (long long)workspace_bytes(plan, seqs, q_heads, p.D));
     p.starts = static_cast<int64_t*>(workspace);
-    p.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + (starts_bytes(seqs) + 15) / 16 * 16);
-    p.part_o = p.part_ml + (int64_t{plan.units} + seqs) * q_heads * 2;
+    char* parts = static_cast<char*>(workspace) + round16(starts_bytes(seqs));
+    p.part_ml = reinterpret_cast<float*>(parts);
+    p.part_o = reinterpret_cast<float*>(parts + round16((int64_t{plan.units} + seqs) * q_heads * 8));
     const dim3 grid(plan.grid_x, plan.grid_y);
     const int threads = plan.wg_sets * plan.streams * kWave;
-    if (fp8) launch_vector<BF16, true>(p, grid, threads, stream);
+    if (mfma_takes(*cache)) launch_mfma(p, BF16, fp8, grid, threads, stream);
+    else if (fp8) launch_vector<BF16, true>(p, grid, threads, stream);
     else launch_vector<BF16, false>(p, grid, threads, stream);
     const int launched = kc::check_launch(fn);
     if (launched != KC_SUCCESS || plan.units == 0) return launched;
@@ -313,7 +320,9 @@ extern "C" int64_t kc_kv_cache_attention_workspace(const kc_kv_cache* cache, int
     const char* fn = "kc_kv_cache_attention_workspace";
     if (check(fn, cache, max_pages, seqs, q_heads) != KC_SUCCESS) return -1;
     if (seqs == 0 || q_heads == 0) return 0;
-    return workspace_bytes(vector_plan(cache, max_pages, seqs, q_heads), seqs, q_heads, cache->head_dim);
+    const int D = cache->head_dim;
+    return std::max(workspace_bytes(plan_for(cache, true, max_pages, seqs, q_heads), seqs, q_heads, D),
+                    workspace_bytes(plan_for(cache, false, max_pages, seqs, q_heads), seqs, q_heads, D));
 }
 
 extern "C" int kc_kv_cache_attention_bf16(const uint16_t* d_q, int64_t q_stride, int q_heads, const kc_kv_cache* cache,

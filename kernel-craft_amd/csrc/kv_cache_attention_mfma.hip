@@ -1,0 +1,565 @@
+// kv_cache_attention_mfma.hip -- attention of each sequence's newest token over the
+// quantized paged cache on gfx950's matrix cores, for head_dims of whole 16-byte rows.
+//
+// A wave takes a set of query heads of one key/value head and a stretch of tiles of 32
+// positions (kv_attention.hpp).  Keys and values are turned from codes into bf16, which
+// holds every E4M3 and E2M1 value (times a power of two) exactly, in registers: no tile
+// goes through LDS.  With lane = 16 g + c:
+//   S^T = K Q^T    16 positions x 16 columns a product; a lane's 8 scores are those of
+//                  column c at positions 4g .. 4g + 3 of both halves of the tile
+//   O^T = V^T P^T  the sum over positions may take them in any order: with the values of
+//                  just those 8 positions in a lane, its own 8 weights are its operand,
+//                  and nothing crosses lanes but the maximum
+// so that a column's maximum, sum and output all live in the lanes of column c.
+//
+// The 16 columns are N query heads in 16 / N pieces.  bf16 queries: 8 heads, the weights
+// as the sum of two bf16 values (2^-17), one in each piece.  fp32 queries: 4 heads, queries
+// and weights as sums of three bf16 values (2^-25).  The pieces cost no product more, since
+// groups of up to 8 (4) query heads leave those columns empty.
+#include <type_traits>
+
+#include "kv_attention.hpp"
+
+namespace {
+
+using namespace kc::kv;
+using namespace kc::mx;
+using kc::kWave;
+
+typedef short bf16x8 __attribute__((ext_vector_type(8)));  // as the matrix instructions take it
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+template <bool BF16>
+using Elem = std::conditional_t<BF16, uint16_t, float>;
+
+constexpr float kLazy = 8.0f;  // a maximum may be passed by 2^8 before the sums are scaled down to a new one
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, true));
+}
+constexpr int kRor4 = 0x124, kRor8 = 0x128;  // within 16 lanes
+
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t w, bool high) {
+    const bf16x2 r = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), 1.0f, true)
+                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), 1.0f, false);
+    return __builtin_bit_cast(uint32_t, r);
+}
+
+// Codes 2 BYTE and 2 BYTE + 1 of w times the scale 2^(b - 127), b's value as scale_operand gives it.
+template <int BYTE>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, BYTE));
+}
+
+__device__ __forceinline__ bf16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(bf16x8, u32x4{a, b, c, d});
+}
+
+__device__ __forceinline__ f32x4 product(bf16x8 a, bf16x8 b, f32x4 c) {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+// A row of RB bytes spread over LANES lanes in pieces, each of L bytes per lane one after
+// the other: as many of the largest L as fit, then one of each smaller power of two that
+// is left.
+template <int RB, int LANES, int MOST>
+struct Cut {
+    static constexpr int kLane = RB / LANES;
+    static constexpr int pieces() {
+        int n = kLane / MOST;
+        for (int l = MOST / 2; l > 0; l /= 2) n += (kLane % MOST & l) != 0;
+        return n;
+    }
+    static constexpr int lane_bytes(int i) {
+        if (i < kLane / MOST) return MOST;
+        i -= kLane / MOST;
+        for (int l = MOST / 2; l > 0; l /= 2)
+            if ((kLane % MOST & l) != 0 && i-- == 0) return l;
+        return 0;
+    }
+    static constexpr int start(int i) {  // byte of the row
+        int at = 0;
+        for (int j = 0; j < i; ++j) at += LANES * lane_bytes(j);
+        return at;
+    }
+    static constexpr int dword(int i) {  // of the lane's registers
+        int at = 0;
+        for (int j = 0; j < i; ++j) at += (lane_bytes(j) + 3) / 4;
+        return at;
+    }
+    static constexpr int dwords() { return dword(pieces()); }
+};
+
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+template <int BYTES>
+__device__ __forceinline__ void load_bytes(const uint8_t* from, uint32_t* to) {
+    if constexpr (BYTES == 16) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(from);
+        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+    } else if constexpr (BYTES == 8) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(from);
+        to[0] = v.x, to[1] = v.y;
+    } else if constexpr (BYTES == 4) {
+        to[0] = *reinterpret_cast<const uint32_t*>(from);
+    } else if constexpr (BYTES == 2) {
+        to[0] = *reinterpret_cast<const uint16_t*>(from);
+    } else {
+        to[0] = *from;
+    }
+}
+
+// out[k]: byte k of t0 .. t3.
+__device__ __forceinline__ void transpose4(uint32_t t0, uint32_t t1, uint32_t t2, uint32_t t3, uint32_t (&out)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(t1, t0, 0x05010400), b = __builtin_amdgcn_perm(t3, t2, 0x05010400);
+    const uint32_t c = __builtin_amdgcn_perm(t1, t0, 0x07030602), d = __builtin_amdgcn_perm(t3, t2, 0x07030602);
+    out[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
+    out[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    out[2] = __builtin_amdgcn_perm(d, c, 0x05040100);
+    out[3] = __builtin_amdgcn_perm(d, c, 0x07060302);
+}
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_perm(b, a, 0x05040100);
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+    return __builtin_amdgcn_perm(b, a, 0x07060302);
+}
+
+template <bool FP8, int D>
+struct Shape {
+    static constexpr int kRow = FP8 ? D : D / 2;   // bytes
+    static constexpr int kBlocks = D / 32;         // MXFP4 scales of a row
+    using K = Cut<kRow, 4, 16>;                    // 16 positions by up to 64 bytes a load
+    using V = Cut<kRow, 16, 16>;                   // 4 positions by up to 256 bytes a load
+    // a lane's K dwords: two are a step of 32 products (FP8; an odd last one has zeros behind it), or one (MXFP4)
+    static constexpr int kSteps = FP8 ? (K::dwords() + 1) / 2 : K::dwords();
+    static constexpr int kTiles = D / 16;          // of O^T
+};
+
+// LDS of a wave: slots of two tiles in turn, scales of one.
+template <bool FP8, int D>
+struct WaveShared {
+    int slots[2][kTile];
+    union {
+        float f[2][kTile];                                        // FP8: keys, values
+        uint8_t b[2][FP8 ? 1 : Shape<FP8, D>::kBlocks][kTile];    // MXFP4
+    } scales;
+};
+
+template <bool BF16, bool FP8, int D>
+__global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) {
+    using S = Shape<FP8, D>;
+    using KC = typename S::K;
+    using VC = typename S::V;
+    constexpr int kN = BF16 ? 8 : 4;  // query heads of a set
+    __shared__ PlanShared plan;
+    __shared__ WaveShared<FP8, D> shared[kMaxWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int c = lane & 15, g = lane >> 4, t = lane & (kTile - 1), part = c / kN;
+    WaveShared<FP8, D>& lds = shared[wave];
+    const int set = blockIdx.y * p.wg_sets + wave % p.wg_sets;
+    Stretch s = find_stretch(p, plan, wave / p.wg_sets);
+    if (s.b < 0 || set >= p.sets) return;
+    const int per_kv = (p.group + kN - 1) / kN, h = set / per_kv, q0 = (set - h * per_kv) * kN;
+    const int heads = min(kN, p.group - q0), qi = c & (kN - 1);
+    const int64_t head0 = static_cast<int64_t>(h) * p.group + q0;
+    const float nan = __uint_as_float(0x7FC00000u), inf = __uint_as_float(0x7F800000u);
+    const uint32_t row_bytes = static_cast<uint32_t>(p.kv_heads) * S::kRow;
+    const uint8_t* kbase = p.k_codes + static_cast<int64_t>(h) * S::kRow;
+    const uint8_t* vbase = p.v_codes + static_cast<int64_t>(h) * S::kRow;
+    // lanes 0 .. 31 fetch the scales of keys, the others those of values
+    const uint8_t* sbase = static_cast<const uint8_t*>(lane < kTile ? p.k_scales : p.v_scales) +
+                           static_cast<int64_t>(h) * (FP8 ? 4 : S::kBlocks);
+    const uint32_t scale_bytes = static_cast<uint32_t>(p.kv_heads) * (FP8 ? 4 : S::kBlocks);
+
+    for (int b = s.b; b < p.seqs; ++b) {
+        const Visible vis = visible(p, b);
+        const int tiles = vis.tiles();
+        Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(b) * p.q_heads + head0 + qi) * D;
+        if (tiles == 0) {
+            if (p.units != 0) continue;  // the join's
+            if (qi < heads)
+                for (int d = g * (16 / kN) + part; d < D; d += 4 * (16 / kN)) out[d] = 0;
+            return;
+        }
+        const int64_t end = min(s.end, s.first + tiles);
+        const int first_tile = vis.first / kTile + static_cast<int>(s.tile - s.first);
+        const int last_tile = vis.first / kTile + static_cast<int>(end - s.first) - 1;
+
+        // ---- queries: the operand of every step ----
+        bf16x8 q[S::kSteps];
+        {
+            const Elem<BF16>* from =
+                static_cast<const Elem<BF16>*>(p.q) + b * p.q_stride + (head0 + (qi < heads ? qi : 0)) * D;
+            each<KC::pieces()>([&](auto piece) {
+                constexpr int kP = piece, kBytes = KC::lane_bytes(kP), kAt = KC::dword(kP);
+                constexpr int kValues = FP8 ? kBytes : 2 * kBytes, kStep = kValues < 8 ? kValues : 8;
+                const int d0 = (FP8 ? 1 : 2) * (KC::start(kP) + g * kBytes);
+#pragma unroll
+                for (int i = 0; i < kValues / kStep; ++i) {
+                    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int e = 0; e < kStep; e += 2) {
+                        float x[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            if constexpr (BF16) {
+                                x[k] = kc::bf16_to_f32(from[d0 + 8 * i + e + k]);
+                            } else {  // the piece of the value that this column holds
+                                x[k] = from[d0 + 8 * i + e + k];
+                                const float hi = kc::bf16_to_f32(kc::f32_to_bf16(x[k]));
+                                const float r = x[k] - hi, mid = kc::bf16_to_f32(kc::f32_to_bf16(r));
+                                x[k] = part == 0 ? hi : part == 1 ? mid : part == 2 ? r - mid : 0.0f;
+                            }
+                        }
+                        w[e / 2] = kc::pack_bf16x2(x[0], x[1]);
+                    }
+                    q[(FP8 ? kAt / 2 : kAt) + i] = operand(w[0], w[1], w[2], w[3]);
+                }
+            });
+        }
+
+        // ---- the pipeline's steps ----
+        int entry, offset;  // of this lane's position t, two tiles ahead
+        auto fetch = [&](int tile) {
+            const int pos = tile * kTile + t;
+            entry = -1;
+            offset = 0;
+            if (tile <= last_tile && pos >= vis.first && pos < vis.end) {
+                const int at = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page;
+                offset = pos - at * p.page;
+                if (at < p.max_pages) entry = p.table[b * p.max_pages + at];
+            }
+        };
+        uint32_t k[2][KC::dwords()], v[8][VC::dwords()];
+        uint32_t sc[FP8 ? 1 : (S::kBlocks + 3) / 4];
+        i32x4 vslot[2];
+        bool holes = false;  // a position of the tile is not there, or not seen
+        auto place = [&](int buffer) {  // slots of the fetched tile
+            const int slot = entry >= 0 && entry < p.num_pages ? entry * p.page + offset : -1;
+            lds.slots[buffer][t] = slot;
+            __builtin_amdgcn_wave_barrier();
+            return slot;
+        };
+        auto load_keys = [&](int buffer, int slot) {
+            const uint8_t* at = sbase + static_cast<uint64_t>(static_cast<uint32_t>(max(slot, 0))) * scale_bytes;
+            if constexpr (FP8) {
+                sc[0] = slot < 0 ? 0u : *reinterpret_cast<const uint32_t*>(at);
+            } else {
+                constexpr int kUnit = S::kBlocks % 4 == 0 ? 4 : S::kBlocks % 2 == 0 ? 2 : 1;
+#pragma unroll
+                for (int i = 0; i < (S::kBlocks + 3) / 4; ++i) sc[i] = 0;
+#pragma unroll
+                for (int i = 0; i < S::kBlocks; i += kUnit) {
+                    uint32_t w;
+                    load_bytes<kUnit>(at + i, &w);
+                    sc[i / 4] |= w << (8 * (i % 4));
+                }
+                if (slot < 0) {
+#pragma unroll
+                    for (int i = 0; i < (S::kBlocks + 3) / 4; ++i) sc[i] = 0x7F7F7F7Fu;
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = lds.slots[buffer][16 * half + c];
+                const uint8_t* from = kbase + static_cast<uint64_t>(static_cast<uint32_t>(max(row, 0))) * row_bytes;
+                each<KC::pieces()>([&](auto piece) {
+                    constexpr int kP = piece;
+                    load_bytes<KC::lane_bytes(kP)>(from + KC::start(kP) + g * KC::lane_bytes(kP),
+                                                   &k[half][KC::dword(kP)]);
+                });
+            }
+        };
+        auto load_values = [&](int buffer) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                vslot[half] = *reinterpret_cast<const i32x4*>(&lds.slots[buffer][16 * half + 4 * g]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int row = vslot[i / 4][i % 4];
+                const uint8_t* from = vbase + static_cast<uint64_t>(static_cast<uint32_t>(max(row, 0))) * row_bytes;
+                each<VC::pieces()>([&](auto piece) {
+                    constexpr int kP = piece;
+                    load_bytes<VC::lane_bytes(kP)>(from + VC::start(kP) + c * VC::lane_bytes(kP), &v[i][VC::dword(kP)]);
+                });
+            }
+        };
+
+        f32x4 o[S::kTiles];
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -inf, l = 0.0f;
+
+        fetch(first_tile);
+        int slot = place(0), buffer = 0;
+        load_keys(0, slot);
+        load_values(0);
+        bool next_holes = __any(slot < 0);
+        fetch(first_tile + 1);
+        for (int tile = first_tile; tile <= last_tile; ++tile, buffer ^= 1) {
+            holes = next_holes;
+            // the next tile's slots
+            slot = place(buffer ^ 1);
+            next_holes = __any(slot < 0);
+            fetch(tile + 2);
+            // this tile's scales
+            if constexpr (FP8) {
+                lds.scales.f[lane / kTile][t] = __uint_as_float(sc[0]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::kBlocks; ++i)
+                    lds.scales.b[lane / kTile][i][t] = static_cast<uint8_t>(sc[i / 4] >> (8 * (i % 4)));
+            }
+            __builtin_amdgcn_wave_barrier();
+
+            // ---- scores ----
+            float x[8];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                f32x4 a{0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (FP8) {
+#pragma unroll
+                    for (int i = 0; i < S::kSteps; ++i) {
+                        const uint32_t w0 = k[half][2 * i];
+                        const bool pair = 2 * i + 1 < KC::dwords();
+                        const uint32_t w1 = pair ? k[half][pair ? 2 * i + 1 : 0] : 0u;
+                        a = product(operand(fp8_pair(w0, false), fp8_pair(w0, true), pair ? fp8_pair(w1, false) : 0u,
+                                            pair ? fp8_pair(w1, true) : 0u),
+                                    q[i], a);
+                    }
+                } else {
+                    each<KC::pieces()>([&](auto piece) {
+                        constexpr int kP = piece, kBytes = KC::lane_bytes(kP);
+                        const int block = (2 * KC::start(kP) + g * 2 * kBytes) / kBlock;
+                        const float f = scale_operand(lds.scales.b[0][block][16 * half + c]);
+#pragma unroll
+                        for (int i = 0; i < kBytes / 4; ++i) {
+                            const uint32_t w = k[half][KC::dword(kP) + i];
+                            a = product(operand(fp4_pair<0>(w, f), fp4_pair<1>(w, f), fp4_pair<2>(w, f),
+                                                fp4_pair<3>(w, f)),
+                                        q[KC::dword(kP) + i], a);
+                        }
+                    });
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = a[i];
+                    if constexpr (!BF16) {  // the same sum in every piece, bit for bit
+                        v += dpp<kRor8>(v);
+                        v += dpp<kRor4>(v);
+                    }
+                    x[4 * half + i] = v * p.scale;
+                }
+                if constexpr (FP8) {
+                    const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.scales.f[0][16 * half + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[4 * half + i] *= f[i];
+                }
+            }
+            if (holes) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const i32x4 at = *reinterpret_cast<const i32x4*>(&lds.slots[buffer][16 * half + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int pos = tile * kTile + 16 * half + 4 * g + i;
+                        if (pos < vis.first || pos >= vis.end) x[4 * half + i] = -inf;
+                        else if (at[i] < 0) x[4 * half + i] = nan;
+#pragma unroll
+                        for (int w = 0; w < VC::dwords(); ++w)
+                            if (at[i] < 0) v[4 * half + i][w] = 0;
+                    }
+                }
+            }
+            float vs[8];
+            if constexpr (FP8) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.scales.f[1][16 * half + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vs[4 * half + i] = f[i];
+                }
+            }
+            if (tile < last_tile) load_keys(buffer ^ 1, slot);
+
+            // ---- weights ----
+            float most = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i]);
+            most = fmaxf(most, __shfl_xor(most, 16, kWave));
+            most = fmaxf(most, __shfl_xor(most, 32, kWave));
+            if (__any(most > m + kLazy)) {  // a column's own decision: the others go on by 1
+                const float to = most > m + kLazy ? most : m;
+                const float by = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+                m = to;
+                l *= by;
+#pragma unroll
+                for (int i = 0; i < S::kTiles; ++i) o[i] *= by;
+            }
+            const float at = m == -inf ? 0.0f : m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = __builtin_amdgcn_exp2f(x[i] - at);
+                sum += x[i];
+                if constexpr (FP8) x[i] *= vs[i];
+            }
+            l += sum;
+            uint32_t pw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float a = x[2 * i], e = x[2 * i + 1];
+#pragma unroll
+                for (int n = 1; n < (BF16 ? 2 : 3); ++n) {  // what the pieces before this column's hold is taken off
+                    const uint32_t w = kc::pack_bf16x2(a, e);
+                    if (part >= n) {
+                        a -= __uint_as_float(w << 16);
+                        e -= __uint_as_float(w & 0xFFFF0000u);
+                    }
+                }
+                pw[i] = kc::pack_bf16x2(a, e);
+                if (!BF16 && part == 3) pw[i] = 0;
+            }
+            const bf16x8 weights = operand(pw[0], pw[1], pw[2], pw[3]);
+
+            // ---- output ----
+            each<VC::pieces()>([&](auto piece) {
+                constexpr int kP = piece, kBytes = VC::lane_bytes(kP), kAt = VC::dword(kP);
+                constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16;
+                if constexpr (FP8) {
+#pragma unroll
+                    for (int w = 0; w < (kBytes + 3) / 4; ++w) {
+                        uint32_t lo[4], hi[4];
+                        transpose4(v[0][kAt + w], v[1][kAt + w], v[2][kAt + w], v[3][kAt + w], lo);
+                        transpose4(v[4][kAt + w], v[5][kAt + w], v[6][kAt + w], v[7][kAt + w], hi);
+#pragma unroll
+                        for (int j = 0; j < (kBytes < 4 ? kBytes : 4); ++j)
+                            o[kTile0 + 4 * w + j] =
+                                product(operand(fp8_pair(lo[j], false), fp8_pair(lo[j], true), fp8_pair(hi[j], false),
+                                                fp8_pair(hi[j], true)),
+                                        weights, o[kTile0 + 4 * w + j]);
+                    }
+                } else {
+                    const int block = 2 * (VC::start(kP) + c * kBytes) / kBlock;
+                    float f[8];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(&lds.scales.b[1][block][16 * half + 4 * g]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) f[4 * half + i] = scale_operand((w >> (8 * i)) & 255u);
+                    }
+                    each<kBytes>([&](auto byte) {
+                        constexpr int kB = byte;
+                        uint32_t e[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) e[i] = fp4_pair<kB % 4>(v[i][kAt + kB / 4], f[i]);
+                        o[kTile0 + 2 * kB] = product(operand(low_halves(e[0], e[1]), low_halves(e[2], e[3]),
+                                                             low_halves(e[4], e[5]), low_halves(e[6], e[7])),
+                                                     weights, o[kTile0 + 2 * kB]);
+                        o[kTile0 + 2 * kB + 1] = product(operand(high_halves(e[0], e[1]), high_halves(e[2], e[3]),
+                                                                 high_halves(e[4], e[5]), high_halves(e[6], e[7])),
+                                                         weights, o[kTile0 + 2 * kB + 1]);
+                    });
+                }
+            });
+            if (tile < last_tile) load_values(buffer ^ 1);
+        }
+
+        // ---- result ----
+        l += __shfl_xor(l, 16, kWave);
+        l += __shfl_xor(l, 32, kWave);
+        const bool whole = holds_all(s, s.tile, end, tiles);
+        const int64_t segment = (static_cast<int64_t>(s.unit) + b) * p.q_heads + head0 + qi;
+        const float by = whole ? 1.0f / l : 1.0f;
+        each<VC::pieces()>([&](auto piece) {
+            constexpr int kP = piece, kValues = (FP8 ? 1 : 2) * VC::lane_bytes(kP);
+            constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16, kD0 = (FP8 ? 1 : 2) * VC::start(kP);
+            // a column's pieces share its rows out
+#pragma unroll
+            for (int i = 0; i < 4 * kN / 16; ++i) {
+                const int r = part * (4 * kN / 16) + i;
+                float y[kValues];
+#pragma unroll
+                for (int j = 0; j < kValues; ++j) {
+                    f32x4 a = o[kTile0 + j];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        a[e] += dpp<kRor8>(a[e]);
+                        if constexpr (!BF16) a[e] += dpp<kRor4>(a[e]);
+                    }
+                    y[j] = r == 0 ? a[0] : r == 1 ? a[1] : r == 2 ? a[2] : a[3];
+                }
+                const int d = kD0 + (4 * g + r) * kValues;
+                if (qi < heads) {
+#pragma unroll
+                    for (int j = 0; j < kValues; ++j) {
+                        if (!whole) p.part_o[segment * D + d + j] = y[j];
+                        else if constexpr (BF16) out[d + j] = kc::f32_to_bf16(y[j] * by);
+                        else out[d + j] = y[j] / l;
+                    }
+                }
+            }
+        });
+        if (!whole && qi < heads && part == 0 && g == 0) {
+            p.part_ml[segment * 2] = m;
+            p.part_ml[segment * 2 + 1] = l;
+        }
+        s.first += tiles;
+        s.tile = end;
+        if (p.units == 0 || end == s.end) return;
+    }
+}
+
+template <bool BF16, bool FP8>
+bool launch(const Attention& p, dim3 grid, int threads, hipStream_t stream) {
+    switch (p.D) {
+        case 64: attention_mfma_kernel<BF16, FP8, 64><<<grid, threads, 0, stream>>>(p); return true;
+        case 96: attention_mfma_kernel<BF16, FP8, 96><<<grid, threads, 0, stream>>>(p); return true;
+        case 128: attention_mfma_kernel<BF16, FP8, 128><<<grid, threads, 0, stream>>>(p); return true;
+        case 192: attention_mfma_kernel<BF16, FP8, 192><<<grid, threads, 0, stream>>>(p); return true;
+        case 256: attention_mfma_kernel<BF16, FP8, 256><<<grid, threads, 0, stream>>>(p); return true;
+        default: break;
+    }
+    if constexpr (FP8) {
+        switch (p.D) {
+            case 80: attention_mfma_kernel<BF16, FP8, 80><<<grid, threads, 0, stream>>>(p); return true;
+            case 112: attention_mfma_kernel<BF16, FP8, 112><<<grid, threads, 0, stream>>>(p); return true;
+            default: break;
+        }
+    }
+    return false;
+}
+
+}  // namespace
+
+namespace kc {
+namespace kv {
+
+bool mfma_takes(const kc_kv_cache& c) {
+    const bool fp8 = c.format == KC_KV_FP8;
+    const int blocks = c.head_dim / 32;
+    // rows of codes in whole 16 bytes, scales in the units that they are loaded in
+    const uintptr_t unit = fp8 ? 4 : blocks % 4 == 0 ? 4 : blocks % 2 == 0 ? 2 : 1;
+    const bool size = c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 192 ||
+                      c.head_dim == 256 || (fp8 && (c.head_dim == 80 || c.head_dim == 112));
+    return size && c.num_pages > 0 && aligned(c.k_codes, 16) && aligned(c.v_codes, 16) && aligned(c.k_scales, unit) &&
+           aligned(c.v_scales, unit);
+}
+
+bool launch_mfma(const Attention& p, bool bf16, bool fp8, dim3 grid, int threads, hipStream_t stream) {
+    if (bf16) return fp8 ? launch<true, true>(p, grid, threads, stream) : launch<true, false>(p, grid, threads, stream);
+    return fp8 ? launch<false, true>(p, grid, threads, stream) : launch<false, false>(p, grid, threads, stream);
+}
+
+}  // namespace kv
+}  // namespace kc
