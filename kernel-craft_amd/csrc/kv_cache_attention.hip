@@ -39,28 +39,25 @@ __device__ __forceinline__ float value(const uint8_t* codes, const void* scales,
     return decode4_f32(c & 15u, scale_value(static_cast<const uint8_t*>(scales)[(row * D + d) / kBlock])).x;
 }
 
-// A wave takes kHeads query heads of one key/value head.  Scores: a lane per position and
-// half of the head; output: a lane per NI values of the head.
+// A workgroup is one wave: kHeads query heads of one key/value head.  Scores: a lane per
+// position and half of the head; output: a lane per NI values of the head.
 template <bool BF16, bool FP8, int NI>
-__global__ __launch_bounds__(256) void attention_kernel(const Attention p) {
+__global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
     __shared__ PlanShared plan;
-    extern __shared__ float lds[];
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    float* ql = lds + wave * (kHeads * p.D + (kHeads + 1) * kTile);
-    float* pl = ql + kHeads * p.D;
-    int* sl = reinterpret_cast<int*>(pl + kHeads * kTile);
-    const int set = blockIdx.y * p.wg_sets + wave % p.wg_sets;
-    Stretch s = find_stretch(p, plan, wave / p.wg_sets);
-    if (s.b < 0 || set >= p.sets) return;
+    __shared__ float ql[kHeads * NI * kWave], pl[kHeads * kTile];
+    __shared__ int sl[kTile];
+    const int lane = threadIdx.x;
+    const int set = blockIdx.y;
+    Stretch s = find_stretch(p, plan, blockIdx.x, 0, blockIdx.x == 0 && set == 0);
+    if (s.b < 0) return;
     const int per_kv = (p.group + kHeads - 1) / kHeads, h = set / per_kv, q0 = (set - h * per_kv) * kHeads;
     const int heads = min(kHeads, p.group - q0);
+    const int64_t head0 = static_cast<int64_t>(h) * p.group + q0;
     const float nan = __uint_as_float(0x7FC00000u), inf = __uint_as_float(0x7F800000u);
 
     for (int b = s.b; b < p.seqs; ++b) {
         const Visible vis = visible(p, b);
-        const int tiles = vis.tiles();
-        const int64_t end = min(s.end, s.first + tiles);
-        const int64_t head0 = static_cast<int64_t>(h) * p.group + q0;
+        const int tiles = vis.tiles(), end = min(s.end, s.first + tiles);
         Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(b) * p.q_heads + head0) * p.D;
         if (tiles == 0) {
             if (p.units != 0) continue;  // the join's
@@ -77,8 +74,9 @@ __global__ __launch_bounds__(256) void attention_kernel(const Attention p) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) acc[j][i] = 0.0f;
         }
-        for (int64_t tile = s.tile; tile < end; ++tile) {
-            const int base = (vis.first / kTile + static_cast<int>(tile - s.first)) * kTile;
+        __syncthreads();
+        for (int tile = s.tile; tile < end; ++tile) {
+            const int base = (vis.first / kTile + (tile - s.first)) * kTile;
             const int t = lane & (kTile - 1), half = lane / kTile, pos = base + t;
             const bool seen = pos >= vis.first && pos < vis.end;
             const int slot = seen ? slot_of(p, b, pos) : -1;
@@ -112,7 +110,7 @@ __global__ __launch_bounds__(256) void attention_kernel(const Attention p) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i) acc[j][i] *= by;
             }
-            __builtin_amdgcn_wave_barrier();
+            __syncthreads();
             for (int u = 0; u < kTile; ++u) {
                 const int at = sl[u];
                 const int64_t row = static_cast<int64_t>(at) * p.kv_heads + h;
@@ -124,9 +122,9 @@ __global__ __launch_bounds__(256) void attention_kernel(const Attention p) {
                     for (int j = 0; j < kHeads; ++j) acc[j][i] = fmaf(pl[j * kTile + u], v, acc[j][i]);
                 }
             }
-            __builtin_amdgcn_wave_barrier();
+            __syncthreads();
         }
-        const bool whole = holds_all(s, s.tile, end, tiles);
+        const bool whole = s.tile == s.first && end == s.first + tiles;
         const int64_t segment = (static_cast<int64_t>(s.unit) + b) * p.q_heads + head0;
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
@@ -149,82 +147,107 @@ __global__ __launch_bounds__(256) void attention_kernel(const Attention p) {
     }
 }
 
-// A workgroup per sequence and query head.
+// blockDim.x / 64 waves, `split` of them for a query head of a sequence: each joins some of
+// its segments, then one all of theirs.
 template <bool BF16>
-__global__ __launch_bounds__(256) void join_kernel(const Attention p) {
-    __shared__ float weight[kMaxUnits + 1], part[2][4];
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int b = blockIdx.x, head = blockIdx.y;
-    const int64_t tile = p.starts[b], end = p.starts[b + 1], per = p.starts[p.seqs + 1];
+__global__ __launch_bounds__(1024) void join_kernel(const Attention p, int split) {
+    __shared__ float part_ml[16][2];
+    extern __shared__ float part_o[];  // [waves][D] where split > 1
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int b = blockIdx.x, head = blockIdx.y * (blockDim.x / kWave / split) + wave / split, sub = wave % split;
+    const int tile = p.starts[b], end = p.starts[b + 1], per = p.starts[p.seqs + 1];
+    const bool mine = head < p.q_heads;
     Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(b) * p.q_heads + head) * p.D;
     if (tile == end) {
-        for (int d = tid; d < p.D; d += 256) put<BF16>(out, d, 0.0f);
+        if (mine && sub == 0)
+            for (int d = lane; d < p.D; d += kWave) put<BF16>(out, d, 0.0f);
         return;
     }
-    const int unit = static_cast<int>(tile / per), n = static_cast<int>((end - 1) / per) - unit + 1;
-    if (n == 1) return;
-    const int64_t first = static_cast<int64_t>(unit + b) * p.q_heads + head;
+    const int unit = tile / per, n = (end - 1) / per - unit + 1;
+    if (n == 1) return;  // the same for the whole workgroup
     const float inf = __uint_as_float(0x7F800000u);
-    float m = -inf;
-    for (int i = tid; i < n; i += 256) m = fmaxf(m, p.part_ml[(first + static_cast<int64_t>(i) * p.q_heads) * 2]);
-    m = kc::wave_max(m);
-    if (lane == 0) part[0][wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(part[0][0], part[0][1]), fmaxf(part[0][2], part[0][3]));
-    if (m == -inf) m = 0.0f;
-    float l = 0.0f;
-    for (int i = tid; i < n; i += 256) {
-        const float* ml = p.part_ml + (first + static_cast<int64_t>(i) * p.q_heads) * 2;
-        const float w = __builtin_amdgcn_exp2f(ml[0] - m);
-        weight[i] = w;
-        l = fmaf(w, ml[1], l);
+    const int64_t first = static_cast<int64_t>(unit + b) * p.q_heads + head;
+    float m = -inf, l = 0.0f;
+    if (mine) {
+        for (int i = sub + lane * split; i < n; i += kWave * split)
+            m = fmaxf(m, p.part_ml[(first + static_cast<int64_t>(i) * p.q_heads) * 2]);
+        m = kc::wave_max(m);
+        const float at = m == -inf ? 0.0f : m;
+        for (int d0 = 0; d0 < p.D; d0 += 2 * kWave) {
+            float o[2] = {};
+            l = 0.0f;
+            const int d = d0 + lane, d1 = min(d, p.D - 1), d2 = min(d + kWave, p.D - 1);
+#pragma unroll 8
+            for (int i = sub; i < n; i += split) {
+                const int64_t row = first + static_cast<int64_t>(i) * p.q_heads;
+                const float w = __builtin_amdgcn_exp2f(p.part_ml[row * 2] - at);
+                l = fmaf(w, p.part_ml[row * 2 + 1], l);
+                o[0] = fmaf(w, p.part_o[row * p.D + d1], o[0]);
+                o[1] = fmaf(w, p.part_o[row * p.D + d2], o[1]);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (d + e * kWave >= p.D) break;
+                if (split > 1) part_o[wave * p.D + d + e * kWave] = o[e];
+                else put<BF16>(out, d + e * kWave, o[e] / l);
+            }
+        }
+        if (lane == 0) {
+            part_ml[wave][0] = m;
+            part_ml[wave][1] = l;
+        }
     }
-    l = kc::wave_sum(l);
-    if (lane == 0) part[1][wave] = l;
+    if (split == 1) return;
     __syncthreads();
-    l = (part[1][0] + part[1][1]) + (part[1][2] + part[1][3]);
-    for (int d = tid; d < p.D; d += 256) {
+    if (!mine || sub != 0) return;
+    const int w1 = wave + min(split, n);
+    for (int w = wave; w < w1; ++w) m = fmaxf(m, part_ml[w][0]);
+    const float at = m == -inf ? 0.0f : m;
+    l = 0.0f;
+    for (int w = wave; w < w1; ++w) l = fmaf(__builtin_amdgcn_exp2f(part_ml[w][0] - at), part_ml[w][1], l);
+    for (int d = lane; d < p.D; d += kWave) {
         float o = 0.0f;
-        for (int i = 0; i < n; ++i)
-            o = fmaf(weight[i], p.part_o[(first + static_cast<int64_t>(i) * p.q_heads) * p.D + d], o);
+        for (int w = wave; w < w1; ++w) o = fmaf(__builtin_amdgcn_exp2f(part_ml[w][0] - at), part_o[w * p.D + d], o);
         put<BF16>(out, d, o / l);
     }
 }
 
 struct Plan {
-    int sets, wg_sets, streams, units;
-    unsigned grid_x, grid_y;
+    int sets, units, wg_sets, streams;
+    dim3 grid;
 };
 
-constexpr int kMinTiles = 2;
+constexpr int kMinTiles = 2;      // of a stretch
+constexpr int kDirectTiles = 32;  // of a sequence that one workgroup takes
 
-// Waves of `heads` query heads each, up to `waves` to a workgroup.
-Plan plan_of(int heads, int waves, const kc_kv_cache* c, int64_t max_pages, int seqs, int q_heads) {
+// Sets of `heads` query heads, workgroups of up to `waves` waves, `resident` of which run at once.
+Plan plan_of(int heads, int waves, int resident, const kc_kv_cache* c, int64_t max_pages, int seqs, int q_heads) {
     Plan p{};
     const int group = q_heads / c->kv_heads;
     p.sets = c->kv_heads * ((group + heads - 1) / heads);
-    p.grid_y = static_cast<unsigned>((p.sets + waves - 1) / waves);
-    p.wg_sets = static_cast<int>((p.sets + p.grid_y - 1) / p.grid_y);
-    p.streams = std::max(1, waves / p.wg_sets);
     const int64_t tiles = (std::min<int64_t>(max_pages * c->page_size, INT32_MAX) + kTile - 1) / kTile;
-    if (tiles <= kMinTiles) {  // nothing to split
-        p.grid_x = static_cast<unsigned>((seqs + p.streams - 1) / p.streams);
+    if (tiles <= kDirectTiles) {
+        p.wg_sets = 1;
+        p.streams = static_cast<int>(std::clamp<int64_t>(tiles, 1, waves));
+        p.grid = dim3(seqs, p.sets);
         return p;
     }
+    const int rows = (p.sets + waves - 1) / waves;
+    p.wg_sets = (p.sets + rows - 1) / rows;
+    p.streams = waves / p.wg_sets;
     const int64_t most = (tiles * seqs + kMinTiles - 1) / kMinTiles;
-    const int64_t wgs = std::max<int64_t>(1, 512 / p.grid_y);
-    p.grid_x = static_cast<unsigned>(std::min({wgs, (most + p.streams - 1) / p.streams, int64_t{kMaxUnits / p.streams}}));
-    p.units = static_cast<int>(p.grid_x) * p.streams;
+    const int64_t wgs = std::min<int64_t>(std::max(1, resident / rows), (most + p.streams - 1) / p.streams);
+    p.grid = dim3(static_cast<unsigned>(std::clamp<int64_t>(wgs, 1, kMaxUnits / p.streams)), rows);
+    p.units = static_cast<int>(p.grid.x) * p.streams;
     return p;
 }
 
 Plan plan_for(const kc_kv_cache* c, bool bf16, int64_t max_pages, int seqs, int q_heads) {
-    if (mfma_takes(*c)) return plan_of(bf16 ? 8 : 4, kMaxWaves, c, max_pages, seqs, q_heads);
-    // queries in LDS: 64 KB hold four waves of heads of up to 768
-    return plan_of(kHeads, c->head_dim > 768 ? 2 : 4, c, max_pages, seqs, q_heads);
+    if (mfma_takes(*c, max_pages)) return plan_of(bf16 ? 8 : 4, kMaxWaves, 256, c, max_pages, seqs, q_heads);
+    return plan_of(kHeads, 1, 2048, c, max_pages, seqs, q_heads);
 }
 
-int64_t starts_bytes(int seqs) { return (int64_t{seqs} + 2) * 8; }
+int64_t starts_bytes(int seqs) { return (int64_t{seqs} + 2) * 4; }
 
 int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
@@ -246,15 +269,18 @@ int check(const char* fn, const kc_kv_cache* cache, int64_t max_pages, int seqs,
                              (long long)max_pages, seqs, q_heads);
     if (cache->num_pages * cache->page_size > INT32_MAX)
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the cache has over 2^31 - 1 slots", fn);
+    const int64_t tiles = (std::min<int64_t>(max_pages * cache->page_size, INT32_MAX) + kTile - 1) / kTile;
+    if (tiles * seqs > (1 << 30))
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: seqs=%d max_pages=%lld page_size=%d too large", fn, seqs,
+                             (long long)max_pages, cache->page_size);
     return KC_SUCCESS;
 }
 
 template <bool BF16, bool FP8>
-void launch_vector(const Attention& p, dim3 grid, int threads, hipStream_t stream) {
-    const size_t lds = static_cast<size_t>(threads / kWave) * (kHeads * p.D + (kHeads + 1) * kTile) * sizeof(float);
-    if (p.D <= 64) attention_kernel<BF16, FP8, 1><<<grid, threads, lds, stream>>>(p);
-    else if (p.D <= 256) attention_kernel<BF16, FP8, 4><<<grid, threads, lds, stream>>>(p);
-    else attention_kernel<BF16, FP8, 16><<<grid, threads, lds, stream>>>(p);
+void launch_vector(const Attention& p, dim3 grid, hipStream_t stream) {
+    if (p.D <= 64) attention_kernel<BF16, FP8, 1><<<grid, kWave, 0, stream>>>(p);
+    else if (p.D <= 256) attention_kernel<BF16, FP8, 4><<<grid, kWave, 0, stream>>>(p);
+    else attention_kernel<BF16, FP8, 16><<<grid, kWave, 0, stream>>>(p);
 }
 
 template <bool BF16>
@@ -292,24 +318,26 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     const Plan plan = plan_for(cache, BF16, max_pages, seqs, q_heads);
     p.units = plan.units;
     p.min_tiles = kMinTiles;
-    p.streams = plan.streams;
     p.sets = plan.sets;
     p.wg_sets = plan.wg_sets;
+    p.streams = plan.streams;
     if (bytes < workspace_bytes(plan, seqs, q_heads, p.D) || (plan.units > 0 && (!workspace || !kc::aligned(workspace, 16))))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: the workspace has %lld bytes, needs %lld, 16-byte aligned", fn,
                              (long long)bytes, (long long)workspace_bytes(plan, seqs, q_heads, p.D));
-    p.starts = static_cast<int64_t*>(workspace);
+    p.starts = static_cast<int*>(workspace);
     char* parts = static_cast<char*>(workspace) + round16(starts_bytes(seqs));
     p.part_ml = reinterpret_cast<float*>(parts);
     p.part_o = reinterpret_cast<float*>(parts + round16((int64_t{plan.units} + seqs) * q_heads * 8));
-    const dim3 grid(plan.grid_x, plan.grid_y);
-    const int threads = plan.wg_sets * plan.streams * kWave;
-    if (mfma_takes(*cache)) launch_mfma(p, BF16, fp8, grid, threads, stream);
-    else if (fp8) launch_vector<BF16, true>(p, grid, threads, stream);
-    else launch_vector<BF16, false>(p, grid, threads, stream);
+    if (mfma_takes(*cache, max_pages)) launch_mfma(p, BF16, fp8, plan.grid, stream);
+    else if (fp8) launch_vector<BF16, true>(p, plan.grid, stream);
+    else launch_vector<BF16, false>(p, plan.grid, stream);
     const int launched = kc::check_launch(fn);
     if (launched != KC_SUCCESS || plan.units == 0) return launched;
-    join_kernel<BF16><<<dim3(seqs, q_heads), 256, 0, stream>>>(p);
+    // one wave per query head of a sequence where that makes waves enough, else 4 or 16
+    const int64_t pairs = int64_t{seqs} * q_heads;
+    const int split = pairs >= 2048 ? 1 : pairs >= 512 ? 4 : 16, waves = std::max(split, 4), per_wg = waves / split;
+    join_kernel<BF16><<<dim3(seqs, (q_heads + per_wg - 1) / per_wg), waves * kWave, split > 1 ? waves * p.D * 4 : 0,
+                        stream>>>(p, split);
     return kc::check_launch(fn);
 }
 

@@ -134,6 +134,19 @@ __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
     return __builtin_amdgcn_perm(b, a, 0x07060302);
 }
 
+// N values at any alignment of their type.
+template <bool BF16, int N>
+__device__ __forceinline__ void store_values(Elem<BF16>* to, const float (&v)[N]) {
+    if constexpr (BF16) {
+        uint32_t w[(N + 1) / 2];
+#pragma unroll
+        for (int i = 0; i < N; i += 2) w[i / 2] = kc::pack_bf16x2(v[i], i + 1 < N ? v[i + 1] : 0.0f);
+        __builtin_memcpy(to, w, 2 * N);
+    } else {
+        __builtin_memcpy(to, v, 4 * N);
+    }
+}
+
 template <bool FP8, int D>
 struct Shape {
     static constexpr int kRow = FP8 ? D : D / 2;   // bytes
@@ -161,13 +174,16 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
     using KC = typename S::K;
     using VC = typename S::V;
     constexpr int kN = BF16 ? 8 : 4;  // query heads of a set
+    constexpr int kRow = D + 4;       // floats of a head in LDS: heads begin at different banks
     __shared__ PlanShared plan;
     __shared__ WaveShared<FP8, D> shared[kMaxWaves];
+    __shared__ float joint_ml[kMaxWaves][2][kN];
+    extern __shared__ float joint[];  // [waves][kN][kRow], for whole sequences
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int c = lane & 15, g = lane >> 4, t = lane & (kTile - 1), part = c / kN;
     WaveShared<FP8, D>& lds = shared[wave];
     const int set = blockIdx.y * p.wg_sets + wave % p.wg_sets;
-    Stretch s = find_stretch(p, plan, wave / p.wg_sets);
+    const Stretch s = find_stretch(p, plan, blockIdx.x, wave / p.wg_sets, blockIdx.x == 0 && blockIdx.y == 0);
     if (s.b < 0 || set >= p.sets) return;
     const int per_kv = (p.group + kN - 1) / kN, h = set / per_kv, q0 = (set - h * per_kv) * kN;
     const int heads = min(kN, p.group - q0), qi = c & (kN - 1);
@@ -181,71 +197,70 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                            static_cast<int64_t>(h) * (FP8 ? 4 : S::kBlocks);
     const uint32_t scale_bytes = static_cast<uint32_t>(p.kv_heads) * (FP8 ? 4 : S::kBlocks);
 
-    for (int b = s.b; b < p.seqs; ++b) {
-        const Visible vis = visible(p, b);
-        const int tiles = vis.tiles();
-        Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(b) * p.q_heads + head0 + qi) * D;
-        if (tiles == 0) {
-            if (p.units != 0) continue;  // the join's
-            if (qi < heads)
-                for (int d = g * (16 / kN) + part; d < D; d += 4 * (16 / kN)) out[d] = 0;
-            return;
+    // ---- a tile's place: sequence b, positions from base on, of which [first, end) are seen ----
+    struct Place {
+        int b, base, first, end;
+    };
+    int seq = s.b, seq_first = s.first;
+    Visible vis = visible_scalar(p, seq);
+    auto find = [&](int tile) {
+        if (tile >= s.end) return Place{-1, 0, 0, 0};
+        for (int n = vis.tiles(); tile >= seq_first + n; n = vis.tiles()) {  // tile < s.end ends it
+            seq_first += n;
+            vis = visible_scalar(p, ++seq);
         }
-        const int64_t end = min(s.end, s.first + tiles);
-        const int first_tile = vis.first / kTile + static_cast<int>(s.tile - s.first);
-        const int last_tile = vis.first / kTile + static_cast<int>(end - s.first) - 1;
+        return Place{seq, (vis.first / kTile + tile - seq_first) * kTile, vis.first, vis.end};
+    };
 
-        // ---- queries: the operand of every step ----
-        bf16x8 q[S::kSteps];
-        {
-            const Elem<BF16>* from =
-                static_cast<const Elem<BF16>*>(p.q) + b * p.q_stride + (head0 + (qi < heads ? qi : 0)) * D;
-            each<KC::pieces()>([&](auto piece) {
-                constexpr int kP = piece, kBytes = KC::lane_bytes(kP), kAt = KC::dword(kP);
-                constexpr int kValues = FP8 ? kBytes : 2 * kBytes, kStep = kValues < 8 ? kValues : 8;
-                const int d0 = (FP8 ? 1 : 2) * (KC::start(kP) + g * kBytes);
+    // ---- queries: the operand of every step ----
+    bf16x8 q[S::kSteps];
+    auto load_queries = [&](int b) {
+        const Elem<BF16>* from =
+            static_cast<const Elem<BF16>*>(p.q) + b * p.q_stride + (head0 + (qi < heads ? qi : 0)) * D;
+        each<KC::pieces()>([&](auto piece) {
+            constexpr int kP = piece, kBytes = KC::lane_bytes(kP), kAt = KC::dword(kP);
+            constexpr int kValues = FP8 ? kBytes : 2 * kBytes, kStep = kValues < 8 ? kValues : 8;
+            const int d0 = (FP8 ? 1 : 2) * (KC::start(kP) + g * kBytes);
 #pragma unroll
-                for (int i = 0; i < kValues / kStep; ++i) {
-                    uint32_t w[4] = {0, 0, 0, 0};
+            for (int i = 0; i < kValues / kStep; ++i) {
+                uint32_t w[4] = {0, 0, 0, 0};
+                if constexpr (BF16) {
+                    __builtin_memcpy(w, from + d0 + 8 * i, 2 * kStep);
+                } else {
 #pragma unroll
                     for (int e = 0; e < kStep; e += 2) {
                         float x[2];
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            if constexpr (BF16) {
-                                x[k] = kc::bf16_to_f32(from[d0 + 8 * i + e + k]);
-                            } else {  // the piece of the value that this column holds
-                                x[k] = from[d0 + 8 * i + e + k];
-                                const float hi = kc::bf16_to_f32(kc::f32_to_bf16(x[k]));
-                                const float r = x[k] - hi, mid = kc::bf16_to_f32(kc::f32_to_bf16(r));
-                                x[k] = part == 0 ? hi : part == 1 ? mid : part == 2 ? r - mid : 0.0f;
-                            }
+                        for (int k = 0; k < 2; ++k) {  // the piece of the value that this column holds
+                            x[k] = from[d0 + 8 * i + e + k];
+                            const float hi = kc::bf16_to_f32(kc::f32_to_bf16(x[k]));
+                            const float r = x[k] - hi, mid = kc::bf16_to_f32(kc::f32_to_bf16(r));
+                            x[k] = part == 0 ? hi : part == 1 ? mid : part == 2 ? r - mid : 0.0f;
                         }
                         w[e / 2] = kc::pack_bf16x2(x[0], x[1]);
                     }
-                    q[(FP8 ? kAt / 2 : kAt) + i] = operand(w[0], w[1], w[2], w[3]);
                 }
-            });
-        }
-
-        // ---- the pipeline's steps ----
-        int entry, offset;  // of this lane's position t, two tiles ahead
-        auto fetch = [&](int tile) {
-            const int pos = tile * kTile + t;
-            entry = -1;
-            offset = 0;
-            if (tile <= last_tile && pos >= vis.first && pos < vis.end) {
-                const int at = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page;
-                offset = pos - at * p.page;
-                if (at < p.max_pages) entry = p.table[b * p.max_pages + at];
+                q[(FP8 ? kAt / 2 : kAt) + i] = operand(w[0], w[1], w[2], w[3]);
             }
+        });
+    };
+
+    // ---- the pipeline's steps ----
+    // Every load of the loop is unconditional, and its order is that of the lines before the
+    // loop, so that the waits in it count loads instead of draining them.
+        int entry, offset;  // of this lane's position t, two tiles ahead; offset < 0: not seen, or past the table
+        auto fetch = [&](const Place& at) {
+            const int pos = at.base + t, near = min(max(pos, at.first), at.end - 1);
+            const int page = p.page_shift >= 0 ? near >> p.page_shift : near / p.page;
+            entry = p.table[max(at.b, 0) * p.max_pages + max(min(page, static_cast<int>(p.max_pages) - 1), 0)];
+            offset = near == pos && page < p.max_pages ? near - page * p.page : -1;
         };
         uint32_t k[2][KC::dwords()], v[8][VC::dwords()];
-        uint32_t sc[FP8 ? 1 : (S::kBlocks + 3) / 4];
+        constexpr int kScaleUnit = S::kBlocks % 4 == 0 ? 4 : S::kBlocks % 2 == 0 ? 2 : 1;  // MXFP4 scales of a load
+        uint32_t sc[FP8 ? 1 : S::kBlocks / kScaleUnit];
         i32x4 vslot[2];
-        bool holes = false;  // a position of the tile is not there, or not seen
         auto place = [&](int buffer) {  // slots of the fetched tile
-            const int slot = entry >= 0 && entry < p.num_pages ? entry * p.page + offset : -1;
+            const int slot = offset >= 0 && entry >= 0 && entry < p.num_pages ? entry * p.page + offset : -1;
             lds.slots[buffer][t] = slot;
             __builtin_amdgcn_wave_barrier();
             return slot;
@@ -253,22 +268,12 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
         auto load_keys = [&](int buffer, int slot) {
             const uint8_t* at = sbase + static_cast<uint64_t>(static_cast<uint32_t>(max(slot, 0))) * scale_bytes;
             if constexpr (FP8) {
-                sc[0] = slot < 0 ? 0u : *reinterpret_cast<const uint32_t*>(at);
+                sc[0] = *reinterpret_cast<const uint32_t*>(at);
             } else {
-                constexpr int kUnit = S::kBlocks % 4 == 0 ? 4 : S::kBlocks % 2 == 0 ? 2 : 1;
 #pragma unroll
-                for (int i = 0; i < (S::kBlocks + 3) / 4; ++i) sc[i] = 0;
-#pragma unroll
-                for (int i = 0; i < S::kBlocks; i += kUnit) {
-                    uint32_t w;
-                    load_bytes<kUnit>(at + i, &w);
-                    sc[i / 4] |= w << (8 * (i % 4));
-                }
-                if (slot < 0) {
-#pragma unroll
-                    for (int i = 0; i < (S::kBlocks + 3) / 4; ++i) sc[i] = 0x7F7F7F7Fu;
-                }
+                for (int i = 0; i < S::kBlocks / kScaleUnit; ++i) load_bytes<kScaleUnit>(at + i * kScaleUnit, &sc[i]);
             }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int row = lds.slots[buffer][16 * half + c];
@@ -296,29 +301,36 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
         };
 
         f32x4 o[S::kTiles];
-#pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -inf, l = 0.0f;
 
-        fetch(first_tile);
-        int slot = place(0), buffer = 0;
+        Place here = find(s.tile), next = find(s.tile + s.step);
+        if (here.b >= 0) load_queries(here.b);
+        fetch(here);
+        int slot = place(0), next_slot, buffer = 0;
+        fetch(next);
+        __builtin_amdgcn_sched_barrier(0);
         load_keys(0, slot);
+        __builtin_amdgcn_sched_barrier(0);
         load_values(0);
-        bool next_holes = __any(slot < 0);
-        fetch(first_tile + 1);
-        for (int tile = first_tile; tile <= last_tile; ++tile, buffer ^= 1) {
-            holes = next_holes;
+        __builtin_amdgcn_sched_barrier(0);
+        int from = here.base;  // the first tile of this sequence here
+#pragma unroll
+        for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int tile = s.tile; here.b >= 0; tile += s.step, buffer ^= 1, slot = next_slot) {
+            const bool holes = __any(slot < 0);  // a position of the tile is not there, or not seen
             // the next tile's slots
-            slot = place(buffer ^ 1);
-            next_holes = __any(slot < 0);
-            fetch(tile + 2);
-            // this tile's scales
+            next_slot = place(buffer ^ 1);
+            const Place after = find(tile + 2 * s.step);
+            fetch(after);
+            __builtin_amdgcn_sched_barrier(0);
+            // this tile's scales; without a slot 0, or 2^0 for the zeros there
             if constexpr (FP8) {
-                lds.scales.f[lane / kTile][t] = __uint_as_float(sc[0]);
+                lds.scales.f[lane / kTile][t] = slot < 0 ? 0.0f : __uint_as_float(sc[0]);
             } else {
 #pragma unroll
                 for (int i = 0; i < S::kBlocks; ++i)
-                    lds.scales.b[lane / kTile][i][t] = static_cast<uint8_t>(sc[i / 4] >> (8 * (i % 4)));
+                    lds.scales.b[lane / kTile][i][t] =
+                        static_cast<uint8_t>(slot < 0 ? kOne : sc[i / kScaleUnit] >> (8 * (i % kScaleUnit)));
             }
             __builtin_amdgcn_wave_barrier();
 
@@ -372,12 +384,11 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                     const i32x4 at = *reinterpret_cast<const i32x4*>(&lds.slots[buffer][16 * half + 4 * g]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int pos = tile * kTile + 16 * half + 4 * g + i;
-                        if (pos < vis.first || pos >= vis.end) x[4 * half + i] = -inf;
-                        else if (at[i] < 0) x[4 * half + i] = nan;
+                        const int pos = here.base + 16 * half + 4 * g + i;
+                        const float y = at[i] < 0 ? nan : x[4 * half + i];
+                        x[4 * half + i] = pos >= here.first && pos < here.end ? y : -inf;
 #pragma unroll
-                        for (int w = 0; w < VC::dwords(); ++w)
-                            if (at[i] < 0) v[4 * half + i][w] = 0;
+                        for (int w = 0; w < VC::dwords(); ++w) v[4 * half + i][w] &= ~(at[i] >> 31);
                     }
                 }
             }
@@ -390,7 +401,12 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                     for (int i = 0; i < 4; ++i) vs[4 * half + i] = f[i];
                 }
             }
-            if (tile < last_tile) load_keys(buffer ^ 1, slot);
+            // in front of the keys that will meet them: the wait for those is the wait for both
+            __builtin_amdgcn_sched_barrier(0);
+            if (next.b != here.b && next.b >= 0) load_queries(next.b);
+            __builtin_amdgcn_sched_barrier(0);
+            load_keys(buffer ^ 1, next_slot);  // behind the last tile: row 0
+            __builtin_amdgcn_sched_barrier(0);
 
             // ---- weights ----
             float most = x[0];
@@ -472,72 +488,107 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                     });
                 }
             });
-            if (tile < last_tile) load_values(buffer ^ 1);
-        }
+            __builtin_amdgcn_sched_barrier(0);
+            load_values(buffer ^ 1);
+            __builtin_amdgcn_sched_barrier(0);
 
-        // ---- result ----
-        l += __shfl_xor(l, 16, kWave);
-        l += __shfl_xor(l, 32, kWave);
-        const bool whole = holds_all(s, s.tile, end, tiles);
-        const int64_t segment = (static_cast<int64_t>(s.unit) + b) * p.q_heads + head0 + qi;
-        const float by = whole ? 1.0f / l : 1.0f;
-        each<VC::pieces()>([&](auto piece) {
-            constexpr int kP = piece, kValues = (FP8 ? 1 : 2) * VC::lane_bytes(kP);
-            constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16, kD0 = (FP8 ? 1 : 2) * VC::start(kP);
-            // a column's pieces share its rows out
+            // ---- the sequence's end here ----
+            if (next.b != here.b) {
+                l += __shfl_xor(l, 16, kWave);
+                l += __shfl_xor(l, 32, kWave);
+                const bool whole = from == here.first / kTile * kTile && here.base == (here.end - 1) / kTile * kTile;
+                const int64_t row = (static_cast<int64_t>(s.unit) + here.b) * p.q_heads + head0 + qi;
+                const float by = p.units != 0 && whole ? 1.0f / l : 1.0f;
+                each<VC::pieces()>([&](auto piece) {
+                    constexpr int kP = piece, kValues = (FP8 ? 1 : 2) * VC::lane_bytes(kP);
+                    constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16, kD0 = (FP8 ? 1 : 2) * VC::start(kP);
+                    // a column's pieces share its rows out
 #pragma unroll
-            for (int i = 0; i < 4 * kN / 16; ++i) {
-                const int r = part * (4 * kN / 16) + i;
-                float y[kValues];
+                    for (int i = 0; i < 4 * kN / 16; ++i) {
+                        const int r = part * (4 * kN / 16) + i;
+                        float y[kValues];
 #pragma unroll
-                for (int j = 0; j < kValues; ++j) {
-                    f32x4 a = o[kTile0 + j];
+                        for (int j = 0; j < kValues; ++j) {
+                            f32x4 a = o[kTile0 + j];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        a[e] += dpp<kRor8>(a[e]);
-                        if constexpr (!BF16) a[e] += dpp<kRor4>(a[e]);
+                            for (int e = 0; e < 4; ++e) {
+                                a[e] += dpp<kRor8>(a[e]);
+                                if constexpr (!BF16) a[e] += dpp<kRor4>(a[e]);
+                            }
+                            y[j] = (r == 0 ? a[0] : r == 1 ? a[1] : r == 2 ? a[2] : a[3]) * by;
+                        }
+                        const int d = kD0 + (4 * g + r) * kValues;
+                        if (qi >= heads) continue;
+                        if (p.units == 0) store_values<false, kValues>(joint + (wave * kN + qi) * kRow + d, y);
+                        else if (!whole) store_values<false, kValues>(p.part_o + row * D + d, y);
+                        else
+                            store_values<BF16, kValues>(static_cast<Elem<BF16>*>(p.out) +
+                                                            (static_cast<int64_t>(here.b) * p.q_heads + head0 + qi) * D + d,
+                                                        y);
                     }
-                    y[j] = r == 0 ? a[0] : r == 1 ? a[1] : r == 2 ? a[2] : a[3];
-                }
-                const int d = kD0 + (4 * g + r) * kValues;
-                if (qi < heads) {
-#pragma unroll
-                    for (int j = 0; j < kValues; ++j) {
-                        if (!whole) p.part_o[segment * D + d + j] = y[j];
-                        else if constexpr (BF16) out[d + j] = kc::f32_to_bf16(y[j] * by);
-                        else out[d + j] = y[j] / l;
+                });
+                if (lane < heads) {
+                    if (p.units == 0) {
+                        joint_ml[wave][0][lane] = m;
+                        joint_ml[wave][1][lane] = l;
+                    } else if (!whole) {
+                        p.part_ml[row * 2] = m;
+                        p.part_ml[row * 2 + 1] = l;
                     }
                 }
+                from = next.base;
+#pragma unroll
+                for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                m = -inf;
+                l = 0.0f;
             }
-        });
-        if (!whole && qi < heads && part == 0 && g == 0) {
-            p.part_ml[segment * 2] = m;
-            p.part_ml[segment * 2 + 1] = l;
+            here = next;
+            next = after;
         }
-        s.first += tiles;
-        s.tile = end;
-        if (p.units == 0 || end == s.end) return;
+    if (p.units != 0) return;
+
+    // ---- a whole sequence: all waves' parts; the workgroup has one set ----
+    __syncthreads();
+    Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(s.b) * p.q_heads + head0) * D;
+    const int parts = min(p.streams, s.end);
+    for (int i = threadIdx.x; i < heads * (D / 4); i += blockDim.x) {
+        const int head = i / (D / 4), d = (i - head * (D / 4)) * 4;
+        float most = -inf, sum = 0.0f;
+        for (int w = 0; w < parts; ++w) most = fmaxf(most, joint_ml[w][0][head]);
+        const float at = most == -inf ? 0.0f : most;
+        f32x4 y{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < parts; ++w) {
+            const float by = __builtin_amdgcn_exp2f(joint_ml[w][0][head] - at);
+            sum = fmaf(by, joint_ml[w][1][head], sum);
+            const f32x4 a = *reinterpret_cast<const f32x4*>(joint + (w * kN + head) * kRow + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = fmaf(by, a[e], y[e]);
+        }
+        const float by = parts == 0 ? 0.0f : 1.0f / sum;  // no position: zeros
+        const float r[4] = {y.x * by, y.y * by, y.z * by, y.w * by};
+        store_values<BF16, 4>(out + head * D + d, r);
     }
 }
 
 template <bool BF16, bool FP8>
-bool launch(const Attention& p, dim3 grid, int threads, hipStream_t stream) {
+void launch(const Attention& p, dim3 grid, hipStream_t stream) {
+    const int waves = p.wg_sets * p.streams;
+    const unsigned lds = p.units == 0 ? waves * (BF16 ? 8 : 4) * (p.D + 4) * 4 : 0;
     switch (p.D) {
-        case 64: attention_mfma_kernel<BF16, FP8, 64><<<grid, threads, 0, stream>>>(p); return true;
-        case 96: attention_mfma_kernel<BF16, FP8, 96><<<grid, threads, 0, stream>>>(p); return true;
-        case 128: attention_mfma_kernel<BF16, FP8, 128><<<grid, threads, 0, stream>>>(p); return true;
-        case 192: attention_mfma_kernel<BF16, FP8, 192><<<grid, threads, 0, stream>>>(p); return true;
-        case 256: attention_mfma_kernel<BF16, FP8, 256><<<grid, threads, 0, stream>>>(p); return true;
+        case 64: attention_mfma_kernel<BF16, FP8, 64><<<grid, waves * kWave, lds, stream>>>(p); return;
+        case 96: attention_mfma_kernel<BF16, FP8, 96><<<grid, waves * kWave, lds, stream>>>(p); return;
+        case 128: attention_mfma_kernel<BF16, FP8, 128><<<grid, waves * kWave, lds, stream>>>(p); return;
+        case 192: attention_mfma_kernel<BF16, FP8, 192><<<grid, waves * kWave, lds, stream>>>(p); return;
+        case 256: attention_mfma_kernel<BF16, FP8, 256><<<grid, waves * kWave, lds, stream>>>(p); return;
         default: break;
     }
     if constexpr (FP8) {
         switch (p.D) {
-            case 80: attention_mfma_kernel<BF16, FP8, 80><<<grid, threads, 0, stream>>>(p); return true;
-            case 112: attention_mfma_kernel<BF16, FP8, 112><<<grid, threads, 0, stream>>>(p); return true;
+            case 80: attention_mfma_kernel<BF16, FP8, 80><<<grid, waves * kWave, lds, stream>>>(p); return;
+            case 112: attention_mfma_kernel<BF16, FP8, 112><<<grid, waves * kWave, lds, stream>>>(p); return;
             default: break;
         }
     }
-    return false;
 }
 
 }  // namespace
@@ -545,20 +596,20 @@ bool launch(const Attention& p, dim3 grid, int threads, hipStream_t stream) {
 namespace kc {
 namespace kv {
 
-bool mfma_takes(const kc_kv_cache& c) {
+bool mfma_takes(const kc_kv_cache& c, int64_t max_pages) {
     const bool fp8 = c.format == KC_KV_FP8;
     const int blocks = c.head_dim / 32;
     // rows of codes in whole 16 bytes, scales in the units that they are loaded in
     const uintptr_t unit = fp8 ? 4 : blocks % 4 == 0 ? 4 : blocks % 2 == 0 ? 2 : 1;
     const bool size = c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 192 ||
                       c.head_dim == 256 || (fp8 && (c.head_dim == 80 || c.head_dim == 112));
-    return size && c.num_pages > 0 && aligned(c.k_codes, 16) && aligned(c.v_codes, 16) && aligned(c.k_scales, unit) &&
+    return size && c.num_pages > 0 && max_pages > 0 && aligned(c.k_codes, 16) && aligned(c.v_codes, 16) && aligned(c.k_scales, unit) &&
            aligned(c.v_scales, unit);
 }
 
-bool launch_mfma(const Attention& p, bool bf16, bool fp8, dim3 grid, int threads, hipStream_t stream) {
-    if (bf16) return fp8 ? launch<true, true>(p, grid, threads, stream) : launch<true, false>(p, grid, threads, stream);
-    return fp8 ? launch<false, true>(p, grid, threads, stream) : launch<false, false>(p, grid, threads, stream);
+void launch_mfma(const Attention& p, bool bf16, bool fp8, dim3 grid, hipStream_t stream) {
+    if (bf16) return fp8 ? launch<true, true>(p, grid, stream) : launch<true, false>(p, grid, stream);
+    return fp8 ? launch<false, true>(p, grid, stream) : launch<false, false>(p, grid, stream);
 }
 
 }  // namespace kv
