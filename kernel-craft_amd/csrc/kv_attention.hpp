@@ -32,6 +32,7 @@ struct Attention {
     const int32_t *table, *lens;
     int64_t q_stride, max_pages, num_pages;
     int page, page_shift;  // page_shift: its logarithm, or -1
+    int room;              // positions of a row of the table, at most 2^31 - 1
     int kv_heads, D, q_heads, group, seqs, window;
     float scale;       // times log2(e)
     int units;         // stretches; 0: whole sequences, and no join
@@ -52,17 +53,33 @@ struct Visible {
 
 __device__ __forceinline__ Visible visible_of(const Attention& p, int len) {
     len = max(len, 0);
-    const int64_t room = p.max_pages * p.page;
-    if (len > room) return {static_cast<int>(room), static_cast<int>(room) + 1};
+    if (len > p.room) return {p.room, p.room + 1};
     return {p.window > 0 && p.window < len ? len - p.window : 0, len};
 }
 
 __device__ __forceinline__ Visible visible(const Attention& p, int b) { return visible_of(p, p.lens[b]); }
 
-// The same for a wave-uniform b: a scalar load, which vector loads in flight do not hold up.
+// An element of memory that nothing writes while the kernel runs, at a wave-uniform index: a
+// scalar load, which vector loads in flight do not hold up.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* from, int64_t i) {
+    typedef const __attribute__((address_space(4))) T* Constant;
+    return reinterpret_cast<Constant>(reinterpret_cast<uintptr_t>(from))[i];
+}
+
 __device__ __forceinline__ Visible visible_scalar(const Attention& p, int b) {
-    typedef const __attribute__((address_space(4))) int32_t* Constant;
-    return visible_of(p, reinterpret_cast<Constant>(reinterpret_cast<uintptr_t>(p.lens))[__builtin_amdgcn_readfirstlane(b)]);
+    return visible_of(p, scalar_load(p.lens, __builtin_amdgcn_readfirstlane(b)));
+}
+
+// Inclusive scan over the 64 lanes.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);   // from 1, 2, 4, 8 lanes below in a row of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, true);   // the row below's last lane, in rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, true);   // lane 31's, in the upper half
+    return v;
 }
 
 // Slot of a position; -1 where its page is missing.  num_pages * page_size is below 2^31.
@@ -77,38 +94,60 @@ __device__ __forceinline__ int slot_of(const Attention& p, int b, int pos) {
 // first tile is `first`.  b < 0: nothing.
 struct Stretch {
     int tile, end, step, first, b, unit;
+    Visible vis;  // of sequence b
 };
 
 struct PlanShared {
     int part[kMaxWaves], first[kMaxWaves], b[kMaxWaves];
 };
 
-// The stretch of this wave (wave-uniform), found by the whole workgroup `at` (of those with
-// the same sets): thread i counts the tiles of its own sequences, a scan puts them in a
-// row, and the thread whose sequences hold a stretch's first tile says so.
+// The stretch of this wave (wave-uniform) of workgroup `at` of those with the same sets.  Up
+// to 64 sequences, every wave counts all tiles by itself: a load, a scan and no barrier.
+// Beyond, the workgroup does: thread i counts the tiles of its own sequences, a scan puts
+// them in a row, and the thread whose sequences hold a stretch's first tile says so.
 __device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& s, int at, int stream, bool says_starts) {
     Stretch r;
     if (p.units == 0) {
         r.unit = at;
         r.b = at < p.seqs ? at : -1;
+        r.vis = at < p.seqs ? visible_scalar(p, at) : Visible{0, 0};
         r.first = 0;
         r.tile = stream;
         r.step = p.streams;
-        r.end = at < p.seqs ? visible_scalar(p, at).tiles() : 0;
+        r.end = r.vis.tiles();
         return r;
     }
-    const int threads = blockDim.x, tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
-    const int each = (p.seqs + threads - 1) / threads;
+    r.unit = at * p.streams + stream;
+    r.step = 1;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    if (p.seqs <= kWave) {
+        const Visible mine = lane < p.seqs ? visible(p, lane) : Visible{0, 0};
+        const int n = mine.tiles(), up = wave_scan(n), total = __builtin_amdgcn_readlane(up, kWave - 1);
+        const int per = max((total + p.units - 1) / p.units, p.min_tiles);
+        r.tile = r.unit * per;  // below 2^30 + units * min_tiles
+        r.end = min(r.tile + per, total);
+        if (says_starts && wave == 0) {  // for the join
+            if (lane < p.seqs) p.starts[lane] = up - n;
+            if (lane == 0) {
+                p.starts[p.seqs] = total;
+                p.starts[p.seqs + 1] = per;
+            }
+        }
+        // the first sequence that ends behind the stretch's first tile
+        const int b = __builtin_popcountll(__ballot(up <= r.tile));
+        r.b = r.tile < total ? b : -1;
+        const int from = b < kWave ? b : 0;
+        r.vis.first = __builtin_amdgcn_readlane(mine.first, from);
+        r.vis.end = __builtin_amdgcn_readlane(mine.end, from);
+        r.first = __builtin_amdgcn_readlane(up - n, from);
+        return r;
+    }
+    const int threads = blockDim.x, each = (p.seqs + threads - 1) / threads;
     const int b0 = min(tid * each, p.seqs), b1 = min(b0 + each, p.seqs);
     const int n0 = b0 < b1 ? visible(p, b0).tiles() : 0;  // most often all
     int mine = n0;
     for (int b = b0 + 1; b < b1; ++b) mine += visible(p, b).tiles();
-    int up = mine;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const int below = __shfl_up(up, off, kWave);
-        if (lane >= off) up += below;
-    }
+    const int up = wave_scan(mine);
     if (lane == kWave - 1) s.part[wave] = up;
     if (tid < kMaxWaves) s.b[tid] = -1;
     __syncthreads();
@@ -120,14 +159,14 @@ __device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& 
     before += up - mine;
     const int per = max((total + p.units - 1) / p.units, p.min_tiles);
     for (int i = 0; i < p.streams; ++i) {
-        const int t = (at * p.streams + i) * per;  // below 2^30 + units * min_tiles
+        const int t = (at * p.streams + i) * per;
         if (t < before || t >= before + mine) continue;
         int to = before, b = b0;
         for (int n = n0; t >= to + n; n = visible(p, ++b).tiles()) to += n;
         s.b[i] = b;
         s.first[i] = to;
     }
-    if (says_starts) {  // for the join
+    if (says_starts) {
         int to = before;
         for (int b = b0; b < b1; ++b) {
             p.starts[b] = to;
@@ -139,11 +178,10 @@ __device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& 
         }
     }
     __syncthreads();
-    r.unit = at * p.streams + stream;
     r.b = __builtin_amdgcn_readfirstlane(s.b[stream]);
     r.first = __builtin_amdgcn_readfirstlane(s.first[stream]);
+    r.vis = r.b >= 0 ? visible_scalar(p, r.b) : Visible{0, 0};
     r.tile = r.unit * per;
-    r.step = 1;
     r.end = min(r.tile + per, total);
     return r;
 }

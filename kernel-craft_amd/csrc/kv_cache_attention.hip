@@ -147,15 +147,33 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
     }
 }
 
-// blockDim.x / 64 waves, `split` of them for a query head of a sequence: each joins some of
-// its segments, then one all of theirs.
-template <bool BF16>
+// What parts of a sum have come to: maximum, sum and W values of the output.
+template <int W>
+struct Joined {
+    float m, l, o[W];
+
+    __device__ __forceinline__ void add(float m1, float l1, const float (&o1)[W]) {
+        const float most = fmaxf(m, m1), at = most == -__builtin_inff() ? 0.0f : most;
+        const float by = __builtin_amdgcn_exp2f(m - at), by1 = __builtin_amdgcn_exp2f(m1 - at);
+        m = most;
+        l = fmaf(l, by, l1 * by1);
+#pragma unroll
+        for (int e = 0; e < W; ++e) o[e] = fmaf(o[e], by, o1[e] * by1);
+    }
+};
+
+// blockDim.x / 64 waves, `split` of them for a query head of a sequence.  A row of a segment
+// takes D / W lanes (at most 64), so that a wave loads several segments at once, kAhead
+// times; the lanes of a value then join theirs, and the waves in LDS.
+template <bool BF16, int W>
 __global__ __launch_bounds__(1024) void join_kernel(const Attention p, int split) {
+    constexpr int kAhead = 4;
     __shared__ float part_ml[16][2];
     extern __shared__ float part_o[];  // [waves][D] where split > 1
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int b = blockIdx.x, head = blockIdx.y * (blockDim.x / kWave / split) + wave / split, sub = wave % split;
-    const int tile = p.starts[b], end = p.starts[b + 1], per = p.starts[p.seqs + 1];
+    const int tile = scalar_load(p.starts, b), end = scalar_load(p.starts, b + 1);
+    const int per = scalar_load(p.starts, p.seqs + 1);
     const bool mine = head < p.q_heads;
     Elem<BF16>* out = static_cast<Elem<BF16>*>(p.out) + (static_cast<int64_t>(b) * p.q_heads + head) * p.D;
     if (tile == end) {
@@ -165,50 +183,60 @@ __global__ __launch_bounds__(1024) void join_kernel(const Attention p, int split
     }
     const int unit = tile / per, n = (end - 1) / per - unit + 1;
     if (n == 1) return;  // the same for the whole workgroup
-    const float inf = __uint_as_float(0x7F800000u);
     const int64_t first = static_cast<int64_t>(unit + b) * p.q_heads + head;
-    float m = -inf, l = 0.0f;
+    int row_lanes = kWave;
+    while (row_lanes / 2 * W >= p.D) row_lanes /= 2;
+    const int groups = kWave / row_lanes, group = lane / row_lanes, at = lane - group * row_lanes;
     if (mine) {
-        for (int i = sub + lane * split; i < n; i += kWave * split)
-            m = fmaxf(m, p.part_ml[(first + static_cast<int64_t>(i) * p.q_heads) * 2]);
-        m = kc::wave_max(m);
-        const float at = m == -inf ? 0.0f : m;
-        for (int d0 = 0; d0 < p.D; d0 += 2 * kWave) {
-            float o[2] = {};
-            l = 0.0f;
-            const int d = d0 + lane, d1 = min(d, p.D - 1), d2 = min(d + kWave, p.D - 1);
-#pragma unroll 8
-            for (int i = sub; i < n; i += split) {
-                const int64_t row = first + static_cast<int64_t>(i) * p.q_heads;
-                const float w = __builtin_amdgcn_exp2f(p.part_ml[row * 2] - at);
-                l = fmaf(w, p.part_ml[row * 2 + 1], l);
-                o[0] = fmaf(w, p.part_o[row * p.D + d1], o[0]);
-                o[1] = fmaf(w, p.part_o[row * p.D + d2], o[1]);
-            }
+        for (int d0 = 0; d0 < p.D; d0 += row_lanes * W) {
+            const int d = d0 + at * W, from = min(d, p.D - W);
+            Joined<W> j{-__builtin_inff(), 0.0f, {}};
+            for (int i0 = sub * groups + group; i0 < n; i0 += kAhead * split * groups) {
+                float sm[kAhead], sl[kAhead], so[kAhead][W];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (d + e * kWave >= p.D) break;
-                if (split > 1) part_o[wave * p.D + d + e * kWave] = o[e];
-                else put<BF16>(out, d + e * kWave, o[e] / l);
+                for (int i = 0; i < kAhead; ++i) {  // behind the last segment: that one again, without weight
+                    const int seg = i0 + i * split * groups;
+                    const int64_t row = first + static_cast<int64_t>(min(seg, n - 1)) * p.q_heads;
+                    sm[i] = p.part_ml[row * 2];
+                    sl[i] = p.part_ml[row * 2 + 1];
+                    __builtin_memcpy(so[i], __builtin_assume_aligned(p.part_o + row * p.D + from, 4 * W), 4 * W);
+                }
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i)
+                    if (i0 + i * split * groups < n) j.add(sm[i], sl[i], so[i]);
             }
-        }
-        if (lane == 0) {
-            part_ml[wave][0] = m;
-            part_ml[wave][1] = l;
+            for (int off = row_lanes; off < kWave; off *= 2) {
+                float o1[W];
+                const float m1 = __shfl_xor(j.m, off, kWave), l1 = __shfl_xor(j.l, off, kWave);
+#pragma unroll
+                for (int e = 0; e < W; ++e) o1[e] = __shfl_xor(j.o[e], off, kWave);
+                j.add(m1, l1, o1);
+            }
+            if (group == 0 && d < p.D) {
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    if (split > 1) part_o[wave * p.D + d + e] = j.o[e];
+                    else put<BF16>(out, d + e, j.o[e] / j.l);
+                }
+            }
+            if (lane == 0) {
+                part_ml[wave][0] = j.m;
+                part_ml[wave][1] = j.l;
+            }
         }
     }
     if (split == 1) return;
     __syncthreads();
-    if (!mine || sub != 0) return;
-    const int w1 = wave + min(split, n);
-    for (int w = wave; w < w1; ++w) m = fmaxf(m, part_ml[w][0]);
-    const float at = m == -inf ? 0.0f : m;
-    l = 0.0f;
-    for (int w = wave; w < w1; ++w) l = fmaf(__builtin_amdgcn_exp2f(part_ml[w][0] - at), part_ml[w][1], l);
-    for (int d = lane; d < p.D; d += kWave) {
-        float o = 0.0f;
-        for (int w = wave; w < w1; ++w) o = fmaf(__builtin_amdgcn_exp2f(part_ml[w][0] - at), part_o[w * p.D + d], o);
-        put<BF16>(out, d, o / l);
+    if (!mine) return;
+    // the waves of a head share its values out
+    const int w0 = wave - sub;
+    for (int d = lane + sub * kWave; d < p.D; d += kWave * split) {
+        Joined<1> j{-__builtin_inff(), 0.0f, {}};
+        for (int w = w0; w < w0 + split; ++w) {
+            const float o1[1] = {part_o[w * p.D + d]};
+            j.add(part_ml[w][0], part_ml[w][1], o1);
+        }
+        put<BF16>(out, d, j.o[0] / j.l);
     }
 }
 
@@ -307,6 +335,7 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     p.num_pages = cache->num_pages;
     p.page = cache->page_size;
     p.page_shift = kc::is_pow2(p.page) ? kc::ilog2(p.page) : -1;
+    p.room = static_cast<int>(std::min<int64_t>(max_pages * p.page, INT32_MAX));
     p.kv_heads = cache->kv_heads;
     p.D = cache->head_dim;
     p.q_heads = q_heads;
@@ -336,8 +365,10 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     // one wave per query head of a sequence where that makes waves enough, else 4 or 16
     const int64_t pairs = int64_t{seqs} * q_heads;
     const int split = pairs >= 2048 ? 1 : pairs >= 512 ? 4 : 16, waves = std::max(split, 4), per_wg = waves / split;
-    join_kernel<BF16><<<dim3(seqs, (q_heads + per_wg - 1) / per_wg), waves * kWave, split > 1 ? waves * p.D * 4 : 0,
-                        stream>>>(p, split);
+    const dim3 join_grid(seqs, (q_heads + per_wg - 1) / per_wg);
+    const unsigned lds = split > 1 ? waves * p.D * sizeof(float) : 0;
+    if (p.D % 4 == 0) join_kernel<BF16, 4><<<join_grid, waves * kWave, lds, stream>>>(p, split);
+    else join_kernel<BF16, 1><<<join_grid, waves * kWave, lds, stream>>>(p, split);
     return kc::check_launch(fn);
 }
 

@@ -202,7 +202,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
         int b, base, first, end;
     };
     int seq = s.b, seq_first = s.first;
-    Visible vis = visible_scalar(p, seq);
+    Visible vis = s.vis;
     auto find = [&](int tile) {
         if (tile >= s.end) return Place{-1, 0, 0, 0};
         for (int n = vis.tiles(); tile >= seq_first + n; n = vis.tiles()) {  // tile < s.end ends it
