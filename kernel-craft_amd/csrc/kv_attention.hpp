@@ -30,8 +30,8 @@ struct Attention {
     const uint8_t *k_codes, *v_codes;
     const void *k_scales, *v_scales;
     const int32_t *table, *lens;
-    int64_t q_stride, max_pages, num_pages;
-    int page, page_shift;  // page_shift: its logarithm, or -1
+    int64_t q_stride;
+    int max_pages, num_pages, page, page_shift;  // page_shift: its logarithm, or -1
     int room;              // positions of a row of the table, at most 2^31 - 1
     int kv_heads, D, q_heads, group, seqs, window;
     float scale;       // times log2(e)
@@ -44,11 +44,13 @@ struct Attention {
     float* part_ml;    // [units + seqs][q_heads][2]
 };
 
+__device__ __forceinline__ int tile_of(int pos) { return static_cast<uint32_t>(pos) / kTile; }
+
 // Visible positions [first, end) of a sequence.  A length past the table sees a page that
 // is missing, hence one position there in place of all.
 struct Visible {
     int first, end;
-    __device__ __forceinline__ int tiles() const { return end > first ? (end - 1) / kTile - first / kTile + 1 : 0; }
+    __device__ __forceinline__ int tiles() const { return end > first ? tile_of(end - 1) - tile_of(first) + 1 : 0; }
 };
 
 __device__ __forceinline__ Visible visible_of(const Attention& p, int len) {
@@ -86,7 +88,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 __device__ __forceinline__ int slot_of(const Attention& p, int b, int pos) {
     const int at = pos / p.page;
     if (at >= p.max_pages) return -1;
-    const int32_t page = p.table[b * p.max_pages + at];
+    const int32_t page = p.table[static_cast<int64_t>(b) * p.max_pages + at];
     return page < 0 || page >= p.num_pages ? -1 : page * p.page + (pos - at * p.page);
 }
 

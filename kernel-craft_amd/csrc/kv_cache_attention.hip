@@ -331,8 +331,8 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     p.table = table;
     p.lens = lens;
     p.q_stride = q_stride;
-    p.max_pages = max_pages;
-    p.num_pages = cache->num_pages;
+    p.max_pages = static_cast<int>(max_pages);
+    p.num_pages = static_cast<int>(cache->num_pages);
     p.page = cache->page_size;
     p.page_shift = kc::is_pow2(p.page) ? kc::ilog2(p.page) : -1;
     p.room = static_cast<int>(std::min<int64_t>(max_pages * p.page, INT32_MAX));

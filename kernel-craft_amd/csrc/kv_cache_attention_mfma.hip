@@ -158,10 +158,12 @@ struct Shape {
     static constexpr int kTiles = D / 16;          // of O^T
 };
 
-// LDS of a wave: slots of two tiles in turn, scales of one.
+// LDS of a wave: slots of two tiles in turn, where the rows of the coming one lie (in 16
+// bytes; the first row for positions without a slot), scales of one.
 template <bool FP8, int D>
 struct WaveShared {
     int slots[2][kTile];
+    uint32_t rows[kTile];
     union {
         float f[2][kTile];                                        // FP8: keys, values
         uint8_t b[2][FP8 ? 1 : Shape<FP8, D>::kBlocks][kTile];    // MXFP4
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
     const int heads = min(kN, p.group - q0), qi = c & (kN - 1);
     const int64_t head0 = static_cast<int64_t>(h) * p.group + q0;
     const float nan = __uint_as_float(0x7FC00000u), inf = __uint_as_float(0x7F800000u);
-    const uint32_t row_bytes = static_cast<uint32_t>(p.kv_heads) * S::kRow;
+    const uint32_t row_units = static_cast<uint32_t>(p.kv_heads) * (S::kRow / 16);  // 16 bytes
     const uint8_t* kbase = p.k_codes + static_cast<int64_t>(h) * S::kRow;
     const uint8_t* vbase = p.v_codes + static_cast<int64_t>(h) * S::kRow;
     // lanes 0 .. 31 fetch the scales of keys, the others those of values
@@ -201,15 +203,17 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
     struct Place {
         int b, base, first, end;
     };
-    int seq = s.b, seq_first = s.first;
+    int seq = s.b, seq_end = s.first + s.vis.tiles();  // the sequence that find() is at, the tile behind its last
     Visible vis = s.vis;
+    int shift = tile_of(vis.first) - s.first;
     auto find = [&](int tile) {
-        if (tile >= s.end) return Place{-1, 0, 0, 0};
-        for (int n = vis.tiles(); tile >= seq_first + n; n = vis.tiles()) {  // tile < s.end ends it
-            seq_first += n;
+        if (tile >= s.end) return Place{-1, kTile, 1, 1};
+        while (tile >= seq_end) {  // tile < s.end ends it
             vis = visible_scalar(p, ++seq);
+            shift = tile_of(vis.first) - seq_end;
+            seq_end += vis.tiles();
         }
-        return Place{seq, (vis.first / kTile + tile - seq_first) * kTile, vis.first, vis.end};
+        return Place{seq, (tile + shift) * kTile, vis.first, vis.end};
     };
 
     // ---- queries: the operand of every step ----
@@ -251,21 +255,31 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
         int entry, offset;  // of this lane's position t, two tiles ahead; offset < 0: not seen, or past the table
         auto fetch = [&](const Place& at) {
             const int pos = at.base + t, near = min(max(pos, at.first), at.end - 1);
-            const int page = p.page_shift >= 0 ? near >> p.page_shift : near / p.page;
-            entry = p.table[max(at.b, 0) * p.max_pages + max(min(page, static_cast<int>(p.max_pages) - 1), 0)];
+            const int page = p.page_shift >= 0 ? near >> p.page_shift : static_cast<uint32_t>(near) / p.page;
+            const int32_t* row = p.table + static_cast<int64_t>(max(at.b, 0)) * p.max_pages;
+            entry = row[static_cast<uint32_t>(min(page, p.max_pages - 1))];
             offset = near == pos && page < p.max_pages ? near - page * p.page : -1;
         };
         uint32_t k[2][KC::dwords()], v[8][VC::dwords()];
         constexpr int kScaleUnit = S::kBlocks % 4 == 0 ? 4 : S::kBlocks % 2 == 0 ? 2 : 1;  // MXFP4 scales of a load
         uint32_t sc[FP8 ? 1 : S::kBlocks / kScaleUnit];
-        i32x4 vslot[2];
-        auto place = [&](int buffer) {  // slots of the fetched tile
-            const int slot = offset >= 0 && entry >= 0 && entry < p.num_pages ? entry * p.page + offset : -1;
+        uint32_t krow[2];
+        u32x4 vrow[2];
+        auto place = [&](int buffer) {  // slots of the fetched tile, and where their rows lie
+            const bool there = offset >= 0 && static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_pages);
+            const int slot = there ? entry * p.page + offset : -1;
             lds.slots[buffer][t] = slot;
+            lds.rows[t] = there ? static_cast<uint32_t>(slot) * row_units : 0u;
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                krow[half] = lds.rows[16 * half + c];
+                vrow[half] = *reinterpret_cast<const u32x4*>(&lds.rows[16 * half + 4 * g]);
+            }
             __builtin_amdgcn_wave_barrier();
             return slot;
         };
-        auto load_keys = [&](int buffer, int slot) {
+        auto load_keys = [&](int slot) {
             const uint8_t* at = sbase + static_cast<uint64_t>(static_cast<uint32_t>(max(slot, 0))) * scale_bytes;
             if constexpr (FP8) {
                 sc[0] = *reinterpret_cast<const uint32_t*>(at);
@@ -276,8 +290,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int row = lds.slots[buffer][16 * half + c];
-                const uint8_t* from = kbase + static_cast<uint64_t>(static_cast<uint32_t>(max(row, 0))) * row_bytes;
+                const uint8_t* from = kbase + (static_cast<uint64_t>(krow[half]) << 4);
                 each<KC::pieces()>([&](auto piece) {
                     constexpr int kP = piece;
                     load_bytes<KC::lane_bytes(kP)>(from + KC::start(kP) + g * KC::lane_bytes(kP),
@@ -285,14 +298,10 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                 });
             }
         };
-        auto load_values = [&](int buffer) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-                vslot[half] = *reinterpret_cast<const i32x4*>(&lds.slots[buffer][16 * half + 4 * g]);
+        auto load_values = [&]() {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int row = vslot[i / 4][i % 4];
-                const uint8_t* from = vbase + static_cast<uint64_t>(static_cast<uint32_t>(max(row, 0))) * row_bytes;
+                const uint8_t* from = vbase + (static_cast<uint64_t>(vrow[i / 4][i % 4]) << 4);
                 each<VC::pieces()>([&](auto piece) {
                     constexpr int kP = piece;
                     load_bytes<VC::lane_bytes(kP)>(from + VC::start(kP) + c * VC::lane_bytes(kP), &v[i][VC::dword(kP)]);
@@ -301,7 +310,8 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
         };
 
         f32x4 o[S::kTiles];
-        float m = -inf, l = 0.0f;
+        float m = -inf, l = 0.0f, at = 0.0f;  // at: m, or 0 while that is -inf
+        const float off1 = part >= 1 ? -1.0f : 0.0f, off2 = part >= 2 ? -1.0f : 0.0f;
 
         Place here = find(s.tile), next = find(s.tile + s.step);
         if (here.b >= 0) load_queries(here.b);
@@ -309,9 +319,9 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
         int slot = place(0), next_slot, buffer = 0;
         fetch(next);
         __builtin_amdgcn_sched_barrier(0);
-        load_keys(0, slot);
+        load_keys(slot);
         __builtin_amdgcn_sched_barrier(0);
-        load_values(0);
+        load_values();
         __builtin_amdgcn_sched_barrier(0);
         int from = here.base;  // the first tile of this sequence here
 #pragma unroll
@@ -325,7 +335,8 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
             __builtin_amdgcn_sched_barrier(0);
             // this tile's scales; without a slot 0, or 2^0 for the zeros there
             if constexpr (FP8) {
-                lds.scales.f[lane / kTile][t] = slot < 0 ? 0.0f : __uint_as_float(sc[0]);
+                lds.scales.f[lane / kTile][t] =
+                    slot < 0 ? 0.0f : __uint_as_float(sc[0]) * (lane < kTile ? p.scale : 1.0f);
             } else {
 #pragma unroll
                 for (int i = 0; i < S::kBlocks; ++i)
@@ -370,7 +381,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                         v += dpp<kRor8>(v);
                         v += dpp<kRor4>(v);
                     }
-                    x[4 * half + i] = v * p.scale;
+                    x[4 * half + i] = FP8 ? v : v * p.scale;
                 }
                 if constexpr (FP8) {
                     const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.scales.f[0][16 * half + 4 * g]);
@@ -405,32 +416,29 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
             __builtin_amdgcn_sched_barrier(0);
             if (next.b != here.b && next.b >= 0) load_queries(next.b);
             __builtin_amdgcn_sched_barrier(0);
-            load_keys(buffer ^ 1, next_slot);  // behind the last tile: row 0
+            load_keys(next_slot);  // behind the last tile: the first row
             __builtin_amdgcn_sched_barrier(0);
 
             // ---- weights ----
-            float most = x[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) most = fmaxf(most, x[i]);
-            most = fmaxf(most, __shfl_xor(most, 16, kWave));
-            most = fmaxf(most, __shfl_xor(most, 32, kWave));
-            if (__any(most > m + kLazy)) {  // a column's own decision: the others go on by 1
-                const float to = most > m + kLazy ? most : m;
+            const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            if (__any(most > m + kLazy)) {
+                float to = fmaxf(most, __shfl_xor(most, 16, kWave));
+                to = fmaxf(to, __shfl_xor(to, 32, kWave));
+                to = to > m + kLazy ? to : m;  // a column's own decision: the others go on by 1
                 const float by = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
                 m = to;
+                at = m == -inf ? 0.0f : m;
                 l *= by;
 #pragma unroll
                 for (int i = 0; i < S::kTiles; ++i) o[i] *= by;
             }
-            const float at = m == -inf ? 0.0f : m;
-            float sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = __builtin_amdgcn_exp2f(x[i] - at);
-                sum += x[i];
-                if constexpr (FP8) x[i] *= vs[i];
+            for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - at);
+            l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+            if constexpr (FP8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= vs[i];
             }
-            l += sum;
             uint32_t pw[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -438,10 +446,9 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
 #pragma unroll
                 for (int n = 1; n < (BF16 ? 2 : 3); ++n) {  // what the pieces before this column's hold is taken off
                     const uint32_t w = kc::pack_bf16x2(a, e);
-                    if (part >= n) {
-                        a -= __uint_as_float(w << 16);
-                        e -= __uint_as_float(w & 0xFFFF0000u);
-                    }
+                    const float off = n == 1 ? off1 : off2;
+                    a = fmaf(off, __uint_as_float(w << 16), a);
+                    e = fmaf(off, __uint_as_float(w & 0xFFFF0000u), e);
                 }
                 pw[i] = kc::pack_bf16x2(a, e);
                 if (!BF16 && part == 3) pw[i] = 0;
@@ -489,14 +496,14 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                 }
             });
             __builtin_amdgcn_sched_barrier(0);
-            load_values(buffer ^ 1);
+            load_values();
             __builtin_amdgcn_sched_barrier(0);
 
             // ---- the sequence's end here ----
             if (next.b != here.b) {
                 l += __shfl_xor(l, 16, kWave);
                 l += __shfl_xor(l, 32, kWave);
-                const bool whole = from == here.first / kTile * kTile && here.base == (here.end - 1) / kTile * kTile;
+                const bool whole = from == tile_of(here.first) * kTile && here.base == tile_of(here.end - 1) * kTile;
                 const int64_t row = (static_cast<int64_t>(s.unit) + here.b) * p.q_heads + head0 + qi;
                 const float by = p.units != 0 && whole ? 1.0f / l : 1.0f;
                 each<VC::pieces()>([&](auto piece) {
@@ -540,7 +547,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
 #pragma unroll
                 for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 m = -inf;
-                l = 0.0f;
+                l = at = 0.0f;
             }
             here = next;
             next = after;
@@ -604,7 +611,9 @@ bool mfma_takes(const kc_kv_cache& c, int64_t max_pages) {
     const bool size = c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 192 ||
                       c.head_dim == 256 || (fp8 && (c.head_dim == 80 || c.head_dim == 112));
     return size && c.num_pages > 0 && max_pages > 0 && aligned(c.k_codes, 16) && aligned(c.v_codes, 16) && aligned(c.k_scales, unit) &&
-           aligned(c.v_scales, unit);
+           aligned(c.v_scales, unit) &&
+           // rows are found by 32 bits of 16 bytes
+           c.num_pages * c.page_size * (fp8 ? c.head_dim : c.head_dim / 2) / 16 * c.kv_heads <= UINT32_MAX;
 }
 
 void launch_mfma(const Attention& p, bool bf16, bool fp8, dim3 grid, hipStream_t stream) {
