@@ -824,7 +824,10 @@ def _one_gpu(op: str, *tensors) -> int:
 def _launch(index: int, fn, *args) -> int:
     """fn(*args, stream) on the current stream of GPU ``index``."""
     import torch
-    if index == torch.cuda.current_device():
+    # the tensors are on a GPU, so torch has set CUDA up: the bare function without
+    # current_device()'s look at that (0.5 -> 0.1 us), where a torch has it
+    current = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+    if index == current():
         return fn(*args, _stream())
     with torch.cuda.device(index):
         return fn(*args, _stream())
@@ -987,6 +990,26 @@ def _kv_cache(op: str, k_codes, k_scales, v_codes, v_scales):
     """(kc_kv_cache, kv_heads, head_dim) of a cache's four tensors, which must be contiguous
     (they are written to); fp32 scales mean FP8 rows, u8 scales MXFP4 rows."""
     import torch
+    ct, st, shape = k_codes.dtype, k_scales.dtype, k_codes.shape
+    fp8 = st is torch.float32
+    if not (v_codes.dtype is ct and v_scales.dtype is st and k_codes.is_contiguous()
+            and v_codes.is_contiguous() and k_scales.is_contiguous() and v_scales.is_contiguous()
+            and (ct is torch.uint8 and (fp8 or st is torch.uint8) or fp8 and ct is torch.int8)
+            and len(shape) == 4 and v_codes.shape == shape):
+        _refuse_kv_cache(op, k_codes, k_scales, v_codes, v_scales)
+    pages, page, heads, width = shape
+    D = width if fp8 else 2 * width
+    want = (pages, page, heads) if fp8 else (pages, page, heads, D // 32)
+    if k_scales.shape != want or v_scales.shape != want or (not fp8 and D % 32):
+        raise ValueError(f"{op}: k_scales {tuple(k_scales.shape)} and v_scales "
+                         f"{tuple(v_scales.shape)} must be {want} (head_dim {D})")
+    return KvCache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+                   pages, page, heads, D, 0 if fp8 else 1), heads, D
+
+
+def _refuse_kv_cache(op: str, k_codes, k_scales, v_codes, v_scales):
+    """ValueError that says what is wrong with a cache's tensors."""
+    import torch
     fp8 = k_scales.dtype is torch.float32
     for name, t, dtypes in (("k_codes", k_codes, (torch.int8, torch.uint8) if fp8 else (torch.uint8,)),
                             ("v_codes", v_codes, (k_codes.dtype,)),
@@ -997,17 +1020,8 @@ def _kv_cache(op: str, k_codes, k_scales, v_codes, v_scales):
                              f"{' or '.join(str(d) for d in dtypes)}")
         if not t.is_contiguous():
             raise ValueError(f"{op}: {name} must be contiguous")
-    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
-        raise ValueError(f"{op}: k_codes {tuple(k_codes.shape)} and v_codes {tuple(v_codes.shape)} "
-                         "must both be [pages, page_size, kv_heads, codes of a head]")
-    pages, page, heads, width = k_codes.shape
-    D = width if fp8 else 2 * width
-    want = (pages, page, heads) if fp8 else (pages, page, heads, D // 32)
-    if k_scales.shape != want or v_scales.shape != want or (not fp8 and D % 32):
-        raise ValueError(f"{op}: k_scales {tuple(k_scales.shape)} and v_scales "
-                         f"{tuple(v_scales.shape)} must be {want} (head_dim {D})")
-    return KvCache(_ptr(k_codes), _ptr(k_scales), _ptr(v_codes), _ptr(v_scales), pages, page, heads,
-                   D, 0 if fp8 else 1), heads, D
+    raise ValueError(f"{op}: k_codes {tuple(k_codes.shape)} and v_codes {tuple(v_codes.shape)} "
+                     "must both be [pages, page_size, kv_heads, codes of a head]")
 
 
 def qk_norm_rope(q, k, q_gamma, k_gamma, cos, sin, positions, eps: float = 1e-6,
@@ -1145,14 +1159,18 @@ def kv_cache_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq
     import torch
     op = "kv_cache_attention"
     cache, Hkv, D = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
-    q = _heads(op, "q", q, (torch.bfloat16, torch.float32), (None, None, D))
-    B, Hq, _ = q.shape
+    dtype, shape = q.dtype, q.shape
+    bf16 = dtype is torch.bfloat16
+    whole = q.is_contiguous()
+    if not (whole and (bf16 or dtype is torch.float32) and len(shape) == 3 and shape[2] == D):
+        q = _heads(op, "q", q, (torch.bfloat16, torch.float32), (None, None, D))
+    B, Hq, _ = shape
     if Hq % Hkv:
         raise ValueError(f"{op}: q has {Hq} heads, not a multiple of the cache's {Hkv}")
     block_table = _take(op, "block_table", block_table, torch.int32)
     seq_lens = _take(op, "seq_lens", seq_lens, torch.int32)
     table = block_table.shape
-    if len(table) != 2 or table[0] != B or seq_lens.shape != (B,):
+    if len(table) != 2 or table[0] != B or seq_lens.shape != table[:1]:
         raise ValueError(f"{op}: block_table {tuple(table)} and seq_lens {tuple(seq_lens.shape)} "
                          f"must be [{B}, pages] and [{B}]")
     if window < 0:
@@ -1163,13 +1181,13 @@ def kv_cache_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq
     need = lib.kc_kv_cache_attention_workspace(ref, table[1], B, Hq)
     if need < 0:
         _check(op)
-    work = torch.empty(max(need, 0), dtype=torch.uint8, device=q.device)
-    out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-    fn = lib.kc_kv_cache_attention_bf16 if q.dtype == torch.bfloat16 else lib.kc_kv_cache_attention_f32
+    out = torch.empty_like(q) if whole else torch.empty(shape, dtype=dtype, device=q.device)
+    work = torch.empty(need, dtype=torch.uint8, device=q.device).data_ptr() if need else None
+    fn = lib.kc_kv_cache_attention_bf16 if bf16 else lib.kc_kv_cache_attention_f32
     with kernel_span(op, sequences=B, heads=Hq, kv_heads=Hkv, head_dim=D):
-        st = _launch(gpu, fn, _ptr(q), q.stride(0), Hq, ref, _ptr(block_table), table[1],
-                     _ptr(seq_lens), B, D ** -0.5 if scale is None else scale, min(window, 2 ** 31 - 1),
-                     _ptr(work), need, _ptr(out))
+        st = _launch(gpu, fn, q.data_ptr(), q.stride(0), Hq, ref, block_table.data_ptr(), table[1],
+                     seq_lens.data_ptr(), B, D ** -0.5 if scale is None else scale,
+                     min(window, 2 ** 31 - 1), work, need, out.data_ptr())
     _check(op, st)
     return out
 
@@ -1182,30 +1200,28 @@ class KvPages(ctypes.Structure):
 
 
 def _kv_pages(op: str, seq_lens, block_table, free_pages, free_count, page_size: int, written):
-    """(seq_lens, free_count, kc_kv_pages) of a cache's pages; the tensor named ``written`` must
-    be contiguous, as it is written to."""
+    """(seq_lens, block_table, free_pages, free_count, kc_kv_pages) of a cache's pages;
+    ``written`` is the one of the tensors that must be contiguous, as it is written to."""
     import torch
+    if not written.is_contiguous():
+        raise ValueError(f"{op}: {'block_table' if written is block_table else 'free_pages'} must "
+                         "be contiguous")
     seq_lens = _take(op, "seq_lens", seq_lens, torch.int32)
     free_count = _take(op, "free_count", free_count, torch.int32)
-    shaped = {"block_table": block_table, "free_pages": free_pages}
-    if not shaped[written].is_contiguous():
-        raise ValueError(f"{op}: {written} must be contiguous")
     block_table = _take(op, "block_table", block_table, torch.int32)
     free_pages = _take(op, "free_pages", free_pages, torch.int32)
-    table = block_table.shape
+    table, free = block_table.shape, free_pages.shape
     if len(table) != 2 or seq_lens.shape != table[:1]:
         raise ValueError(f"{op}: block_table {tuple(table)} and seq_lens {tuple(seq_lens.shape)} "
                          "must be [requests, pages] and [requests]")
-    if free_pages.dim() != 1 or free_count.shape != (1,):
-        raise ValueError(f"{op}: free_pages {tuple(free_pages.shape)} and free_count "
+    if len(free) != 1 or free_count.shape != (1,):
+        raise ValueError(f"{op}: free_pages {tuple(free)} and free_count "
                          f"{tuple(free_count.shape)} must be [pages] and [1]")
     if page_size <= 0:
         raise ValueError(f"{op}: page_size={page_size} must be positive")
-    # the copies that _take may have made live as long as the structure
-    pages = KvPages(_ptr(block_table), _ptr(free_pages), _ptr(free_count), table[1],
-                    free_pages.shape[0], page_size, table[0])
-    pages.keep = (block_table, free_pages, free_count)
-    return seq_lens, free_count, pages
+    return seq_lens, block_table, free_pages, free_count, KvPages(
+        block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), table[1], free[0],
+        page_size, table[0])
 
 
 def kv_cache_extend(seq_lens, new_lens, block_table, free_pages, free_count, page_size: int,
@@ -1225,25 +1241,26 @@ def kv_cache_extend(seq_lens, new_lens, block_table, free_pages, free_count, pag
     they are but for block_table's new entries (kc_kv_cache_extend)."""
     import torch
     op = "kv_cache_extend"
-    seq_lens, free_count, pages = _kv_pages(op, seq_lens, block_table, free_pages, free_count,
-                                            page_size, "block_table")
+    seq_lens, table, free_pages, free_count, pages = _kv_pages(
+        op, seq_lens, block_table, free_pages, free_count, page_size, block_table)
     new_lens = _take(op, "new_lens", new_lens, torch.int32)
-    B = seq_lens.shape[0]
-    if new_lens.shape != (B,):
-        raise ValueError(f"{op}: new_lens {tuple(new_lens.shape)} must be [{B}]")
+    if new_lens.shape != seq_lens.shape:
+        raise ValueError(f"{op}: new_lens {tuple(new_lens.shape)} must be {tuple(seq_lens.shape)}")
     if not 0 <= total_new < 2 ** 31:
         raise ValueError(f"{op}: total_new={total_new} must be from 0 to 2^31 - 1")
-    gpu = _one_gpu(op, seq_lens, new_lens, block_table, free_pages, free_count)
-    dev = seq_lens.device
+    gpu = _one_gpu(op, seq_lens, new_lens, table, free_pages, free_count)
+    B, dev = pages.seqs, seq_lens.device
     # one allocation for the int32 results
-    parts = torch.empty(3 * B + 3 + total_new, dtype=torch.int32, device=dev).split(
-        (B, 1, B + 1, B + 1, total_new))
+    results = torch.empty(3 * B + 3 + total_new, dtype=torch.int32, device=dev)
+    lens, count, cu_new, cu, positions = results.split_with_sizes((B, 1, B + 1, B + 1, total_new))
     slots = torch.empty(total_new, dtype=torch.int64, device=dev)
+    at = results.data_ptr()
     with kernel_span(op, requests=B, tokens=total_new, page_size=page_size):
-        st = _launch(gpu, _get_lib().kc_kv_cache_extend, ctypes.byref(pages), _ptr(seq_lens),
-                     _ptr(new_lens), total_new, *[_ptr(t) for t in parts], _ptr(slots))
+        st = _launch(gpu, _get_lib().kc_kv_cache_extend, ctypes.byref(pages), seq_lens.data_ptr(),
+                     new_lens.data_ptr(), total_new, at, at + 4 * B, at + 4 * B + 4,
+                     at + 8 * B + 8, at + 12 * B + 12, slots.data_ptr())
     _check(op, st)
-    return (*parts, slots)
+    return lens, count, cu_new, cu, positions, slots
 
 
 def kv_cache_release(finished, seq_lens, block_table, free_pages, free_count,
@@ -1257,16 +1274,15 @@ def kv_cache_release(finished, seq_lens, block_table, free_pages, free_count,
     if finished.dtype not in (torch.bool, torch.uint8):
         raise ValueError(f"{op}: finished has dtype {finished.dtype}; expected torch.bool or torch.uint8")
     finished = finished.contiguous()
-    seq_lens, free_count, pages = _kv_pages(op, seq_lens, block_table, free_pages, free_count,
-                                            page_size, "free_pages")
-    B = seq_lens.shape[0]
-    if finished.shape != (B,):
-        raise ValueError(f"{op}: finished {tuple(finished.shape)} must be [{B}]")
-    gpu = _one_gpu(op, seq_lens, finished, block_table, free_pages, free_count)
-    lens, count = torch.empty(B + 1, dtype=torch.int32, device=seq_lens.device).split((B, 1))
-    with kernel_span(op, requests=B, page_size=page_size):
-        st = _launch(gpu, _get_lib().kc_kv_cache_release, ctypes.byref(pages), _ptr(finished),
-                     _ptr(seq_lens), _ptr(lens), _ptr(count))
+    seq_lens, block_table, free, free_count, pages = _kv_pages(
+        op, seq_lens, block_table, free_pages, free_count, page_size, free_pages)
+    if finished.shape != seq_lens.shape:
+        raise ValueError(f"{op}: finished {tuple(finished.shape)} must be {tuple(seq_lens.shape)}")
+    gpu = _one_gpu(op, seq_lens, finished, block_table, free, free_count)
+    lens, count = torch.empty_like(seq_lens), torch.empty_like(free_count)
+    with kernel_span(op, requests=pages.seqs, page_size=page_size):
+        st = _launch(gpu, _get_lib().kc_kv_cache_release, ctypes.byref(pages), finished.data_ptr(),
+                     seq_lens.data_ptr(), lens.data_ptr(), count.data_ptr())
     _check(op, st)
     return lens, count
 
@@ -1280,49 +1296,72 @@ class Residual(ctypes.Structure):
                 ("alpha", ctypes.c_float), ("eps", ctypes.c_float)]
 
 
-def _residual_args(op: str, y, h, gamma, post_gamma, gate, alpha: float, eps: float):
-    """(gpu, suffix of the entry point, kc_residual) of validated arguments; rows with values one
+def _residual(op: str, y, h, gamma, post_gamma, gate, alpha: float, eps: float, fp8: bool) -> Tuple:
+    """residual_rmsnorm, and with ``fp8`` residual_rmsnorm_fp8_quantize.  Rows with values one
     after the other are read in place, anything else is copied."""
     import torch
-    if y.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{op}: y has dtype {y.dtype}; expected torch.bfloat16 or torch.float32")
-    if h.dtype is not y.dtype and h.dtype is not torch.float32:
-        raise ValueError(f"{op}: h has dtype {h.dtype}; expected {y.dtype} or torch.float32")
-    if y.dim() != 2 or h.shape != y.shape:
-        raise ValueError(f"{op}: y {tuple(y.shape)} and h {tuple(h.shape)} must both be [rows, cols]")
-    T, D = y.shape
-    gamma = _take(op, "gamma", gamma, y.dtype)
-    given = [y, h, gamma]
+    ydt, hdt, shape = y.dtype, h.dtype, y.shape
+    bf16 = ydt is torch.bfloat16
+    if not bf16 and ydt is not torch.float32:
+        raise ValueError(f"{op}: y has dtype {ydt}; expected torch.bfloat16 or torch.float32")
+    if hdt is not ydt and hdt is not torch.float32:
+        raise ValueError(f"{op}: h has dtype {hdt}; expected {ydt} or torch.float32")
+    if len(shape) != 2 or h.shape != shape:
+        raise ValueError(f"{op}: y {tuple(shape)} and h {tuple(h.shape)} must both be [rows, cols]")
+    T, D = shape
+    gamma = _take(op, "gamma", gamma, ydt)
+    width = shape[1:]
+    if gamma.shape != width:
+        raise ValueError(f"{op}: gamma {tuple(gamma.shape)} must be [{D}]")
+    given, post, gated, gate_stride = [y, h, gamma], None, None, 0
     if post_gamma is not None:
-        post_gamma = _take(op, "post_gamma", post_gamma, y.dtype)
+        post_gamma = _take(op, "post_gamma", post_gamma, ydt)
+        if post_gamma.shape != width:
+            raise ValueError(f"{op}: post_gamma {tuple(post_gamma.shape)} must be [{D}]")
         given.append(post_gamma)
-    if gamma.shape != (D,) or (post_gamma is not None and post_gamma.shape != (D,)):
-        raise ValueError(f"{op}: gamma and post_gamma must be [{D}]")
-
-    def rows(t):
-        return t if t.stride(1) == 1 or D <= 1 else t.contiguous()
-
-    y, h = rows(y), rows(h)
-    gate_stride = 0
+        post = post_gamma.data_ptr()
+    if D > 1:
+        if y.stride(1) != 1:
+            y = y.contiguous()
+        if h.stride(1) != 1:
+            h = h.contiguous()
     if gate is not None:
-        if gate.dtype is not y.dtype:
-            raise ValueError(f"{op}: gate has dtype {gate.dtype}; expected {y.dtype}")
-        if gate.shape == (D,):
+        if gate.dtype is not ydt:
+            raise ValueError(f"{op}: gate has dtype {gate.dtype}; expected {ydt}")
+        if gate.shape == width:
             gate = gate.contiguous()
-        elif gate.shape == (T, D):
-            gate = rows(gate)
+        elif gate.shape == shape:
+            if D > 1 and gate.stride(1) != 1:
+                gate = gate.contiguous()
             gate_stride = gate.stride(0)
         else:
             raise ValueError(f"{op}: gate {tuple(gate.shape)} must be [{D}] or [{T}, {D}]")
         given.append(gate)
+        gated = gate.data_ptr()
     gpu = _one_gpu(op, *given)
-    args = Residual(_ptr(y), _ptr(h), None if gate is None else _ptr(gate),
-                    None if post_gamma is None else _ptr(post_gamma), _ptr(gamma), y.stride(0),
+    args = Residual(y.data_ptr(), h.data_ptr(), gated, post, gamma.data_ptr(), y.stride(0),
                     h.stride(0), gate_stride, T, D, alpha, eps)
-    # the copies made above live as long as the structure
-    args.keep = (y, h, gate, post_gamma, gamma)
-    suffix = "f32" if y.dtype == torch.float32 else "bf16" if h.dtype == y.dtype else "bf16_f32"
-    return gpu, suffix, args
+    dev = y.device
+    h_new = torch.empty(shape, dtype=hdt, device=dev)
+    lib = _get_lib()
+    mixed = hdt is not ydt
+    if fp8:
+        n = torch.empty(shape, dtype=torch.int8, device=dev)
+        # scale 1 for empty rows (absmax 0), which the library does not write
+        scales = (torch.empty if D else torch.ones)(T, dtype=torch.float32, device=dev)
+        fn = (lib.kc_residual_rmsnorm_quantize_fp8_bf16_f32 if mixed else
+              lib.kc_residual_rmsnorm_quantize_fp8_bf16 if bf16 else
+              lib.kc_residual_rmsnorm_quantize_fp8_f32)
+        out = (h_new.data_ptr(), n.data_ptr(), scales.data_ptr())
+    else:
+        n = torch.empty(shape, dtype=ydt, device=dev)
+        fn = (lib.kc_residual_rmsnorm_bf16_f32 if mixed else
+              lib.kc_residual_rmsnorm_bf16 if bf16 else lib.kc_residual_rmsnorm_f32)
+        out = (h_new.data_ptr(), n.data_ptr())
+    with kernel_span(op, rows=T, cols=D):
+        st = _launch(gpu, fn, ctypes.byref(args), *out)
+    _check(op, st)
+    return (h_new, n, scales) if fp8 else (h_new, n)
 
 
 def residual_rmsnorm(y, h, gamma, post_gamma=None, gate=None, alpha: float = 1.0,
@@ -1333,16 +1372,7 @@ def residual_rmsnorm(y, h, gamma, post_gamma=None, gate=None, alpha: float = 1.0
     n = rmsnorm(h_new) * gamma.  gate is None (1), [cols] or [rows, cols].  Returns (h_new, n),
     h_new of h's type and n of y's; fp32 arithmetic, each rounded once, n from the h_new that is
     not rounded yet (kc_residual_rmsnorm_*)."""
-    import torch
-    op = "residual_rmsnorm"
-    gpu, suffix, args = _residual_args(op, y, h, gamma, post_gamma, gate, alpha, eps)
-    h_new = torch.empty(args.rows, args.cols, dtype=h.dtype, device=h.device)
-    n = torch.empty(args.rows, args.cols, dtype=y.dtype, device=h.device)
-    with kernel_span(op, rows=args.rows, d=args.cols):
-        st = _launch(gpu, getattr(_get_lib(), "kc_residual_rmsnorm_" + suffix), ctypes.byref(args),
-                     _ptr(h_new), _ptr(n))
-    _check(op, st)
-    return h_new, n
+    return _residual("residual_rmsnorm", y, h, gamma, post_gamma, gate, alpha, eps, False)
 
 
 def residual_rmsnorm_fp8_quantize(y, h, gamma, post_gamma=None, gate=None, alpha: float = 1.0,
@@ -1350,18 +1380,7 @@ def residual_rmsnorm_fp8_quantize(y, h, gamma, post_gamma=None, gate=None, alpha
     """residual_rmsnorm with n quantized per token in the same pass, from fp32 as
     fp8_quantize_rows does: (h_new, int8 codes [rows, cols], fp32 scales [rows]), what
     fp8_gemm_w8a8 takes (kc_residual_rmsnorm_quantize_fp8_*)."""
-    import torch
-    op = "residual_rmsnorm_fp8_quantize"
-    gpu, suffix, args = _residual_args(op, y, h, gamma, post_gamma, gate, alpha, eps)
-    h_new = torch.empty(args.rows, args.cols, dtype=h.dtype, device=h.device)
-    codes = torch.empty(args.rows, args.cols, dtype=torch.int8, device=h.device)
-    # scale 1 for empty rows (absmax 0), which the library does not write
-    scales = (torch.empty if args.cols else torch.ones)(args.rows, dtype=torch.float32, device=h.device)
-    with kernel_span(op, rows=args.rows, cols=args.cols):
-        st = _launch(gpu, getattr(_get_lib(), "kc_residual_rmsnorm_quantize_fp8_" + suffix),
-                     ctypes.byref(args), _ptr(h_new), _ptr(codes), _ptr(scales))
-    _check(op, st)
-    return h_new, codes, scales
+    return _residual("residual_rmsnorm_fp8_quantize", y, h, gamma, post_gamma, gate, alpha, eps, True)
 
 
 # ---------------------------------------------------------------------------

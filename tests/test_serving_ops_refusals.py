@@ -151,9 +151,9 @@ def _res(**kw):
     (lambda L: _call(L, table=None), "null"),
     (lambda L: _call(L, lens=None), "null"),
     (lambda L: _call(L, out=None), "null"),
-    (lambda L: _call(L, size=100), "workspace"),
-    (lambda L: _call(L, work=None), "workspace"),
-    (lambda L: _call(L, work=ODD), "workspace"),
+    (lambda L: _call(L, pages=200, size=100), "workspace"),
+    (lambda L: _call(L, pages=200, work=None), "workspace"),
+    (lambda L: _call(L, pages=200, work=ODD), "workspace"),
     (lambda L: L.kc_kv_cache_attention_f32(P, 512, 8, None, P, 20, P, 3, 1.0, 0, P, 1 << 40, P, None), "null"),
     (lambda L: L.kc_kv_cache_extend(None, P, P, 3, P, P, P, P, P, P, None), "null"),
     (lambda L: L.kc_kv_cache_extend(_pages(page_size=0), P, P, 3, P, P, P, P, P, P, None), "shape"),
@@ -203,4 +203,5 @@ def test_workspace_of_refused_calls():
     L = kc_abi.lib()
     assert L.kc_kv_cache_attention_workspace(_cache(), 20, 3, 7) == -1 and L.kc_get_last_error() == 1
     assert L.kc_kv_cache_attention_workspace(_cache(), 20, 0, 8) == 0
-    assert L.kc_kv_cache_attention_workspace(_cache(), 20, 3, 8) > 0
+    assert L.kc_kv_cache_attention_workspace(_cache(), 20, 3, 8) == 0  # short tables are not split
+    assert L.kc_kv_cache_attention_workspace(_cache(), 200, 3, 8) > 0
