@@ -1,5 +1,5 @@
 // kv_attention.hpp -- how attention of one token per sequence over the quantized cache is
-// split: shared by its kernels (kv_cache_attention.hip, kv_cache_attention_mfma.hip).
+// split: shared by its kernels (kv_cache_attention.hip, kv_attention_mfma.hpp).
 //
 // The visible positions of a sequence are cut into tiles of 32 (at multiples of 32), the
 // tiles of all sequences stand in one row, and `units` waves for each set of query heads
@@ -188,9 +188,11 @@ __device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& 
     return r;
 }
 
-// The matrix-core kernel (kv_cache_attention_mfma.hip): sets of 8 query heads in bf16, 4 in fp32.
-bool mfma_takes(const kc_kv_cache& cache, int64_t max_pages);
-void launch_mfma(const Attention& p, bool bf16, bool fp8, dim3 grid, hipStream_t stream);
+constexpr int kMaxMfmaD = 256;
+
+// The matrix-core kernel (kv_attention_mfma.hpp): sets of 8 query heads in bf16, 4 in fp32.
+void launch_mfma_bf16(const Attention& p, bool fp8, dim3 grid, hipStream_t stream);
+void launch_mfma_f32(const Attention& p, bool fp8, dim3 grid, hipStream_t stream);
 
 }  // namespace kv
 }  // namespace kc

@@ -1,5 +1,6 @@
-// kv_cache_attention_mfma.hip -- attention of each sequence's newest token over the
-// quantized paged cache on gfx950's matrix cores, for head_dims of whole 16-byte rows.
+// kv_attention_mfma.hpp -- attention of each sequence's newest token over the
+// quantized paged cache on gfx950's matrix cores, for head_dims up to 256 whose rows of codes
+// are whole 16 bytes.
 //
 // A wave takes a set of query heads of one key/value head and a stretch of tiles of 32
 // positions (kv_attention.hpp).  Keys and values are turned from codes into bf16, which
@@ -16,6 +17,8 @@
 // as the sum of two bf16 values (2^-17), one in each piece.  fp32 queries: 4 heads, queries
 // and weights as sums of three bf16 values (2^-25).  The pieces cost no product more, since
 // groups of up to 8 (4) query heads leave those columns empty.
+#pragma once
+
 #include <type_traits>
 
 #include "kv_attention.hpp"
@@ -577,49 +580,18 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
     }
 }
 
-template <bool BF16, bool FP8>
+template <bool BF16, bool FP8, int D>
 void launch(const Attention& p, dim3 grid, hipStream_t stream) {
-    const int waves = p.wg_sets * p.streams;
-    const unsigned lds = p.units == 0 ? waves * (BF16 ? 8 : 4) * (p.D + 4) * 4 : 0;
-    switch (p.D) {
-        case 64: attention_mfma_kernel<BF16, FP8, 64><<<grid, waves * kWave, lds, stream>>>(p); return;
-        case 96: attention_mfma_kernel<BF16, FP8, 96><<<grid, waves * kWave, lds, stream>>>(p); return;
-        case 128: attention_mfma_kernel<BF16, FP8, 128><<<grid, waves * kWave, lds, stream>>>(p); return;
-        case 192: attention_mfma_kernel<BF16, FP8, 192><<<grid, waves * kWave, lds, stream>>>(p); return;
-        case 256: attention_mfma_kernel<BF16, FP8, 256><<<grid, waves * kWave, lds, stream>>>(p); return;
-        default: break;
-    }
-    if constexpr (FP8) {
-        switch (p.D) {
-            case 80: attention_mfma_kernel<BF16, FP8, 80><<<grid, waves * kWave, lds, stream>>>(p); return;
-            case 112: attention_mfma_kernel<BF16, FP8, 112><<<grid, waves * kWave, lds, stream>>>(p); return;
-            default: break;
-        }
+    constexpr int kStep = FP8 ? 16 : 32;
+    if constexpr (D > kMaxMfmaD) {
+        return;
+    } else if (p.D != D) {
+        launch<BF16, FP8, D + kStep>(p, grid, stream);
+    } else {
+        const int waves = p.wg_sets * p.streams;
+        const unsigned lds = p.units == 0 ? waves * (BF16 ? 8 : 4) * (D + 4) * 4 : 0;
+        attention_mfma_kernel<BF16, FP8, D><<<grid, waves * kWave, lds, stream>>>(p);
     }
 }
 
 }  // namespace
-
-namespace kc {
-namespace kv {
-
-bool mfma_takes(const kc_kv_cache& c, int64_t max_pages) {
-    const bool fp8 = c.format == KC_KV_FP8;
-    const int blocks = c.head_dim / 32;
-    // rows of codes in whole 16 bytes, scales in the units that they are loaded in
-    const uintptr_t unit = fp8 ? 4 : blocks % 4 == 0 ? 4 : blocks % 2 == 0 ? 2 : 1;
-    const bool size = c.head_dim == 64 || c.head_dim == 96 || c.head_dim == 128 || c.head_dim == 192 ||
-                      c.head_dim == 256 || (fp8 && (c.head_dim == 80 || c.head_dim == 112));
-    return size && c.num_pages > 0 && max_pages > 0 && aligned(c.k_codes, 16) && aligned(c.v_codes, 16) && aligned(c.k_scales, unit) &&
-           aligned(c.v_scales, unit) &&
-           // rows are found by 32 bits of 16 bytes
-           c.num_pages * c.page_size * (fp8 ? c.head_dim : c.head_dim / 2) / 16 * c.kv_heads <= UINT32_MAX;
-}
-
-void launch_mfma(const Attention& p, bool bf16, bool fp8, dim3 grid, hipStream_t stream) {
-    if (bf16) return fp8 ? launch<true, true>(p, grid, stream) : launch<true, false>(p, grid, stream);
-    return fp8 ? launch<false, true>(p, grid, stream) : launch<false, false>(p, grid, stream);
-}
-
-}  // namespace kv
-}  // namespace kc

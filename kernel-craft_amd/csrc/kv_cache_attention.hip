@@ -240,6 +240,19 @@ __global__ __launch_bounds__(1024) void join_kernel(const Attention p, int split
     }
 }
 
+// Whether the matrix-core kernel takes this cache.
+bool mfma_takes(const kc_kv_cache& c, int64_t max_pages) {
+    const bool fp8 = c.format == KC_KV_FP8;
+    const int blocks = c.head_dim / 32, row = fp8 ? c.head_dim : c.head_dim / 2;
+    // rows of codes in whole 16 bytes, scales in the units that they are loaded in
+    const uintptr_t unit = fp8 ? 4 : blocks % 4 == 0 ? 4 : blocks % 2 == 0 ? 2 : 1;
+    return row % 16 == 0 && c.head_dim <= kMaxMfmaD && c.num_pages > 0 && max_pages > 0 &&
+           kc::aligned(c.k_codes, 16) && kc::aligned(c.v_codes, 16) && kc::aligned(c.k_scales, unit) &&
+           kc::aligned(c.v_scales, unit) &&
+           // rows are found by 32 bits of 16 bytes
+           c.num_pages * c.page_size * (row / 16) * c.kv_heads <= UINT32_MAX;
+}
+
 struct Plan {
     int sets, units, wg_sets, streams;
     dim3 grid;
@@ -368,7 +381,7 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     char* parts = static_cast<char*>(workspace) + round16(starts_bytes(seqs));
     p.part_ml = reinterpret_cast<float*>(parts);
     p.part_o = reinterpret_cast<float*>(parts + round16((int64_t{plan.units} + seqs) * q_heads * 8));
-    if (mfma_takes(*cache, max_pages)) launch_mfma(p, BF16, fp8, plan.grid, stream);
+    if (mfma_takes(*cache, max_pages)) (BF16 ? launch_mfma_bf16 : launch_mfma_f32)(p, fp8, plan.grid, stream);
     else if (fp8) launch_vector<BF16, true>(p, plan.grid, stream);
     else launch_vector<BF16, false>(p, plan.grid, stream);
     const int launched = kc::check_launch(fn);

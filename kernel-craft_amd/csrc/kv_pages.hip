@@ -11,7 +11,8 @@
 //
 // Bound by latency: a few bytes per request and 12 per token.  One launch: every
 // workgroup scans all requests by itself (three block scans, 8 bytes a request from the
-// cache), so that none waits for another, and takes 1024 rows of the batch.
+// cache), so that none waits for another, and takes as many rows of the batch as it has
+// threads.
 #include <algorithm>
 
 #include "kc_common.hpp"
@@ -20,9 +21,9 @@ namespace {
 
 using kc::kWave;
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
-constexpr int64_t kMaxGrid = (1 << 22) - 1;  // workgroups of 1024: a launch holds fewer than 2^32 threads
+// Threads of a workgroup: 256 where that is one request each, else 1024 (a scan over 16
+// waves and 1024 LDS entries: 256 requests 5.2 us, 6.5 with 1024 threads).
+constexpr int kFew = 256, kMany = 1024;
 
 struct Pages {
     int32_t* table;
@@ -34,7 +35,8 @@ struct Pages {
     const int32_t* lens;
 };
 
-// Sum of v over the threads before this one; `total` over all.  `part` is LDS of kWaves.
+// Sum of v over the threads before this one; `total` over all.  `part` is LDS of a sum per wave.
+template <int kThreads>
 __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t& total) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     int64_t up = v;
@@ -49,7 +51,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t&
     int64_t before = 0;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kThreads / kWave; ++w) {
         if (w < wave) before += part[w];
         total += part[w];
     }
@@ -57,6 +59,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* part, int64_t&
 }
 
 // The last thread whose first item is at most `at` (starts ascend from 0).
+template <int kThreads>
 __device__ __forceinline__ int last_at_most(const int64_t* starts, int64_t at) {
     int lo = 0;
 #pragma unroll
@@ -92,10 +95,11 @@ __device__ __forceinline__ Request request(const Pages& p, const int32_t* fresh,
     return r;
 }
 
+template <int kThreads>
 __global__ __launch_bounds__(kThreads) void extend_kernel(const Pages p, const int32_t* __restrict__ fresh,
                                                           int64_t rows, int32_t* cu_new, int32_t* cu_after,
                                                           int32_t* positions, int64_t* slots) {
-    __shared__ int64_t part[kWaves], first_row[kThreads], first_ask[kThreads];
+    __shared__ int64_t part[kThreads / kWave], first_row[kThreads], first_ask[kThreads];
     __shared__ unsigned long long used;
     const int tid = threadIdx.x, each = (p.seqs + kThreads - 1) / kThreads;
     const int b0 = min(tid * each, p.seqs), b1 = min(b0 + each, p.seqs);
@@ -104,14 +108,14 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(const Pages p, const i
 
     int64_t sum = 0, total_rows, total;
     for (int b = b0; b < b1; ++b) sum += max(fresh[b], 0);
-    const int64_t row0 = block_scan(sum, part, total_rows);
+    const int64_t row0 = block_scan<kThreads>(sum, part, total_rows);
     sum = 0;
     for (int64_t b = b0, at = row0; b < b1; ++b) {
         const Request r = request(p, fresh, rows, b, at);
         at += r.fresh;
         sum += r.ask;
     }
-    const int64_t ask0 = block_scan(sum, part, total);
+    const int64_t ask0 = block_scan<kThreads>(sum, part, total);
     first_row[tid] = row0;
     first_ask[tid] = ask0;
     if (blockIdx.x == 0) {  // what there is one of for each request
@@ -131,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(const Pages p, const i
             after += len;
             most = max(most, upto);
         });
-        int64_t cu = block_scan(after, part, total);
+        int64_t cu = block_scan<kThreads>(after, part, total);
         if (most > 0) atomicMax(&used, static_cast<unsigned long long>(most));
         walk([&](int b, int64_t at, int64_t len, int64_t) {
             p.lens_out[b] = static_cast<int32_t>(len);
@@ -152,7 +156,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(const Pages p, const i
     int32_t pos = -1;
     int64_t slot = -1;
     if (row < total_rows) {
-        const int t = last_at_most(first_row, row);
+        const int t = last_at_most<kThreads>(first_row, row);
         int64_t at = first_row[t], ask = first_ask[t];
         int b = t * each;
         Request r = request(p, fresh, rows, b, at);
@@ -180,8 +184,9 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(const Pages p, const i
     slots[row] = slot;
 }
 
+template <int kThreads>
 __global__ __launch_bounds__(kThreads) void release_kernel(const Pages p, const uint8_t* __restrict__ finished) {
-    __shared__ int64_t part[kWaves], first[kThreads];
+    __shared__ int64_t part[kThreads / kWave], first[kThreads];
     const int tid = threadIdx.x, each = (p.seqs + kThreads - 1) / kThreads;
     const int b0 = min(tid * each, p.seqs), b1 = min(b0 + each, p.seqs);
     const int64_t free = min(static_cast<int64_t>(max(p.count[0], 0)), p.capacity);
@@ -190,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void release_kernel(const Pages p, const 
     };
     int64_t sum = 0, total;
     for (int b = b0; b < b1; ++b) sum += pages(b);
-    first[tid] = block_scan(sum, part, total);
+    first[tid] = block_scan<kThreads>(sum, part, total);
     const int64_t back = min(total, p.capacity - free);
     if (blockIdx.x == 0) {
         for (int b = b0; b < b1; ++b) p.lens_out[b] = finished[b] ? 0 : max(p.lens[b], 0);
@@ -199,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void release_kernel(const Pages p, const 
     __syncthreads();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < back;
          i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int t = last_at_most(first, i);
+        const int t = last_at_most<kThreads>(first, i);
         int64_t at = first[t];
         int b = t * each;
         for (int64_t n = pages(b); i >= at + n; n = pages(++b)) at += n;
@@ -243,9 +248,16 @@ extern "C" int kc_kv_cache_extend(const kc_kv_pages* pages, const int32_t* d_seq
     if (!d_cu_new || !d_cu_seqlens || (pages->seqs > 0 && !d_new_lens) ||
         (total_new > 0 && (!d_positions || !d_slots)))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
-    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, (total_new + kThreads - 1) / kThreads));
-    extend_kernel<<<grid, kThreads, 0, stream>>>(args(pages, d_seq_lens, d_seq_lens_out, d_free_count_out), d_new_lens,
-                                                 total_new, d_cu_new, d_cu_seqlens, d_positions, d_slots);
+    const Pages p = args(pages, d_seq_lens, d_seq_lens_out, d_free_count_out);
+    const bool few = pages->seqs <= kFew;
+    const int threads = few ? kFew : kMany;
+    const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, (total_new + threads - 1) / threads));
+    if (few)
+        extend_kernel<kFew><<<grid, kFew, 0, stream>>>(p, d_new_lens, total_new, d_cu_new, d_cu_seqlens, d_positions,
+                                                       d_slots);
+    else
+        extend_kernel<kMany><<<grid, kMany, 0, stream>>>(p, d_new_lens, total_new, d_cu_new, d_cu_seqlens, d_positions,
+                                                         d_slots);
     return kc::check_launch(fn);
 }
 
@@ -256,11 +268,13 @@ extern "C" int kc_kv_cache_release(const kc_kv_pages* pages, const uint8_t* d_fi
     if (st != KC_SUCCESS) return st;
     if (pages->seqs > 0 && !d_finished)
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null device pointer", fn);
-    // One workgroup per 1024 entries of the block table, as far as 256 take all
-    // that there is at once.
+    const Pages p = args(pages, d_seq_lens, d_seq_lens_out, d_free_count_out);
+    const bool few = pages->seqs <= kFew;
+    const int threads = few ? kFew : kMany;
+    // A thread for each entry of the block table, as far as 256 workgroups go.
     const int64_t most = std::min<int64_t>(pages->seqs * pages->max_pages, pages->num_pages);
-    const unsigned grid = static_cast<unsigned>(std::clamp<int64_t>((most + kThreads - 1) / kThreads, 1, 256));
-    release_kernel<<<grid, kThreads, 0, stream>>>(args(pages, d_seq_lens, d_seq_lens_out, d_free_count_out),
-                                                  d_finished);
+    const unsigned grid = static_cast<unsigned>(std::clamp<int64_t>((most + threads - 1) / threads, 1, 256));
+    if (few) release_kernel<kFew><<<grid, kFew, 0, stream>>>(p, d_finished);
+    else release_kernel<kMany><<<grid, kMany, 0, stream>>>(p, d_finished);
     return kc::check_launch(fn);
 }

@@ -83,6 +83,8 @@ SHAPES = [  # q heads, kv heads, D, page, format
     (5, 1, 80, 16, "fp8"), (28, 4, 96, 5, "fp8"), (12, 3, 256, 16, "fp8"), (4, 1, 256, 33, "mxfp4"),
     (6, 3, 33, 16, "fp8"), (2, 2, 1, 3, "fp8"), (4, 2, 32, 16, "mxfp4"), (3, 1, 192, 16, "fp8"), (6, 1, 192, 8, "mxfp4"),
     (2, 1, 576, 16, "fp8"), (2, 1, 1024, 16, "mxfp4"), (9, 9, 16, 4, "fp8"), (66, 11, 64, 16, "fp8"), (10, 5, 112, 16, "fp8"),
+    (4, 2, 48, 16, "fp8"), (4, 1, 144, 3, "fp8"), (8, 2, 160, 16, "fp8"), (8, 2, 160, 16, "mxfp4"), (2, 1, 176, 16, "fp8"),
+    (2, 1, 208, 16, "fp8"), (2, 1, 224, 64, "fp8"), (5, 1, 224, 16, "mxfp4"), (3, 1, 240, 16, "fp8"),
     (72, 72, 64, 16, "fp8"), (64, 1, 128, 16, "fp8"), (1, 1, 1000, 16, "fp8"),
 ]
 

@@ -49,7 +49,7 @@ def _extend(torch, ops, lens, new, table, stack, count, page, rows):
 EXTENDS = [  # requests, longest, new, page, width to spare, share of the pages that there are, rows to spare
     (1, 0, 1, 16, 0, 1.0, 0), (1, 16, 1, 16, 0, 1.0, 0), (1, 700, 1, 16, 3, 0.0, 0), (64, 500, 1, 16, 2, 1.0, 0),
     (64, 500, 1, 16, 2, 0.5, 0), (9, 100, 60, 7, 1, 1.0, 5), (9, 100, 60, 7, 1, 0.6, 0), (33, 40, 90, 1, 0, 0.7, 3),
-    (1000, 300, 1, 32, 1, 0.9, 0), (1024, 60, 3, 16, 1, 1.0, 1), (1025, 60, 3, 16, 1, 0.5, 0),
+    (256, 300, 1, 16, 1, 0.8, 0), (257, 30, 4, 16, 1, 1.0, 2), (1000, 300, 1, 32, 1, 0.9, 0), (1024, 60, 3, 16, 1, 1.0, 1), (1025, 60, 3, 16, 1, 0.5, 0),
     (3000, 50, 2, 8, 1, 0.8, 700), (5, 9000, 3000, 64, 2, 1.0, 0), (2, 1, 5000, 3, 0, 1.0, 0),
 ]
 
@@ -96,7 +96,7 @@ def test_extend_keeps_pages_that_were_marked_missing(gpu, ops):
     assert got[4].tolist() == [5, 6, 7, 20, 21, 22] and got[5].tolist() == [-1] * 6
 
 
-RELEASES = [(1, 0, 16), (1, 100, 16), (64, 500, 16), (64, 33, 1), (1000, 300, 32), (1025, 90, 7), (3000, 40, 8), (3, 40000, 2)]
+RELEASES = [(256, 70, 16), (257, 70, 16), (1, 0, 16), (1, 100, 16), (64, 500, 16), (64, 33, 1), (1000, 300, 32), (1025, 90, 7), (3000, 40, 8), (3, 40000, 2)]
 
 
 @pytest.mark.parametrize("B,ctx,page", RELEASES)
