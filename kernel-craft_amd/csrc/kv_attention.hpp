@@ -6,8 +6,8 @@
 // take equal stretches of that row, whatever the lengths are: no wave waits for a longest
 // sequence, and the host need not know the lengths.  A stretch that holds all tiles of a
 // sequence writes its output; the others write sums and their maximum to the workspace
-// (segment number: unit + sequence, which no two segments share), and a second launch
-// joins them:  m = max m_i,  l = sum l_i 2^(m_i - m),  o = sum o_i 2^(m_i - m) / l.
+// (segment 2 unit where it begins with the stretch, 2 unit + 1 where it ends with it: a
+// stretch cuts two sequences at most), and a second launch joins them:  m = max m_i,  l = sum l_i 2^(m_i - m),  o = sum o_i 2^(m_i - m) / l.
 // Scores are kept times log2(e).  A part without a finite score has m = -inf, l = 0, o = 0.
 //
 // Where the block table has few tiles a row, a workgroup takes whole sequences instead, its
@@ -40,8 +40,8 @@ struct Attention {
     int sets;          // of query heads that share a key/value head and a wave
     int wg_sets, streams;  // sets of a workgroup, and its waves for each of them
     int* starts;       // workspace: first tile of each sequence, their number, tiles per stretch
-    float* part_o;     // [units + seqs][q_heads][D]
-    float* part_ml;    // [units + seqs][q_heads][2]
+    float* part_o;     // [2 units][q_heads][D]
+    float* part_ml;    // [2 units][q_heads][2]
 };
 
 __device__ __forceinline__ int tile_of(int pos) { return static_cast<uint32_t>(pos) / kTile; }
@@ -164,7 +164,7 @@ __device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& 
         const int t = (at * p.streams + i) * per;
         if (t < before || t >= before + mine) continue;
         int to = before, b = b0;
-        for (int n = n0; t >= to + n; n = visible(p, ++b).tiles()) to += n;
+        for (int n = n0; t >= to + n && b + 1 < b1; n = visible(p, ++b).tiles()) to += n;
         s.b[i] = b;
         s.first[i] = to;
     }

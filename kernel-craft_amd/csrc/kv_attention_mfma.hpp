@@ -211,7 +211,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
     int shift = tile_of(vis.first) - s.first;
     auto find = [&](int tile) {
         if (tile >= s.end) return Place{-1, kTile, 1, 1};
-        while (tile >= seq_end) {  // tile < s.end ends it
+        while (tile >= seq_end && seq + 1 < p.seqs) {  // tile < s.end ends it
             vis = visible_scalar(p, ++seq);
             shift = tile_of(vis.first) - seq_end;
             seq_end += vis.tiles();
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                 l += __shfl_xor(l, 16, kWave);
                 l += __shfl_xor(l, 32, kWave);
                 const bool whole = from == tile_of(here.first) * kTile && here.base == tile_of(here.end - 1) * kTile;
-                const int64_t row = (static_cast<int64_t>(s.unit) + here.b) * p.q_heads + head0 + qi;
+                const int64_t row = (int64_t{2} * s.unit + (here.b == s.b ? 0 : 1)) * p.q_heads + head0 + qi;
                 const float by = p.units != 0 && whole ? 1.0f / l : 1.0f;
                 each<VC::pieces()>([&](auto piece) {
                     constexpr int kP = piece, kValues = (FP8 ? 1 : 2) * VC::lane_bytes(kP);

@@ -54,6 +54,7 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
     const int heads = min(kHeads, p.group - q0);
     const int64_t head0 = static_cast<int64_t>(h) * p.group + q0;
     const float nan = __uint_as_float(0x7FC00000u), inf = __uint_as_float(0x7F800000u);
+    int64_t segment = static_cast<int64_t>(s.unit) * 2 * p.q_heads + head0;
 
     for (int b = s.b; b < p.seqs; ++b) {
         const Visible vis = visible(p, b);
@@ -125,7 +126,6 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
             __syncthreads();
         }
         const bool whole = s.tile == s.first && end == s.first + tiles;
-        const int64_t segment = (static_cast<int64_t>(s.unit) + b) * p.q_heads + head0;
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
             if (j >= heads) break;
@@ -141,6 +141,7 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
                 p.part_ml[(segment + j) * 2 + 1] = l[j];
             }
         }
+        if (b == s.b) segment += p.q_heads;  // what follows begins behind the stretch's first tile
         s.first += tiles;
         s.tile = end;
         if (p.units == 0 || end == s.end) return;
@@ -183,7 +184,6 @@ __global__ __launch_bounds__(1024) void join_kernel(const Attention p, int split
     }
     const int unit = tile / per, n = (end - 1) / per - unit + 1;
     if (n == 1) return;  // the same for the whole workgroup
-    const int64_t first = static_cast<int64_t>(unit + b) * p.q_heads + head;
     int row_lanes = kWave;
     while (row_lanes / 2 * W >= p.D) row_lanes /= 2;
     const int groups = kWave / row_lanes, group = lane / row_lanes, at = lane - group * row_lanes;
@@ -196,7 +196,8 @@ __global__ __launch_bounds__(1024) void join_kernel(const Attention p, int split
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {  // behind the last segment: that one again, without weight
                     const int seg = i0 + i * split * groups;
-                    const int64_t row = first + static_cast<int64_t>(min(seg, n - 1)) * p.q_heads;
+                    const int slot = 2 * (unit + min(seg, n - 1)) + (min(seg, n - 1) == 0 && tile % per != 0);
+                    const int64_t row = static_cast<int64_t>(slot) * p.q_heads + head;
                     sm[i] = p.part_ml[row * 2];
                     sl[i] = p.part_ml[row * 2 + 1];
                     __builtin_memcpy(so[i], __builtin_assume_aligned(p.part_o + row * p.D + from, 4 * W), 4 * W);
@@ -304,7 +305,7 @@ int64_t starts_bytes(int seqs) { return (int64_t{seqs} + 2) * 4; }
 int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 int64_t workspace_bytes(const Plan& p, int seqs, int q_heads, int D) {
-    const int64_t rows = (int64_t{p.units} + seqs) * q_heads;
+    const int64_t rows = int64_t{p.units} * 2 * q_heads;
     return p.units == 0 ? 0 : round16(starts_bytes(seqs)) + round16(rows * 8) + rows * D * 4;
 }
 
@@ -380,7 +381,7 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     p.starts = static_cast<int*>(workspace);
     char* parts = static_cast<char*>(workspace) + round16(starts_bytes(seqs));
     p.part_ml = reinterpret_cast<float*>(parts);
-    p.part_o = reinterpret_cast<float*>(parts + round16((int64_t{plan.units} + seqs) * q_heads * 8));
+    p.part_o = reinterpret_cast<float*>(parts + round16(int64_t{plan.units} * 2 * q_heads * 8));
     if (mfma_takes(*cache, max_pages)) (BF16 ? launch_mfma_bf16 : launch_mfma_f32)(p, fp8, plan.grid, stream);
     else if (fp8) launch_vector<BF16, true>(p, plan.grid, stream);
     else launch_vector<BF16, false>(p, plan.grid, stream);

@@ -1182,12 +1182,14 @@ def kv_cache_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq
     if need < 0:
         _check(op)
     out = torch.empty_like(q) if whole else torch.empty(shape, dtype=dtype, device=q.device)
-    work = torch.empty(need, dtype=torch.uint8, device=q.device).data_ptr() if need else None
+    # held until the launch: freed before, another thread's tensor could have its memory
+    work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     fn = lib.kc_kv_cache_attention_bf16 if bf16 else lib.kc_kv_cache_attention_f32
     with kernel_span(op, sequences=B, heads=Hq, kv_heads=Hkv, head_dim=D):
         st = _launch(gpu, fn, q.data_ptr(), q.stride(0), Hq, ref, block_table.data_ptr(), table[1],
                      seq_lens.data_ptr(), B, D ** -0.5 if scale is None else scale,
-                     min(window, 2 ** 31 - 1), work, need, out.data_ptr())
+                     min(window, 2 ** 31 - 1), None if work is None else work.data_ptr(), need,
+                     out.data_ptr())
     _check(op, st)
     return out
 
@@ -1342,7 +1344,7 @@ def _residual(op: str, y, h, gamma, post_gamma, gate, alpha: float, eps: float, 
     args = Residual(y.data_ptr(), h.data_ptr(), gated, post, gamma.data_ptr(), y.stride(0),
                     h.stride(0), gate_stride, T, D, alpha, eps)
     dev = y.device
-    h_new = torch.empty(shape, dtype=hdt, device=dev)
+    h_new = torch.empty_like(h) if h.is_contiguous() else torch.empty(shape, dtype=hdt, device=dev)
     lib = _get_lib()
     mixed = hdt is not ydt
     if fp8:
