@@ -8,7 +8,10 @@
 //
 // Bound by memory: y, h and a gate per value once in, h' and n (or codes) once out.  A
 // workgroup holds a row in registers, W units of 8 values per thread; its gammas and a
-// channel gate stay in registers from row to row.
+// channel gate stay in registers from row to row.  8000 rows of 4096 in bf16 with both norms
+// and a channel gate, to codes: 229 MB in 46 us, 5.0 TB/s, as fast as a copy; 2003 of 5120 on an
+// fp32 stream: 143 MB in 24 us, 5.9 TB/s, part of it from cache; one row 3.6 us, all of it the
+// launch, the trip to memory and the row's sums.
 #include <algorithm>
 #include <type_traits>
 
@@ -60,49 +63,72 @@ __device__ __forceinline__ Unit<BF16> pack(const float (&v)[kUnit]) {
     return u;
 }
 
-// Unit u of a row of D values; zeros past its end.
-template <bool BF16, bool VEC>
-__device__ __forceinline__ Unit<BF16> load(const Elem<BF16>* row, int u, int D) {
-    Unit<BF16> r;
-    if constexpr (VEC) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(row + u * kUnit);
+// How rows lie: kWhole in whole units, every one aligned to 16 bytes; kAny of at least a unit's
+// values, at any address; kShort of fewer than that.  Any address costs no loads value by value:
+// the memory unit takes 16 bytes as they come (4000 rows of 4097 in bf16, to codes: 29 us; value
+// by value 114, and 21 for 4096).
+enum Lie { kWhole, kAny, kShort };
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+
+// Where a unit begins in a row of D values.  The last one of kAny is moved back to end with the
+// row: its first `again` values are the unit's before too, come out the same and are stored
+// twice, but count once in sums.
+struct Place {
+    int at, again;  // again >= kUnit: past the row
+};
+
+template <Lie LIE>
+__device__ __forceinline__ Place place(int unit, int D) {
+    const int at = unit * kUnit;
+    if (LIE != kAny) return {at, at < D ? 0 : kUnit};
+    const int back = max(0, at + kUnit - D);
+    return {at - back, back};
+}
+
+// The values of a unit's that count in sums, the others as zeros.
+template <Lie LIE>
+__device__ __forceinline__ float counted(float v, int e, Place a) {
+    return LIE != kAny || e >= a.again ? v : 0.0f;
+}
+
+// A row's unit; zeros past its end.
+template <bool BF16, Lie LIE>
+__device__ __forceinline__ Unit<BF16> load(const Elem<BF16>* row, int unit, int D) {
+    using Load = std::conditional_t<LIE == kWhole, u32x4, u32x4_any>;
+    const Place a = place<LIE>(unit, D);
+    Unit<BF16> r{};
+    if constexpr (LIE != kShort) {
+        const Load* p = reinterpret_cast<const Load*>(row + a.at);
 #pragma unroll
-        for (int i = 0; i < (BF16 ? 1 : 2); ++i) r.w[i] = u * kUnit < D ? p[i] : u32x4{0u, 0u, 0u, 0u};
-    } else {
-        float v[kUnit];
+        for (int k = 0; k < (BF16 ? 1 : 2); ++k) r.w[k] = a.again < kUnit ? u32x4(p[k]) : u32x4{0u, 0u, 0u, 0u};
+    } else if (a.again == 0) {
 #pragma unroll
-        for (int i = 0; i < kUnit; ++i) {
-            v[i] = 0.0f;
-            if (u * kUnit + i < D) {
-                if constexpr (BF16) v[i] = kc::bf16_to_f32(row[u * kUnit + i]);
-                else v[i] = row[u * kUnit + i];
-            }
-        }
-        if constexpr (BF16) {  // exact
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                r.w[0][i] = __float_as_uint(v[2 * i]) >> 16 | (__float_as_uint(v[2 * i + 1]) & 0xFFFF0000u);
-        } else {
-            r = pack<false>(v);
+        for (int e = 0; e < kUnit; ++e) {
+            if (e >= D) break;
+            if constexpr (BF16) r.w[0][e / 2] |= static_cast<uint32_t>(row[e]) << (16 * (e % 2));
+            else r.w[e / 4][e % 4] = __float_as_uint(row[e]);
         }
     }
     return r;
 }
 
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void store(Elem<BF16>* row, int u, int D, const float (&v)[kUnit]) {
+template <bool BF16, Lie LIE>
+__device__ __forceinline__ void store(Elem<BF16>* row, int unit, int D, const float (&v)[kUnit]) {
+    using Store = std::conditional_t<LIE == kWhole, u32x4, u32x4_any>;
+    const Place a = place<LIE>(unit, D);
     const Unit<BF16> r = pack<BF16>(v);
-    if constexpr (VEC) {
-        if (u * kUnit >= D) return;
+    if (a.again >= kUnit) return;
+    if constexpr (LIE != kShort) {
 #pragma unroll
-        for (int i = 0; i < (BF16 ? 1 : 2); ++i)
-            __builtin_nontemporal_store(r.w[i], reinterpret_cast<u32x4*>(row + u * kUnit) + i);
+        for (int k = 0; k < (BF16 ? 1 : 2); ++k)
+            __builtin_nontemporal_store(Store(r.w[k]), reinterpret_cast<Store*>(row + a.at) + k);
     } else {
 #pragma unroll
-        for (int i = 0; i < kUnit; ++i) {
-            if (u * kUnit + i >= D) break;
-            if constexpr (BF16) row[u * kUnit + i] = static_cast<uint16_t>(r.w[0][i / 2] >> (16 * (i % 2)));
-            else row[u * kUnit + i] = v[i];
+        for (int e = 0; e < kUnit; ++e) {
+            if (e >= D) break;
+            if constexpr (BF16) row[e] = static_cast<uint16_t>(r.w[0][e / 2] >> (16 * (e % 2)));
+            else row[e] = v[e];
         }
     }
 }
@@ -130,8 +156,8 @@ __device__ __forceinline__ float over_row(float v, float* part) {
     return r;
 }
 
-template <bool YB, bool HB, bool FP8, bool VEC, int THREADS, int W>
-__global__ __launch_bounds__(THREADS) void residual_kernel(const Args p) {
+template <bool YB, bool HB, bool FP8, Lie LIE, int THREADS, int W>
+__global__ __launch_bounds__(THREADS, 4) void residual_kernel(const Args p) {
     using namespace kc::fp8;
     constexpr int kParts = THREADS / kWave;
     __shared__ float part[2][3][kParts];
@@ -145,10 +171,9 @@ __global__ __launch_bounds__(THREADS) void residual_kernel(const Args p) {
     Unit<YB> gamma[W], post[W], cgate[W];
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const int u = tid + i * THREADS;
-        gamma[i] = load<YB, VEC>(static_cast<const Y*>(p.gamma), u, p.D);
-        if (p.post) post[i] = load<YB, VEC>(static_cast<const Y*>(p.post), u, p.D);
-        if (channel) cgate[i] = load<YB, VEC>(gate, u, p.D);
+        gamma[i] = load<YB, LIE>(static_cast<const Y*>(p.gamma), tid + i * THREADS, p.D);
+        if (p.post) post[i] = load<YB, LIE>(static_cast<const Y*>(p.post), tid + i * THREADS, p.D);
+        if (channel) cgate[i] = load<YB, LIE>(gate, tid + i * THREADS, p.D);
     }
     int turn = 0;  // rows take the two sets of partial results in turn
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
@@ -156,20 +181,20 @@ __global__ __launch_bounds__(THREADS) void residual_kernel(const Args p) {
         Unit<HB> hv[W];
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            const int u = tid + i * THREADS;
-            yv[i] = load<YB, VEC>(y + row * p.y_stride, u, p.D);
-            hv[i] = load<HB, VEC>(h + row * p.h_stride, u, p.D);
-            if (gate && !channel) gv[i] = load<YB, VEC>(gate + row * p.gate_stride, u, p.D);
+            yv[i] = load<YB, LIE>(y + row * p.y_stride, tid + i * THREADS, p.D);
+            hv[i] = load<HB, LIE>(h + row * p.h_stride, tid + i * THREADS, p.D);
+            if (gate && !channel) gv[i] = load<YB, LIE>(gate + row * p.gate_stride, tid + i * THREADS, p.D);
         }
         float inv = 1.0f;
         if (p.post) {
             float ss = 0.0f;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
+                const Place a = place<LIE>(tid + i * THREADS, p.D);
                 float v[kUnit];
                 unpack<YB>(yv[i], v);
 #pragma unroll
-                for (int e = 0; e < kUnit; ++e) ss = fmaf(v[e], v[e], ss);
+                for (int e = 0; e < kUnit; ++e) ss = fmaf(v[e], counted<LIE>(v[e], e, a), ss);
             }
             ss = over_row<THREADS, false>(ss, part[turn][0]);
             inv = 1.0f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
@@ -177,6 +202,7 @@ __global__ __launch_bounds__(THREADS) void residual_kernel(const Args p) {
         float x[W][kUnit], ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
+            const Place a = place<LIE>(tid + i * THREADS, p.D);
             float b[kUnit], g[kUnit];
             unpack<YB>(yv[i], b);
             unpack<HB>(hv[i], x[i]);
@@ -193,9 +219,9 @@ __global__ __launch_bounds__(THREADS) void residual_kernel(const Args p) {
 #pragma unroll
             for (int e = 0; e < kUnit; ++e) {
                 x[i][e] = fmaf(p.alpha, b[e], x[i][e]);
-                ss = fmaf(x[i][e], x[i][e], ss);
+                ss = fmaf(x[i][e], counted<LIE>(x[i][e], e, a), ss);
             }
-            store<HB, VEC>(static_cast<H*>(p.h_out) + row * p.D, tid + i * THREADS, p.D, x[i]);
+            store<HB, LIE>(static_cast<H*>(p.h_out) + row * p.D, tid + i * THREADS, p.D, x[i]);
         }
         ss = over_row<THREADS, false>(ss, part[turn][1]);
         inv = 1.0f / sqrtf(ss / static_cast<float>(p.D) + p.eps);
@@ -209,7 +235,7 @@ __global__ __launch_bounds__(THREADS) void residual_kernel(const Args p) {
                 x[i][e] = (g[e] * x[i][e]) * inv;
                 if constexpr (FP8) most = fmaxf(most, fabsf(x[i][e]));
             }
-            if constexpr (!FP8) store<YB, VEC>(static_cast<Y*>(p.out) + row * p.D, tid + i * THREADS, p.D, x[i]);
+            if constexpr (!FP8) store<YB, LIE>(static_cast<Y*>(p.out) + row * p.D, tid + i * THREADS, p.D, x[i]);
         }
         if constexpr (FP8) {
             const RowDiv d = row_div(over_row<THREADS, true>(most, part[turn][2]));
@@ -217,31 +243,40 @@ __global__ __launch_bounds__(THREADS) void residual_kernel(const Args p) {
             uint8_t* codes = static_cast<uint8_t*>(p.out) + row * p.D;
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                const int at = (tid + i * THREADS) * kUnit;
-                if (at >= p.D) break;
+                const Place a = place<LIE>(tid + i * THREADS, p.D);
+                if (a.again >= kUnit) break;
                 const f32x4 lo{x[i][0], x[i][1], x[i][2], x[i][3]}, hi{x[i][4], x[i][5], x[i][6], x[i][7]};
                 const u32x2 c = d.fast ? u32x2{e4m3x4_div<true>(lo, d), e4m3x4_div<true>(hi, d)}
                                        : u32x2{e4m3x4_div<false>(lo, d), e4m3x4_div<false>(hi, d)};
-                if constexpr (VEC) {
-                    __builtin_nontemporal_store(c, reinterpret_cast<u32x2*>(codes + at));
+                if constexpr (LIE != kShort) {
+                    using Store = std::conditional_t<LIE == kWhole, u32x2, u32x2_any>;
+                    __builtin_nontemporal_store(Store(c), reinterpret_cast<Store*>(codes + a.at));
                 } else {
 #pragma unroll
                     for (int e = 0; e < kUnit; ++e)
-                        if (at + e < p.D) codes[at + e] = static_cast<uint8_t>(c[e / 4] >> (8 * (e % 4)));
+                        if (e < p.D) codes[e] = static_cast<uint8_t>(c[e / 4] >> (8 * (e % 4)));
                 }
             }
         }
     }
 }
 
-template <bool YB, bool HB, bool FP8, bool VEC>
+// One thread per unit while a row fits 256 of them, two units per thread to 16384 values; small
+// rows get small workgroups (32000 rows of 512 24 us, 256 threads 36), and 4 waves stay on a SIMD
+// with two units held.  Four units, for rows past 16384, spill (1000 rows of 28672 in bf16 72 us,
+// 3.2 TB/s); 1000 of 14336 took 49 us that way and take 19 with two.
+template <bool YB, bool HB, bool FP8, Lie LIE>
 void launch(const Args& p, hipStream_t stream) {
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(p.rows, 2048));
     const int units = (p.D + kUnit - 1) / kUnit;
-    if (units <= 256) residual_kernel<YB, HB, FP8, VEC, 256, 1><<<grid, 256, 0, stream>>>(p);
-    else if (units <= 512) residual_kernel<YB, HB, FP8, VEC, 256, 2><<<grid, 256, 0, stream>>>(p);
-    else if (units <= 1024) residual_kernel<YB, HB, FP8, VEC, 512, 2><<<grid, 512, 0, stream>>>(p);
-    else residual_kernel<YB, HB, FP8, VEC, 1024, 4><<<grid, 1024, 0, stream>>>(p);
+    if constexpr (LIE == kShort) residual_kernel<YB, HB, FP8, LIE, 64, 1><<<grid, 64, 0, stream>>>(p);
+    else if (units <= 64) residual_kernel<YB, HB, FP8, LIE, 64, 1><<<grid, 64, 0, stream>>>(p);
+    else if (units <= 128) residual_kernel<YB, HB, FP8, LIE, 128, 1><<<grid, 128, 0, stream>>>(p);
+    else if (units <= 256) residual_kernel<YB, HB, FP8, LIE, 256, 1><<<grid, 256, 0, stream>>>(p);
+    else if (units <= 512) residual_kernel<YB, HB, FP8, LIE, 256, 2><<<grid, 256, 0, stream>>>(p);
+    else if (units <= 1024) residual_kernel<YB, HB, FP8, LIE, 512, 2><<<grid, 512, 0, stream>>>(p);
+    else if (units <= 2048) residual_kernel<YB, HB, FP8, LIE, 1024, 2><<<grid, 1024, 0, stream>>>(p);
+    else residual_kernel<YB, HB, FP8, LIE, 1024, 4><<<grid, 1024, 0, stream>>>(p);
 }
 
 template <bool YB, bool HB, bool FP8>
@@ -258,12 +293,13 @@ int residual(const char* fn, const kc_residual* a, void* h_out, void* out, float
     const Args p{a->y,    a->h,    a->gate,  a->post_gamma, a->gamma, a->y_stride, a->h_stride, a->gate_stride,
                  a->rows, a->cols, a->alpha, a->eps,        h_out,    out,         scales};
     constexpr int y_step = YB ? 8 : 4, h_step = HB ? 8 : 4;  // values in 16 bytes
-    const bool vec = p.D % kUnit == 0 && p.y_stride % y_step == 0 && p.h_stride % h_step == 0 &&
+    const bool whole = p.D % kUnit == 0 && p.y_stride % y_step == 0 && p.h_stride % h_step == 0 &&
                      (!p.gate || p.gate_stride % y_step == 0) && kc::aligned(p.y, 16) && kc::aligned(p.h, 16) &&
                      kc::aligned(p.gate, 16) && kc::aligned(p.post, 16) && kc::aligned(p.gamma, 16) &&
                      kc::aligned(h_out, 16) && kc::aligned(out, FP8 ? 8 : 16);
-    if (vec) launch<YB, HB, FP8, true>(p, stream);
-    else launch<YB, HB, FP8, false>(p, stream);
+    if (whole) launch<YB, HB, FP8, kWhole>(p, stream);
+    else if (p.D >= kUnit) launch<YB, HB, FP8, kAny>(p, stream);
+    else launch<YB, HB, FP8, kShort>(p, stream);
     return kc::check_launch(fn);
 }
 
