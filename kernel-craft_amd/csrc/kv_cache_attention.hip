@@ -7,7 +7,8 @@
 //
 // The vector kernel is for what the matrix cores' does not take (heads over 256, rows of codes
 // that are no whole 16 bytes, unaligned pools).  It decodes value by value and is bound by that:
-// 4 sequences of 30000 tokens, 32 query heads on 8 of 72 in FP8: 164 us for 138 MB, 0.8 TB/s.
+// 4 sequences of up to 30000 tokens, 16 query heads on 8 of 72 in FP8: 70 us for 57 MB, 0.8 TB/s;
+// 16 on one of 576: 180 us for 54 MB.
 #include <algorithm>
 #include <type_traits>
 
@@ -33,22 +34,40 @@ __device__ __forceinline__ void put(Elem<BF16>* p, int64_t i, float v) {
     else p[i] = v;
 }
 
+__device__ __forceinline__ int wave_max_int(int v) {
+#pragma unroll
+    for (int off = kWave / 2; off > 0; off >>= 1) v = max(v, __shfl_xor(v, off, kWave));
+    return v;
+}
+
 constexpr int kHeads = 4;  // query heads of a wave of the vector kernel
 
-// Value d of the row `row` (slot * kv_heads + head); FP8 without its scale.
-template <bool FP8>
-__device__ __forceinline__ float value(const uint8_t* codes, const void* scales, int64_t row, int D, int d) {
-    if constexpr (FP8) return __builtin_amdgcn_cvt_f32_fp8(codes[row * D + d], 0);
-    const uint32_t c = codes[(row * D + d) / 2] >> (4 * (d & 1));
-    return decode4_f32(c & 15u, scale_value(static_cast<const uint8_t*>(scales)[(row * D + d) / kBlock])).x;
+// Values d .. d + W - 1 of the row `row` (slot * kv_heads + head); FP8 without its scale.
+template <bool FP8, int W>
+__device__ __forceinline__ void values(const uint8_t* codes, const void* scales, int64_t row, int D, int d,
+                                       float (&v)[W]) {
+    if constexpr (W == 1) {
+        static_assert(FP8, "rows of MXFP4 are whole blocks");
+        v[0] = __builtin_amdgcn_cvt_f32_fp8(codes[row * D + d], 0);
+    } else if constexpr (FP8) {
+        int w;
+        __builtin_memcpy(&w, codes + row * D + d, 4);
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+        v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
+    } else {
+        uint16_t w;
+        __builtin_memcpy(&w, codes + (row * D + d) / 2, 2);
+        const f32x4 f = decode4_f32(w, scale_value(static_cast<const uint8_t*>(scales)[(row * D + d) / kBlock]));
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    }
 }
 
 // A workgroup is one wave: kHeads query heads of one key/value head.  Scores: a lane per
-// position and half of the head; output: a lane per NI values of the head.
-template <bool BF16, bool FP8, int NI>
+// position and half of the head, W values at a time; output: a lane per NI times W values.
+template <bool BF16, bool FP8, int W, int NI>
 __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
     __shared__ PlanShared plan;
-    __shared__ float ql[kHeads * NI * kWave], pl[kHeads * kTile];
+    __shared__ float ql[kHeads * NI * W * kWave], pl[kHeads * kTile];
     __shared__ int sl[kTile];
     const int lane = threadIdx.x;
     const int set = blockIdx.y;
@@ -71,13 +90,15 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
         }
         const Elem<BF16>* q = static_cast<const Elem<BF16>*>(p.q) + b * p.q_stride + head0 * p.D;
         for (int i = lane; i < kHeads * p.D; i += kWave) ql[i] = i < heads * p.D ? get<BF16>(q, i) : 0.0f;
-        float m[kHeads], l[kHeads], acc[kHeads][NI];
+        float m[kHeads], l[kHeads], acc[kHeads][NI][W];
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
             m[j] = -inf;
             l[j] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NI; ++i) acc[j][i] = 0.0f;
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int e = 0; e < W; ++e) acc[j][i][e] = 0.0f;
         }
         __syncthreads();
         for (int tile = s.tile; tile < end; ++tile) {
@@ -88,10 +109,14 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
             float sc[kHeads] = {}, vs = 1.0f;
             if (slot >= 0) {
                 const int64_t row = static_cast<int64_t>(slot) * p.kv_heads + h;
-                for (int d = half; d < p.D; d += 2) {
-                    const float k = value<FP8>(p.k_codes, p.k_scales, row, p.D, d);
+#pragma unroll 4
+                for (int d = half * W; d < p.D; d += 2 * W) {
+                    float k[W];
+                    values<FP8, W>(p.k_codes, p.k_scales, row, p.D, d, k);
 #pragma unroll
-                    for (int j = 0; j < kHeads; ++j) sc[j] = fmaf(ql[j * p.D + d], k, sc[j]);
+                    for (int j = 0; j < kHeads; ++j)
+#pragma unroll
+                        for (int e = 0; e < W; ++e) sc[j] = fmaf(ql[j * p.D + d + e], k[e], sc[j]);
                 }
                 float ks = p.scale;
                 if constexpr (FP8) {
@@ -101,7 +126,9 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
 #pragma unroll
                 for (int j = 0; j < kHeads; ++j) sc[j] *= ks;
             }
-            if (half == 0) sl[t] = slot;
+            // positions without a row read another's: a weight of zero, or NaN, is all they have
+            const int some = wave_max_int(slot);
+            if (half == 0) sl[t] = slot >= 0 ? slot : some;
 #pragma unroll
             for (int j = 0; j < kHeads; ++j) {
                 float v = sc[j] + __shfl_xor(sc[j], kTile, kWave);
@@ -113,18 +140,25 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
                 l[j] = fmaf(l[j], by, kc::wave_sum(half == 0 ? e : 0.0f));
                 if (half == 0) pl[j * kTile + t] = seen ? e * vs : 0.0f;
 #pragma unroll
-                for (int i = 0; i < NI; ++i) acc[j][i] *= by;
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int e = 0; e < W; ++e) acc[j][i][e] *= by;
             }
             __syncthreads();
-            for (int u = 0; u < kTile; ++u) {
-                const int at = sl[u];
-                const int64_t row = static_cast<int64_t>(at) * p.kv_heads + h;
+            if (some >= 0) {  // else the sums of the weights say it all
+#pragma unroll 4
+                for (int u = 0; u < kTile; ++u) {
+                    const int64_t row = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(sl[u])) * p.kv_heads + h;
 #pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int d = lane + i * kWave;
-                    const float v = at >= 0 && d < p.D ? value<FP8>(p.v_codes, p.v_scales, row, p.D, d) : 0.0f;
+                    for (int i = 0; i < NI; ++i) {
+                        const int d = (lane + i * kWave) * W;
+                        float v[W] = {};
+                        if (d < p.D) values<FP8, W>(p.v_codes, p.v_scales, row, p.D, d, v);
 #pragma unroll
-                    for (int j = 0; j < kHeads; ++j) acc[j][i] = fmaf(pl[j * kTile + u], v, acc[j][i]);
+                        for (int j = 0; j < kHeads; ++j)
+#pragma unroll
+                            for (int e = 0; e < W; ++e) acc[j][i][e] = fmaf(pl[j * kTile + u], v[e], acc[j][i][e]);
+                    }
                 }
             }
             __syncthreads();
@@ -135,10 +169,13 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
             if (j >= heads) break;
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int d = lane + i * kWave;
+                const int d = (lane + i * kWave) * W;
                 if (d >= p.D) break;
-                if (whole) put<BF16>(out, j * p.D + d, acc[j][i] / l[j]);
-                else p.part_o[(segment + j) * p.D + d] = acc[j][i];
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    if (whole) put<BF16>(out, j * p.D + d + e, acc[j][i][e] / l[j]);
+                    else p.part_o[(segment + j) * p.D + d + e] = acc[j][i][e];
+                }
             }
             if (!whole && lane == 0) {
                 p.part_ml[(segment + j) * 2] = m[j];
@@ -266,10 +303,8 @@ struct Plan {
 constexpr int kMinTiles = 2;      // of a stretch
 constexpr int kDirectTiles = 5;   // of a sequence for each wave of a workgroup that takes all of it
 
-constexpr int kResident = 2048;   // waves that run at once: two a SIMD
-
-// Sets of `heads` query heads, workgroups of up to `waves` waves.
-Plan plan_of(int heads, int waves, const kc_kv_cache* c, int64_t max_pages, int seqs, int q_heads, int window) {
+// Sets of `heads` query heads, workgroups of up to `waves` waves, `resident` waves at once.
+Plan plan_of(int heads, int waves, int resident, const kc_kv_cache* c, int64_t max_pages, int seqs, int q_heads, int window) {
     Plan p{};
     const int group = q_heads / c->kv_heads;
     p.sets = c->kv_heads * ((group + heads - 1) / heads);
@@ -281,7 +316,7 @@ Plan plan_of(int heads, int waves, const kc_kv_cache* c, int64_t max_pages, int 
     // its waves end at different times and it reads heads apart, but nothing is joined.  fp32
     // or bf16, FP8, 8 sets: 24 sequences of 33 tiles 12.6 us against 20.3, one of 22 9.5
     // (12.4), one of 63 17.3 (13.1); in two rounds, 64 of 32 21.1 (18.1).
-    const int64_t rounds = (int64_t{seqs} * p.sets * waves + kResident - 1) / kResident;
+    const int64_t rounds = (int64_t{seqs} * p.sets * waves + resident - 1) / resident;
     if (tiles * std::max<int64_t>(rounds, 1) <= kDirectTiles * waves) {
         p.wg_sets = 1;
         p.streams = static_cast<int>(std::clamp<int64_t>(tiles, 1, waves));
@@ -292,7 +327,7 @@ Plan plan_of(int heads, int waves, const kc_kv_cache* c, int64_t max_pages, int 
     p.wg_sets = (p.sets + rows - 1) / rows;
     p.streams = waves / p.wg_sets;
     const int64_t most = (tiles * seqs + kMinTiles - 1) / kMinTiles;
-    const int at_once = std::max(1, kResident / (p.wg_sets * p.streams * rows));
+    const int at_once = std::max(1, resident / (p.wg_sets * p.streams * rows));
     const int64_t wgs = std::min<int64_t>(at_once, (most + p.streams - 1) / p.streams);
     p.grid = dim3(static_cast<unsigned>(std::clamp<int64_t>(wgs, 1, kMaxUnits / p.streams)), rows);
     p.units = static_cast<int>(p.grid.x) * p.streams;
@@ -300,8 +335,11 @@ Plan plan_of(int heads, int waves, const kc_kv_cache* c, int64_t max_pages, int 
 }
 
 Plan plan_for(const kc_kv_cache* c, bool bf16, int64_t max_pages, int seqs, int q_heads, int window) {
-    if (mfma_takes(*c, max_pages)) return plan_of(bf16 ? 8 : 4, kMaxWaves, c, max_pages, seqs, q_heads, window);
-    return plan_of(kHeads, 1, c, max_pages, seqs, q_heads, window);
+    // waves at once: of the matrix cores' kernel two a SIMD, of the vector kernel as many as
+    // its registers let: four, three, two
+    if (mfma_takes(*c, max_pages)) return plan_of(bf16 ? 8 : 4, kMaxWaves, 2048, c, max_pages, seqs, q_heads, window);
+    const int resident = c->head_dim <= 256 ? 4096 : c->head_dim <= 512 ? 3072 : 2048;
+    return plan_of(kHeads, 1, resident, c, max_pages, seqs, q_heads, window);
 }
 
 int64_t starts_bytes(int seqs) { return (int64_t{seqs} + 2) * 4; }
@@ -333,11 +371,17 @@ int check(const char* fn, const kc_kv_cache* cache, int64_t max_pages, int seqs,
     return KC_SUCCESS;
 }
 
+// Four values at a time where a head is whole fours (every MXFP4 one is).
 template <bool BF16, bool FP8>
 void launch_vector(const Attention& p, dim3 grid, hipStream_t stream) {
-    if (p.D <= 64) attention_kernel<BF16, FP8, 1><<<grid, kWave, 0, stream>>>(p);
-    else if (p.D <= 256) attention_kernel<BF16, FP8, 4><<<grid, kWave, 0, stream>>>(p);
-    else attention_kernel<BF16, FP8, 16><<<grid, kWave, 0, stream>>>(p);
+    if (p.D % 4 == 0) {
+        if (p.D <= 256) attention_kernel<BF16, FP8, 4, 1><<<grid, kWave, 0, stream>>>(p);
+        else if (p.D <= 512) attention_kernel<BF16, FP8, 4, 2><<<grid, kWave, 0, stream>>>(p);
+        else attention_kernel<BF16, FP8, 4, 4><<<grid, kWave, 0, stream>>>(p);
+    } else if constexpr (FP8) {
+        if (p.D <= 256) attention_kernel<BF16, FP8, 1, 4><<<grid, kWave, 0, stream>>>(p);
+        else attention_kernel<BF16, FP8, 1, 16><<<grid, kWave, 0, stream>>>(p);
+    }
 }
 
 template <bool BF16>
