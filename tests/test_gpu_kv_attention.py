@@ -85,7 +85,8 @@ SHAPES = [  # q heads, kv heads, D, page, format
     (2, 1, 576, 16, "fp8"), (2, 1, 1024, 16, "mxfp4"), (9, 9, 16, 4, "fp8"), (66, 11, 64, 16, "fp8"), (10, 5, 112, 16, "fp8"),
     (4, 2, 48, 16, "fp8"), (4, 1, 144, 3, "fp8"), (8, 2, 160, 16, "fp8"), (8, 2, 160, 16, "mxfp4"), (2, 1, 176, 16, "fp8"),
     (2, 1, 208, 16, "fp8"), (2, 1, 224, 64, "fp8"), (5, 1, 224, 16, "mxfp4"), (3, 1, 240, 16, "fp8"),
-    (72, 72, 64, 16, "fp8"), (64, 1, 128, 16, "fp8"), (1, 1, 1000, 16, "fp8"),
+    (72, 72, 64, 16, "fp8"), (64, 1, 128, 16, "fp8"), (1, 1, 1000, 16, "fp8"), (3, 1, 257, 16, "fp8"), (2, 1, 999, 5, "fp8"),
+    (6, 2, 300, 16, "fp8"), (5, 1, 512, 16, "fp8"), (8, 2, 320, 16, "mxfp4"), (4, 4, 72, 16, "fp8"), (7, 1, 65, 16, "fp8"),
 ]
 
 
@@ -250,6 +251,28 @@ def test_results_repeat(gpu, ops):
                 got.append(ops.kv_cache_attention(q, *pool, table, d_lens))
     gpu.cuda.synchronize()
     assert all(gpu.equal(y, want) for y in got)
+
+
+def test_pages_in_several_places(gpu, ops):
+    """Sequences that share the pages of a prefix, and a page twice in one: the
+    values of a cache that holds copies."""
+    lens = [100, 90, 64, 3]
+    for D, fmt in ((128, "fp8"), (64, "mxfp4"), (33, "fp8")):
+        pool, table = fill(gpu, ops, lens, 2, D, 16, fmt)
+        table[1, :5] = table[0, :5]
+        table[2, 2] = table[2, 0]
+        table[3, 0] = table[0, 1]
+        for dtype in (gpu.bfloat16, gpu.float32):
+            check(gpu, ops, queries(gpu, 4, 8, D, dtype), pool, table, lens, fmt)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_windows_of_a_large_batch(gpu, ops, dtype):
+    """More sequences than a wave has lanes, some empty, some within the window."""
+    lens = [(37 * i * i) % 301 * (i % 7 != 3) for i in range(150)] + [2500, 0]
+    for Hq, H, D, page, fmt in ((16, 4, 128, 16, "fp8"), (8, 1, 64, 48, "mxfp4"), (3, 1, 20, 16, "fp8")):
+        pool, table = fill(gpu, ops, lens, H, D, page, fmt, window=129)
+        check(gpu, ops, queries(gpu, len(lens), Hq, D, getattr(gpu, dtype)), pool, table, lens, fmt, 129)
 
 
 def test_two_graphs_replayed_in_turn(gpu, ops):

@@ -142,6 +142,27 @@ def test_views_and_streams(gpu, ops):
     assert all(np.array_equal(g, w) for g, w in zip(got, want))
 
 
+def test_two_pools_on_two_streams(gpu, ops):
+    """Steps over tables of their own, at once: each as alone."""
+    rng = np.random.default_rng(8)
+    jobs = []
+    for B in (300, 40):
+        lens, fresh = rng.integers(0, 90, B), rng.integers(0, 5, B)
+        table, stack = _state(rng, lens, 16, 8, B)
+        rows = int(fresh.sum())
+        want = ref.extend(lens, fresh, table, stack, B, 16, rows)
+        jobs.append(([_dev(gpu, np.asarray(a, np.int32)) for a in (lens, fresh, table, stack, [B])], rows, want))
+    streams = [gpu.cuda.Stream() for _ in jobs]
+    gpu.cuda.synchronize()
+    got = []
+    for _ in range(6):
+        for s, (args, rows, want) in zip(streams, jobs):
+            with gpu.cuda.stream(s):
+                got.append(((*ops.kv_cache_extend(*args, 16, rows), args[2]), want))
+    gpu.cuda.synchronize()
+    assert all(np.array_equal(g.cpu().numpy(), w) for gs, ws in got for g, w in zip(gs, ws))
+
+
 def test_many_steps_in_a_graph(gpu, ops):
     """A step that extends, releases and feeds its results back, captured once
     and replayed, against the rules on the host; other eager work between."""

@@ -10,7 +10,8 @@ pytestmark = pytest.mark.gpu
 
 TYPES = [("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float32", "float32")]
 SHAPES = [(1, 4096), (1, 1), (3, 8), (5, 33), (2, 2048), (4, 2056), (7, 4104), (2, 5120), (3, 8192), (2, 8200), (1, 14336),
-          (2, 32768), (1, 32761), (300, 512), (2100, 1024), (2, 777), (0, 64), (4, 0)]
+          (2, 32768), (1, 32761), (2, 16384), (2, 16385), (3, 8193), (5, 7), (4, 15), (3, 1023), (2, 1031), (300, 512),
+          (2100, 1024), (2, 777), (0, 64), (4, 0)]
 FORMS = [(False, None), (True, None), (False, "channel"), (True, "channel"), (False, "value"), (True, "value")]
 
 
@@ -91,6 +92,56 @@ def test_views(gpu, ops, ydt, hdt):
         got = ops.residual_rmsnorm(y[:1].expand(6, D), h, gamma, post, gate[:1].expand(6, D), 0.5)
         want = ops.residual_rmsnorm(y[:1].repeat(6, 1), h, gamma, post, gate[0], 0.5)
         assert all(gpu.equal(g, w) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize("ydt,hdt", TYPES)
+@pytest.mark.parametrize("D", [7, 8, 520, 523, 4104])
+def test_gammas_and_gates_at_any_address(gpu, ops, D, ydt, hdt):
+    """Rows of weights that begin between 16 bytes, in both forms: the bits of
+    aligned ones."""
+    ydt, hdt = getattr(gpu, ydt), getattr(gpu, hdt)
+    y, h, gamma, post, gate = _inputs(gpu, 5, D, ydt, hdt, True, "channel")
+    def moved(t):
+        return gpu.cat([t[:1], t])[1:]
+    for f in (ops.residual_rmsnorm, ops.residual_rmsnorm_fp8_quantize):
+        want = f(y, h, gamma, post, gate, 0.7)
+        for a in ((moved(gamma), post, gate), (gamma, moved(post), gate), (gamma, post, moved(gate))):
+            assert all(gpu.equal(g, w) for g, w in zip(f(y, h, *a, 0.7), want))
+
+
+@pytest.mark.parametrize("D", [3, 13, 64, 515])
+def test_nothing_behind_the_rows(gpu, ops, D):
+    """Outputs at odd addresses between other bytes: those stay."""
+    import ctypes
+    import kc_abi
+    L, T = kc_abi.lib(), 3
+    y, h, gamma, post, gate = _inputs(gpu, T, D, gpu.bfloat16, gpu.bfloat16, True, "value")
+    want = ops.residual_rmsnorm_fp8_quantize(y, h, gamma, post, gate, 0.5)
+    h_out = gpu.full((T * D + 9,), 7.0, device="cuda").bfloat16()
+    codes = gpu.full((T * D + 9,), 99, dtype=gpu.int8, device="cuda")
+    scales = gpu.full((T + 2,), 7.0, device="cuda")
+    a = ops.Residual(y.data_ptr(), h.data_ptr(), gate.data_ptr(), post.data_ptr(), gamma.data_ptr(), D, D, D, T, D, 0.5,
+                     1e-6)
+    assert L.kc_residual_rmsnorm_quantize_fp8_bf16(ctypes.byref(a), kc_abi.ptr(h_out[1:]), kc_abi.ptr(codes[1:]),
+                                                   kc_abi.ptr(scales[1:]), kc_abi.stream()) == 0
+    for got, w, was in zip((h_out, codes, scales), want, (7, 99, 7)):
+        n = w.numel()
+        assert gpu.equal(got[1:1 + n], w.flatten())
+        assert bool((got[:1] == was).all()) and bool((got[1 + n:] == was).all())
+
+
+def test_two_streams_at_once(gpu, ops):
+    args = [_inputs(gpu, 700, 515 + i, gpu.bfloat16, gpu.float32, True, "value") for i in range(2)]
+    want = [ops.residual_rmsnorm(*a) for a in args]
+    streams = [gpu.cuda.Stream() for _ in args]
+    gpu.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, a in zip(streams, args):
+            with gpu.cuda.stream(s):
+                got.append(ops.residual_rmsnorm(*a))
+    gpu.cuda.synchronize()
+    assert all(gpu.equal(g, w) for i, o in enumerate(got) for g, w in zip(o, want[i % 2]))
 
 
 def test_extreme_rows(gpu, ops):

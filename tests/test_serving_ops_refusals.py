@@ -142,6 +142,8 @@ def _res(**kw):
     (lambda L: _call(L, seqs=1 << 22), "too large"),
     (lambda L: _call(L, heads=1 << 16), "too large"),
     (lambda L: _call(L, pages=1 << 31), "too large"),
+    (lambda L: _call(L, pages=1 << 27, seqs=17), "too large"),
+    (lambda L: _call(L, pages=(1 << 31) - 1, seqs=17), "too large"),
     (lambda L: _call(L, cache=_cache(num_pages=1 << 28)), "slots"),
     (lambda L: _call(L, cache=_cache(head_dim=1025)), "1024"),
     (lambda L: _call(L, cache=_cache(head_dim=48, format=1)), "multiple of 32"),
