@@ -15,7 +15,7 @@
 //
 // The 16 columns are N query heads in 16 / N pieces.  bf16 queries: 8 heads, the weights
 // as the sum of two bf16 values (2^-17), one in each piece.  fp32 queries: 4 heads, queries
-// and weights as sums of three bf16 values (2^-25).  The pieces cost no product more, since
+// and weights as sums of three bf16 values (exact, and 2^-25).  The pieces cost no product more, since
 // groups of up to 8 (4) query heads leave those columns empty.
 //
 // Two waves a SIMD, each with the next tile's codes, scales and row numbers in flight (the
@@ -57,6 +57,10 @@ __device__ __forceinline__ uint32_t fp8_pair(uint32_t w, bool high) {
                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), 1.0f, false);
     return __builtin_bit_cast(uint32_t, r);
 }
+
+// The value's first 8 significant bits: fp32 is the sum of three such pieces, exactly, and none
+// of them is past the largest bf16 value where the fp32 is.
+__device__ __forceinline__ float top_half(float v) { return __uint_as_float(__float_as_uint(v) & 0xFFFF0000u); }
 
 // Codes 2 BYTE and 2 BYTE + 1 of w times the scale 2^(b - 127), b's value as scale_operand gives it.
 template <int BYTE>
@@ -249,8 +253,7 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {  // the piece of the value that this column holds
                             x[k] = from[d0 + 8 * i + e + k];
-                            const float hi = kc::bf16_to_f32(kc::f32_to_bf16(x[k]));
-                            const float r = x[k] - hi, mid = kc::bf16_to_f32(kc::f32_to_bf16(r));
+                            const float hi = top_half(x[k]), r = x[k] - hi, mid = top_half(r);
                             x[k] = part == 0 ? hi : part == 1 ? mid : part == 2 ? r - mid : 0.0f;
                         }
                         w[e / 2] = kc::pack_bf16x2(x[0], x[1]);

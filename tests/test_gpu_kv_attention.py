@@ -174,6 +174,23 @@ def test_large_and_equal_scores(gpu, ops, D, fmt):
             check(gpu, ops, queries(gpu, 4, 8, D, dtype, size=size), pool, table, lens, fmt, scale=scale)
 
 
+@pytest.mark.parametrize("D", [128, 288])
+def test_the_largest_queries(gpu, ops, D):
+    """fp32 queries that bf16 would round to infinity: one value a head, against
+    keys of a quarter there, so that every product and sum stays in fp32."""
+    lens = [90, 3, 300]
+    pool, table = fill(gpu, ops, lens, 2, D, 16, "mxfp4")
+    k = gpu.ones(90, 2, D, device="cuda")
+    at = gpu.arange(90, device="cuda")
+    slots = table[0, at // 16].long() * 16 + at % 16
+    q = gpu.zeros(3, 8, D, device="cuda")
+    for h in range(8):
+        k[:, h // 4, 3 * h] = 0.25 * (1 - 2 * (at % (h + 2) == 0).float())
+        q[0, h, 3 * h] = 3.402e38 * (-1.0) ** h
+    ops.kv_cache_write(k, gpu.randn(90, 2, D, device="cuda"), slots, *pool)
+    check(gpu, ops, q, pool, table, lens, "mxfp4", scale=2.0 ** -126)
+
+
 @pytest.mark.parametrize("D,fmt", [(128, "fp8"), (64, "mxfp4"), (33, "fp8")])
 def test_nan_and_infinite_queries(gpu, ops, D, fmt):
     """A query head's NaN or infinity, and a key's or value's NaN, stay where they are."""
