@@ -527,7 +527,7 @@ typedef struct kc_kv_pages {
  *     served and for rows behind the last request
  * (cu_* past 2^31 - 1 stay at it).  Inputs are left as they are but for new
  * entries of block_table, and no output may overlap them, so a call that is
- * repeated gives the same again.  seqs up to 2^24. */
+ * repeated gives the same again.  seqs up to 2^20. */
 int kc_kv_cache_extend(const kc_kv_pages* pages, const int32_t* d_seq_lens,
                        const int32_t* d_new_lens, int64_t total_new,
                        int32_t* d_seq_lens_out, int32_t* d_free_count_out,
@@ -536,7 +536,9 @@ int kc_kv_cache_extend(const kc_kv_pages* pages, const int32_t* d_seq_lens,
                        kc_stream_t stream);
 /* The pages of the sequences with finished[b] != 0 (u8 [seqs]) back onto the
  * stack, in order: free_pages is written from free_count on (pages past
- * num_pages are dropped), seq_lens_out is 0 for them.  block_table stays. */
+ * num_pages are dropped), seq_lens_out is 0 for them.  block_table stays.
+ * Entries go back as they stand: a page that two sequences hold, or an entry
+ * that is no page, must not reach this call. */
 int kc_kv_cache_release(const kc_kv_pages* pages, const uint8_t* d_finished,
                         const int32_t* d_seq_lens, int32_t* d_seq_lens_out,
                         int32_t* d_free_count_out, kc_stream_t stream);

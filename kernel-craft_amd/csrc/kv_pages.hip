@@ -26,6 +26,8 @@ using kc::kWave;
 // waves and 1024 LDS entries: 256 requests 5.2 us, 6.5 with 1024 threads).
 constexpr int kFew = 256, kMany = 1024;
 
+constexpr int kMaxRequests = 1 << 20;  // every workgroup goes over all of them
+
 struct Pages {
     int32_t* table;
     int32_t* stack;
@@ -220,7 +222,7 @@ int check(const char* fn, const kc_kv_pages* pages, const int32_t* lens, const i
         return kc::set_error(KC_ERR_INVALID_ARGUMENT,
                              "%s: bad shape seqs=%d max_pages=%lld num_pages=%lld page_size=%d", fn, pages->seqs,
                              (long long)pages->max_pages, (long long)pages->num_pages, pages->page_size);
-    if (pages->max_pages > INT32_MAX || pages->num_pages > INT32_MAX || pages->seqs > (1 << 24))
+    if (pages->max_pages > INT32_MAX || pages->num_pages > INT32_MAX || pages->seqs > kMaxRequests)
         return kc::set_error(KC_ERR_INVALID_ARGUMENT, "%s: seqs=%d max_pages=%lld num_pages=%lld too large", fn,
                              pages->seqs, (long long)pages->max_pages, (long long)pages->num_pages);
     const bool table = pages->seqs > 0 && pages->max_pages > 0;

@@ -1219,8 +1219,8 @@ def _kv_pages(op: str, seq_lens, block_table, free_pages, free_count, page_size:
     if len(free) != 1 or free_count.shape != (1,):
         raise ValueError(f"{op}: free_pages {tuple(free)} and free_count "
                          f"{tuple(free_count.shape)} must be [pages] and [1]")
-    if page_size <= 0:
-        raise ValueError(f"{op}: page_size={page_size} must be positive")
+    if not 0 < page_size < 2 ** 31:
+        raise ValueError(f"{op}: page_size={page_size} must be from 1 to 2^31 - 1")
     return seq_lens, block_table, free_pages, free_count, KvPages(
         block_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(), table[1], free[0],
         page_size, table[0])
@@ -1270,7 +1270,8 @@ def kv_cache_release(finished, seq_lens, block_table, free_pages, free_count,
     """The pages of the sequences that ``finished`` (bool or u8 [requests]) names, back onto the
     stack of free pages (kv_cache_extend's tensors; free_pages is written in place from
     free_count on).  Returns (seq_lens, free_count), lengths of 0 for those sequences; their
-    entries of block_table stay (kc_kv_cache_release)."""
+    entries of block_table stay.  Entries go back as they stand: pages that sequences share are
+    the caller's to count, and must not come here twice (kc_kv_cache_release)."""
     import torch
     op = "kv_cache_release"
     if finished.dtype not in (torch.bool, torch.uint8):

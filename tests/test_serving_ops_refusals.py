@@ -76,6 +76,8 @@ def _residual(y=None, h=None, gamma=None, **kw):
     (lambda: _extend(count=z(2)), "free_count"),
     (lambda: _extend(count=z(1, dtype=torch.int64)), "dtype"),
     (lambda: _extend(page=0), "page_size"),
+    (lambda: _extend(page=2 ** 32 + 16), "page_size"),
+    (lambda: _release(page=2 ** 31), "page_size"),
     (lambda: _extend(total=-1), "total_new"),
     (lambda: _extend(total=2 ** 31), "total_new"),
     (lambda: _extend(), "GPU only"),
@@ -162,7 +164,7 @@ def _res(**kw):
     (lambda L: L.kc_kv_cache_extend(_pages(seqs=-1), P, P, 3, P, P, P, P, P, P, None), "shape"),
     (lambda L: L.kc_kv_cache_extend(_pages(max_pages=-1), P, P, 3, P, P, P, P, P, P, None), "shape"),
     (lambda L: L.kc_kv_cache_extend(_pages(num_pages=1 << 31), P, P, 3, P, P, P, P, P, P, None), "too large"),
-    (lambda L: L.kc_kv_cache_extend(_pages(seqs=(1 << 24) + 1), P, P, 3, P, P, P, P, P, P, None), "too large"),
+    (lambda L: L.kc_kv_cache_extend(_pages(seqs=(1 << 20) + 1), P, P, 3, P, P, P, P, P, P, None), "too large"),
     (lambda L: L.kc_kv_cache_extend(_pages(), P, P, -1, P, P, P, P, P, P, None), "total_new"),
     (lambda L: L.kc_kv_cache_extend(_pages(), P, P, 1 << 31, P, P, P, P, P, P, None), "total_new"),
     (lambda L: L.kc_kv_cache_extend(_pages(block_table=None), P, P, 3, P, P, P, P, P, P, None), "null"),
