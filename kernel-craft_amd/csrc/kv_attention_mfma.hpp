@@ -23,9 +23,10 @@
 // read: 4 sequences of 131072 tokens, 32 query heads on 8 of 128 in FP8: 430 MB in 92 us, 4.7
 // TB/s, the same time with the arithmetic left out, and 5.9 TB/s is what rows of a
 // paged cache can be read at in this order at all.  64 of up to 2000: 92 MB in 26 us, of which
-// the split, the first trips to memory and the join are 9.  In MXFP4 the decoding is what
-// bounds long caches: 4 of 131072 take 62 us for 227 MB, the vector units busy for 8 parts in
-// 10.  Three or four waves a SIMD, a barrier a tile and two tiles in flight were no faster.
+// the split, the first trips to memory and the join are 9.  In MXFP4
+// a trip to memory brings half the bytes: 4 of 131072 take 61 us for 222 MB, and leaving the
+// decoding out changes nothing.  Three or four waves a SIMD, a barrier a tile and two tiles in
+// flight were no faster.
 #pragma once
 
 #include <type_traits>
