@@ -23,7 +23,6 @@ namespace kv {
 constexpr int kTile = 32;          // positions
 constexpr int kMaxUnits = 4096;    // stretches of a set of query heads
 constexpr int kMaxWaves = 8;       // of a workgroup
-constexpr int kXcds = 8;           // workgroups go round them in turn
 
 struct Attention {
     const void* q;

@@ -335,10 +335,10 @@ Plan plan_of(int heads, int waves, int resident, const kc_kv_cache* c, int64_t m
 }
 
 Plan plan_for(const kc_kv_cache* c, bool bf16, int64_t max_pages, int seqs, int q_heads, int window) {
-    // waves at once: of the matrix cores' kernel two a SIMD, of the vector kernel as many as
-    // its registers let: four, three, two
+    // waves at once: of the matrix cores' kernel two a SIMD, of the vector kernel four (heads
+    // past 256, three of which fit, take no longer with them), or the two that fit
     if (mfma_takes(*c, max_pages)) return plan_of(bf16 ? 8 : 4, kMaxWaves, 2048, c, max_pages, seqs, q_heads, window);
-    const int resident = c->head_dim <= 256 ? 4096 : c->head_dim <= 512 ? 3072 : 2048;
+    const int resident = c->head_dim <= 512 ? 4096 : 2048;
     return plan_of(kHeads, 1, resident, c, max_pages, seqs, q_heads, window);
 }
 
