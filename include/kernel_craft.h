@@ -474,8 +474,9 @@ int kc_kv_cache_read_f32(const kc_kv_cache* cache, const int32_t* d_block_table,
  * without tokens (a length of 0 or below) gives zeros; one with a visible
  * position whose page is missing (past max_pages, or an entry outside the
  * pool) gives NaN.  What the cache holds behind a sequence's end, or outside
- * of its window, does not matter, NaN included.  At most 2^31 - 1 slots,
- * seqs * q_heads below 2^24, seqs * max_pages * page_size up to 2^35.
+ * of its window, does not matter, NaN included.  out overlaps no input.  At
+ * most 2^31 - 1 slots, seqs * q_heads below 2^24, seqs * max_pages * page_size
+ * up to 2^35.
  *
  * The workspace (16-byte aligned) holds what the parts of a long sequence
  * give before they are joined: kc_kv_cache_attention_workspace() bytes (-1
