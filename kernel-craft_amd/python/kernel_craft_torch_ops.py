@@ -1165,7 +1165,7 @@ def kv_cache_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq
     if not (whole and (bf16 or dtype is torch.float32) and len(shape) == 3 and shape[2] == D):
         q = _heads(op, "q", q, (torch.bfloat16, torch.float32), (None, None, D))
     B, Hq, _ = shape
-    if Hq % Hkv:
+    if not Hkv or Hq % Hkv:
         raise ValueError(f"{op}: q has {Hq} heads, not a multiple of the cache's {Hkv}")
     block_table = _take(op, "block_table", block_table, torch.int32)
     seq_lens = _take(op, "seq_lens", seq_lens, torch.int32)

@@ -106,6 +106,13 @@ def test_operators_refuse(call, match):
         call()
 
 
+@pytest.mark.parametrize("heads", [0, 4])
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+def test_a_cache_without_heads(fmt, heads):
+    with pytest.raises(ValueError, match="multiple"):
+        _attend(q=z(3, heads, 64, dtype=BF), pool=_pool(H=0, fmt=fmt))
+
+
 P = ctypes.c_void_p(0x1000)
 ODD = ctypes.c_void_p(0x1008)
 
