@@ -53,10 +53,30 @@ __device__ __forceinline__ float dpp(float v) {
 }
 constexpr int kRor4 = 0x124, kRor8 = 0x128;  // within 16 lanes
 
-__device__ __forceinline__ uint32_t fp8_pair(uint32_t w, bool high) {
-    const bf16x2 r = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), 1.0f, true)
-                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), 1.0f, false);
+// Codes of w times a power of two.
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t w, bool high, float power = 1.0f) {
+    const bf16x2 r = high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), power, true)
+                          : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(static_cast<int>(w), power, false);
     return __builtin_bit_cast(uint32_t, r);
+}
+
+// An FP8 key's scale as power * rest: the power of two goes into its values as they are decoded,
+// so that products with the query are past fp32 only where those with the key are, and the rest,
+// from 1 to 2 (past 2^126 to 4, below 2^-100 less than 1), is the score's.  Between the bounds
+// every E4M3 value times the power is a normal bf16, and the power's inverse a normal fp32.
+__device__ __forceinline__ float power_of(float scale) {
+    const uint32_t e = __float_as_uint(scale) & 0x7F800000u;
+    return __uint_as_float(min(max(e, 0x0D800000u), 0x7E800000u));
+}
+__device__ __forceinline__ float inverse(float power) { return __uint_as_float(0x7F000000u - __float_as_uint(power)); }
+
+// Lanes 0 .. 15 and 16 .. 31 of v, to all four rows of 16 lanes each.
+__device__ __forceinline__ void spread_rows(float v, float& first, float& second) {
+    const uint32_t b = __float_as_uint(v);
+    const auto low = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    const auto rows = __builtin_amdgcn_permlane16_swap(low[0], low[0], false, false);
+    first = __uint_as_float(rows[0]);
+    second = __uint_as_float(rows[1]);
 }
 
 // The value's first 8 significant bits: fp32 is the sum of three such pieces, exactly, and none
@@ -350,9 +370,12 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
         fetch(after);
         __builtin_amdgcn_sched_barrier(0);
         // this tile's scales; without a slot 0, or 2^0 for the zeros there
+        float power[2];
         if constexpr (FP8) {
-            lds.scales.f[lane / kTile][t] =
-                slot < 0 ? 0.0f : __uint_as_float(sc[0]) * (lane < kTile ? p.scale : 1.0f);
+            const float scale = __uint_as_float(sc[0]), own = power_of(scale);
+            spread_rows(own, power[0], power[1]);
+            const float rest = lane < kTile ? scale * inverse(own) * p.scale : scale;
+            lds.scales.f[lane / kTile][t] = slot < 0 ? 0.0f : rest;
         } else {
 #pragma unroll
             for (int i = 0; i < S::kBlocks; ++i)
@@ -372,8 +395,9 @@ __global__ __launch_bounds__(512) void attention_mfma_kernel(const Attention p) 
                     const uint32_t w0 = k[half][2 * i];
                     const bool pair = 2 * i + 1 < KC::dwords();
                     const uint32_t w1 = pair ? k[half][pair ? 2 * i + 1 : 0] : 0u;
-                    a = product(operand(fp8_pair(w0, false), fp8_pair(w0, true), pair ? fp8_pair(w1, false) : 0u,
-                                        pair ? fp8_pair(w1, true) : 0u),
+                    a = product(operand(fp8_pair(w0, false, power[half]), fp8_pair(w0, true, power[half]),
+                                        pair ? fp8_pair(w1, false, power[half]) : 0u,
+                                        pair ? fp8_pair(w1, true, power[half]) : 0u),
                                 q[i], a);
                 }
             } else {

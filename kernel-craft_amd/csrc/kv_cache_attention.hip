@@ -109,22 +109,26 @@ __global__ __launch_bounds__(kWave) void attention_kernel(const Attention p) {
             float sc[kHeads] = {}, vs = 1.0f;
             if (slot >= 0) {
                 const int64_t row = static_cast<int64_t>(slot) * p.kv_heads + h;
+                float ks = 1.0f;
+                if constexpr (FP8) {
+                    ks = static_cast<const float*>(p.k_scales)[row];
+                    vs = static_cast<const float*>(p.v_scales)[row];
+                }
 #pragma unroll 4
                 for (int d = half * W; d < p.D; d += 2 * W) {
                     float k[W];
                     values<FP8, W>(p.k_codes, p.k_scales, row, p.D, d, k);
+                    if constexpr (FP8) {  // before the products: those with the codes may be past fp32
+#pragma unroll
+                        for (int e = 0; e < W; ++e) k[e] *= ks;
+                    }
 #pragma unroll
                     for (int j = 0; j < kHeads; ++j)
 #pragma unroll
                         for (int e = 0; e < W; ++e) sc[j] = fmaf(ql[j * p.D + d + e], k[e], sc[j]);
                 }
-                float ks = p.scale;
-                if constexpr (FP8) {
-                    ks *= static_cast<const float*>(p.k_scales)[row];
-                    vs = static_cast<const float*>(p.v_scales)[row];
-                }
 #pragma unroll
-                for (int j = 0; j < kHeads; ++j) sc[j] *= ks;
+                for (int j = 0; j < kHeads; ++j) sc[j] *= p.scale;
             }
             // positions without a row read another's: a weight of zero, or NaN, is all they have
             const int some = wave_max_int(slot);

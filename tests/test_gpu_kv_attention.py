@@ -191,6 +191,43 @@ def test_the_largest_queries(gpu, ops, D):
     check(gpu, ops, q, pool, table, lens, "mxfp4", scale=2.0 ** -126)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("D", [128, 16, 33, 288])
+def test_the_range_of_fp8_scores(gpu, ops, D, dtype):
+    """Queries and keys whose products with each other stay in fp32, but not those
+    with the keys' codes (up to 448) or the scales' with the scale of the call."""
+    lens = [90, 3, 300]
+    pool, table = fill(gpu, ops, lens, 2, D, 16, "fp8")
+    at = gpu.arange(90, device="cuda")
+    slots = table[0, at // 16].long() * 16 + at % 16
+    v = gpu.randn(90, 2, D, device="cuda")
+    # one value a head, of nearly fp32's largest, against keys of a quarter there
+    k = gpu.ones(90, 2, D, device="cuda")
+    q = gpu.zeros(3, 8, D, device="cuda")
+    for h in range(8):
+        k[:, h // 4, 2 * h] = 0.25 * (1 - 2 * (at % (h + 2) == 0).float())
+        q[0, h, 2 * h] = 3.3e38 * (-1.0) ** h
+    ops.kv_cache_write(k, v, slots, *pool)
+    check(gpu, ops, q.to(getattr(gpu, dtype)), pool, table, lens, "fp8", scale=2.0 ** -126)
+    # large against small, both ways
+    for size in (3e35, 1e-30):
+        ops.kv_cache_write(gpu.randn(90, 2, D, device="cuda") / size, v, slots, *pool)
+        q = queries(gpu, 3, 8, D, getattr(gpu, dtype))
+        q[0] = (size * queries(gpu, 1, 8, D, gpu.float32)[0]).to(q.dtype)
+        check(gpu, ops, q, pool, table, lens, "fp8")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("D", [128, 33])
+def test_any_finite_scale_of_a_key(gpu, ops, D, dtype):
+    """Zero, negative, denormal and far apart, in one tile."""
+    lens = [70, 40]
+    pool, table = fill(gpu, ops, lens, 2, D, 16, "fp8")
+    at = gpu.arange(70, device="cuda")
+    kinds = gpu.tensor([0.0, -0.01, 2.0 ** -140, 2.0 ** -149, 0.02, 2.0 ** -101, -(2.0 ** -130)], device="cuda")
+    pool[1][table[0, at // 16].long(), at % 16] = kinds[at % 7, None].expand(70, 2).contiguous()
+    check(gpu, ops, queries(gpu, 2, 8, D, getattr(gpu, dtype)), pool, table, lens, "fp8")
+
 @pytest.mark.parametrize("D,fmt", [(128, "fp8"), (64, "mxfp4"), (33, "fp8")])
 def test_nan_and_infinite_queries(gpu, ops, D, fmt):
     """A query head's NaN or infinity, and a key's or value's NaN, stay where they are."""
