@@ -425,3 +425,230 @@ def test_serving_steps(gpu, ops, fmt):
         lens, count = ops.kv_cache_release(done, lens, table, free, count, page)
         held = sum(-(-n // page) for n in lens.tolist())
         assert int(count) == pages - held and len(free[:pages - held].unique()) == pages - held
+
+
+def workspace(ops, pool, table, B, Hq):
+    """Bytes that attention over this cache needs; 0 where no sequence is split."""
+    import kc_abi
+    pages, page, H = pool[0].shape[:3]
+    fp8 = pool[1].dim() == 3
+    D = pool[0].shape[3] * (1 if fp8 else 2)
+    cache = ops.KvCache(*(t.data_ptr() for t in pool), pages, page, H, D, 0 if fp8 else 1)
+    return kc_abi.lib().kc_kv_cache_attention_workspace(ctypes.byref(cache), table.shape[1], B, Hq), cache
+
+
+def split(ops, pool, table, B, Hq):
+    need, _ = workspace(ops, pool, table, B, Hq)
+    assert need > 0
+    return need
+
+
+def wide_for(page, positions=2000):
+    return -(-positions // page)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("Hq,H,D,page,fmt", SHAPES)
+def test_split_against_64_bits(gpu, ops, Hq, H, D, page, fmt, dtype):
+    """Tables so wide that every sequence is cut into stretches and joined: ends
+    of sequences inside a stretch, whole ones, empty ones between them."""
+    lens = LENS + [700, 3]
+    pool, table = fill(gpu, ops, lens, H, D, page, fmt, seed=Hq + D, wide=wide_for(page))
+    split(ops, pool, table, len(lens), Hq)
+    check(gpu, ops, queries(gpu, len(lens), Hq, D, getattr(gpu, dtype)), pool, table, lens, fmt)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("window", [1300, 1313, 1999])
+def test_split_windows(gpu, ops, window, dtype):
+    import kc_abi
+    lens = [3000, window - 1, window, window + 1, 0, 5, 2500]
+    for Hq, H, D, page, fmt in ((8, 2, 128, 16, "fp8"), (8, 2, 64, 7, "mxfp4"), (3, 1, 40, 16, "fp8")):
+        pool, table = fill(gpu, ops, lens, H, D, page, fmt, seed=window, window=window)
+        q = queries(gpu, len(lens), Hq, D, getattr(gpu, dtype))
+        d_lens = gpu.tensor(lens, dtype=gpu.int32, device="cuda")
+        assert any("join_kernel" in n for n in kc_abi.kernels_of(
+            lambda: ops.kv_cache_attention(q, *pool, table, d_lens, window=window)))
+        check(gpu, ops, q, pool, table, lens, fmt, window)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_split_lengths_that_the_table_does_not_have(gpu, ops, dtype):
+    for D in (128, 80, 33):
+        pool, table = fill(gpu, ops, [40, 20, 16, 900], 2, D, 16, "fp8", wide=wide_for(16))
+        split(ops, pool, table, 4, 4)
+        room = table.shape[1] * 16
+        table = table.where((table >= 0) & (table < len(pool[0])), table.new_zeros(()))
+        q = queries(gpu, 4, 4, D, getattr(gpu, dtype))
+        check(gpu, ops, q, pool, table, [room + 1, -3, 16, 900], "fp8")
+        check(gpu, ops, q, pool, table, [40, 2 ** 31 - 1, -2 ** 31, 900], "fp8")
+        check(gpu, ops, q, pool, table, [40, 7, 2 ** 31 - 1, 900], "fp8", window=1500)
+
+
+@pytest.mark.parametrize("fmt,D", [("fp8", 128), ("mxfp4", 64), ("fp8", 208), ("fp8", 33)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_split_missing_pages(gpu, ops, D, fmt, dtype):
+    """NaN through the join, for the sequence whose page is missing alone."""
+    lens = [100, 100, 100, 700, 5, 300]
+    pool, table = fill(gpu, ops, lens, 2, D, 16, fmt, wide=wide_for(16))
+    split(ops, pool, table, 6, 8)
+    table[1, 6] = -1
+    table[3, 40] = len(pool[0])
+    y = check(gpu, ops, queries(gpu, 6, 8, D, getattr(gpu, dtype)), pool, table, lens, fmt)
+    assert gpu.isnan(y).flatten(1).all(1).tolist() == [False, True, False, True, False, False]
+
+
+@pytest.mark.parametrize("D,fmt", [(128, "fp8"), (64, "mxfp4"), (160, "fp8"), (33, "fp8")])
+def test_split_nan_and_infinite_queries(gpu, ops, D, fmt):
+    lens = [200, 200, 70]
+    pool, table = fill(gpu, ops, lens, 2, D, 16, fmt, wide=wide_for(16))
+    split(ops, pool, table, 3, 8)
+    d_lens = gpu.tensor(lens, dtype=gpu.int32, device="cuda")
+    for dtype in (gpu.bfloat16, gpu.float32):
+        q = queries(gpu, 3, 8, D, dtype)
+        plain = check(gpu, ops, q, pool, table, lens, fmt)
+        q[0, 1, 5] = float("nan")
+        q[1, 6, 0] = float("inf")
+        y = ops.kv_cache_attention(q, *pool, table, d_lens)
+        bad = gpu.zeros(3, 8, dtype=gpu.bool, device="cuda")
+        bad[0, 1] = bad[1, 6] = True
+        assert bool(gpu.isnan(y[bad]).all()) and gpu.equal(y[~bad], plain[~bad])
+    one = [t.clone() for t in pool]
+    one[3][int(table[1, 3]), 2, 1] = float("nan") if fmt == "fp8" else 255  # one value row's scale, of the second head
+    y = ops.kv_cache_attention(queries(gpu, 3, 8, D, gpu.bfloat16), *one, table, d_lens)
+    assert bool(gpu.isnan(y[1, 4:]).all()) and not bool(gpu.isnan(y[1, :4]).any()) and not bool(gpu.isnan(y[[0, 2]]).any())
+
+
+def test_split_large_and_equal_scores(gpu, ops):
+    lens = [300, 1, 64, 2000]
+    for D, fmt in ((128, "fp8"), (128, "mxfp4"), (33, "fp8")):
+        pool, table = fill(gpu, ops, lens, 2, D, 16, fmt, wide=wide_for(16))
+        split(ops, pool, table, 4, 8)
+        for dtype in (gpu.bfloat16, gpu.float32):
+            for size, scale in ((100.0, None), (0.0, None), (1.0, 0.0), (1.0, 50.0), (1.0, -3.0)):
+                check(gpu, ops, queries(gpu, 4, 8, D, dtype, size=size), pool, table, lens, fmt, scale=scale)
+
+
+def test_split_views(gpu, ops):
+    """Queries that are views, a cache that begins at 16 bytes and no more: the
+    same values from the same kernel."""
+    lens = [50, 333, 0, 64, 900]
+    for D, fmt in ((128, "fp8"), (128, "mxfp4"), (64, "fp8")):
+        pool, table = fill(gpu, ops, lens, 2, D, 16, fmt, wide=wide_for(16))
+        split(ops, pool, table, 5, 8)
+        d_lens = gpu.tensor(lens, dtype=gpu.int32, device="cuda")
+        rows = gpu.randn(5, 12 * D + 8, device="cuda").bfloat16()
+        for lead in (0, 8, 1):
+            q = rows[:, lead:lead + 8 * D].unflatten(1, (8, D))
+            want = ops.kv_cache_attention(q.contiguous(), *pool, table, d_lens)
+            assert gpu.equal(ops.kv_cache_attention(q, *pool, table, d_lens), want)
+
+            def moved(t):
+                raw = gpu.zeros(t.numel() * t.element_size() + 16, dtype=gpu.uint8, device="cuda")
+                return raw[16:].view(t.dtype).view(t.shape).copy_(t)
+            assert gpu.equal(ops.kv_cache_attention(q, *[moved(t) for t in pool], table, d_lens), want)
+
+
+def test_split_offsets_past_32_bits(gpu, ops):
+    """Pages whose codes lie beyond 4 GiB."""
+    H, D, page, pages = 8, 128, 64, 70000
+    lens = [2000, 90]
+    for dtype in (gpu.bfloat16, gpu.float32):
+        pool, table = fill(gpu, ops, lens, H, D, page, "fp8")
+        split(ops, pool, table, 2, 32)
+        far = [gpu.zeros((pages,) + t.shape[1:], dtype=t.dtype, device="cuda") for t in pool]
+        for t, s in zip(far, pool):
+            t[pages - len(s):] = s
+        q = queries(gpu, 2, 32, D, dtype)
+        d_lens = gpu.tensor(lens, dtype=gpu.int32, device="cuda")
+        real = (table >= 0) & (table < len(pool[0]))
+        moved = gpu.where(real, table + (pages - len(pool[0])), -1)
+        assert gpu.equal(ops.kv_cache_attention(q, *far, moved, d_lens), ops.kv_cache_attention(q, *pool, table, d_lens))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("B", [65, 600, 1100])
+def test_split_more_sequences_than_threads(gpu, ops, B, dtype):
+    """A thread counts the tiles of several sequences, some of them empty."""
+    lens = [(37 * i) % 90 * (i % 5 != 2) for i in range(B)]
+    lens[B // 2] = 4000
+    lens[-1] = 0
+    for Hq, H, D, page, fmt in ((8, 2, 64, 16, "fp8"), (2, 1, 128, 32, "mxfp4"), (2, 1, 20, 16, "fp8")):
+        pool, table = fill(gpu, ops, lens, H, D, page, fmt, seed=B)
+        split(ops, pool, table, B, Hq)
+        check(gpu, ops, queries(gpu, B, Hq, D, getattr(gpu, dtype)), pool, table, lens, fmt)
+
+
+@pytest.mark.parametrize("D", [64, 33])
+def test_any_content_of_the_workspace(gpu, ops, D):
+    """What the workspace holds does not matter, NaN included; nothing is written
+    behind it or the output; one byte less is refused."""
+    import kc_abi
+    lens = [4000, 1, 0, 700]
+    pool, table = fill(gpu, ops, lens, 2, D, 16, "fp8")
+    d_lens = gpu.tensor(lens, dtype=gpu.int32, device="cuda")
+    need, cache = workspace(ops, pool, table, 4, 6)
+    assert need > 64
+    L = kc_abi.lib()
+    for fn, dtype in ((L.kc_kv_cache_attention_f32, gpu.float32), (L.kc_kv_cache_attention_bf16, gpu.bfloat16)):
+        q = queries(gpu, 4, 6, D, dtype)
+        want = check(gpu, ops, q, pool, table, lens, "fp8")
+
+        def call(work, bytes_, out):
+            return fn(kc_abi.ptr(q), q.stride(0), 6, ctypes.byref(cache), kc_abi.ptr(table), table.shape[1],
+                      kc_abi.ptr(d_lens), 4, D ** -0.5, 0, kc_abi.ptr(work), bytes_, kc_abi.ptr(out), kc_abi.stream())
+        for byte in (0, 255, 127, 129):
+            work = gpu.full((need + 256,), byte, dtype=gpu.uint8, device="cuda")
+            out = gpu.full((5, 6, D), 9.0, dtype=dtype, device="cuda")
+            assert call(work, need, out) == 0
+            assert gpu.equal(out[:4], want) and bool((out[4] == 9).all()) and bool((work[need:] == byte).all())
+        assert call(work, need - 1, out) == 1 and L.kc_get_last_error() == 1
+
+
+@pytest.mark.parametrize("fmt,D", [("fp8", 128), ("mxfp4", 128), ("fp8", 33)])
+def test_split_graphs_replayed_in_turn(gpu, ops, fmt, D):
+    """Two captured calls, replayed while lengths that move every stretch's bounds,
+    and queries, change in place, with eager calls between."""
+    most = [4000, 20, 0, 64, 1200]
+    pool, table = fill(gpu, ops, most, 2, D, 16, fmt)
+    split(ops, pool, table, 5, 8)
+    d_lens = gpu.tensor(most, dtype=gpu.int32, device="cuda")
+    qs = [queries(gpu, 5, 8, D, dtype, seed=5) for dtype in (gpu.bfloat16, gpu.float32)]
+    side = gpu.cuda.Stream()
+    side.wait_stream(gpu.cuda.current_stream())
+    with gpu.cuda.stream(side):
+        for q in qs:
+            ops.kv_cache_attention(q, *pool, table, d_lens)
+    gpu.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for q in qs:
+        g = gpu.cuda.CUDAGraph()
+        with gpu.cuda.graph(g):
+            outs.append(ops.kv_cache_attention(q, *pool, table, d_lens))
+        graphs.append(g)
+    for lens in (most, [3999, 0, 0, 64, 1199], [17, 20, 0, 0, 1200], [0] * 5, [4000, 1, 0, 33, 3], [2048, 20, 0, 1, 0]):
+        d_lens.copy_(gpu.tensor(lens, dtype=gpu.int32))
+        for q in qs:
+            q.normal_()
+        want = [check(gpu, ops, q, pool, table, lens, fmt) for q in qs]
+        for _ in range(2):
+            for g in graphs:
+                g.replay()
+        gpu.cuda.synchronize()
+        assert all(gpu.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "mxfp4"])
+def test_long_results_repeat(gpu, ops, fmt):
+    """The same bits behind other calls, which leave other parts in the same memory."""
+    lens = [0, 5000, 18000, 40000]
+    pool, table = fill(gpu, ops, lens, 2, 128, 64, fmt, wide=0)
+    split(ops, pool, table, 4, 8)
+    d_lens = gpu.tensor(lens, dtype=gpu.int32, device="cuda")
+    q, other = (queries(gpu, 4, 8, 128, gpu.bfloat16, seed=s) for s in (1, 2))
+    want = check(gpu, ops, q, pool, table, lens, fmt)
+    got = []
+    for _ in range(20):
+        ops.kv_cache_attention(other, *pool, table, d_lens)
+        got.append(ops.kv_cache_attention(q, *pool, table, d_lens))
+    assert all(gpu.equal(y, want) for y in got)
