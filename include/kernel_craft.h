@@ -469,14 +469,17 @@ int kc_kv_cache_read_f32(const kc_kv_cache* cache, const int32_t* d_block_table,
  * over the positions t of the sequence: all of the seq_lens[b] (int32) that it
  * has in the cache, the new token's own among them, or the last `window` of
  * them (0: all).  Computed in fp32 from the values that kc_kv_cache_read_f32
- * gives and rounded once; results do not depend on what other sequences of
- * the batch hold beyond the order in which a long sum is split.  A sequence
- * without tokens (a length of 0 or below) gives zeros; one with a visible
- * position whose page is missing (past max_pages, or an entry outside the
- * pool) gives NaN.  What the cache holds behind a sequence's end, or outside
- * of its window, does not matter, NaN included.  out overlaps no input.  At
- * most 2^31 - 1 slots, seqs * q_heads below 2^24, seqs * max_pages * page_size
- * up to 2^35.
+ * gives and rounded once, but that with bf16 queries a weight p_t (times the
+ * scale of its row of values, in FP8) may be held to 2^-17 of itself, far below
+ * the output's 2^-8.  Sums may hold weights up to 2^8 before the division, so
+ * values past 2^120 / seq_lens[b] may overflow them.  Results do not depend on
+ * what other sequences of the batch hold beyond the order in which a long sum
+ * is split.  A sequence without tokens (a length of 0 or below) gives zeros;
+ * one with a visible position whose page is missing (past max_pages, or an
+ * entry outside the pool) gives NaN.  What the cache holds behind a sequence's
+ * end, or outside of its window, does not matter, NaN included.  out overlaps
+ * no input.  At most 2^31 - 1 slots, seqs * q_heads below 2^24, seqs *
+ * max_pages * page_size up to 2^35.
  *
  * The workspace (16-byte aligned) holds what the parts of a long sequence
  * give before they are joined: kc_kv_cache_attention_workspace() bytes (-1

@@ -6,9 +6,9 @@
 // says how the work is split.
 //
 // The vector kernel is for what the matrix cores' does not take (heads over 256, rows of codes
-// that are no whole 16 bytes, unaligned pools).  It decodes value by value and is bound by that:
-// 4 sequences of up to 30000 tokens, 16 query heads on 8 of 72 in FP8: 70 us for 57 MB, 0.8 TB/s;
-// 16 on one of 576: 180 us for 54 MB.
+// that are no whole 16 bytes, unaligned pools, keys past 64 GiB).  It decodes value by value and
+// is bound by that: 4 sequences of up to 30000 tokens, 16 query heads on 8 of 72 in FP8: 71 us for
+// 57 MB, 7 of them the join; 16 on one of 576: 184 us for 54 MB, 23 of them the join.
 #include <algorithm>
 #include <type_traits>
 
@@ -317,9 +317,10 @@ Plan plan_of(int heads, int waves, int resident, const kc_kv_cache* c, int64_t m
     const int64_t seen = window > 0 ? std::min<int64_t>(room, int64_t{window} + kTile - 1) : room;
     const int64_t tiles = (seen + kTile - 1) / kTile;
     // A workgroup per sequence and set where all of them run at once and none has many tiles:
-    // its waves end at different times and it reads heads apart, but nothing is joined.  fp32
-    // or bf16, FP8, 8 sets: 24 sequences of 33 tiles 12.6 us against 20.3, one of 22 9.5
-    // (12.4), one of 63 17.3 (13.1); in two rounds, 64 of 32 21.1 (18.1).
+    // its waves end at different times and it reads heads apart, but nothing is joined.  FP8, 8
+    // sets: one sequence of 22 tiles 9.9 us against 12.8 split and joined, 24 of 33 in fp32 11.9
+    // (17.8), one of 63 17.6 (13.3); in two rounds, 64 of up to 32 21.7 (18.1).  A table's width
+    // is what the host knows: the one of 22 tiles in a table of 4096 is split, 13.2.
     const int64_t rounds = (int64_t{seqs} * p.sets * waves + resident - 1) / resident;
     if (tiles * std::max<int64_t>(rounds, 1) <= kDirectTiles * waves) {
         p.wg_sets = 1;
@@ -440,8 +441,10 @@ int attention(const char* fn, const Elem<BF16>* q, int64_t q_stride, int q_heads
     else launch_vector<BF16, false>(p, plan.grid, stream);
     const int launched = kc::check_launch(fn);
     if (launched != KC_SUCCESS || plan.units == 0) return launched;
-    // one wave per query head of a sequence where that makes waves enough, else 4 or 8 (16 with half
-    // the segments in flight: 4 sequences of 16384 tokens 19.4 us, so 18.8)
+    // One wave per query head of a sequence where that makes waves enough, else 4 or 8.  The join
+    // with 1, 4 and 8 of them: 128 pairs (4 sequences of up to 131072 tokens) 16.2, 7.2 and 7.5 us,
+    // 512 5.4, 4.5 and 5.7, 1024 4.3, 5.2 and 8.4, 2048 (64 of up to 2000) 4.3, 7.4 and 12.6.
+    // Lengths are not looked at: one of 100000 among 63 of 100 takes 20.8, 18.1 and 17.6.
     const int64_t pairs = int64_t{seqs} * q_heads;
     const int split = pairs >= 2048 ? 1 : pairs >= 512 ? 4 : 8, waves = std::max(split, 4), per_wg = waves / split;
     const dim3 join_grid(seqs, (q_heads + per_wg - 1) / per_wg);

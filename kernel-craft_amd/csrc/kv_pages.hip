@@ -12,8 +12,8 @@
 // Bound by latency: a few bytes per request and 12 per token.  One launch: every
 // workgroup scans all requests by itself (three block scans, 8 bytes a request from the
 // cache), so that none waits for another, and takes as many rows of the batch as it has
-// threads.  256 requests of a token each 5.2 us, 40 chunks of 16384 tokens together 5.6 us;
-// releasing 64 or 1000 of 1000 requests 3.2 and 4.8 us, where an empty launch takes 1.5.
+// threads.  256 requests of a token each 5.0 us, 40 chunks of 16000 tokens together 5.3;
+// releasing half of 64 or of 1000 requests 3.5 and 5.1, where an empty launch takes 1.5.
 #include <algorithm>
 
 #include "kc_common.hpp"
@@ -23,7 +23,7 @@ namespace {
 using kc::kWave;
 
 // Threads of a workgroup: 256 where that is one request each, else 1024 (a scan over 16
-// waves and 1024 LDS entries: 256 requests 5.2 us, 6.5 with 1024 threads).
+// waves and 1024 LDS entries: 1.3 us more for 256 requests).
 constexpr int kFew = 256, kMany = 1024;
 
 constexpr int kMaxRequests = 1 << 20;  // every workgroup goes over all of them

@@ -9,8 +9,8 @@
 // Bound by memory: y, h and a gate per value once in, h' and n (or codes) once out.  A
 // workgroup holds a row in registers, W units of 8 values per thread; its gammas and a
 // channel gate stay in registers from row to row.  8000 rows of 4096 in bf16 with both norms
-// and a channel gate, to codes: 229 MB in 46 us, 5.0 TB/s, as fast as a copy; 2003 of 5120 on an
-// fp32 stream: 143 MB in 24 us, 5.9 TB/s, part of it from cache; one row 3.6 us, all of it the
+// and a channel gate, to codes: 229 MB in 44 us, 5.2 TB/s (a copy of 1 GiB 5.0); 2003 of 5120 on
+// an fp32 stream: 144 MB in 25 us, 5.8 TB/s, part of it from cache; one row 3.2 us, all of it the
 // launch, the trip to memory and the row's sums.
 #include <algorithm>
 #include <type_traits>

@@ -1153,9 +1153,9 @@ def kv_cache_attention(q, k_codes, k_scales, v_codes, v_scales, block_table, seq
     (int32) positions that sequence b has in the cache, its newest token's among them, in the
     pages block_table[b] (int32 [sequences, most pages]); only the last ``window`` of them if it
     is not 0.  q_heads is a multiple of the cache's kv_heads, scale 1 / sqrt(D) by default.  fp32
-    arithmetic on the values that kv_cache_read gives, rounded once.  A sequence of length 0
-    gives zeros, one with a visible position whose page is missing NaN
-    (kc_kv_cache_attention_*)."""
+    arithmetic on the values that kv_cache_read gives, rounded once; with bf16 queries the weights
+    are held to 2^-17.  A sequence of length 0 gives zeros, one with a visible position whose page
+    is missing NaN (kc_kv_cache_attention_*)."""
     import torch
     op = "kv_cache_attention"
     cache, Hkv, D = _kv_cache(op, k_codes, k_scales, v_codes, v_scales)
